@@ -472,6 +472,120 @@ int pk_features_push(const pk_features_desc *fe, const float *samples, int64_t s
                      int32_t batch, void *out, int32_t out_dtype, int32_t max_frames,
                      int32_t *num_frames, void *stream);
 
+/* ---------------- token pools: paged K/V that grows with its requests ------
+ * The cache of a text decoder behind the transcripts (a decoder that checks
+ * the greedy path and its alternatives as a tree of drafted tokens): one table
+ * row of pages per request slot, pages taken from one LIFO free stack, every
+ * length on the device.  The reference has no such cache; the calls follow
+ * the windowed pool's (begin_step, append, attention, end_step). */
+typedef struct pk_token_kv_desc {
+    void *kv;             /* [num_pages][num_layers][2][num_kv_heads][page_size][head_dim] */
+    int32_t *page_table;  /* [num_slots][table_width], -1 = no page           */
+    int32_t *free_pages;  /* [num_pages] stack of free page ids               */
+    int32_t *free_count;  /* [1] entries on the stack                         */
+    int32_t *lengths;     /* [num_slots] tokens kept                          */
+    int32_t *held;        /* [num_slots] pages held                           */
+    int32_t *scratch;     /* [4 * num_slots + 16] working space of the calls  */
+    int32_t *error;       /* [1] device error word (PK_DEV_* bits)            */
+    int32_t num_pages;
+    int32_t num_slots;
+    int32_t num_layers;
+    int32_t num_heads;    /* query heads, a multiple of num_kv_heads          */
+    int32_t num_kv_heads;
+    int32_t head_dim;     /* 64 or 128                                        */
+    int32_t page_size;    /* tokens per page, a power of two in [8, 256]      */
+    int32_t table_width;  /* pages a request can hold                         */
+    int32_t dtype;        /* PK_DTYPE_*                                       */
+} pk_token_kv_desc;
+
+typedef struct pk_token_kv pk_token_kv; /* opaque: desc + TMA descriptor */
+
+int pk_token_kv_create(const pk_token_kv_desc *desc, pk_token_kv **out);
+int pk_token_kv_destroy(pk_token_kv *kv);
+
+/* Every page free, every request empty.  The stack is filled with `init_order`
+ * (device int32 [num_pages], a permutation) or 0..num_pages-1 when NULL; pages
+ * are taken from its end. */
+int pk_token_reset(pk_token_kv *kv, const int32_t *init_order, void *stream);
+
+/* Words (int32) of a step block for `batch` requests and `rows` token rows, and
+ * where its arrays begin.  offsets (int64 [PK_TOK_OFFSETS]) may be NULL:
+ *   PK_TOK_ROW_START  [batch + 1] first row of each request, clamped to `rows`
+ *   PK_TOK_CONTEXT    [batch]  tokens kept before the step; -1: request refused
+ *   PK_TOK_REQUEST    [rows]   the row's request, -1 behind the last request
+ *   PK_TOK_POSITION   [rows]   context + depth in the tree
+ *   PK_TOK_SLOT_MAP   [rows]   page * page_size + row in the page, -1: none
+ *   PK_TOK_MASK       [rows]   int64 bits of the row's ancestors and itself
+ *                              (only with parents)
+ * The other entries are the library's. */
+#define PK_TOK_ROW_START 0
+#define PK_TOK_CONTEXT 1
+#define PK_TOK_SLOT 2
+#define PK_TOK_UNIT_START 3
+#define PK_TOK_PART_START 4
+#define PK_TOK_TAKE 5
+#define PK_TOK_HELD 6
+#define PK_TOK_REQUEST 7
+#define PK_TOK_POSITION 8
+#define PK_TOK_SLOT_MAP 9
+#define PK_TOK_UNITS 10
+#define PK_TOK_MASK 11
+#define PK_TOK_OFFSETS 12
+#define PK_TOK_MAX_TREE 64      /* most nodes of one tree                     */
+#define PK_TOK_MAX_BATCH 65536  /* most requests of one step                  */
+int64_t pk_token_step_words(const pk_token_kv *kv, int32_t batch, int32_t rows, int32_t trees,
+                            int64_t *offsets);
+
+/* Start of one step of `batch` requests (slots: distinct rows of the table,
+ * counts: their new tokens, packed in this order into `rows` rows): takes pages
+ * for the tokens that the held pages do not cover, in batch order, and writes
+ * the step block.  parents (int32 [rows], NULL = each token follows the one
+ * before): the parent node of each token inside its request, below the token's
+ * own index, -1 = the context; at most PK_TOK_MAX_TREE tokens then.
+ * A request that cannot be served (slot out of range or twice, count out of
+ * range, no room in its table row, rows past `rows`, no pages left) sets its
+ * error bit and is left out: CONTEXT -1, its rows' SLOT_MAP -1, no state
+ * changed; the others are served.  A bad parent counts as -1 (PK_DEV_BAD_COUNT).
+ * Needs no host read: lengths stay on the device, so a step can be captured. */
+int pk_token_begin_step(pk_token_kv *kv, const int32_t *slots, const int32_t *counts,
+                        int32_t batch, const int32_t *parents, int32_t rows, int32_t *step,
+                        void *stream);
+
+/* K and V rows of layers [layer0, layer0 + num_layers) into the pages: element
+ * (l, r, h, c) at l*layer_stride + r*row_stride + h*head_stride + c.  Rows with
+ * SLOT_MAP -1 are skipped. */
+int pk_token_append(pk_token_kv *kv, int32_t layer0, int32_t num_layers, const void *key,
+                    const void *value, int64_t layer_stride, int64_t row_stride,
+                    int64_t head_stride, int32_t batch, int32_t rows, int32_t trees,
+                    const int32_t *step, void *stream);
+
+/* Attention of the step's rows over their request's context and their
+ * ancestors (without parents: the rows before), themselves among them:
+ *   out[r][h] = softmax(scale * q[r][h] . k[j][h / group]) . v[j][h / group].
+ * query (r, h, c) at r*q_row_stride + h*q_head_stride + c, out likewise.  Keys
+ * that a row does not see have no part in it, whatever they hold.  Rows behind
+ * the last request and of refused requests are left as they were.  workspace:
+ * pk_token_attention_workspace() bytes (0: may be NULL), for this call alone. */
+int64_t pk_token_attention_workspace(const pk_token_kv *kv, int32_t batch, int32_t rows);
+int pk_token_attention(pk_token_kv *kv, int32_t layer, const void *query, int64_t q_row_stride,
+                       int64_t q_head_stride, float scale, int32_t batch, int32_t rows,
+                       int32_t trees, const int32_t *step, void *out, int64_t o_row_stride,
+                       int64_t o_head_stride, void *workspace, void *stream);
+
+/* End of the step: last[b] is the deepest kept node of request b (-1: none).
+ * The rows on its path are moved behind the context in order of depth, in
+ * every layer, and lengths grow by the path's tokens.  Pages stay with the
+ * request (the next step's tokens need them).  A bad last[b] sets
+ * PK_DEV_BAD_COUNT and keeps nothing. */
+int pk_token_end_step(pk_token_kv *kv, const int32_t *last, int32_t batch, int32_t rows,
+                      int32_t trees, const int32_t *step, void *stream);
+
+/* Requests cut to lengths[b] tokens (0: released); pages past the end go back
+ * on the stack, the last taken on top.  A length above the present one, or a
+ * slot out of range or twice, sets its error bit and leaves the request. */
+int pk_token_truncate(pk_token_kv *kv, const int32_t *slots, const int32_t *lengths,
+                      int32_t batch, void *stream);
+
 /* Self-test of the failure path of every TMA pipeline here: the bounded
  * mbarrier wait that gives up after a time limit and records PK_DEV_TIMEOUT in
  * *error (instead of hanging the GPU), leaving the context usable.  One CTA

@@ -1,0 +1,200 @@
+// C-ABI entry points of the token pools (include/pk.h): argument checks on the
+// host, the pool's TMA descriptor, dispatch.
+#include <math.h>
+#include <stdlib.h>
+
+#include "pk_internal.h"
+
+using namespace pk;
+
+#define PK_CHECK(cond, ...)             \
+    do {                                \
+        if (!(cond)) {                  \
+            pk::set_error(__VA_ARGS__); \
+            return PK_EINVAL;           \
+        }                               \
+    } while (0)
+
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What every call on a step block needs.
+#define PK_CHECK_STEP(kv, batch, rows, step)                                                   \
+    PK_CHECK(kv, "null pool");                                                                 \
+    PK_CHECK((batch) >= 0 && (batch) <= PK_TOK_MAX_BATCH && (batch) <= (kv)->d.num_slots,       \
+             "batch %d outside [0, min(num_slots, %d)]", (batch), PK_TOK_MAX_BATCH);           \
+    PK_CHECK((rows) >= 0 && (int64_t)(rows) * (kv)->d.num_heads <= 0x7fffffff,                 \
+             "rows %d: negative or too many", (rows));                                         \
+    PK_CHECK((batch) == 0 || ((step) && aligned16(step)), "step block null or not 16-byte aligned")
+
+extern "C" {
+
+int pk_token_kv_create(const pk_token_kv_desc *desc, pk_token_kv **out) {
+    PK_CHECK(desc && out, "null argument");
+    const pk_token_kv_desc &d = *desc;
+    PK_CHECK(d.kv && d.page_table && d.free_pages && d.free_count && d.lengths && d.held &&
+                 d.scratch && d.error,
+             "null device buffer in descriptor");
+    PK_CHECK(d.dtype == PK_DTYPE_F32 || d.dtype == PK_DTYPE_BF16, "bad dtype %d", d.dtype);
+    PK_CHECK(d.num_pages > 0 && d.num_slots > 0 && d.num_layers > 0 && d.table_width > 0,
+             "empty pool");
+    PK_CHECK(d.num_kv_heads > 0 && d.num_heads > 0 && d.num_heads % d.num_kv_heads == 0,
+             "num_heads (%d) must be a multiple of num_kv_heads (%d)", d.num_heads, d.num_kv_heads);
+    PK_CHECK(d.head_dim == 64 || d.head_dim == 128, "head_dim %d: 64 or 128", d.head_dim);
+    PK_CHECK(d.page_size >= 8 && d.page_size <= 256 && (d.page_size & (d.page_size - 1)) == 0,
+             "page_size must be a power of two in [8, 256]");
+    PK_CHECK((int64_t)d.num_pages * d.page_size <= 0x7fffffff &&
+                 (int64_t)d.table_width * d.page_size <= 0x7fffffff - 65536,
+             "more tokens than 32 bits count");
+    const int64_t planes = (int64_t)d.num_pages * d.num_layers * 2 * d.num_kv_heads;
+    PK_CHECK(planes <= 0x7fffffff, "more (page, layer, head) planes than 32 bits count");
+    PK_CHECK(aligned16(d.kv), "kv pool not 16-byte aligned");
+    pk_token_kv *kv = static_cast<pk_token_kv *>(calloc(1, sizeof(pk_token_kv)));
+    PK_CHECK(kv, "out of host memory");
+    kv->d = d;
+    kv->esize = d.dtype == PK_DTYPE_BF16 ? 2 : 4;
+    kv->group = d.num_heads / d.num_kv_heads;
+    while ((1 << kv->ps_shift) < d.page_size) ++kv->ps_shift;
+    // two waves of two CTAs an SM
+    kv->target = (4 * (int64_t)current_sms() + d.num_kv_heads - 1) / d.num_kv_heads;
+    if (d.dtype == PK_DTYPE_BF16) {
+        const uint64_t row = (uint64_t)d.head_dim * 2;
+        int st = encode_tmap_3d(&kv->kv_map, d.dtype, d.kv, d.head_dim, d.page_size,
+                                (uint64_t)planes, row, row * d.page_size, 64,
+                                d.page_size < kTokTile ? d.page_size : kTokTile, 1);
+        if (st != PK_OK) {
+            free(kv);
+            return st;
+        }
+    }
+    *out = kv;
+    return PK_OK;
+}
+
+int pk_token_kv_destroy(pk_token_kv *kv) {
+    free(kv);
+    return PK_OK;
+}
+
+int pk_token_reset(pk_token_kv *kv, const int32_t *init_order, void *stream) {
+    PK_CHECK(kv, "null pool");
+    return launch_token_reset(kv, init_order, static_cast<cudaStream_t>(stream));
+}
+
+int64_t pk_token_step_words(const pk_token_kv *kv, int32_t batch, int32_t rows, int32_t trees,
+                            int64_t *offsets) {
+    if (!kv || batch < 0 || rows < 0) return -1;
+    const TokLayout l = tok_layout(kv, batch, rows, trees);
+    if (offsets) {
+        offsets[PK_TOK_ROW_START] = l.row_start;
+        offsets[PK_TOK_CONTEXT] = l.context;
+        offsets[PK_TOK_SLOT] = l.slot;
+        offsets[PK_TOK_UNIT_START] = l.unit_start;
+        offsets[PK_TOK_PART_START] = l.part_start;
+        offsets[PK_TOK_TAKE] = l.take;
+        offsets[PK_TOK_HELD] = l.held;
+        offsets[PK_TOK_REQUEST] = l.request;
+        offsets[PK_TOK_POSITION] = l.position;
+        offsets[PK_TOK_SLOT_MAP] = l.slot_map;
+        offsets[PK_TOK_UNITS] = l.units;
+        offsets[PK_TOK_MASK] = l.mask;
+    }
+    return l.words;
+}
+
+int pk_token_begin_step(pk_token_kv *kv, const int32_t *slots, const int32_t *counts,
+                        int32_t batch, const int32_t *parents, int32_t rows, int32_t *step,
+                        void *stream) {
+    PK_CHECK_STEP(kv, batch, rows, step);
+    if (batch == 0) return PK_OK;
+    PK_CHECK(slots && counts, "null slots/counts");
+    return launch_token_begin(kv, slots, counts, batch, parents, rows, step,
+                              static_cast<cudaStream_t>(stream));
+}
+
+int pk_token_append(pk_token_kv *kv, int32_t layer0, int32_t num_layers, const void *key,
+                    const void *value, int64_t layer_stride, int64_t row_stride,
+                    int64_t head_stride, int32_t batch, int32_t rows, int32_t trees,
+                    const int32_t *step, void *stream) {
+    PK_CHECK_STEP(kv, batch, rows, step);
+    PK_CHECK(layer0 >= 0 && num_layers >= 0 && num_layers <= kv->d.num_layers - layer0,
+             "layers [%d, +%d) outside [0, %d)", layer0, num_layers, kv->d.num_layers);
+    PK_CHECK(num_layers <= 65535, "more than 65535 layers in one call");
+    if (batch == 0 || rows == 0 || num_layers == 0) return PK_OK;
+    PK_CHECK(key && value && aligned16(key) && aligned16(value),
+             "key/value null or not 16-byte aligned");
+    const int es = kv->esize;
+    PK_CHECK((layer_stride * es) % 16 == 0 && (row_stride * es) % 16 == 0 &&
+                 (head_stride * es) % 16 == 0,
+             "strides must be multiples of 16 bytes");
+    TokAppendArgs a;
+    a.key = key;
+    a.value = value;
+    a.ls = layer_stride;
+    a.rs = row_stride;
+    a.hs = head_stride;
+    a.layer0 = layer0;
+    a.nlayers = num_layers;
+    a.batch = batch;
+    a.rows = rows;
+    a.trees = trees;
+    a.step = step;
+    return launch_token_append(kv, a, static_cast<cudaStream_t>(stream));
+}
+
+int64_t pk_token_attention_workspace(const pk_token_kv *kv, int32_t batch, int32_t rows) {
+    return kv && batch >= 0 && rows >= 0 ? tree_attn_workspace(kv, batch, rows) : -1;
+}
+
+int pk_token_attention(pk_token_kv *kv, int32_t layer, const void *query, int64_t q_row_stride,
+                       int64_t q_head_stride, float scale, int32_t batch, int32_t rows,
+                       int32_t trees, const int32_t *step, void *out, int64_t o_row_stride,
+                       int64_t o_head_stride, void *workspace, void *stream) {
+    PK_CHECK_STEP(kv, batch, rows, step);
+    PK_CHECK(layer >= 0 && layer < kv->d.num_layers, "layer out of range");
+    PK_CHECK(scale > 0.f && isfinite(scale), "scale must be positive and finite");
+    if (batch == 0 || rows == 0) return PK_OK;
+    PK_CHECK(query && out && aligned16(query) && aligned16(out),
+             "query/out null or not 16-byte aligned");
+    const int es = kv->esize;
+    PK_CHECK((q_row_stride * es) % 16 == 0 && (q_head_stride * es) % 16 == 0 &&
+                 (o_row_stride * es) % 16 == 0 && (o_head_stride * es) % 16 == 0,
+             "strides must be multiples of 16 bytes");
+    PK_CHECK((workspace && aligned16(workspace)) || tree_attn_workspace(kv, batch, rows) == 0,
+             "workspace null or not 16-byte aligned");
+    TreeAttnArgs a;
+    a.q = query;
+    a.q_rs = q_row_stride;
+    a.q_hs = q_head_stride;
+    a.out = out;
+    a.o_rs = o_row_stride;
+    a.o_hs = o_head_stride;
+    a.scale = scale;
+    a.layer = layer;
+    a.batch = batch;
+    a.rows = rows;
+    a.trees = trees != 0;
+    a.step = step;
+    a.ws = static_cast<float *>(workspace);
+    return launch_tree_attention(kv, a, static_cast<cudaStream_t>(stream));
+}
+
+int pk_token_end_step(pk_token_kv *kv, const int32_t *last, int32_t batch, int32_t rows,
+                      int32_t trees, const int32_t *step, void *stream) {
+    PK_CHECK_STEP(kv, batch, rows, step);
+    if (batch == 0) return PK_OK;
+    PK_CHECK(last, "null last");
+    PK_CHECK(kv->d.num_layers <= 65535, "more than 65535 layers");
+    return launch_token_end(kv, last, batch, rows, trees, step, static_cast<cudaStream_t>(stream));
+}
+
+int pk_token_truncate(pk_token_kv *kv, const int32_t *slots, const int32_t *lengths,
+                      int32_t batch, void *stream) {
+    PK_CHECK(kv, "null pool");
+    PK_CHECK(batch >= 0 && batch <= kv->d.num_slots && batch <= PK_TOK_MAX_BATCH,
+             "batch %d outside [0, min(num_slots, %d)]", batch, PK_TOK_MAX_BATCH);
+    if (batch == 0) return PK_OK;
+    PK_CHECK(slots && lengths, "null slots/lengths");
+    return launch_token_truncate(kv, slots, lengths, batch, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "pk.h"
 
 struct pk_paged_kv {
@@ -203,5 +205,113 @@ struct FeArgs {
     int32_t *nframes;
 };
 int launch_features(const FeArgs &a, cudaStream_t s);
+
+// pk_tokens.cu / pk_tree_attn.cu: token pools
+}  // namespace pk
+
+struct pk_token_kv {
+    pk_token_kv_desc d;
+    CUtensorMap kv_map;  // bf16 pools: {head_dim, page_size, pages*layers*2*kv_heads}, boxes of
+                         // 64 columns x min(page_size, 64) rows, 128B-swizzled
+    int ps_shift, esize, group;
+    int64_t target;      // attention units per K/V head that a step aims at
+};
+
+namespace pk {
+
+// Key tokens of one attention tile.
+constexpr int kTokTile = 64;
+
+// Step block, int32 words: header, then arrays at these offsets.
+enum TokHeader { kTokChunk = 0, kTokUnits, kTokRows, kTokFree, kTokHeaderWords = 16 };
+struct TokLayout {
+    int64_t row_start, context, slot, unit_start, part_start, take, held, request, position,
+        slot_map, units, mask, words;
+};
+// One attention unit (a row tile of one request over a range of key tiles), 8
+// words, for every K/V head: slot, first row, tokens, context, row tile, first
+// and end key tile, partial (-1: the only range of its rows).
+constexpr int kTokUnitWords = 8;
+
+// Query rows (token x group) of one attention tile: the narrowest of 16, 32 and
+// 64 that holds an average request, since a tile's K/V is read once per row tile.
+inline int tok_tile_rows(const pk_token_kv *kv, int batch, int rows) {
+    if (kv->d.dtype == PK_DTYPE_F32) return 16;
+    const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
+    return mean <= 16 ? 16 : (mean <= 32 ? 32 : 64);
+}
+// Most units of a step: the aimed-at number plus one for each row tile's last range.
+inline int64_t tok_max_units(const pk_token_kv *kv, int batch, int rows) {
+    const int bm = tok_tile_rows(kv, batch, rows);
+    return kv->target + ((int64_t)rows * kv->group) / bm + batch;
+}
+// Ranges of row tiles that have more than one: at most twice the aimed-at number.
+inline int64_t tok_max_parts(const pk_token_kv *kv) { return 2 * kv->target; }
+// Key tiles below which a range is not split.
+constexpr int kTokMinChunk = 8;
+inline TokLayout tok_layout(const pk_token_kv *kv, int batch, int rows, int trees) {
+    TokLayout l;
+    int64_t o = kTokHeaderWords;
+    auto take = [&](int64_t n) {
+        const int64_t at = o;
+        o += n;
+        return at;
+    };
+    l.row_start = take(batch + 1);
+    l.context = take(batch);
+    l.slot = take(batch);
+    l.unit_start = take(batch + 1);
+    l.part_start = take(batch + 1);
+    l.take = take(batch + 1);
+    l.held = take(batch);
+    l.request = take(rows);
+    l.position = take(rows);
+    l.slot_map = take(rows);
+    o = (o + 3) / 4 * 4;
+    l.units = take(tok_max_units(kv, batch, rows) * kTokUnitWords);
+    l.mask = take(trees ? 2 * (int64_t)rows : 0);
+    l.words = o;
+    return l;
+}
+int launch_token_reset(const pk_token_kv *kv, const int32_t *init_order, cudaStream_t s);
+int launch_token_begin(const pk_token_kv *kv, const int32_t *slots, const int32_t *counts,
+                       int batch, const int32_t *parents, int rows, int32_t *step, cudaStream_t s);
+struct TokAppendArgs {
+    const void *key, *value;
+    int64_t ls, rs, hs;
+    int layer0, nlayers, batch, rows, trees;
+    const int32_t *step;
+};
+int launch_token_append(const pk_token_kv *kv, const TokAppendArgs &a, cudaStream_t s);
+int launch_token_end(const pk_token_kv *kv, const int32_t *last, int batch, int rows, int trees,
+                     const int32_t *step, cudaStream_t s);
+int launch_token_truncate(const pk_token_kv *kv, const int32_t *slots, const int32_t *lengths,
+                          int batch, cudaStream_t s);
+struct TreeAttnArgs {
+    const void *q;
+    int64_t q_rs, q_hs, o_rs, o_hs;
+    void *out;
+    float scale;
+    int layer, batch, rows, trees;
+    const int32_t *step;
+    float *ws;
+};
+int64_t tree_attn_workspace(const pk_token_kv *kv, int batch, int rows);
+int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStream_t s);
+
+// Allow `bytes` of dynamic shared memory for `kernel` on the current device, once
+// per device (`done`: a bit per device, of the kernel's own).
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+int current_sms();   // multiprocessors of the current device
 
 }  // namespace pk

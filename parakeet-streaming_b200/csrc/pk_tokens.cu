@@ -1,0 +1,629 @@
+// Token pools: page tables, slot maps and tree masks from request lengths, and
+// the cache traffic of a step (append, keep the accepted path, cut).
+//
+// For request b with len tokens kept, held pages and n new tokens:
+//   take(b)  = max(ceil((len + n) / page_size) - held, 0)
+//   page i of the step's new pages = free_pages[free_count - 1 - i], batch order
+//   node j's cache row = table[(len + j) / page_size] * page_size + (len + j) % page_size
+//   mask(j) = bit j | mask(parent(j)),  position(j) = len + |ancestors of j|
+//
+// The prefix sums over the batch (rows, pages, attention units) need every
+// request, so one CTA makes them; what they place (rows, table entries, unit
+// records) is written by that CTA too while there is little of it, and by a grid
+// otherwise.  Masks come by doubling over the ancestors (mask |= mask[jump],
+// jump = jump[jump]): 6 rounds of warp shuffles for 64 nodes, whatever the depth.
+// Everything is integer work bound by latency: a few thousand rows are written
+// faster than a second launch starts.  The pages go back in the order that
+// restores the stack exactly, so a step that is cut back leaves no trace.
+#include "pk_common.cuh"
+#include "pk_internal.h"
+
+namespace pk {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+// Rows (and twice the table entries) that the planning CTA writes itself: above
+// it a second launch over the whole GPU is faster.
+constexpr int kOneCtaRows = 2048;
+
+struct TokParams {
+    pk_token_kv_desc d;
+    TokLayout l;
+    int ps_shift, group, tile_rows, batch, rows;
+    int64_t target, max_units;
+    const int32_t *slots, *counts, *parents;
+    int32_t *step;
+};
+
+__device__ int64_t block_exclusive_sum64(int64_t v, int64_t &total, int64_t *s_warp) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[wid] = x;
+    __syncthreads();
+    if (wid == 0) {
+        int64_t t = lane < nw ? s_warp[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += y;
+        }
+        if (lane < nw) s_warp[lane] = t;
+        if (lane == 31) s_warp[32] = t;
+    }
+    __syncthreads();
+    total = s_warp[32];
+    const int64_t res = (wid > 0 ? s_warp[wid - 1] : 0) + x - v;
+    __syncthreads();
+    return res;
+}
+
+// Marks every slot of the batch with the first request that names it; a slot
+// out of range is nobody's.  scratch[0 .. num_slots) is the mark.
+__device__ void mark_slots(const pk_token_kv_desc &d, const int32_t *slots, int batch) {
+    for (int b = threadIdx.x; b < batch; b += blockDim.x) {
+        const int s = slots[b];
+        if (s >= 0 && s < d.num_slots) d.scratch[s] = 0x7fffffff;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < batch; b += blockDim.x) {
+        const int s = slots[b];
+        if (s >= 0 && s < d.num_slots) atomicMin(&d.scratch[s], b);
+    }
+    __syncthreads();
+}
+__device__ bool owns_slot(const pk_token_kv_desc &d, int slot, int b) {
+    return slot >= 0 && slot < d.num_slots && d.scratch[slot] == b;
+}
+
+__device__ __forceinline__ int ceil_shift(int64_t n, int shift) {
+    return (int)((n + (1 << shift) - 1) >> shift);
+}
+
+// Page i of a request: a held one, or the step's (free stack, top first).
+__device__ __forceinline__ int page_of(const TokParams &p, int slot, int held, int first,
+                                       int free_n, int i) {
+    return i < held ? p.d.page_table[(int64_t)slot * p.d.table_width + i]
+                    : p.d.free_pages[free_n - 1 - (first + i - held)];
+}
+
+// The planning CTA.  Thread t owns the requests [t * nk, (t + 1) * nk), so that
+// each prefix sum is one scan over the threads' sums.
+__device__ void begin_plan(const TokParams &p) {
+    __shared__ int64_t s_scan[33];
+    __shared__ unsigned long long s_take;
+    const pk_token_kv_desc &d = p.d;
+    int32_t *st = p.step;
+    const int nk = (p.batch + blockDim.x - 1) / blockDim.x;
+    const int b0 = threadIdx.x * nk, b1 = min(b0 + nk, p.batch);
+    const int free_n = *d.free_count;
+    if (threadIdx.x == 0) s_take = 0;
+    mark_slots(d, p.slots, p.batch);
+
+    // rows; which requests can be served but for their pages
+    int64_t sum = 0, total;
+    for (int b = b0; b < b1; ++b) sum += max(p.counts[b], 0);
+    int64_t at = block_exclusive_sum64(sum, total, s_scan);
+    int64_t takes = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int slot = p.slots[b], n = p.counts[b];
+        const int64_t end = at + max(n, 0);
+        int ctx = -1, held = 0, take = 0, err = 0;
+        if (!owns_slot(d, slot, b)) {
+            err = PK_DEV_BAD_SLOT;
+        } else if (n < 0 || end > p.rows || (p.parents && n > PK_TOK_MAX_TREE)) {
+            err = PK_DEV_BAD_COUNT;
+        } else {
+            const int len = d.lengths[slot];
+            const int need = ceil_shift((int64_t)len + n, p.ps_shift);
+            held = d.held[slot];
+            if (need > d.table_width || (int64_t)len + n > 0x7fffffff) {
+                err = PK_DEV_BAD_COUNT;
+            } else {
+                ctx = len;
+                take = max(need - held, 0);
+            }
+        }
+        if (err) raise(d.error, err);
+        st[p.l.row_start + b] = (int)min(at, (int64_t)p.rows);
+        st[p.l.context + b] = ctx;
+        st[p.l.slot + b] = slot;
+        st[p.l.held + b] = held;
+        takes += take;
+        at = end;
+    }
+    if (threadIdx.x == 0) {
+        const int used = (int)min(total, (int64_t)p.rows);
+        st[p.l.row_start + p.batch] = used;
+        st[kTokRows] = used;
+        st[kTokFree] = free_n;
+    }
+
+    // pages, in batch order: requests past the end of the stack are left out
+    int64_t first = block_exclusive_sum64(takes, total, s_scan);
+    int64_t tiles = 0, taken = 0;
+    const int bm = p.tile_rows;
+    for (int b = b0; b < b1; ++b) {
+        int ctx = st[p.l.context + b];
+        const int held = st[p.l.held + b], n = max(p.counts[b], 0);
+        const int take = ctx < 0 ? 0 : max(ceil_shift((int64_t)ctx + n, p.ps_shift) - held, 0);
+        st[p.l.take + b] = (int)min(first, (int64_t)0x7fffffff);
+        if (take > 0 && first + take > free_n) {
+            raise(d.error, PK_DEV_POOL_EXHAUSTED);
+            st[p.l.context + b] = ctx = -1;
+        } else if (take > 0) {
+            taken += take;
+            d.held[st[p.l.slot + b]] = held + take;
+        }
+        first += take;
+        if (ctx >= 0 && n > 0)
+            tiles += ((int64_t)n * p.group + bm - 1) / bm *
+                     (((int64_t)ctx + n + kTokTile - 1) / kTokTile);
+    }
+    if (taken) atomicAdd(&s_take, (unsigned long long)taken);
+
+    // attention units: ranges of `chunk` key tiles, so that there are about
+    // `target` of them per K/V head
+    block_exclusive_sum64(tiles, total, s_scan);
+    const int chunk = (int)max((total + p.target - 1) / p.target, (int64_t)kTokMinChunk);
+    int64_t units = 0;
+    auto ranges = [&](int b, int64_t &rt, int64_t &ns) {
+        const int ctx = st[p.l.context + b], n = max(p.counts[b], 0);
+        rt = ctx >= 0 && n > 0 ? ((int64_t)n * p.group + bm - 1) / bm : 0;
+        ns = rt ? (((int64_t)ctx + n + kTokTile - 1) / kTokTile + chunk - 1) / chunk : 0;
+    };
+    for (int b = b0; b < b1; ++b) {
+        int64_t rt, ns;
+        ranges(b, rt, ns);
+        units += rt * ns + (ns > 1 ? (rt * ns) << 32 : 0);   // units low, partials high
+    }
+    int64_t u = block_exclusive_sum64(units, total, s_scan);
+    for (int b = b0; b < b1; ++b) {
+        int64_t rt, ns;
+        ranges(b, rt, ns);
+        st[p.l.unit_start + b] = (int)(u & 0xffffffff);
+        st[p.l.part_start + b] = (int)(u >> 32);
+        u += rt * ns + (ns > 1 ? (rt * ns) << 32 : 0);
+    }
+    if (threadIdx.x == 0) {
+        st[kTokChunk] = chunk;
+        st[kTokUnits] = (int)min(total & 0xffffffff, p.max_units);
+        st[p.l.unit_start + p.batch] = (int)(total & 0xffffffff);
+        st[p.l.part_start + p.batch] = (int)(total >> 32);
+        *d.free_count = free_n - (int)s_take;
+    }
+}
+
+// One value of a 64-entry array held two entries a lane (j, j + 32).
+template <typename T>
+__device__ __forceinline__ T shfl64(T lo, T hi, int j) {
+    const T a = __shfl_sync(0xffffffffu, lo, j & 31), b = __shfl_sync(0xffffffffu, hi, j & 31);
+    return j & 32 ? b : a;
+}
+
+// A tree's rows, by one warp: nodes lane and lane + 32.
+__device__ void tree_rows(const TokParams &p, int b, int lane) {
+    int32_t *st = p.step;
+    const int r0 = st[p.l.row_start + b], n = st[p.l.row_start + b + 1] - r0;
+    const int ctx = st[p.l.context + b], slot = st[p.l.slot + b], held = st[p.l.held + b];
+    const int first = st[p.l.take + b], free_n = st[kTokFree];
+    int64_t *mask = reinterpret_cast<int64_t *>(st + p.l.mask);
+    if (ctx < 0) {   // left out: its rows may be more than a tree's
+        for (int j = lane; j < n; j += 32) {
+            st[p.l.request + r0 + j] = b;
+            st[p.l.position + r0 + j] = 0;
+            st[p.l.slot_map + r0 + j] = -1;
+            mask[r0 + j] = 0;
+        }
+        return;
+    }
+    unsigned long long m[2];
+    int jump[2], depth[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int j = lane + 32 * h;
+        int par = -1;
+        if (j < n) {
+            par = p.parents[r0 + j];
+            if (par < -1 || par >= j) {
+                raise(p.d.error, PK_DEV_BAD_COUNT);
+                par = -1;
+            }
+        }
+        m[h] = 1ull << j;
+        jump[h] = par;
+        depth[h] = par >= 0;
+    }
+#pragma unroll 1
+    for (int round = 0; round < 6; ++round) {
+        unsigned long long nm[2];
+        int nj[2], nd[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int j = max(jump[h], 0);
+            const unsigned long long am = shfl64(m[0], m[1], j);
+            const int aj = shfl64(jump[0], jump[1], j), ad = shfl64(depth[0], depth[1], j);
+            const bool live = jump[h] >= 0;
+            nm[h] = live ? m[h] | am : m[h];
+            nd[h] = live ? depth[h] + ad : depth[h];
+            nj[h] = live ? aj : -1;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            m[h] = nm[h];
+            jump[h] = nj[h];
+            depth[h] = nd[h];
+        }
+        if (__all_sync(0xffffffffu, jump[0] < 0 && jump[1] < 0)) break;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int j = lane + 32 * h;
+        if (j < n) {
+            const int tok = ctx + j;
+            const int page = page_of(p, slot, held, first, free_n, tok >> p.ps_shift);
+            st[p.l.request + r0 + j] = b;
+            st[p.l.position + r0 + j] = ctx + depth[h];
+            st[p.l.slot_map + r0 + j] =
+                (page << p.ps_shift) | (tok & ((1 << p.ps_shift) - 1));
+            mask[r0 + j] = (int64_t)m[h];
+        }
+    }
+}
+
+// What the prefix sums place, by warps w of nw: the requests' new table entries,
+// unit records and tree rows a request at a time; chain rows and the rows behind
+// the last request a row at a time.
+__device__ void begin_fill(const TokParams &p, int w, int nw) {
+    int32_t *st = p.step;
+    const int lane = threadIdx.x & 31;
+    const int free_n = st[kTokFree], chunk = st[kTokChunk];
+    for (int b = w; b < p.batch; b += nw) {
+        const int ctx = st[p.l.context + b];
+        if (ctx >= 0) {
+            const int r0 = st[p.l.row_start + b], n = st[p.l.row_start + b + 1] - r0;
+            const int slot = st[p.l.slot + b], held = st[p.l.held + b], first = st[p.l.take + b];
+            const int need = ceil_shift((int64_t)ctx + n, p.ps_shift);
+            for (int i = held + lane; i < need; i += 32)
+                p.d.page_table[(int64_t)slot * p.d.table_width + i] =
+                    p.d.free_pages[free_n - 1 - (first + i - held)];
+            const int u0 = st[p.l.unit_start + b], nu = st[p.l.unit_start + b + 1] - u0;
+            const int part0 = st[p.l.part_start + b];
+            const int nr = n > 0 ? (int)(((int64_t)n * p.group + p.tile_rows - 1) / p.tile_rows) : 1;
+            for (int i = lane; i < nu; i += 32) {
+                const int rt = i % nr, split = i / nr;
+                // keys that the tile's last row sees: for a chain, up to itself
+                const int64_t last = ((int64_t)(rt + 1) * p.tile_rows + p.group - 1) / p.group;
+                const int seen = ctx + (p.parents ? n : (int)min(last, (int64_t)n));
+                const int kt = (seen + kTokTile - 1) / kTokTile;
+                if (u0 + i < p.max_units) {
+                    int4 *rec = reinterpret_cast<int4 *>(st + p.l.units +
+                                                         (int64_t)(u0 + i) * kTokUnitWords);
+                    rec[0] = make_int4(slot, r0, n, ctx);
+                    rec[1] = make_int4(rt, min(split * chunk, kt), min((split + 1) * chunk, kt),
+                                       nu > nr ? part0 + i : -1);
+                }
+            }
+        }
+        if (p.parents) tree_rows(p, b, lane);
+    }
+    const int used = st[kTokRows];
+    for (int r = (p.parents ? used : 0) + w * 32 + lane; r < p.rows; r += nw * 32) {
+        int req = -1, pos = 0, map = -1;
+        if (r < used) {
+            int lo = 0, hi = p.batch;   // the last request that starts at or before row r
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (st[p.l.row_start + mid] <= r) lo = mid;
+                else hi = mid;
+            }
+            req = lo;
+            const int ctx = st[p.l.context + lo];
+            if (ctx >= 0) {
+                pos = ctx + r - st[p.l.row_start + lo];
+                const int page = page_of(p, st[p.l.slot + lo], st[p.l.held + lo],
+                                         st[p.l.take + lo], free_n, pos >> p.ps_shift);
+                map = (page << p.ps_shift) | (pos & ((1 << p.ps_shift) - 1));
+            }
+        }
+        st[p.l.request + r] = req;
+        st[p.l.position + r] = pos;
+        st[p.l.slot_map + r] = map;
+        if (p.parents) reinterpret_cast<int64_t *>(st + p.l.mask)[r] = 0;
+    }
+}
+
+template <bool kFill>
+__global__ void __launch_bounds__(kPlanThreads) token_begin_kernel(const TokParams p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    begin_plan(p);
+    if (kFill) {
+        __syncthreads();
+        begin_fill(p, threadIdx.x >> 5, blockDim.x >> 5);
+    }
+}
+
+__global__ void __launch_bounds__(256) token_fill_kernel(const TokParams p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    begin_fill(p, (blockIdx.x * blockDim.x + threadIdx.x) >> 5, (gridDim.x * blockDim.x) >> 5);
+}
+
+__global__ void token_reset_kernel(pk_token_kv_desc d, const int32_t *order) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t tid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t n = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = tid; i < d.num_pages; i += n) d.free_pages[i] = order ? order[i] : (int)i;
+    for (int64_t i = tid; i < (int64_t)d.num_slots * d.table_width; i += n) d.page_table[i] = -1;
+    for (int64_t i = tid; i < d.num_slots; i += n) {
+        d.lengths[i] = 0;
+        d.held[i] = 0;
+    }
+    if (tid == 0) {
+        *d.free_count = d.num_pages;
+        *d.error = 0;
+    }
+}
+
+// ------------------------------------------------------------------ append
+// 16 bytes a thread: a row's K and V of one layer, head by head.
+__global__ void __launch_bounds__(256)
+    token_append_kernel(pk_token_kv_desc d, TokAppendArgs a, int64_t slot_map, int ps_shift,
+                        int esize) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int per_head = d.head_dim * esize / 16, per_row = per_head * d.num_kv_heads;
+    const int64_t n = (int64_t)a.rows * per_row;
+    const int layer = blockIdx.y;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+         i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / per_row;
+        const int c = (int)(i - r * per_row), h = c / per_head, e = c - h * per_head;
+        const int map = a.step[slot_map + r];
+        if (map < 0) continue;
+        const int64_t src = (layer * a.ls + r * a.rs + h * a.hs) * esize + e * 16;
+        const uint4 k = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.key) + src);
+        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.value) + src);
+        const int64_t page = map >> ps_shift, off = map & (d.page_size - 1);
+        const int64_t plane = ((page * d.num_layers + a.layer0 + layer) * 2) * d.num_kv_heads + h;
+        char *kv = static_cast<char *>(d.kv) + (plane * d.page_size + off) * d.head_dim * esize +
+                   e * 16;
+        *reinterpret_cast<uint4 *>(kv) = k;
+        *reinterpret_cast<uint4 *>(kv + (int64_t)d.num_kv_heads * d.page_size * d.head_dim *
+                                            esize) = v;
+    }
+}
+
+// --------------------------------------------------------------- acceptance
+// One CTA per (request, layer).  The path's nodes p_0 < p_1 < ... go to rows
+// len, len + 1, ...: p_i >= i, so in ascending order no row is overwritten before
+// it has been read, and kAhead rows are read before the first of them is written.
+constexpr int kAhead = 8;
+__global__ void __launch_bounds__(256)
+    token_end_kernel(pk_token_kv_desc d, TokLayout l, const int32_t *last, int trees,
+                     const int32_t *step, int ps_shift, int esize) {
+    __shared__ int s_src[PK_TOK_MAX_TREE], s_dst[PK_TOK_MAX_TREE], s_n;
+    grid_dep_wait();
+    grid_dep_launch();
+    const int b = blockIdx.x, layer = blockIdx.y;
+    const int ctx = step[l.context + b];
+    if (ctx < 0) return;
+    const int r0 = step[l.row_start + b], n = step[l.row_start + b + 1] - r0;
+    int keep = last[b];
+    if (keep < -1 || keep >= n) {
+        if (layer == 0 && threadIdx.x == 0) raise(d.error, PK_DEV_BAD_COUNT);
+        keep = -1;
+    }
+    unsigned long long path = 0;
+    if (trees && keep >= 0)
+        path = (unsigned long long)reinterpret_cast<const int64_t *>(step + l.mask)[r0 + keep];
+    const int kept = trees ? __popcll(path) : keep + 1;
+    if (layer == 0 && threadIdx.x == 0) d.lengths[step[l.slot + b]] = ctx + kept;
+    // a path of nodes 0, 1, ... is in place already (every chain)
+    if (!trees || path == (kept >= 64 ? ~0ull : (1ull << kept) - 1ull)) return;
+    const int in_place = __ffsll(~path) - 1;   // nodes 0 .. in_place - 1 stay
+    if (threadIdx.x < PK_TOK_MAX_TREE && (path >> threadIdx.x & 1) &&
+        (int)threadIdx.x >= in_place) {
+        const int rank = __popcll(path & ((1ull << threadIdx.x) - 1ull));
+        s_src[rank - in_place] = step[l.slot_map + r0 + threadIdx.x];
+        s_dst[rank - in_place] = step[l.slot_map + r0 + rank];
+    }
+    if (threadIdx.x == 0) s_n = kept - in_place;
+    __syncthreads();
+    const int moves = s_n;
+    const int per_head = d.head_dim * esize / 16;
+    const int64_t row_bytes = (int64_t)d.head_dim * esize;
+    for (int c = threadIdx.x; c < 2 * d.num_kv_heads * per_head; c += blockDim.x) {
+        const int plane = c / per_head, e = c - plane * per_head;   // (K|V, head)
+        auto at = [&](int map) {
+            const int64_t page = map >> ps_shift, off = map & (d.page_size - 1);
+            return static_cast<char *>(d.kv) +
+                   (((page * d.num_layers + layer) * 2 * d.num_kv_heads + plane) * d.page_size +
+                    off) * row_bytes + e * 16;
+        };
+        for (int i = 0; i < moves; i += kAhead) {
+            uint4 v[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (i + k < moves) v[k] = *reinterpret_cast<const uint4 *>(at(s_src[i + k]));
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (i + k < moves) *reinterpret_cast<uint4 *>(at(s_dst[i + k])) = v[k];
+        }
+    }
+}
+
+// -------------------------------------------------------------------- cutting
+// scratch: the slots' marks, then per request give's prefix, pages kept and given.
+struct TokCut {
+    pk_token_kv_desc d;
+    const int32_t *slots, *lengths;
+    int batch, ps_shift;
+};
+__device__ void cut_plan(const TokCut &p) {
+    __shared__ int64_t s_scan[33];
+    const pk_token_kv_desc &d = p.d;
+    int32_t *head = d.scratch + d.num_slots, *tmp = head + 16;
+    const int free_n = *d.free_count;
+    mark_slots(d, p.slots, p.batch);
+    const int nk = (p.batch + blockDim.x - 1) / blockDim.x;
+    const int b0 = threadIdx.x * nk, b1 = min(b0 + nk, p.batch);
+    int64_t sum = 0, total;
+    for (int b = b0; b < b1; ++b) {
+        const int slot = p.slots[b], len = p.lengths[b];
+        int keep = 0, give = 0;
+        if (!owns_slot(d, slot, b)) {
+            raise(d.error, PK_DEV_BAD_SLOT);
+        } else if (len < 0 || len > d.lengths[slot]) {
+            raise(d.error, PK_DEV_BAD_COUNT);
+        } else {
+            const int held = d.held[slot];
+            keep = min(ceil_shift(len, p.ps_shift), held);
+            give = held - keep;
+            d.held[slot] = keep;
+            d.lengths[slot] = len;
+        }
+        tmp[3 * b + 1] = keep;
+        tmp[3 * b + 2] = give;
+        sum += give;
+    }
+    int64_t first = block_exclusive_sum64(sum, total, s_scan);
+    for (int b = b0; b < b1; ++b) {
+        tmp[3 * b] = (int)first;
+        first += tmp[3 * b + 2];
+    }
+    if (threadIdx.x == 0) {
+        head[0] = free_n + (int)total;
+        *d.free_count = free_n + (int)total;
+    }
+}
+__device__ void cut_fill(const TokCut &p, int w, int nw) {
+    const pk_token_kv_desc &d = p.d;
+    const int32_t *head = d.scratch + d.num_slots, *tmp = head + 16;
+    const int top = head[0], lane = threadIdx.x & 31;
+    for (int b = w; b < p.batch; b += nw) {
+        const int first = tmp[3 * b], keep = tmp[3 * b + 1], give = tmp[3 * b + 2];
+        if (!give) continue;
+        int32_t *row = d.page_table + (int64_t)p.slots[b] * d.table_width + keep;
+        for (int i = lane; i < give; i += 32) {
+            d.free_pages[top - 1 - (first + i)] = row[i];
+            row[i] = -1;
+        }
+    }
+}
+template <bool kFill>
+__global__ void __launch_bounds__(kPlanThreads) token_cut_kernel(const TokCut p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    cut_plan(p);
+    if (kFill) {
+        __syncthreads();
+        cut_fill(p, threadIdx.x >> 5, blockDim.x >> 5);
+    }
+}
+__global__ void __launch_bounds__(256) token_cut_fill_kernel(const TokCut p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    cut_fill(p, (blockIdx.x * blockDim.x + threadIdx.x) >> 5, (gridDim.x * blockDim.x) >> 5);
+}
+
+int grid_for(int64_t threads, int block) {
+    const int64_t n = (threads + block - 1) / block, most = (int64_t)current_sms() * (2048 / block);
+    return (int)(n < 1 ? 1 : (n < most ? n : most));
+}
+
+}  // namespace
+
+int current_sms() {
+    static std::atomic<int> sms[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    int n = sms[dev & 63].load(std::memory_order_relaxed);
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+        sms[dev & 63].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+int launch_token_reset(const pk_token_kv *kv, const int32_t *init_order, cudaStream_t s) {
+    const pk_token_kv_desc &d = kv->d;
+    const int64_t n = (int64_t)d.num_slots * d.table_width;
+    return cuda_status(launch_pdl(token_reset_kernel,
+                                  dim3(grid_for(n > d.num_pages ? n : d.num_pages, 256)), dim3(256),
+                                  0, s, d, init_order),
+                       "token_reset_kernel");
+}
+
+int launch_token_begin(const pk_token_kv *kv, const int32_t *slots, const int32_t *counts,
+                       int batch, const int32_t *parents, int rows, int32_t *step,
+                       cudaStream_t s) {
+    TokParams p;
+    p.d = kv->d;
+    p.l = tok_layout(kv, batch, rows, parents != nullptr);
+    p.ps_shift = kv->ps_shift;
+    p.group = kv->group;
+    p.tile_rows = tok_tile_rows(kv, batch, rows);
+    p.batch = batch;
+    p.rows = rows;
+    p.target = kv->target;
+    p.max_units = tok_max_units(kv, batch, rows);
+    p.slots = slots;
+    p.counts = counts;
+    p.parents = parents;
+    p.step = step;
+    if (batch <= 64 && rows <= kOneCtaRows)
+        return cuda_status(launch_pdl(token_begin_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, p),
+                           "token_begin_kernel");
+    cudaError_t e = launch_pdl(token_begin_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, p);
+    if (e != cudaSuccess) return cuda_status(e, "token_begin_kernel");
+    const int64_t warps = parents ? (int64_t)batch : ((int64_t)rows + 31) / 32;
+    return cuda_status(launch_pdl(token_fill_kernel,
+                                  dim3(grid_for((warps > batch ? warps : batch) * 32, 256)),
+                                  dim3(256), 0, s, p),
+                       "token_fill_kernel");
+}
+
+int launch_token_append(const pk_token_kv *kv, const TokAppendArgs &a, cudaStream_t s) {
+    const pk_token_kv_desc &d = kv->d;
+    const TokLayout l = tok_layout(kv, a.batch, a.rows, a.trees);
+    const int64_t n = (int64_t)a.rows * d.num_kv_heads * d.head_dim * kv->esize / 16;
+    return cuda_status(launch_pdl(token_append_kernel, dim3(grid_for(n, 256), a.nlayers), dim3(256),
+                                  0, s, d, a, l.slot_map, kv->ps_shift, kv->esize),
+                       "token_append_kernel");
+}
+
+int launch_token_end(const pk_token_kv *kv, const int32_t *last, int batch, int rows, int trees,
+                     const int32_t *step, cudaStream_t s) {
+    const pk_token_kv_desc &d = kv->d;
+    return cuda_status(launch_pdl(token_end_kernel, dim3(batch, trees ? d.num_layers : 1), dim3(256),
+                                  0, s, d, tok_layout(kv, batch, rows, trees), last, trees, step,
+                                  kv->ps_shift, kv->esize),
+                       "token_end_kernel");
+}
+
+int launch_token_truncate(const pk_token_kv *kv, const int32_t *slots, const int32_t *lengths,
+                          int batch, cudaStream_t s) {
+    TokCut p;
+    p.d = kv->d;
+    p.slots = slots;
+    p.lengths = lengths;
+    p.batch = batch;
+    p.ps_shift = kv->ps_shift;
+    if (batch <= 64 && (int64_t)batch * kv->d.table_width <= 2 * kOneCtaRows)
+        return cuda_status(launch_pdl(token_cut_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, p),
+                           "token_cut_kernel");
+    cudaError_t e = launch_pdl(token_cut_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, p);
+    if (e != cudaSuccess) return cuda_status(e, "token_cut_kernel");
+    return cuda_status(launch_pdl(token_cut_fill_kernel, dim3(grid_for((int64_t)batch * 32, 256)),
+                                  dim3(256), 0, s, p),
+                       "token_cut_fill_kernel");
+}
+
+}  // namespace pk

@@ -1,0 +1,799 @@
+// Attention of a step's token rows over a token pool: each row sees its
+// request's context and, of the step's own tokens, its ancestors (or, in a
+// chain, the rows before it) and itself.
+//
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j - m),  m = max_j
+//
+// One pass over the keys in tiles of 64 with a running maximum and sum (fp32).
+// The rows of a K/V head are its group's query heads of every token, so a
+// request's pages are read once for up to 64 of them (a row tile).  The step
+// block lists units - a row tile over a range of key tiles - of about equal
+// length, some waves of them for the whole GPU however the lengths are spread;
+// a CTA walks its units and a second launch joins rows whose keys were split.
+//
+// bf16: a producer warp brings each tile's pages (TMA boxes of a page's rows x
+// 64 columns, 128B swizzle) into a ring of K and V slots that runs ahead across
+// units; four warps hold 16-row fragments of the row tile and compute
+// S = Q K^T and O += P V with mma.sync m16n8k16.  With fewer than 64 rows the
+// warps share the keys of a tile instead (4 / (rows / 16) ways) and join through
+// shared memory at the end.  P is rounded to bf16 for the product, relative
+// 2^-9 of each weight, below the rounding of the bf16 V that it multiplies; the
+// sum that normalises keeps fp32 weights.
+// Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
+// other waits return at once.
+#include <math.h>
+
+#include "pk_common.cuh"
+#include "pk_internal.h"
+
+namespace pk {
+namespace {
+
+constexpr int kTile = kTokTile;
+constexpr int kConsumers = 128, kThreads = kConsumers + 32;
+
+struct TreeParams {
+    const int32_t *step, *table;
+    TokLayout l;
+    int table_width, num_pages, num_layers, layer, kv_heads, group, ps_shift, trees;
+    int rows, heads, tile_rows;
+    const void *q, *kv;
+    void *out;
+    int64_t q_rs, q_hs, o_rs, o_hs;
+    float scale_log2;
+    float *ws_o, *ws_ml;   // partial outputs [part][kv head][row of tile][dim], (m, l) pairs
+    int32_t *error;
+};
+
+struct Unit {
+    int slot, row0, count, ctx, rt, t0, t1, part;
+};
+__device__ __forceinline__ Unit load_unit(const TreeParams &p, int i) {
+    const int4 *r =
+        reinterpret_cast<const int4 *>(p.step + p.l.units + (int64_t)i * kTokUnitWords);
+    const int4 a = r[0], b = r[1];
+    return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+__device__ __forceinline__ void consumer_sync() {
+    asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory");
+}
+// barrier that also ORs a flag over the consumer warps
+__device__ __forceinline__ bool consumer_any(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v), "n"(kConsumers)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_async_proxy() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Whether row `node` sees the step's token `rel` (>= 0) of its request.
+__device__ __forceinline__ bool sees(int trees, uint64_t mask, int node, int rel) {
+    return trees ? rel < PK_TOK_MAX_TREE && ((mask >> rel) & 1) : rel <= node;
+}
+
+// Bounded wait that gives up at once when another wait of the CTA already has.
+__device__ __forceinline__ void ring_wait(uint64_t *bar, uint32_t parity, volatile int *failed,
+                                          int32_t *error) {
+    if (mbar_try_wait(bar, parity)) return;
+    if (*failed) return;
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity)) {
+        if (*failed) return;
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            *failed = 1;
+            raise(error, PK_DEV_TIMEOUT);
+            return;
+        }
+    }
+}
+
+template <int DH, int BM>
+struct TreeShape {
+    static constexpr int kCols = DH / 64;                    // 128-byte column boxes of a row
+    static constexpr int kBox = kTile * 128;                 // one column box of a tile
+    static constexpr int kSlot = kCols * kBox;               // one tile of K or of V
+    static constexpr int kWm = BM / 16, kWk = 4 / kWm;       // warps over rows, over keys
+    // 96 KB of tiles, or 64 KB beside the join buffer: two CTAs an SM
+    static constexpr int kSlots = (kWk > 1 ? 4 : 6) * (128 / DH);
+    static constexpr int kKeys = kTile / kWk;                // keys of a tile per warp
+    static constexpr int kPad = DH + 4;                      // join buffer row, floats
+    static constexpr int kJoin = kWk > 1 ? 4 * 16 * kPad * 4 + 4 * 16 * 8 : 0;
+    static constexpr int kSmem = kSlots * kSlot + kJoin + 1024;
+};
+
+template <int DH, int BM>
+__global__ void __launch_bounds__(kThreads, 2)
+    tree_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const TreeParams p) {
+    using S = TreeShape<DH, BM>;
+    constexpr int NS = S::kSlots;
+    extern __shared__ uint8_t tree_smem[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
+    float *join = reinterpret_cast<float *>(ring + NS * S::kSlot);
+    __shared__ __align__(8) uint64_t full[NS], empty[NS];
+    __shared__ volatile int failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 4);
+        }
+        failed = 0;
+        fence_mbar_init();
+        prefetch_tmap(&kv_map);
+    }
+    __syncthreads();
+    grid_dep_wait();
+    grid_dep_launch();
+    const int units = p.step[kTokUnits] * p.kv_heads;
+
+    if (warp == 4) {
+        // producer: lanes issue a tile's boxes, K then V
+        const int ps = 1 << p.ps_shift, rows_box = min(ps, kTile);
+        const int box_of = lane / S::kCols, col = lane % S::kCols;
+        const uint32_t bytes = rows_box * 128;
+        int it = 0;   // ring use
+        bool stop = false;   // the warp's, so that its lanes stay together
+        for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
+            const Unit w = load_unit(p, u / p.kv_heads);
+            const int head = u % p.kv_heads;
+            const int32_t *table = p.table + (int64_t)w.slot * p.table_width;
+            const int len = w.ctx + w.count;
+            for (int t = w.t0; t < w.t1 && !stop; ++t) {
+                const int k0 = t * kTile, n = (min(kTile, len - k0) + rows_box - 1) / rows_box;
+                int page = 0;
+                if (box_of < n) {
+                    page = table[(k0 + box_of * rows_box) >> p.ps_shift];
+                    if (page < 0 || page >= p.num_pages) {
+                        raise(p.error, PK_DEV_BAD_PAGE);
+                        page = 0;
+                    }
+                }
+                const int in_page = (k0 + box_of * rows_box) & (ps - 1);
+#pragma unroll
+                for (int v = 0; v < 2; ++v, ++it) {
+                    const int s = it % NS, use = it / NS;
+                    if (use) ring_wait(&empty[s], (use - 1) & 1, &failed, p.error);
+                    stop = __any_sync(0xffffffffu, failed != 0);
+                    if (stop) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * S::kCols * bytes);
+                    __syncwarp();
+                    if (box_of < n)
+                        tma_load_3d(ring + s * S::kSlot + col * S::kBox + box_of * bytes, &kv_map,
+                                    &full[s], col * 64, in_page,
+                                    ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + head);
+                }
+            }
+        }
+        if (stop) {   // leave no copy in flight
+            for (int s = 0; s < NS; ++s)
+                if (it > s) {
+                    const int lastu = (it - 1 - s) / NS;
+                    mbar_wait_bounded(&full[s], lastu & 1, kWaitLimitNs);
+                }
+        }
+        return;
+    }
+
+    const int wm = warp % S::kWm, wk = warp / S::kWm;
+    const int key0 = wk * S::kKeys;
+    const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
+    int it = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const Unit w = load_unit(p, u / p.kv_heads);
+        const int head = u % p.kv_heads;
+        const int m_rows = w.count * p.group;
+        // this thread's two rows of the tile (fragment rows lane / 4 and + 8)
+        uint32_t qf[DH / 16][4];
+        uint64_t mask[2];
+        int node[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = w.rt * BM + wm * 16 + (lane >> 2) + h * 8;
+            node[h] = -1;
+            mask[h] = 0;
+            const __nv_bfloat16 *src = nullptr;
+            if (r < m_rows) {
+                node[h] = r / p.group;
+                const int64_t row = w.row0 + node[h];
+                if (p.trees)
+                    mask[h] = reinterpret_cast<const uint64_t *>(p.step + p.l.mask)[row];
+                src = q + row * p.q_rs + (int64_t)(head * p.group + r - node[h] * p.group) * p.q_hs +
+                      (lane & 3) * 2;
+            }
+#pragma unroll
+            for (int ks = 0; ks < DH / 16; ++ks) {
+                qf[ks][h] = src ? *reinterpret_cast<const uint32_t *>(src + ks * 16) : 0u;
+                qf[ks][h + 2] = src ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8) : 0u;
+            }
+        }
+        float o[DH / 8][4];
+#pragma unroll
+        for (int i = 0; i < DH / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        const int len = w.ctx + w.count;
+
+        for (int t = w.t0; t < w.t1; ++t, it += 2) {
+            const int sk = it % NS, sv = (it + 1) % NS;
+            const int k0 = t * kTile;
+            const uint32_t kb = smem_u32(ring + sk * S::kSlot), vb = smem_u32(ring + sv * S::kSlot);
+            float s[S::kKeys / 8][4];
+#pragma unroll
+            for (int i = 0; i < S::kKeys / 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+            ring_wait(&full[sk], (it / NS) & 1, &failed, p.error);
+            __syncwarp();
+#pragma unroll
+            for (int ks = 0; ks < DH / 16; ++ks) {
+#pragma unroll
+                for (int nb = 0; nb < S::kKeys / 16; ++nb) {
+                    uint32_t b[4];
+                    const uint32_t row = key0 + nb * 16 + ((lane >> 4) << 3) + (lane & 7);
+                    ldsm4(kb + (ks / 4) * S::kBox +
+                              sw128(row, (ks % 4) * 32 + ((lane >> 3) & 1) * 16), b);
+                    mma16816(s[2 * nb], qf[ks], b[0], b[1]);
+                    mma16816(s[2 * nb + 1], qf[ks], b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) arrive(&empty[sk]);
+            const bool own = k0 + kTile > w.ctx;   // some of the step's own tokens, or the end
+            if (own) {
+#pragma unroll
+                for (int i = 0; i < S::kKeys / 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = k0 + key0 + i * 8 + (lane & 3) * 2 + (e & 1), h = e >> 1;
+                        const int rel = key - w.ctx;
+                        if (key >= len || (rel >= 0 && !sees(p.trees, mask[h], node[h], rel)))
+                            s[i][e] = -INFINITY;
+                    }
+            }
+            float keep[2], base[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = m[h];
+#pragma unroll
+                for (int i = 0; i < S::kKeys / 8; ++i)
+                    top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // nothing seen yet: weights and factor are exp2(-inf) = 0
+                base[h] = top == -INFINITY ? 0.f : __fmul_rn(top, p.scale_log2);
+                // both products rounded alike: an unchanged maximum keeps a factor of 1
+                keep[h] = ex2(__fmul_rn(m[h], p.scale_log2) - base[h]);
+                m[h] = top;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < S::kKeys / 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float w2 = ex2(s[i][2 * h + e] * p.scale_log2 - base[h]);
+                        s[i][2 * h + e] = w2;
+                        sum += w2;
+                    }
+                l[h] = l[h] * keep[h] + sum;
+            }
+#pragma unroll
+            for (int i = 0; i < DH / 8; ++i) {
+                o[i][0] *= keep[0];
+                o[i][1] *= keep[0];
+                o[i][2] *= keep[1];
+                o[i][3] *= keep[1];
+            }
+            ring_wait(&full[sv], ((it + 1) / NS) & 1, &failed, p.error);
+            __syncwarp();
+            bool odd = false;   // a value that is not finite among the step's own rows
+            if (own) {
+                // rows past the end hold what the page held before: zero for the
+                // product; a non-finite value of a token that some rows do not see
+                // must not reach them as 0 x inf
+                uint8_t *vs = ring + sv * S::kSlot;
+                bool bad = false;
+                for (int c = threadIdx.x; c < kTile * DH / 8; c += kConsumers) {
+                    const int row = c / (DH / 8), ch = c % (DH / 8);
+                    uint4 *at = reinterpret_cast<uint4 *>(
+                        vs + (ch / 8) * S::kBox + sw128(row, (ch % 8) * 16));
+                    const int key = k0 + row;
+                    if (key >= len) {
+                        *at = make_uint4(0u, 0u, 0u, 0u);
+                    } else if (key >= w.ctx) {
+                        const uint4 x = *at;
+                        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            bad |= (e[i] & 0x7f80u) == 0x7f80u || (e[i] & 0x7f800000u) == 0x7f800000u;
+                    }
+                }
+                odd = consumer_any(bad);
+                fence_async_proxy();   // the slot's next TMA load comes after these writes
+            }
+            if (!odd) {
+#pragma unroll
+                for (int kk = 0; kk < S::kKeys / 16; ++kk) {
+                    const uint32_t a[4] = {
+                        pack2(s[2 * kk][0], s[2 * kk][1]), pack2(s[2 * kk][2], s[2 * kk][3]),
+                        pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]),
+                        pack2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+                    for (int nb = 0; nb < DH / 16; ++nb) {
+                        uint32_t b[4];
+                        const uint32_t row = key0 + kk * 16 + (lane & 15);
+                        ldsm4_t(vb + (nb / 4) * S::kBox +
+                                    sw128(row, (nb % 4) * 32 + (lane >> 4) * 16), b);
+                        mma16816(o[2 * nb], a, b[0], b[1]);
+                        mma16816(o[2 * nb + 1], a, b[2], b[3]);
+                    }
+                }
+            } else {
+                // the same product a key at a time, keys of weight zero left out
+                const uint8_t *vs = ring + sv * S::kSlot;
+#pragma unroll
+                for (int i = 0; i < S::kKeys / 8; ++i) {
+#pragma unroll 1
+                    for (int x = 0; x < 8; ++x) {
+                        const int from = (lane & ~3) | (x >> 1);
+                        const float w0a = __shfl_sync(0xffffffffu, s[i][0], from);
+                        const float w0b = __shfl_sync(0xffffffffu, s[i][1], from);
+                        const float w1a = __shfl_sync(0xffffffffu, s[i][2], from);
+                        const float w1b = __shfl_sync(0xffffffffu, s[i][3], from);
+                        const float w0 = x & 1 ? w0b : w0a, w1 = x & 1 ? w1b : w1a;
+                        const int row = key0 + i * 8 + x;
+#pragma unroll
+                        for (int n = 0; n < DH / 8; ++n) {
+                            const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(
+                                vs + (n / 8) * S::kBox + sw128(row, (n % 8) * 16 + (lane & 3) * 4));
+                            const float2 f = __bfloat1622float2(v);
+                            if (w0 != 0.f) {
+                                o[n][0] += w0 * f.x;
+                                o[n][1] += w0 * f.y;
+                            }
+                            if (w1 != 0.f) {
+                                o[n][2] += w1 * f.x;
+                                o[n][3] += w1 * f.y;
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) arrive(&empty[sv]);
+        }
+        // row sums over the quad's lanes
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        }
+        const int64_t part = ((int64_t)w.part * p.kv_heads + head) * BM;
+        if (S::kWk == 1) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int rt = wm * 16 + (lane >> 2) + h * 8, r = w.rt * BM + rt;
+                if (r >= m_rows) continue;
+                if (w.part >= 0) {
+                    float *dst = p.ws_o + (part + rt) * DH + (lane & 3) * 2;
+#pragma unroll
+                    for (int n = 0; n < DH / 8; ++n)
+                        *reinterpret_cast<float2 *>(dst + n * 8) =
+                            make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                    if ((lane & 3) == 0)
+                        *reinterpret_cast<float2 *>(p.ws_ml + (part + rt) * 2) =
+                            make_float2(__fmul_rn(m[h], p.scale_log2), l[h]);
+                } else {
+                    const float inv = 1.f / l[h];
+                    __nv_bfloat16 *dst = out + (int64_t)(w.row0 + node[h]) * p.o_rs +
+                                         (int64_t)(head * p.group + r - node[h] * p.group) * p.o_hs +
+                                         (lane & 3) * 2;
+#pragma unroll
+                    for (int n = 0; n < DH / 8; ++n)
+                        *reinterpret_cast<uint32_t *>(dst + n * 8) =
+                            pack2(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+                }
+            }
+        } else {
+            // join the warps' shares of the keys: each writes its 16 rows, then every
+            // thread sums 8 columns of a row over the shares
+            float *ml = join + 4 * 16 * S::kPad;
+            const int base = warp * 16;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float *dst = join + (base + (lane >> 2) + h * 8) * S::kPad + (lane & 3) * 2;
+#pragma unroll
+                for (int n = 0; n < DH / 8; ++n)
+                    *reinterpret_cast<float2 *>(dst + n * 8) =
+                        make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                if ((lane & 3) == 0) {
+                    ml[2 * (base + (lane >> 2) + h * 8)] = __fmul_rn(m[h], p.scale_log2);
+                    ml[2 * (base + (lane >> 2) + h * 8) + 1] = l[h];
+                }
+            }
+            consumer_sync();
+            for (int c = threadIdx.x; c < BM * DH / 8; c += kConsumers) {
+                const int rt = c / (DH / 8), ch = c % (DH / 8), r = w.rt * BM + rt;
+                if (r >= m_rows) continue;
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < S::kWk; ++k)   // share k of row rt: warp k * kWm + rt / 16
+                    top = fmaxf(top, ml[2 * (k * BM + rt)]);
+                const float ref = top == -INFINITY ? 0.f : top;
+                float acc[8] = {}, sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < S::kWk; ++k) {
+                    const float f = ex2(ml[2 * (k * BM + rt)] - ref);
+                    sum += f * ml[2 * (k * BM + rt) + 1];
+                    const float4 *src = reinterpret_cast<const float4 *>(
+                        join + (k * BM + rt) * S::kPad + ch * 8);
+                    const float4 a = src[0], b = src[1];
+                    acc[0] += f * a.x;
+                    acc[1] += f * a.y;
+                    acc[2] += f * a.z;
+                    acc[3] += f * a.w;
+                    acc[4] += f * b.x;
+                    acc[5] += f * b.y;
+                    acc[6] += f * b.z;
+                    acc[7] += f * b.w;
+                }
+                if (w.part >= 0) {
+                    float4 *dst = reinterpret_cast<float4 *>(p.ws_o + (part + rt) * DH + ch * 8);
+                    dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                    dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                    if (ch == 0)
+                        *reinterpret_cast<float2 *>(p.ws_ml + (part + rt) * 2) =
+                            make_float2(top, sum);
+                } else {
+                    const float inv = 1.f / sum;
+                    const int nd = r / p.group;
+                    __nv_bfloat16 *dst = out + (int64_t)(w.row0 + nd) * p.o_rs +
+                                         (int64_t)(head * p.group + r - nd * p.group) * p.o_hs +
+                                         ch * 8;
+                    *reinterpret_cast<uint4 *>(dst) =
+                        make_uint4(pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv),
+                                   pack2(acc[4] * inv, acc[5] * inv), pack2(acc[6] * inv, acc[7] * inv));
+                }
+            }
+            consumer_sync();   // the buffer is free again
+        }
+    }
+}
+
+// ------------------------------------------------------------------ float32
+// The parity mode: the same units, fp32 FMAs.  A CTA of four warps holds a
+// 16-row tile; K rows are padded so that a lane per key reads without bank
+// conflicts; a warp computes the scores of its four rows (two keys a lane), then
+// their outputs (DH / 32 columns a lane).
+constexpr int kRowsF32 = 16;
+template <int DH>
+__global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) {
+    constexpr int kKp = DH + 4, NV = DH / 32;
+    extern __shared__ uint8_t tree_smem[];
+    float *sk = reinterpret_cast<float *>(tree_smem);   // [kTile][kKp]
+    float *sv = sk + kTile * kKp;                       // [kTile][DH]
+    float *sq = sv + kTile * DH;                        // [kRowsF32][DH]
+    float *sp = sq + kRowsF32 * DH;                     // [kRowsF32][kTile]
+    grid_dep_wait();
+    grid_dep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int units = p.step[kTokUnits] * p.kv_heads;
+    const float *q = static_cast<const float *>(p.q), *kv = static_cast<const float *>(p.kv);
+    float *out = static_cast<float *>(p.out);
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        const Unit w = load_unit(p, u / p.kv_heads);
+        const int head = u % p.kv_heads, m_rows = w.count * p.group, len = w.ctx + w.count;
+        __syncthreads();
+        for (int c = threadIdx.x; c < kRowsF32 * DH / 4; c += 128) {
+            const int rt = c / (DH / 4), e = c % (DH / 4), r = w.rt * kRowsF32 + rt;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < m_rows) {
+                const int nd = r / p.group;
+                x = *reinterpret_cast<const float4 *>(
+                    q + (int64_t)(w.row0 + nd) * p.q_rs +
+                    (int64_t)(head * p.group + r - nd * p.group) * p.q_hs + e * 4);
+            }
+            reinterpret_cast<float4 *>(sq)[c] = x;
+        }
+        float o[4][NV] = {}, m[4], l[4];
+        uint64_t mask[4];
+        int node[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = w.rt * kRowsF32 + warp * 4 + i;
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+            node[i] = r < m_rows ? r / p.group : -1;
+            mask[i] = p.trees && r < m_rows
+                          ? reinterpret_cast<const uint64_t *>(p.step + p.l.mask)[w.row0 + node[i]]
+                          : 0;
+        }
+        for (int t = w.t0; t < w.t1; ++t) {
+            const int k0 = t * kTile;
+            __syncthreads();   // the previous tile is done with
+            for (int c = threadIdx.x; c < kTile * DH / 4; c += 128) {
+                const int row = c / (DH / 4), e = c % (DH / 4), key = k0 + row;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+                if (key < len) {
+                    int page = p.table[(int64_t)w.slot * p.table_width + (key >> p.ps_shift)];
+                    if (page < 0 || page >= p.num_pages) {
+                        raise(p.error, PK_DEV_BAD_PAGE);
+                        page = 0;
+                    }
+                    const int64_t ps = 1 << p.ps_shift, off = key & (ps - 1);
+                    const int64_t plane =
+                        (((int64_t)page * p.num_layers + p.layer) * 2) * p.kv_heads + head;
+                    const float *src = kv + (plane * ps + off) * DH + e * 4;
+                    a = *reinterpret_cast<const float4 *>(src);
+                    b = *reinterpret_cast<const float4 *>(src + p.kv_heads * ps * DH);
+                }
+                *reinterpret_cast<float4 *>(sk + row * kKp + e * 4) = a;
+                reinterpret_cast<float4 *>(sv)[c] = b;
+            }
+            __syncthreads();
+            float s[4][2] = {};
+#pragma unroll 4
+            for (int e = 0; e < DH / 4; ++e) {
+                const float4 a = *reinterpret_cast<const float4 *>(sk + lane * kKp + e * 4);
+                const float4 b = *reinterpret_cast<const float4 *>(sk + (lane + 32) * kKp + e * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 x =
+                        *reinterpret_cast<const float4 *>(sq + (warp * 4 + i) * DH + e * 4);
+                    s[i][0] += x.x * a.x + x.y * a.y + x.z * a.z + x.w * a.w;
+                    s[i][1] += x.x * b.x + x.y * b.y + x.z * b.z + x.w * b.w;
+                }
+            }
+            const bool own = k0 + kTile > w.ctx;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float top = m[i];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = k0 + lane + 32 * h, rel = key - w.ctx;
+                    if (own && (key >= len ||
+                                (rel >= 0 && !sees(p.trees, mask[i], node[i], rel))))
+                        s[i][h] = -INFINITY;
+                    top = fmaxf(top, s[i][h]);
+                }
+#pragma unroll
+                for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                // exp2 of the scaled difference, so that large scores lose nothing
+                const float ref = top == -INFINITY ? 0.f : top;
+                const float keep = exp2f((m[i] - ref) * p.scale_log2);
+                const float a = exp2f((s[i][0] - ref) * p.scale_log2);
+                const float b = exp2f((s[i][1] - ref) * p.scale_log2);
+                m[i] = top;
+                l[i] = l[i] * keep + a + b;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) o[i][n] *= keep;
+                sp[(warp * 4 + i) * kTile + lane] = a;
+                sp[(warp * 4 + i) * kTile + lane + 32] = b;
+            }
+            __syncwarp();
+            const int end = min(kTile, len - k0);
+#pragma unroll 1
+            for (int j = 0; j < end; ++j) {
+                float v[NV];
+#pragma unroll
+                for (int n = 0; n < NV; ++n) v[n] = sv[j * DH + n * 32 + lane];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = sp[(warp * 4 + i) * kTile + j];
+                    if (x != 0.f) {   // a key that the row does not see has no part, even inf
+#pragma unroll
+                        for (int n = 0; n < NV; ++n) o[i][n] += x * v[n];
+                    }
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int rt = warp * 4 + i, r = w.rt * kRowsF32 + rt;
+            float sum = l[i];
+#pragma unroll
+            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if (r >= m_rows) continue;
+            if (w.part >= 0) {
+                const int64_t part = ((int64_t)w.part * p.kv_heads + head) * kRowsF32 + rt;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) p.ws_o[part * DH + n * 32 + lane] = o[i][n];
+                if (lane == 0) {
+                    p.ws_ml[part * 2] = m[i] * p.scale_log2;
+                    p.ws_ml[part * 2 + 1] = sum;
+                }
+            } else {
+                const float inv = 1.f / sum;
+                float *dst = out + (int64_t)(w.row0 + node[i]) * p.o_rs +
+                             (int64_t)(head * p.group + r - node[i] * p.group) * p.o_hs;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) dst[n * 32 + lane] = o[i][n] * inv;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ the join
+// A warp per (row, head): the row's ranges weighted by exp2(m - max m), in order
+// of the ranges, so that the result does not depend on which finished first.
+template <int DH, typename T>
+__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
+    constexpr int NV = DH / 32;
+    grid_dep_wait();
+    grid_dep_launch();
+    const int lane = threadIdx.x & 31;
+    const int64_t n = (int64_t)p.rows * p.heads;
+    const int chunk = p.step[kTokChunk], bm = p.tile_rows;
+    for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < n;
+         i += ((int64_t)gridDim.x * blockDim.x) >> 5) {
+        const int row = (int)(i / p.heads), qh = (int)(i - (int64_t)row * p.heads);
+        const int b = p.step[p.l.request + row];
+        if (b < 0) continue;
+        const int ctx = p.step[p.l.context + b];
+        if (ctx < 0) continue;
+        const int r0 = p.step[p.l.row_start + b], cnt = p.step[p.l.row_start + b + 1] - r0;
+        const int ns = ((ctx + cnt + kTile - 1) / kTile + chunk - 1) / chunk;
+        if (ns <= 1) continue;
+        const int head = qh / p.group, r = (row - r0) * p.group + qh - head * p.group;
+        const int nr = (cnt * p.group + bm - 1) / bm, rt = r / bm;
+        const int64_t base = p.step[p.l.part_start + b] + rt;
+        auto at = [&](int s) {
+            return ((base + (int64_t)s * nr) * p.kv_heads + head) * bm + (r - rt * bm);
+        };
+        float top = -INFINITY;
+        for (int s = lane; s < ns; s += 32) top = fmaxf(top, p.ws_ml[at(s) * 2]);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        if (top == -INFINITY) top = 0.f;
+        float acc[NV] = {}, sum = 0.f;
+        for (int s = 0; s < ns; ++s) {
+            const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + at(s) * 2);
+            const float f = exp2f(ml.x - top);
+            sum += f * ml.y;
+            const float *src = p.ws_o + at(s) * DH + lane * NV;
+#pragma unroll
+            for (int e = 0; e < NV; ++e) acc[e] += f * src[e];
+        }
+        const float inv = 1.f / sum;
+        T *dst = static_cast<T *>(p.out) + (int64_t)row * p.o_rs + (int64_t)qh * p.o_hs + lane * NV;
+#pragma unroll
+        for (int e = 0; e < NV; ++e) dst[e] = Elem<T>::from_f(acc[e] * inv);
+    }
+}
+
+template <int DH, int BM>
+cudaError_t launch_bf16(const pk_token_kv *kv, const TreeParams &p, int64_t most, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int smem = TreeShape<DH, BM>::kSmem;
+    cudaError_t e = allow_smem(tree_attn_kernel<DH, BM>, smem, done);
+    if (e != cudaSuccess) return e;
+    // two CTAs an SM, which their shared memory allows
+    const int64_t ctas = 2 * current_sms();
+    return launch_pdl(tree_attn_kernel<DH, BM>, dim3((unsigned)(most < ctas ? most : ctas)),
+                      dim3(kThreads), smem, s, kv->kv_map, p);
+}
+template <int DH>
+cudaError_t launch_bm(const pk_token_kv *kv, const TreeParams &p, int64_t most, cudaStream_t s) {
+    switch (p.tile_rows) {
+        case 16: return launch_bf16<DH, 16>(kv, p, most, s);
+        case 32: return launch_bf16<DH, 32>(kv, p, most, s);
+        default: return launch_bf16<DH, 64>(kv, p, most, s);
+    }
+}
+template <int DH>
+cudaError_t launch_f32(const TreeParams &p, int64_t most, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr int smem = (kTile * (DH + 4) + kTile * DH + kRowsF32 * DH + kRowsF32 * kTile) * 4;
+    cudaError_t e = allow_smem(tree_attn_f32_kernel<DH>, smem, done);
+    if (e != cudaSuccess) return e;
+    const int64_t ctas = 2 * current_sms();
+    return launch_pdl(tree_attn_f32_kernel<DH>, dim3((unsigned)(most < ctas ? most : ctas)),
+                      dim3(128), smem, s, p);
+}
+template <int DH>
+cudaError_t launch_join(const TreeParams &p, int dtype, cudaStream_t s) {
+    const int64_t ctas = ((int64_t)p.rows * p.heads + 7) / 8, lim = 8 * current_sms();
+    const dim3 grid((unsigned)(ctas < lim ? ctas : lim));
+    return dtype == PK_DTYPE_BF16
+               ? launch_pdl(tree_join_kernel<DH, __nv_bfloat16>, grid, dim3(256), 0, s, p)
+               : launch_pdl(tree_join_kernel<DH, float>, grid, dim3(256), 0, s, p);
+}
+
+// No request of this pool can be long enough to be split.
+bool never_split(const pk_token_kv *kv) {
+    return (int64_t)kv->d.table_width << kv->ps_shift <= (int64_t)kTokMinChunk * kTile;
+}
+
+}  // namespace
+
+int64_t tree_attn_workspace(const pk_token_kv *kv, int batch, int rows) {
+    if (never_split(kv)) return 0;
+    return tok_max_parts(kv) * kv->d.num_kv_heads * tok_tile_rows(kv, batch, rows) *
+           (kv->d.head_dim + 2) * 4;
+}
+
+int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStream_t s) {
+    const pk_token_kv_desc &d = kv->d;
+    TreeParams p;
+    p.step = a.step;
+    p.table = d.page_table;
+    p.l = tok_layout(kv, a.batch, a.rows, a.trees);
+    p.table_width = d.table_width;
+    p.num_pages = d.num_pages;
+    p.num_layers = d.num_layers;
+    p.layer = a.layer;
+    p.kv_heads = d.num_kv_heads;
+    p.group = kv->group;
+    p.ps_shift = kv->ps_shift;
+    p.trees = a.trees;
+    p.rows = a.rows;
+    p.heads = d.num_heads;
+    p.tile_rows = tok_tile_rows(kv, a.batch, a.rows);
+    p.q = a.q;
+    p.kv = d.kv;
+    p.out = a.out;
+    p.q_rs = a.q_rs;
+    p.q_hs = a.q_hs;
+    p.o_rs = a.o_rs;
+    p.o_hs = a.o_hs;
+    p.scale_log2 = a.scale * 1.44269504088896340736f;
+    p.ws_o = a.ws;
+    p.ws_ml = a.ws ? a.ws + tok_max_parts(kv) * d.num_kv_heads * p.tile_rows * d.head_dim : nullptr;
+    p.error = d.error;
+    const int64_t most = tok_max_units(kv, a.batch, a.rows) * d.num_kv_heads;
+    cudaError_t e;
+    if (d.dtype == PK_DTYPE_BF16)
+        e = d.head_dim == 64 ? launch_bm<64>(kv, p, most, s) : launch_bm<128>(kv, p, most, s);
+    else
+        e = d.head_dim == 64 ? launch_f32<64>(p, most, s) : launch_f32<128>(p, most, s);
+    if (e != cudaSuccess) return cuda_status(e, "tree attention kernel");
+    if (never_split(kv)) return PK_OK;
+    e = d.head_dim == 64 ? launch_join<64>(p, d.dtype, s) : launch_join<128>(p, d.dtype, s);
+    return cuda_status(e, "tree_join_kernel");
+}
+
+}  // namespace pk

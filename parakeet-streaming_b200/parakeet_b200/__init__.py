@@ -6,4 +6,6 @@ Host side mirrors the reference's module and scheduler interfaces
 """
 from .ops import PagedKVPool, pages_per_stream, ring_size
 
-__all__ = ["PagedKVPool", "pages_per_stream", "ring_size"]
+from .tokens import TokenKVPool, TokenStep
+
+__all__ = ["PagedKVPool", "TokenKVPool", "TokenStep", "pages_per_stream", "ring_size"]

@@ -21,6 +21,9 @@ PK_DEV_BAD_COUNT = 16
 PK_GEMM_STORE, PK_GEMM_SILU, PK_GEMM_RESIDUAL, PK_GEMM_RESIDUAL_RELU, PK_GEMM_BIAS = 0, 1, 2, 3, 4
 PK_FE_HIST, PK_FE_META_STRIDE, PK_FE_FIRST, PK_FE_FINAL = 512, 4, 1, 2
 PK_NOALLOC_SCRATCH_BYTES = 32 * 1024 * 1024   # pk_paged_attention_noalloc's static scratch
+PK_TOK_ROW_START, PK_TOK_CONTEXT, PK_TOK_REQUEST, PK_TOK_POSITION = 0, 1, 7, 8
+PK_TOK_SLOT_MAP, PK_TOK_MASK, PK_TOK_OFFSETS = 9, 11, 12
+PK_TOK_MAX_TREE, PK_TOK_MAX_BATCH = 64, 65536   # nodes of a tree, requests of a step
 META_FIRST, META_NEXT, META_WRITTEN, META_PROCESSED, META_CACHE_LEN = 0, 1, 2, 3, 4
 META_STRIDE = 8
 WIN_STRIDE = 128
@@ -49,6 +52,28 @@ class PagedKVDesc(ctypes.Structure):
         ("chunk", ctypes.c_int32),
         ("page_size", ctypes.c_int32),
         ("ring", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class TokenKVDesc(ctypes.Structure):
+    _fields_ = [
+        ("kv", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("held", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+        ("error", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32),
+        ("num_layers", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
     ]
 
@@ -115,10 +140,22 @@ SIGNATURES = {
                            ctypes.POINTER(_I64), ctypes.POINTER(_I32)],
     "pk_features_push": [ctypes.POINTER(FeaturesDesc), _P, _I64, _P, _P, _P, _I32, _P, _I32, _I32,
                          _P, _P],
+    "pk_token_kv_create": [ctypes.POINTER(TokenKVDesc), ctypes.POINTER(ctypes.c_void_p)],
+    "pk_token_kv_destroy": [_P],
+    "pk_token_reset": [_P, _P, _P],
+    "pk_token_step_words": [_P, _I32, _I32, _I32, _P],
+    "pk_token_begin_step": [_P, _P, _P, _I32, _P, _I32, _P, _P],
+    "pk_token_append": [_P, _I32, _I32, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P],
+    "pk_token_attention_workspace": [_P, _I32, _I32],
+    "pk_token_attention": [_P, _I32, _P, _I64, _I64, ctypes.c_float, _I32, _I32, _I32, _P, _P, _I64,
+                           _I64, _P, _P],
+    "pk_token_end_step": [_P, _P, _I32, _I32, _I32, _P, _P],
+    "pk_token_truncate": [_P, _P, _P, _I32, _P],
     "pk_selftest_bounded_wait": [_P, _I32, _I64, _P, _P],
     "pk_last_error": [],
 }
-RESTYPES = {"pk_last_error": ctypes.c_char_p}
+RESTYPES = {"pk_last_error": ctypes.c_char_p, "pk_token_step_words": _I64,
+            "pk_token_attention_workspace": _I64}
 
 _lib = None
 
