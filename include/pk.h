@@ -586,6 +586,34 @@ int pk_token_end_step(pk_token_kv *kv, const int32_t *last, int32_t batch, int32
 int pk_token_truncate(pk_token_kv *kv, const int32_t *slots, const int32_t *lengths,
                       int32_t batch, void *stream);
 
+/* ---------------- adapters of many requests beside a shared projection ------
+ * pk_gemm_bf16 whose rows may each have a low-rank adapter of their own:
+ *   C[m] = epi(A[m] W^T + scale[a] (A[m] down[a]^T) up[a]^T),  a = ids[m]
+ * (ids[m] = -1: none; scale NULL: 1).  down [num_adapters][rank][K] and up
+ * [num_adapters][N][rank], contiguous; rank a multiple of 8 up to
+ * PK_ADAPTER_MAX_RANK (adapters of lower rank are padded with zeros).  One
+ * adapter's weights never meet another one's rows.  The reference has none.
+ *
+ * The plan of a step's ids (rows sorted by adapter) serves every projection
+ * with the same rows; plan is pk_adapter_plan_words() int32, 16-byte aligned.
+ * An id out of range counts as -1 and sets PK_DEV_BAD_SLOT. */
+#define PK_ADAPTER_MAX 8192       /* most adapters of one call                 */
+#define PK_ADAPTER_MAX_RANK 128
+#define PK_ADAPTER_MAX_ROWS 1048576
+int64_t pk_adapter_plan_words(int32_t rows, int32_t num_adapters);
+int pk_adapter_plan(const int32_t *ids, int32_t rows, int32_t num_adapters, int32_t *plan,
+                    int32_t *error, void *stream);
+
+/* Arguments as pk_gemm_bf16's; ids and plan as given to and made by
+ * pk_adapter_plan (rows = M); workspace: pk_adapter_workspace() bytes, 16-byte
+ * aligned, for this call alone. */
+int64_t pk_adapter_workspace(int32_t rows, int32_t rank);
+int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int32_t M, int32_t N,
+                    int32_t K, void *C, int64_t ldc, int32_t epilogue, const void *R, int64_t ldr,
+                    const void *bias, float alpha, const void *down, const void *up, int32_t rank,
+                    int32_t num_adapters, const float *scale, const int32_t *ids,
+                    const int32_t *plan, void *workspace, int32_t *error, void *stream);
+
 /* Self-test of the failure path of every TMA pipeline here: the bounded
  * mbarrier wait that gives up after a time limit and records PK_DEV_TIMEOUT in
  * *error (instead of hanging the GPU), leaving the context usable.  One CTA

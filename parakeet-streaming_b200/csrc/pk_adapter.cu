@@ -1,0 +1,622 @@
+// A projection shared by many requests, with each request's low-rank adapter:
+//
+//   acc[m] = x[m] W^T + S[m] up[a]^T,   S[m] = scale[a] * x[m] down[a]^T,  a = ids[m]
+//   C[m]   = epilogue(acc[m])           (rows with ids[m] = -1: x[m] W^T alone)
+//
+// Three launches:
+//  1. the plan (once per step: every projection of a model uses the same ids)
+//     sorts the rows by adapter, so that a 128-row tile meets few adapters, and
+//     lists each tile's (adapter, rows) pairs;
+//  2. S in bf16, by sorted row.  Bound by reading x: a tile's K is cut over a
+//     cluster of CTAs, whose sums meet in distributed shared memory;
+//  3. the product on the tcgen05 tensor cores.  The A operand's rows are fetched
+//     in sorted order (TMA gather4); after the K blocks of x W^T each pair of the
+//     tile adds one K block S up[a]^T into the same accumulator, with the lanes of
+//     other rows disabled in the MMA: they get no zero products, so one adapter's
+//     weights, whatever they hold, do not reach another's rows.  The epilogue
+//     writes the rows back to their own places.
+//
+// S is rounded to bf16 because the tensor cores take it so: relative 2^-9 of each
+// of its terms, half of what rounding the sum to the bf16 result costs.  Sums are
+// fp32 throughout and in a fixed order.
+#include "pk_common.cuh"
+#include "pk_internal.h"
+#include "pk_umma.cuh"
+
+namespace pk {
+namespace {
+
+constexpr int kTileRows = 128;
+
+// ------------------------------------------------------------------ the plan
+__global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, int rows,
+                                                            int adapters, AdapterLayout l,
+                                                            int32_t *plan, int32_t *error) {
+    extern __shared__ int s_bin[];   // [adapters + 1] (the last: rows without one)
+    __shared__ int s_warp[33], s_base, s_pairs;
+    grid_dep_wait();
+    grid_dep_launch();
+    const int tid = threadIdx.x, lane = tid & 31, bins = adapters + 1;
+    const int tiles = (rows + kTileRows - 1) / kTileRows;
+    for (int i = tid; i < bins; i += blockDim.x) s_bin[i] = 0;
+    if (tid == 0) s_base = s_pairs = 0;
+    __syncthreads();
+    auto bin_of = [&](int r) {
+        const int a = ids[r];
+        return a >= 0 && a < adapters ? a : adapters;
+    };
+    const int padded = (rows + 31) / 32 * 32;
+    for (int r = tid; r < padded; r += blockDim.x) {
+        const int a = r < rows ? bin_of(r) : -1;
+        if (r < rows && (ids[r] < -1 || ids[r] >= adapters)) raise(error, PK_DEV_BAD_SLOT);
+        const unsigned same = __match_any_sync(0xffffffffu, a);
+        if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(&s_bin[a], __popc(same));
+    }
+    __syncthreads();
+    // each adapter's first sorted row and first pair (it has one for each tile that
+    // its rows touch), 1024 adapters at a time
+    int32_t *pair = plan + l.pairs;
+    for (int i = tid; i < tiles + 1; i += blockDim.x) plan[l.tile_pair + i] = 0x7fffffff;
+    for (int a0 = 0; a0 < bins; a0 += blockDim.x) {
+        const int a = a0 + tid, n = a < bins ? s_bin[a] : 0;
+        auto scan = [&](int v, int &total) {
+            int x = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (lane == 31) s_warp[tid >> 5] = x;
+            __syncthreads();
+            if (tid < 32) {
+                int t = s_warp[tid];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, t, o);
+                    if (lane >= o) t += y;
+                }
+                s_warp[tid] = t;
+                if (tid == 31) s_warp[32] = t;
+            }
+            __syncthreads();
+            total = s_warp[32];
+            const int res = (tid >= 32 ? s_warp[(tid >> 5) - 1] : 0) + x - v;
+            __syncthreads();
+            return res;
+        };
+        int total;
+        const int first = s_base + scan(n, total);
+        __syncthreads();
+        if (tid == 0) s_base += total;
+        const int t0 = first / kTileRows, t1 = n ? (first + n - 1) / kTileRows : t0 - 1;
+        const int mine = a < adapters && n ? t1 - t0 + 1 : 0;
+        const int p0 = s_pairs + scan(mine, total);
+        __syncthreads();
+        if (tid == 0) s_pairs += total;
+        if (a < bins) s_bin[a] = first;   // the sort's running position
+        for (int i = 0; i < mine; ++i) {
+            const int t = t0 + i, lo = max(first - t * kTileRows, 0);
+            const int hi = min(first + n - t * kTileRows, kTileRows);
+            pair[2 * (p0 + i)] = a;
+            pair[2 * (p0 + i) + 1] = lo | hi << 16;
+            if (lo == 0) plan[l.tile_pair + t] = p0 + i;
+        }
+        __syncthreads();
+    }
+    // tiles that no adapter's rows begin: past all of them
+    for (int i = tid; i < tiles + 1; i += blockDim.x)
+        if (plan[l.tile_pair + i] == 0x7fffffff) plan[l.tile_pair + i] = s_pairs;
+    for (int r = tid; r < padded; r += blockDim.x) {
+        const int a = r < rows ? bin_of(r) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, a);
+        const int lead = __ffs(same) - 1;
+        int at = 0;
+        if (a >= 0 && lane == lead) at = atomicAdd(&s_bin[a], __popc(same));
+        at = __shfl_sync(0xffffffffu, at, lead) + __popc(same & ((1u << lane) - 1u));
+        if (a >= 0) plan[l.order + at] = r;
+    }
+    for (int r = rows + tid; r < tiles * kTileRows; r += blockDim.x) plan[l.order + r] = rows;
+}
+
+// --------------------------------------------------------------------- S
+// CTA (rank, tile): K blocks rank, rank + C, ... of the tile's 128 rows.  A stage
+// holds 64 columns of the rows and of the down rows of as many pairs as fit 128
+// columns of S; with more pairs the rows are streamed again for the next ones.
+constexpr int kShThreads = 256, kShStages = 3, kShCols = 128;
+constexpr int kShStage = kTileRows * 128 + kShCols * 128;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool full) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(full ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4a(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <int NT>   // 8-column tiles of a pair: rank <= 8 NT
+__global__ void __launch_bounds__(kShThreads, 2)
+    adapter_shrink_kernel(const AdapterArgs p, int cluster) {
+    extern __shared__ uint8_t sh_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(sh_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ int s_row[kTileRows];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+    const int rank = (int)cluster_ctarank(), tile = blockIdx.y, m0 = tile * kTileRows;
+    grid_dep_wait();
+    grid_dep_launch();
+    const int32_t *plan = p.plan;
+    if (tid < kTileRows) s_row[tid] = plan[p.l.order + m0 + tid];
+    const int pair0 = plan[p.l.tile_pair + tile], pair1 = plan[p.l.tile_pair + tile + 1];
+    const int r = p.rank, per = kShCols / r, nk = p.K / 64;
+    const int mine = (nk - rank + cluster - 1) / cluster;   // K blocks of this CTA
+    const int batches = (pair1 - pair0 + per - 1) / per;
+    const __nv_bfloat16 *x = static_cast<const __nv_bfloat16 *>(p.x);
+    const __nv_bfloat16 *down = static_cast<const __nv_bfloat16 *>(p.down);
+    __syncthreads();
+
+    // this thread's shares of a stage: 4 row chunks
+    const char *src[4];
+    bool live[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = tid + i * kShThreads, row = s_row[c >> 3];
+        live[i] = row < p.M;
+        src[i] = reinterpret_cast<const char *>(x + (int64_t)(live[i] ? row : 0) * p.ldx) +
+                 (c & 7) * 16;
+    }
+    auto load = [&](int it) {
+        const int b = it / mine, kb = rank + (it % mine) * cluster;
+        uint8_t *st = smem + (it % kShStages) * kShStage;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = tid + i * kShThreads;
+            cp_async16(smem_u32(st) + sw128(c >> 3, (c & 7) * 16), src[i] + (int64_t)kb * 128, live[i]);
+        }
+        const int np = min(per, pair1 - pair0 - b * per);
+        for (int c = tid; c < np * r * 8; c += kShThreads) {
+            const int col = c >> 3, j = col / r, q = col - j * r;
+            const int a = plan[p.l.pairs + 2 * (pair0 + b * per + j)];
+            cp_async16(smem_u32(st) + kTileRows * 128 + sw128(col, (c & 7) * 16),
+                       reinterpret_cast<const char *>(down + ((int64_t)a * r + q) * p.K) +
+                           (int64_t)kb * 128 + (c & 7) * 16,
+                       true);
+        }
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+    const int total = batches * max(mine, 0);
+    const int row_lo = warp * 16 + (lane >> 2);
+    for (int it = 0; it < kShStages - 1; ++it) {
+        if (it < total) load(it);
+        commit();
+    }
+    for (int it = 0; it < total; ++it) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kShStages - 2) : "memory");
+        __syncthreads();
+        if (it + kShStages - 1 < total) load(it + kShStages - 1);
+        commit();
+        const uint32_t sa = smem_u32(smem + (it % kShStages) * kShStage);
+        const uint32_t sb = sa + kTileRows * 128;
+        const int b = it / mine, np = min(per, pair1 - pair0 - b * per);
+        uint32_t a[4][4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+            ldsm4a(sa + sw128(warp * 16 + (lane & 15), ks * 32 + (lane >> 4) * 16), a[ks]);
+        for (int j = 0; j < np; ++j) {
+            const int range = plan[p.l.pairs + 2 * (pair0 + b * per + j) + 1];
+            const int lo = range & 0xffff, hi = range >> 16;
+            if (hi <= warp * 16 || lo >= warp * 16 + 16) continue;
+            const bool in0 = row_lo >= lo && row_lo < hi, in1 = row_lo + 8 >= lo && row_lo + 8 < hi;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                if (n * 8 >= r) break;
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k2 = 0; k2 < 2; ++k2) {   // 32 columns of K: 4 matrices
+                    uint32_t bm[4];
+                    ldsm4a(sb + sw128(j * r + n * 8 + (lane & 7), k2 * 64 + (lane >> 3) * 16), bm);
+                    mma_16816(t, a[2 * k2], bm[0], bm[1]);
+                    mma_16816(t, a[2 * k2 + 1], bm[2], bm[3]);
+                }
+                // rows of other adapters keep what they have: no product of theirs
+                if (in0) {
+                    acc[n][0] += t[0];
+                    acc[n][1] += t[1];
+                }
+                if (in1) {
+                    acc[n][2] += t[2];
+                    acc[n][3] += t[3];
+                }
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // partial sums [row][r] of this CTA, then rows rank * share .. summed over the
+    // cluster in rank order
+    float *part = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        if (n * 8 >= r) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float2 *>(part + (row_lo + 8 * h) * r + n * 8 + (lane & 3) * 2) =
+                make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+    }
+    cluster_sync_all();
+    const int share = kTileRows / cluster;
+    __nv_bfloat16 *s = static_cast<__nv_bfloat16 *>(p.s);
+    for (int c = tid; c < share * r; c += kShThreads) {
+        const int row = rank * share + c / r, col = c % r;
+        const uint32_t at = smem_u32(part + row * r + col);
+        float v = 0.f;
+        for (int q = 0; q < cluster; ++q) v += ld_cluster(mapa_rank(at, q));
+        const int m = s_row[row];
+        if (p.scale && m < p.M) {
+            const int a = p.ids[m];
+            if (a >= 0 && a < p.adapters) v *= p.scale[a];
+        }
+        s[(int64_t)(m0 + row) * r + col] = __float2bfloat16_rn(v);
+    }
+    cluster_sync_all();   // no CTA leaves while its sums are read
+}
+
+// ------------------------------------------------------------------ the product
+__device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, uint64_t *bar,
+                                            int32_t c0, int4 rows) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(rows.x), "r"(rows.y), "r"(rows.z),
+        "r"(rows.w), "r"(smem_u32(bar))
+        : "memory");
+}
+// umma_bf16 that leaves the accumulator lanes of `off`'s bits as they are
+__device__ __forceinline__ void umma_bf16_lanes(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                                uint32_t idesc, const uint32_t (&off)[4]) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}" ::"r"(
+            tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+        : "memory");
+}
+
+// A warp's rows of C and R in sorted order: the eight that this lane's pieces touch.
+struct SortedRows {
+    int row[8];
+    __device__ __forceinline__ int operator()(int, int i) const { return row[i]; }
+};
+
+constexpr int kAdThreads = 192;
+
+// The persistent GEMM (pk_gemm.cu) with gathered rows and the pairs' K blocks.
+template <int BN, int NS, int EPI>
+__global__ void __launch_bounds__(kAdThreads, 1)
+    adapter_gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
+                        const __grid_constant__ CUtensorMap tm_w,
+                        const __grid_constant__ CUtensorMap tm_s,
+                        const __grid_constant__ CUtensorMap tm_up, const AdapterArgs p) {
+    constexpr int kBBytes = BN * kBK * 2;
+    extern __shared__ uint8_t gemm_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem, *sB = smem + NS * kABytes;
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], tmem_full[2], tmem_empty[2];
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int failed;
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint8_t *stage = sB + NS * kBBytes + (warp & 3) * kStageBytes;
+    const int mtiles = (p.M + kBM - 1) / kBM, tiles = mtiles * (p.N / BN), nk = p.K / kBK;
+    const int rblocks = (p.rank + kBK - 1) / kBK;
+    const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order;
+    const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tmem_full[a], 1);
+            mbar_init(&tmem_empty[a], 4);
+        }
+        failed = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tm_x);
+        prefetch_tmap(&tm_w);
+        prefetch_tmap(&tm_s);
+        prefetch_tmap(&tm_up);
+    }
+    if (warp == 0) {
+        tmem_alloc(&tmem_base, 2 * BN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+
+    if (warp == 0) {
+        // producer.  The weights of the first stages do not depend on the kernel
+        // before: they are requested ahead of the wait for it.
+        const int pre = (int)blockIdx.x < tiles ? (nk < NS ? nk : NS) : 0;
+        if (lane == 0)
+            for (int kb = 0; kb < pre; ++kb) {
+                mbar_arrive_expect_tx(&full[kb], kABytes + kBBytes);
+                tma_load_2d(sB + kb * kBBytes, &tm_w, &full[kb], kb * kBK,
+                            ((int)blockIdx.x / mtiles) * BN);
+            }
+        __syncwarp();
+        grid_dep_wait();
+        int g = 0;
+        bool stop = false;   // the warp's, so that its lanes stay together
+        auto free_stage = [&](int s) {
+            const int u = g / NS;
+            if (u >= 1 && !mbar_wait_bounded(&empty[s], (u - 1) & 1, kWaitLimitNs)) {
+                raise(p.error, PK_DEV_TIMEOUT);
+                failed = 1;
+            }
+            stop = __any_sync(0xffffffffu, failed != 0);
+        };
+        for (int tile = blockIdx.x; tile < tiles && !stop; tile += gridDim.x) {
+            const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
+            const int4 rows = reinterpret_cast<const int4 *>(order + m0)[lane];
+            for (int kb = 0; kb < nk; ++kb, ++g) {
+                const int s = g % NS;
+                if (g >= pre) {
+                    free_stage(s);
+                    if (stop) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
+                        tma_load_2d(sB + s * kBBytes, &tm_w, &full[s], kb * kBK, n0);
+                    }
+                    __syncwarp();
+                }
+                // four rows a lane
+                tma_gather4(sA + s * kABytes + lane * 512, &tm_x, &full[s], kb * kBK, rows);
+            }
+            if (stop) break;
+            const int p1 = tile_pair[mt + 1];
+            for (int pr = tile_pair[mt]; pr < p1 && !stop; ++pr) {
+                const int a = pairs[pr].x;
+                for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                    const int s = g % NS;
+                    free_stage(s);
+                    if (stop) break;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
+                        tma_load_2d(sA + s * kABytes, &tm_s, &full[s], rb * kBK, m0);
+                        tma_load_3d(sB + s * kBBytes, &tm_up, &full[s], rb * kBK, n0, a);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (stop && lane == 0) {   // leave no copy in flight
+            for (int s = 0; s < NS; ++s)
+                if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_bf16(kBM, BN);
+            grid_dep_wait();   // the plan
+            int g = 0, t = 0;
+            auto ready = [&](int s) {
+                if (mbar_wait_bounded(&full[s], (g / NS) & 1, kWaitLimitNs)) return true;
+                raise(p.error, PK_DEV_TIMEOUT);
+                failed = 1;
+                return false;
+            };
+            for (int tile = blockIdx.x; tile < tiles && !failed; tile += gridDim.x, ++t) {
+                const int acc = t & 1, use = t >> 1, mt = tile % mtiles;
+                if (use >= 1 && !mbar_wait_bounded(&tmem_empty[acc], (use - 1) & 1, kWaitLimitNs)) {
+                    raise(p.error, PK_DEV_TIMEOUT);
+                    failed = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem + acc * BN;
+                for (int kb = 0; kb < nk; ++kb, ++g) {
+                    const int s = g % NS;
+                    if (!ready(s)) break;
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 16; ++kk)
+                        umma_bf16(d, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32), idesc,
+                                  (kb | kk) != 0);
+                    umma_commit(&empty[s]);
+                }
+                const int p1 = tile_pair[mt + 1];
+                for (int pr = tile_pair[mt]; pr < p1 && !failed; ++pr) {
+                    const int range = pairs[pr].y, lo = range & 0xffff, hi = range >> 16;
+                    uint32_t off[4];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int a = max(lo - w * 32, 0), b = min(hi - w * 32, 32);
+                        const uint32_t below = b >= 32 ? 0xffffffffu : (b > 0 ? (1u << b) - 1u : 0u);
+                        const uint32_t skip = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+                        off[w] = ~(below & ~skip);
+                    }
+                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                        const int s = g % NS;
+                        if (!ready(s)) break;
+                        tc_fence_after();
+                        const uint32_t a0 = smem_u32(sA + s * kABytes),
+                                       b0 = smem_u32(sB + s * kBBytes);
+                        const int steps = min(kBK, p.rank - rb * kBK);
+                        for (int kk = 0; kk * 16 < steps; ++kk)
+                            umma_bf16_lanes(d, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32),
+                                            idesc, off);
+                        umma_commit(&empty[s]);
+                    }
+                }
+                umma_commit(&tmem_full[acc]);
+            }
+        }
+    } else {
+        // epilogue warps 2..5
+        grid_dep_wait();
+        const int q = warp & 3;
+        int t = 0;
+        uint4 rv[8], rn[8];
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++t) {
+            const int acc = t & 1, use = t >> 1;
+            const int m0 = (tile % mtiles) * kBM, n0 = (tile / mtiles) * BN;
+            SortedRows rows;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int m = order[m0 + q * 32 + i * 4 + (lane >> 3)];
+                rows.row[i] = m < p.M ? m : -1;
+            }
+            __nv_bfloat16 *C = static_cast<__nv_bfloat16 *>(p.C);
+            const __nv_bfloat16 *R = static_cast<const __nv_bfloat16 *>(p.R);
+            if (is_residual(EPI)) load_residual64(rn, rows, n0, R, p.ldr);
+            const bool ok = __all_sync(0xffffffffu,
+                                       mbar_wait_bounded(&tmem_full[acc], use & 1, kWaitLimitNs));
+            if (!ok) {
+                if (lane == 0) raise(p.error, PK_DEV_TIMEOUT);
+                failed = 1;
+                break;
+            }
+            tc_fence_after();
+            if (tile + (int)gridDim.x >= tiles) grid_dep_launch();
+#pragma unroll 1
+            for (int c = 0; c < BN / 64; ++c) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rv[i] = rn[i];
+                if (is_residual(EPI) && c + 1 < BN / 64)
+                    load_residual64(rn, rows, n0 + (c + 1) * 64, R, p.ldr);
+                epilogue_tile64<EPI>(tmem + acc * BN + ((uint32_t)(q * 32) << 16) + c * 64, rows,
+                                     n0 + c * 64, C, p.ldc, rv,
+                                     static_cast<const __nv_bfloat16 *>(p.bias), p.alpha, stage);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cta(&tmem_empty[acc]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 2 * BN);
+    }
+}
+
+template <int NT>
+cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr size_t smem = kShStages * kShStage + 1024;
+    cudaError_t e = allow_smem(adapter_shrink_kernel<NT>, smem, done);
+    if (e != cudaSuccess) return e;
+    int cluster = 1;   // CTAs over K, a block of 64 or more each
+    while (cluster < 8 && 2 * cluster <= p.K / 64) cluster *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster, (p.M + kTileRows - 1) / kTileRows);
+    cfg.blockDim = dim3(kShThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = cluster;
+    attrs[0].val.clusterDim.y = 1;
+    attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, adapter_shrink_kernel<NT>, p, cluster);
+}
+
+template <int BN, int NS, int EPI>
+int launch_product_t(const AdapterArgs &p, const CUtensorMap (&tm)[4], cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    constexpr size_t smem = (size_t)NS * (kABytes + BN * kBK * 2) + 4 * kStageBytes + 1024;
+    cudaError_t e = allow_smem(adapter_gemm_kernel<BN, NS, EPI>, smem, done);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(adapter gemm)");
+    const int tiles = ((p.M + kBM - 1) / kBM) * (p.N / BN), sms = current_sms();
+    e = launch_pdl(adapter_gemm_kernel<BN, NS, EPI>, dim3(tiles < sms ? tiles : sms),
+                   dim3(kAdThreads), smem, s, tm[0], tm[1], tm[2], tm[3], p);
+    return cuda_status(e, "adapter_gemm_kernel");
+}
+
+template <int BN, int NS>
+int launch_product(const AdapterArgs &p, cudaStream_t s) {
+    CUtensorMap tm[4];
+    const uint64_t xd[2] = {(uint64_t)p.K, (uint64_t)p.M}, xs[1] = {(uint64_t)p.ldx * 2};
+    const uint64_t wd[2] = {(uint64_t)p.K, (uint64_t)p.N}, ws[1] = {(uint64_t)p.ldw * 2};
+    const uint64_t padded = (uint64_t)((p.M + kBM - 1) / kBM * kBM), rb = (uint64_t)p.rank * 2;
+    const uint64_t sd[2] = {(uint64_t)p.rank, padded}, ss[1] = {rb};
+    const uint64_t ud[3] = {(uint64_t)p.rank, (uint64_t)p.N, (uint64_t)p.adapters};
+    const uint64_t us[2] = {rb, rb * p.N};
+    const uint32_t one_row[2] = {kBK, 1}, wbox[2] = {kBK, BN}, sbox[2] = {kBK, kBM},
+                   ubox[3] = {kBK, BN, 1};
+    int st = encode_tmap(&tm[0], PK_DTYPE_BF16, p.x, 2, xd, xs, one_row);
+    if (st == PK_OK) st = encode_tmap(&tm[1], PK_DTYPE_BF16, p.W, 2, wd, ws, wbox);
+    if (st == PK_OK) st = encode_tmap(&tm[2], PK_DTYPE_BF16, p.s, 2, sd, ss, sbox);
+    if (st == PK_OK) st = encode_tmap(&tm[3], PK_DTYPE_BF16, p.up, 3, ud, us, ubox);
+    if (st != PK_OK) return st;
+    switch (p.epilogue) {
+        case PK_GEMM_SILU: return launch_product_t<BN, NS, PK_GEMM_SILU>(p, tm, s);
+        case PK_GEMM_RESIDUAL: return launch_product_t<BN, NS, PK_GEMM_RESIDUAL>(p, tm, s);
+        case PK_GEMM_RESIDUAL_RELU: return launch_product_t<BN, NS, PK_GEMM_RESIDUAL_RELU>(p, tm, s);
+        case PK_GEMM_BIAS: return launch_product_t<BN, NS, PK_GEMM_BIAS>(p, tm, s);
+        default: return launch_product_t<BN, NS, PK_GEMM_STORE>(p, tm, s);
+    }
+}
+
+}  // namespace
+
+int launch_adapter_plan(const int32_t *ids, int rows, int adapters, int32_t *plan, int32_t *error,
+                        cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(adapter_plan_kernel, (PK_ADAPTER_MAX + 1) * 4, done);
+    if (e == cudaSuccess)
+        e = launch_pdl(adapter_plan_kernel, dim3(1), dim3(1024), (size_t)(adapters + 1) * 4, s, ids,
+                       rows, adapters, adapter_layout(rows, adapters), plan, error);
+    return cuda_status(e, "adapter_plan_kernel");
+}
+
+int launch_adapter_gemm(const AdapterArgs &a, cudaStream_t s) {
+    AdapterArgs p = a;
+    p.l = adapter_layout(p.M, p.adapters);
+    cudaError_t e = p.rank <= 8    ? launch_shrink<1>(p, s)
+                    : p.rank <= 16 ? launch_shrink<2>(p, s)
+                    : p.rank <= 32 ? launch_shrink<4>(p, s)
+                    : p.rank <= 64 ? launch_shrink<8>(p, s)
+                                   : launch_shrink<16>(p, s);
+    if (e != cudaSuccess) return cuda_status(e, "adapter_shrink_kernel");
+    // wide tiles where they still fill the GPU, narrow ones (more CTAs for the
+    // weight stream) otherwise
+    const int mtiles = (p.M + kBM - 1) / kBM, sms = current_sms();
+    if (p.N % 256 == 0 && mtiles * (p.N / 256) >= 2 * sms) return launch_product<256, 4>(p, s);
+    if (p.N % 128 == 0 && mtiles * (p.N / 128) >= sms) return launch_product<128, 6>(p, s);
+    return launch_product<64, 6>(p, s);
+}
+
+}  // namespace pk

@@ -1,5 +1,5 @@
-// C-ABI entry points of the token pools (include/pk.h): argument checks on the
-// host, the pool's TMA descriptor, dispatch.
+// C-ABI entry points of the token pools and the adapters (include/pk.h): argument
+// checks on the host, the pool's TMA descriptor, dispatch.
 #include <math.h>
 #include <stdlib.h>
 
@@ -195,6 +195,79 @@ int pk_token_truncate(pk_token_kv *kv, const int32_t *slots, const int32_t *leng
     if (batch == 0) return PK_OK;
     PK_CHECK(slots && lengths, "null slots/lengths");
     return launch_token_truncate(kv, slots, lengths, batch, static_cast<cudaStream_t>(stream));
+}
+
+int64_t pk_adapter_plan_words(int32_t rows, int32_t num_adapters) {
+    if (rows < 0 || rows > PK_ADAPTER_MAX_ROWS || num_adapters <= 0 || num_adapters > PK_ADAPTER_MAX)
+        return -1;
+    return adapter_layout(rows, num_adapters).words;
+}
+
+int pk_adapter_plan(const int32_t *ids, int32_t rows, int32_t num_adapters, int32_t *plan,
+                    int32_t *error, void *stream) {
+    PK_CHECK(rows >= 0 && rows <= PK_ADAPTER_MAX_ROWS, "rows %d outside [0, %d]", rows,
+             PK_ADAPTER_MAX_ROWS);
+    PK_CHECK(num_adapters > 0 && num_adapters <= PK_ADAPTER_MAX, "num_adapters %d outside [1, %d]",
+             num_adapters, PK_ADAPTER_MAX);
+    if (rows == 0) return PK_OK;
+    PK_CHECK(ids && plan && error, "null pointer");
+    PK_CHECK(aligned16(plan), "plan not 16-byte aligned");
+    return launch_adapter_plan(ids, rows, num_adapters, plan, error,
+                               static_cast<cudaStream_t>(stream));
+}
+
+int64_t pk_adapter_workspace(int32_t rows, int32_t rank) {
+    if (rows < 0 || rows > PK_ADAPTER_MAX_ROWS || rank <= 0 || rank > PK_ADAPTER_MAX_RANK) return -1;
+    return ((int64_t)rows + 127) / 128 * 128 * rank * 2;
+}
+
+int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int32_t M, int32_t N,
+                    int32_t K, void *C, int64_t ldc, int32_t epilogue, const void *R, int64_t ldr,
+                    const void *bias, float alpha, const void *down, const void *up, int32_t rank,
+                    int32_t num_adapters, const float *scale, const int32_t *ids,
+                    const int32_t *plan, void *workspace, int32_t *error, void *stream) {
+    PK_CHECK(M >= 0 && M <= PK_ADAPTER_MAX_ROWS && N > 0 && K > 0, "bad shape %d x %d x %d", M, N, K);
+    PK_CHECK(num_adapters > 0 && num_adapters <= PK_ADAPTER_MAX, "num_adapters %d outside [1, %d]",
+             num_adapters, PK_ADAPTER_MAX);
+    PK_CHECK(rank > 0 && rank % 8 == 0 && rank <= PK_ADAPTER_MAX_RANK,
+             "rank %d: a multiple of 8 up to %d", rank, PK_ADAPTER_MAX_RANK);
+    if (M == 0) return PK_OK;
+    PK_CHECK(K % 64 == 0 && N % 64 == 0, "K (%d) and N (%d) must be multiples of 64", K, N);
+    PK_CHECK(epilogue >= PK_GEMM_STORE && epilogue <= PK_GEMM_BIAS, "bad epilogue %d", epilogue);
+    PK_CHECK(A && W && C && down && up && ids && plan && workspace && error, "null pointer");
+    PK_CHECK(aligned16(A) && aligned16(W) && aligned16(C) && aligned16(down) && aligned16(up) &&
+                 aligned16(plan) && aligned16(workspace),
+             "operands must be 16-byte aligned");
+    PK_CHECK(lda >= K && ldw >= K && ldc >= N && lda % 8 == 0 && ldw % 8 == 0 && ldc % 8 == 0,
+             "row strides must cover the rows and be multiples of 8 elements");
+    if (epilogue == PK_GEMM_RESIDUAL || epilogue == PK_GEMM_RESIDUAL_RELU)
+        PK_CHECK(R && aligned16(R) && ldr >= N && ldr % 8 == 0, "bad residual operand");
+    if (epilogue == PK_GEMM_BIAS) PK_CHECK(bias && aligned16(bias), "bad bias operand");
+    AdapterArgs a;
+    a.x = A;
+    a.W = W;
+    a.R = R;
+    a.bias = bias;
+    a.down = down;
+    a.up = up;
+    a.ldx = lda;
+    a.ldw = ldw;
+    a.ldc = ldc;
+    a.ldr = ldr;
+    a.C = C;
+    a.s = workspace;
+    a.M = M;
+    a.N = N;
+    a.K = K;
+    a.epilogue = epilogue;
+    a.rank = rank;
+    a.adapters = num_adapters;
+    a.alpha = alpha;
+    a.scale = scale;
+    a.ids = ids;
+    a.plan = plan;
+    a.error = error;
+    return launch_adapter_gemm(a, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

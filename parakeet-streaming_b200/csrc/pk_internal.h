@@ -299,6 +299,34 @@ struct TreeAttnArgs {
 int64_t tree_attn_workspace(const pk_token_kv *kv, int batch, int rows);
 int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStream_t s);
 
+// pk_adapter.cu: plan block, int32 words
+struct AdapterLayout {
+    int64_t tile_pair, order, pairs, words;
+};
+inline AdapterLayout adapter_layout(int rows, int adapters) {
+    AdapterLayout l;
+    const int64_t tiles = ((int64_t)rows + 127) / 128;
+    l.order = 0;                         // sorted row -> row; `rows` past the last
+    l.tile_pair = l.order + tiles * 128; // first pair of each tile
+    l.pairs = (l.tile_pair + tiles + 1 + 1) / 2 * 2;   // adapter, first | end << 16 row in the tile
+    l.words = l.pairs + 2 * (tiles + (adapters < rows ? adapters : rows));
+    return l;
+}
+struct AdapterArgs {
+    const void *x, *W, *R, *bias, *down, *up;
+    int64_t ldx, ldw, ldc, ldr;
+    void *C, *s;
+    int M, N, K, epilogue, rank, adapters;
+    float alpha;
+    const float *scale;
+    const int32_t *ids, *plan;
+    int32_t *error;
+    AdapterLayout l;
+};
+int launch_adapter_plan(const int32_t *ids, int rows, int adapters, int32_t *plan, int32_t *error,
+                        cudaStream_t s);
+int launch_adapter_gemm(const AdapterArgs &a, cudaStream_t s);
+
 // Allow `bytes` of dynamic shared memory for `kernel` on the current device, once
 // per device (`done`: a bit per device, of the kernel's own).
 template <typename K>

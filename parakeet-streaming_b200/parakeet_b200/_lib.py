@@ -24,6 +24,7 @@ PK_NOALLOC_SCRATCH_BYTES = 32 * 1024 * 1024   # pk_paged_attention_noalloc's sta
 PK_TOK_ROW_START, PK_TOK_CONTEXT, PK_TOK_REQUEST, PK_TOK_POSITION = 0, 1, 7, 8
 PK_TOK_SLOT_MAP, PK_TOK_MASK, PK_TOK_OFFSETS = 9, 11, 12
 PK_TOK_MAX_TREE, PK_TOK_MAX_BATCH = 64, 65536   # nodes of a tree, requests of a step
+PK_ADAPTER_MAX, PK_ADAPTER_MAX_RANK, PK_ADAPTER_MAX_ROWS = 8192, 128, 1048576
 META_FIRST, META_NEXT, META_WRITTEN, META_PROCESSED, META_CACHE_LEN = 0, 1, 2, 3, 4
 META_STRIDE = 8
 WIN_STRIDE = 128
@@ -151,11 +152,17 @@ SIGNATURES = {
                            _I64, _P, _P],
     "pk_token_end_step": [_P, _P, _I32, _I32, _I32, _P, _P],
     "pk_token_truncate": [_P, _P, _P, _I32, _P],
+    "pk_adapter_plan_words": [_I32, _I32],
+    "pk_adapter_plan": [_P, _I32, _I32, _P, _P, _P],
+    "pk_adapter_workspace": [_I32, _I32],
+    "pk_adapter_gemm": [_P, _I64, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _P,
+                        ctypes.c_float, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _P],
     "pk_selftest_bounded_wait": [_P, _I32, _I64, _P, _P],
     "pk_last_error": [],
 }
 RESTYPES = {"pk_last_error": ctypes.c_char_p, "pk_token_step_words": _I64,
-            "pk_token_attention_workspace": _I64}
+            "pk_token_attention_workspace": _I64, "pk_adapter_plan_words": _I64,
+            "pk_adapter_workspace": _I64}
 
 _lib = None
 
