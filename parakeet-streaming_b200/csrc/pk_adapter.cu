@@ -10,7 +10,7 @@
 //  2. S in bf16, by sorted row.  Bound by reading x: a tile's K is cut over a
 //     cluster of CTAs, whose sums meet in distributed shared memory;
 //  3. the product on the tcgen05 tensor cores.  The A operand's rows are fetched
-//     in sorted order (TMA gather4); after the K blocks of x W^T each pair of the
+//     in sorted order; after the K blocks of x W^T each pair of the
 //     tile adds one K block S up[a]^T into the same accumulator, with the lanes of
 //     other rows disabled in the MMA: they get no zero products, so one adapter's
 //     weights, whatever they hold, do not reach another's rows.  The epilogue
@@ -284,15 +284,6 @@ __global__ void __launch_bounds__(kShThreads, 2)
 }
 
 // ------------------------------------------------------------------ the product
-__device__ __forceinline__ void tma_gather4(void *dst, const CUtensorMap *map, uint64_t *bar,
-                                            int32_t c0, int4 rows) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(rows.x), "r"(rows.y), "r"(rows.z),
-        "r"(rows.w), "r"(smem_u32(bar))
-        : "memory");
-}
 // umma_bf16 that leaves the accumulator lanes of `off`'s bits as they are
 __device__ __forceinline__ void umma_bf16_lanes(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                                 uint32_t idesc, const uint32_t (&off)[4]) {
@@ -311,16 +302,20 @@ struct SortedRows {
     __device__ __forceinline__ int operator()(int, int i) const { return row[i]; }
 };
 
-constexpr int kAdThreads = 192;
+constexpr int kAdThreads = 320;   // TMA, MMA, 4 epilogue and 4 gather warps
 
-// The persistent GEMM (pk_gemm.cu) with gathered rows and the pairs' K blocks.
+// The persistent GEMM (pk_gemm.cu) with gathered rows and the pairs' K blocks.  A
+// stage's A half is fetched by four warps with 16-byte cp.async (TMA's gather4, four
+// 128-byte rows an instruction, measured 85 cycles each: a sixth of what the MMAs
+// consume), its B half by TMA.
 template <int BN, int NS, int EPI>
 __global__ void __launch_bounds__(kAdThreads, 1)
-    adapter_gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
-                        const __grid_constant__ CUtensorMap tm_w,
-                        const __grid_constant__ CUtensorMap tm_s,
+    adapter_gemm_kernel(const __grid_constant__ CUtensorMap tm_w,
                         const __grid_constant__ CUtensorMap tm_up, const AdapterArgs p) {
     constexpr int kBBytes = BN * kBK * 2;
+    // groups that a gather warp keeps in flight: it has handed over stage g - NS
+    // before it waits for stage g to be free
+    constexpr int kLag = NS - 2;
     extern __shared__ uint8_t gemm_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~uintptr_t(1023));
@@ -337,7 +332,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], 5);   // the TMA lane and the four gather warps
             mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -346,9 +341,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         }
         failed = 0;
         fence_mbar_init();
-        prefetch_tmap(&tm_x);
         prefetch_tmap(&tm_w);
-        prefetch_tmap(&tm_s);
         prefetch_tmap(&tm_up);
     }
     if (warp == 0) {
@@ -359,67 +352,112 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base;
+    // wait until stage g of the ring is free; false when a wait of the CTA gave up
+    auto free_stage = [&](int g) {
+        const int u = g / NS;
+        if (u >= 1 && !failed && !mbar_wait_bounded(&empty[g % NS], (u - 1) & 1, kWaitLimitNs)) {
+            raise(p.error, PK_DEV_TIMEOUT);
+            failed = 1;
+        }
+        return !failed;
+    };
 
     if (warp == 0) {
-        // producer.  The weights of the first stages do not depend on the kernel
-        // before: they are requested ahead of the wait for it.
-        const int pre = (int)blockIdx.x < tiles ? (nk < NS ? nk : NS) : 0;
-        if (lane == 0)
+        if (lane == 0) {
+            // B producer.  The weights of the first stages do not depend on the
+            // kernel before: they are requested ahead of the wait for it.
+            const int pre = (int)blockIdx.x < tiles ? (nk < NS ? nk : NS) : 0;
             for (int kb = 0; kb < pre; ++kb) {
-                mbar_arrive_expect_tx(&full[kb], kABytes + kBBytes);
+                mbar_arrive_expect_tx(&full[kb], kBBytes);
                 tma_load_2d(sB + kb * kBBytes, &tm_w, &full[kb], kb * kBK,
                             ((int)blockIdx.x / mtiles) * BN);
             }
-        __syncwarp();
+            grid_dep_wait();
+            int g = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+                const int mt = tile % mtiles, n0 = (tile / mtiles) * BN;
+                for (int kb = 0; kb < nk && ok; ++kb, ++g) {
+                    if (g < pre) continue;
+                    if (!(ok = free_stage(g))) break;
+                    mbar_arrive_expect_tx(&full[g % NS], kBBytes);
+                    tma_load_2d(sB + (g % NS) * kBBytes, &tm_w, &full[g % NS], kb * kBK, n0);
+                }
+                const int p1 = tile_pair[mt + 1];
+                for (int pr = tile_pair[mt]; pr < p1 && ok; ++pr) {
+                    const int a = pairs[pr].x;
+                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                        if (!(ok = free_stage(g))) break;
+                        mbar_arrive_expect_tx(&full[g % NS], kBBytes);
+                        tma_load_3d(sB + (g % NS) * kBBytes, &tm_up, &full[g % NS], rb * kBK, n0, a);
+                    }
+                }
+            }
+            if (!ok)   // leave no copy in flight
+                for (int s = 0; s < NS; ++s)
+                    if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
+        }
+    } else if (warp >= 6) {
+        // A: thread t brings 16-byte chunk t % 8 of rows t / 8 + 16 i of the tile
+        const int t = threadIdx.x - 6 * 32, chunk = t & 7, row0 = t >> 3;
         grid_dep_wait();
         int g = 0;
-        bool stop = false;   // the warp's, so that its lanes stay together
-        auto free_stage = [&](int s) {
-            const int u = g / NS;
-            if (u >= 1 && !mbar_wait_bounded(&empty[s], (u - 1) & 1, kWaitLimitNs)) {
-                raise(p.error, PK_DEV_TIMEOUT);
-                failed = 1;
-            }
-            stop = __any_sync(0xffffffffu, failed != 0);
+        bool ok = true;
+        // stage `at` has arrived once at most `behind` younger groups are in flight
+        auto hand_over = [&](int at) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cta(&full[at % NS]);
         };
-        for (int tile = blockIdx.x; tile < tiles && !stop; tile += gridDim.x) {
-            const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
-            const int4 rows = reinterpret_cast<const int4 *>(order + m0)[lane];
-            for (int kb = 0; kb < nk; ++kb, ++g) {
-                const int s = g % NS;
-                if (g >= pre) {
-                    free_stage(s);
-                    if (stop) break;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
-                        tma_load_2d(sB + s * kBBytes, &tm_w, &full[s], kb * kBK, n0);
-                    }
-                    __syncwarp();
-                }
-                // four rows a lane
-                tma_gather4(sA + s * kABytes + lane * 512, &tm_x, &full[s], kb * kBK, rows);
+        auto issue = [&](const char *const (&src)[8], const bool (&live)[8], int64_t bytes, int width) {
+            if (!free_stage(g)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            const uint32_t dst = smem_u32(sA + (g % NS) * kABytes);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                const bool in = live[i] && chunk * 16 < width;
+                cp_async16(dst + sw128(row0 + 16 * i, chunk * 16),
+                           in ? src[i] + bytes : static_cast<const char *>(p.x), in);
             }
-            if (stop) break;
-            const int p1 = tile_pair[mt + 1];
-            for (int pr = tile_pair[mt]; pr < p1 && !stop; ++pr) {
-                const int a = pairs[pr].x;
-                for (int rb = 0; rb < rblocks; ++rb, ++g) {
-                    const int s = g % NS;
-                    free_stage(s);
-                    if (stop) break;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
-                        tma_load_2d(sA + s * kABytes, &tm_s, &full[s], rb * kBK, m0);
-                        tma_load_3d(sB + s * kBBytes, &tm_up, &full[s], rb * kBK, n0, a);
-                    }
-                    __syncwarp();
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (g >= kLag) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                hand_over(g - kLag);
+            }
+            ++g;
+        };
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            const int mt = tile % mtiles, m0 = mt * kBM;
+            const char *src[8];
+            bool live[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = order[m0 + row0 + 16 * i];
+                live[i] = row < p.M;
+                src[i] = reinterpret_cast<const char *>(
+                             static_cast<const __nv_bfloat16 *>(p.x) +
+                             (live[i] ? (int64_t)row * p.ldx : 0)) + chunk * 16;
+            }
+            for (int kb = 0; kb < nk && ok; ++kb) issue(src, live, (int64_t)kb * 128, 128);
+            const int np = tile_pair[mt + 1] - tile_pair[mt];
+            if (np) {   // the same S block for every pair: other rows' lanes are off
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    live[i] = true;
+                    src[i] = reinterpret_cast<const char *>(
+                                 static_cast<const __nv_bfloat16 *>(p.s) +
+                                 (int64_t)(m0 + row0 + 16 * i) * p.rank) +
+                             chunk * 16;
                 }
+                for (int pr = 0; pr < np && ok; ++pr)
+                    for (int rb = 0; rb < rblocks && ok; ++rb)
+                        issue(src, live, rb * 128, p.rank * 2 - rb * 128);
             }
         }
-        if (stop && lane == 0) {   // leave no copy in flight
-            for (int s = 0; s < NS; ++s)
-                if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
-        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (int at = max(g - kLag, 0); at < g; ++at) hand_over(at);
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = idesc_bf16(kBM, BN);
@@ -554,32 +592,27 @@ cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
 }
 
 template <int BN, int NS, int EPI>
-int launch_product_t(const AdapterArgs &p, const CUtensorMap (&tm)[4], cudaStream_t s) {
+int launch_product_t(const AdapterArgs &p, const CUtensorMap (&tm)[2], cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr size_t smem = (size_t)NS * (kABytes + BN * kBK * 2) + 4 * kStageBytes + 1024;
     cudaError_t e = allow_smem(adapter_gemm_kernel<BN, NS, EPI>, smem, done);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(adapter gemm)");
     const int tiles = ((p.M + kBM - 1) / kBM) * (p.N / BN), sms = current_sms();
     e = launch_pdl(adapter_gemm_kernel<BN, NS, EPI>, dim3(tiles < sms ? tiles : sms),
-                   dim3(kAdThreads), smem, s, tm[0], tm[1], tm[2], tm[3], p);
+                   dim3(kAdThreads), smem, s, tm[0], tm[1], p);
     return cuda_status(e, "adapter_gemm_kernel");
 }
 
 template <int BN, int NS>
 int launch_product(const AdapterArgs &p, cudaStream_t s) {
-    CUtensorMap tm[4];
-    const uint64_t xd[2] = {(uint64_t)p.K, (uint64_t)p.M}, xs[1] = {(uint64_t)p.ldx * 2};
+    CUtensorMap tm[2];
     const uint64_t wd[2] = {(uint64_t)p.K, (uint64_t)p.N}, ws[1] = {(uint64_t)p.ldw * 2};
-    const uint64_t padded = (uint64_t)((p.M + kBM - 1) / kBM * kBM), rb = (uint64_t)p.rank * 2;
-    const uint64_t sd[2] = {(uint64_t)p.rank, padded}, ss[1] = {rb};
+    const uint64_t rb = (uint64_t)p.rank * 2;
     const uint64_t ud[3] = {(uint64_t)p.rank, (uint64_t)p.N, (uint64_t)p.adapters};
     const uint64_t us[2] = {rb, rb * p.N};
-    const uint32_t one_row[2] = {kBK, 1}, wbox[2] = {kBK, BN}, sbox[2] = {kBK, kBM},
-                   ubox[3] = {kBK, BN, 1};
-    int st = encode_tmap(&tm[0], PK_DTYPE_BF16, p.x, 2, xd, xs, one_row);
-    if (st == PK_OK) st = encode_tmap(&tm[1], PK_DTYPE_BF16, p.W, 2, wd, ws, wbox);
-    if (st == PK_OK) st = encode_tmap(&tm[2], PK_DTYPE_BF16, p.s, 2, sd, ss, sbox);
-    if (st == PK_OK) st = encode_tmap(&tm[3], PK_DTYPE_BF16, p.up, 3, ud, us, ubox);
+    const uint32_t wbox[2] = {kBK, BN}, ubox[3] = {kBK, BN, 1};
+    int st = encode_tmap(&tm[0], PK_DTYPE_BF16, p.W, 2, wd, ws, wbox);
+    if (st == PK_OK) st = encode_tmap(&tm[1], PK_DTYPE_BF16, p.up, 3, ud, us, ubox);
     if (st != PK_OK) return st;
     switch (p.epilogue) {
         case PK_GEMM_SILU: return launch_product_t<BN, NS, PK_GEMM_SILU>(p, tm, s);
