@@ -607,7 +607,7 @@ int pk_adapter_plan(const int32_t *ids, int32_t rows, int32_t num_adapters, int3
 /* Arguments as pk_gemm_bf16's; ids and plan as given to and made by
  * pk_adapter_plan (rows = M); workspace: pk_adapter_workspace() bytes, 16-byte
  * aligned, for this call alone. */
-int64_t pk_adapter_workspace(int32_t rows, int32_t rank);
+int64_t pk_adapter_workspace(int32_t rows, int32_t K, int32_t rank);
 int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int32_t M, int32_t N,
                     int32_t K, void *C, int64_t ldc, int32_t epilogue, const void *R, int64_t ldr,
                     const void *bias, float alpha, const void *down, const void *up, int32_t rank,

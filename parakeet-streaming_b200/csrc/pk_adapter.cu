@@ -33,13 +33,13 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
                                                             int adapters, AdapterLayout l,
                                                             int32_t *plan, int32_t *error) {
     extern __shared__ int s_bin[];   // [adapters + 1] (the last: rows without one)
-    __shared__ int s_warp[33], s_base, s_pairs;
+    __shared__ int s_warp[33], s_base, s_pairs, s_moved;
     grid_dep_wait();
     grid_dep_launch();
     const int tid = threadIdx.x, lane = tid & 31, bins = adapters + 1;
     const int tiles = (rows + kTileRows - 1) / kTileRows;
     for (int i = tid; i < bins; i += blockDim.x) s_bin[i] = 0;
-    if (tid == 0) s_base = s_pairs = 0;
+    if (tid == 0) s_base = s_pairs = s_moved = 0;
     __syncthreads();
     auto bin_of = [&](int r) {
         const int a = ids[r];
@@ -114,7 +114,10 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
         if (a >= 0 && lane == lead) at = atomicAdd(&s_bin[a], __popc(same));
         at = __shfl_sync(0xffffffffu, at, lead) + __popc(same & ((1u << lane) - 1u));
         if (a >= 0) plan[l.order + at] = r;
+        if (a >= 0 && at != r) s_moved = 1;
     }
+    __syncthreads();
+    if (tid == 0) plan[l.sorted] = !s_moved;
     for (int r = rows + tid; r < tiles * kTileRows; r += blockDim.x) plan[l.order + r] = rows;
 }
 
@@ -166,9 +169,11 @@ __global__ void __launch_bounds__(kShThreads, 2)
     const int pair0 = plan[p.l.tile_pair + tile], pair1 = plan[p.l.tile_pair + tile + 1];
     const int r = p.rank, per = kShCols / r, nk = p.K / 64;
     const int mine = (nk - rank + cluster - 1) / cluster;   // K blocks of this CTA
-    const int batches = (pair1 - pair0 + per - 1) / per;
+    const int batches = max((pair1 - pair0 + per - 1) / per, 1);   // one for the copy at least
     const __nv_bfloat16 *x = static_cast<const __nv_bfloat16 *>(p.x);
     const __nv_bfloat16 *down = static_cast<const __nv_bfloat16 *>(p.down);
+    // the rows' sorted copy is made on the way, where their order is another
+    char *copy = plan[p.l.sorted] ? nullptr : static_cast<char *>(p.xs);
     __syncthreads();
 
     // this thread's shares of a stage: 4 row chunks
@@ -219,7 +224,19 @@ __global__ void __launch_bounds__(kShThreads, 2)
         commit();
         const uint32_t sa = smem_u32(smem + (it % kShStages) * kShStage);
         const uint32_t sb = sa + kTileRows * 128;
-        const int b = it / mine, np = min(per, pair1 - pair0 - b * per);
+        const int b = it / mine;
+        if (copy && b == 0) {
+            const uint8_t *st = smem + (it % kShStages) * kShStage;
+            const int64_t kb = rank + it * cluster;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = tid + i * kShThreads, row = c >> 3;
+                *reinterpret_cast<uint4 *>(copy + ((int64_t)(m0 + row) * p.K + kb * 64) * 2 +
+                                           (c & 7) * 16) =
+                    *reinterpret_cast<const uint4 *>(st + sw128(row, (c & 7) * 16));
+            }
+        }
+        const int np = min(per, pair1 - pair0 - b * per);
         uint32_t a[4][4];
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
@@ -296,26 +313,53 @@ __device__ __forceinline__ void umma_bf16_lanes(uint32_t tmem_d, uint64_t adesc,
         : "memory");
 }
 
+__device__ __forceinline__ void umma_bf16_pair_lanes(uint32_t tmem_d, uint64_t adesc,
+                                                     uint64_t bdesc, uint32_t idesc,
+                                                     const uint32_t (&off)[8]) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, "
+        "p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]),
+        "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
+        : "memory");
+}
+// Lanes outside a pair's rows, 32 a word.
+__device__ __forceinline__ void lanes_off(int range, uint32_t *off) {
+    const int lo = range & 0xffff, hi = range >> 16;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int a = max(lo - w * 32, 0), b = min(hi - w * 32, 32);
+        const uint32_t below = b >= 32 ? 0xffffffffu : (b > 0 ? (1u << b) - 1u : 0u);
+        const uint32_t skip = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+        off[w] = ~(below & ~skip);
+    }
+}
+
 // A warp's rows of C and R in sorted order: the eight that this lane's pieces touch.
 struct SortedRows {
     int row[8];
     __device__ __forceinline__ int operator()(int, int i) const { return row[i]; }
 };
 
-constexpr int kAdThreads = 320;   // TMA, MMA, 4 epilogue and 4 gather warps
+struct AdapterMaps {
+    CUtensorMap x, xs, w, s, up;   // rows, sorted copy, weight, S, up
+};
 
-// The persistent GEMM (pk_gemm.cu) with gathered rows and the pairs' K blocks.  A
-// stage's A half is fetched by four warps with 16-byte cp.async (TMA's gather4, four
-// 128-byte rows an instruction, measured 85 cycles each: a sixth of what the MMAs
-// consume), its B half by TMA.
+constexpr int kAdThreads = 192;   // TMA, MMA and 4 epilogue warps
+
+// The persistent GEMM (pk_gemm.cu) over the sorted rows, with the pairs' K blocks.
+// The rows come by TMA tile loads from their sorted copy (from x itself where its
+// order is the sorted one).  Fetching them in place was slower at every size: TMA's
+// gather4 (four 128-byte rows an instruction) takes 85 cycles each, six times what
+// the MMAs of a stage last; 16-byte cp.async by four more warps costs its proxy
+// fences, 0.5 us a stage (6720 x 1024 x 4096: 265 and 98 us against 67 for the
+// plain tile loads).
 template <int BN, int NS, int EPI>
 __global__ void __launch_bounds__(kAdThreads, 1)
-    adapter_gemm_kernel(const __grid_constant__ CUtensorMap tm_w,
-                        const __grid_constant__ CUtensorMap tm_up, const AdapterArgs p) {
+    adapter_gemm_kernel(const __grid_constant__ AdapterMaps tm, const AdapterArgs p) {
     constexpr int kBBytes = BN * kBK * 2;
-    // groups that a gather warp keeps in flight: it has handed over stage g - NS
-    // before it waits for stage g to be free
-    constexpr int kLag = NS - 2;
     extern __shared__ uint8_t gemm_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~uintptr_t(1023));
@@ -328,11 +372,12 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     uint8_t *stage = sB + NS * kBBytes + (warp & 3) * kStageBytes;
     const int mtiles = (p.M + kBM - 1) / kBM, tiles = mtiles * (p.N / BN), nk = p.K / kBK;
     const int rblocks = (p.rank + kBK - 1) / kBK;
-    const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order;
+    const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order,
+                  *sorted = p.plan + p.l.sorted;
     const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
-            mbar_init(&full[s], 5);   // the TMA lane and the four gather warps
+            mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -341,8 +386,9 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         }
         failed = 0;
         fence_mbar_init();
-        prefetch_tmap(&tm_w);
-        prefetch_tmap(&tm_up);
+        prefetch_tmap(&tm.w);
+        prefetch_tmap(&tm.up);
+        prefetch_tmap(&tm.s);
     }
     if (warp == 0) {
         tmem_alloc(&tmem_base, 2 * BN);
@@ -364,32 +410,38 @@ __global__ void __launch_bounds__(kAdThreads, 1)
 
     if (warp == 0) {
         if (lane == 0) {
-            // B producer.  The weights of the first stages do not depend on the
-            // kernel before: they are requested ahead of the wait for it.
+            // producer.  The weights of the first stages do not depend on the kernel
+            // before: they are requested ahead of the wait for it.
             const int pre = (int)blockIdx.x < tiles ? (nk < NS ? nk : NS) : 0;
             for (int kb = 0; kb < pre; ++kb) {
-                mbar_arrive_expect_tx(&full[kb], kBBytes);
-                tma_load_2d(sB + kb * kBBytes, &tm_w, &full[kb], kb * kBK,
+                mbar_arrive_expect_tx(&full[kb], kABytes + kBBytes);
+                tma_load_2d(sB + kb * kBBytes, &tm.w, &full[kb], kb * kBK,
                             ((int)blockIdx.x / mtiles) * BN);
             }
             grid_dep_wait();
+            const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
             int g = 0;
             bool ok = true;
             for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-                const int mt = tile % mtiles, n0 = (tile / mtiles) * BN;
-                for (int kb = 0; kb < nk && ok; ++kb, ++g) {
-                    if (g < pre) continue;
-                    if (!(ok = free_stage(g))) break;
-                    mbar_arrive_expect_tx(&full[g % NS], kBBytes);
-                    tma_load_2d(sB + (g % NS) * kBBytes, &tm_w, &full[g % NS], kb * kBK, n0);
+                const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
+                for (int kb = 0; kb < nk; ++kb, ++g) {
+                    const int s = g % NS;
+                    if (g >= pre) {
+                        if (!(ok = free_stage(g))) break;
+                        mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
+                        tma_load_2d(sB + s * kBBytes, &tm.w, &full[s], kb * kBK, n0);
+                    }
+                    tma_load_2d(sA + s * kABytes, rows, &full[s], kb * kBK, m0);
                 }
                 const int p1 = tile_pair[mt + 1];
                 for (int pr = tile_pair[mt]; pr < p1 && ok; ++pr) {
                     const int a = pairs[pr].x;
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                        const int s = g % NS;
                         if (!(ok = free_stage(g))) break;
-                        mbar_arrive_expect_tx(&full[g % NS], kBBytes);
-                        tma_load_3d(sB + (g % NS) * kBBytes, &tm_up, &full[g % NS], rb * kBK, n0, a);
+                        mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
+                        tma_load_2d(sA + s * kABytes, &tm.s, &full[s], rb * kBK, m0);
+                        tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, a);
                     }
                 }
             }
@@ -397,67 +449,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 for (int s = 0; s < NS; ++s)
                     if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
         }
-    } else if (warp >= 6) {
-        // A: thread t brings 16-byte chunk t % 8 of rows t / 8 + 16 i of the tile
-        const int t = threadIdx.x - 6 * 32, chunk = t & 7, row0 = t >> 3;
-        grid_dep_wait();
-        int g = 0;
-        bool ok = true;
-        // stage `at` has arrived once at most `behind` younger groups are in flight
-        auto hand_over = [&](int at) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cta(&full[at % NS]);
-        };
-        auto issue = [&](const char *const (&src)[8], const bool (&live)[8], int64_t bytes, int width) {
-            if (!free_stage(g)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
-            const uint32_t dst = smem_u32(sA + (g % NS) * kABytes);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-            {
-                const bool in = live[i] && chunk * 16 < width;
-                cp_async16(dst + sw128(row0 + 16 * i, chunk * 16),
-                           in ? src[i] + bytes : static_cast<const char *>(p.x), in);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (g >= kLag) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-                hand_over(g - kLag);
-            }
-            ++g;
-        };
-        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-            const int mt = tile % mtiles, m0 = mt * kBM;
-            const char *src[8];
-            bool live[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = order[m0 + row0 + 16 * i];
-                live[i] = row < p.M;
-                src[i] = reinterpret_cast<const char *>(
-                             static_cast<const __nv_bfloat16 *>(p.x) +
-                             (live[i] ? (int64_t)row * p.ldx : 0)) + chunk * 16;
-            }
-            for (int kb = 0; kb < nk && ok; ++kb) issue(src, live, (int64_t)kb * 128, 128);
-            const int np = tile_pair[mt + 1] - tile_pair[mt];
-            if (np) {   // the same S block for every pair: other rows' lanes are off
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    live[i] = true;
-                    src[i] = reinterpret_cast<const char *>(
-                                 static_cast<const __nv_bfloat16 *>(p.s) +
-                                 (int64_t)(m0 + row0 + 16 * i) * p.rank) +
-                             chunk * 16;
-                }
-                for (int pr = 0; pr < np && ok; ++pr)
-                    for (int rb = 0; rb < rblocks && ok; ++rb)
-                        issue(src, live, rb * 128, p.rank * 2 - rb * 128);
-            }
-        }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        for (int at = max(g - kLag, 0); at < g; ++at) hand_over(at);
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = idesc_bf16(kBM, BN);
@@ -491,19 +482,12 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 }
                 const int p1 = tile_pair[mt + 1];
                 for (int pr = tile_pair[mt]; pr < p1 && !failed; ++pr) {
-                    const int range = pairs[pr].y, lo = range & 0xffff, hi = range >> 16;
                     uint32_t off[4];
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int a = max(lo - w * 32, 0), b = min(hi - w * 32, 32);
-                        const uint32_t below = b >= 32 ? 0xffffffffu : (b > 0 ? (1u << b) - 1u : 0u);
-                        const uint32_t skip = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
-                        off[w] = ~(below & ~skip);
-                    }
+                    lanes_off(pairs[pr].y, off);
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         const int s = g % NS;
                         if (!ready(s)) break;
-                        tc_fence_after();
+                            tc_fence_after();
                         const uint32_t a0 = smem_u32(sA + s * kABytes),
                                        b0 = smem_u32(sB + s * kBBytes);
                         const int steps = min(kBK, p.rank - rb * kBK);
@@ -566,6 +550,221 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     }
 }
 
+// 3-D tile load into this CTA's shared memory, completion on an mbarrier of either
+// CTA of the pair
+__device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *map, uint32_t bar,
+                                                 int32_t c0, int32_t c1, int32_t c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+
+// CTA-pair form (pk_gemm.cu's, 256 x BN tiles): CTA r loads sorted rows 128 r ..
+// of the tile and rows (BN / 2) r .. of W.  The pairs of the tile's two
+// 128-row halves are walked one half after the other, the other half's lanes off.
+template <int BN, int NS, int EPI>
+__global__ void __launch_bounds__(kAdThreads, 1)
+    adapter_gemm_pair_kernel(const __grid_constant__ AdapterMaps tm, const AdapterArgs p) {
+    constexpr int kHalfB = BN / 2;
+    constexpr int kBBytes = kHalfB * kBK * 2;
+    constexpr uint32_t kStageTx = 2 * (kABytes + kBBytes);   // both CTAs' loads
+    extern __shared__ uint8_t gemm_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem, *sB = smem + NS * kABytes;
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], tmem_full[2], tmem_empty[2];
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int failed;
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint8_t *stage = sB + NS * kBBytes + (warp & 3) * kStageBytes;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pair = blockIdx.x / 2, npairs = gridDim.x / 2;
+    const int halves = (p.M + kBM - 1) / kBM, mtiles = (halves + 1) / 2;
+    const int tiles = mtiles * (p.N / BN), nk = p.K / kBK;
+    const int rblocks = (p.rank + kBK - 1) / kBK;
+    const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order,
+                  *sorted = p.plan + p.l.sorted;
+    const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tmem_full[a], 1);
+            mbar_init(&tmem_empty[a], 8);
+        }
+        failed = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tm.w);
+        prefetch_tmap(&tm.up);
+        prefetch_tmap(&tm.s);
+    }
+    if (warp == 0) {
+        tmem_alloc_pair(&tmem_base, 2 * BN);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    auto free_stage = [&](int g) {
+        const int u = g / NS;
+        if (u >= 1 && !failed && !mbar_wait_bounded(&empty[g % NS], (u - 1) & 1, kWaitLimitNs)) {
+            raise(p.error, PK_DEV_TIMEOUT);
+            failed = 1;
+        }
+        return !failed;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            grid_dep_wait();
+            const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
+            int g = 0;
+            bool ok = true;
+            for (int tile = pair; tile < tiles && ok; tile += npairs) {
+                const int mt = tile % mtiles, m0 = mt * 2 * kBM + (int)rank * kBM;
+                const int n0 = (tile / mtiles) * BN + (int)rank * kHalfB;
+                for (int kb = 0; kb < nk; ++kb, ++g) {
+                    if (!(ok = free_stage(g))) break;
+                    const int s = g % NS;
+                    const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
+                    if (leader) mbar_arrive_expect_tx(&full[s], kStageTx);
+                    tma_load_2d_pair(sB + s * kBBytes, &tm.w, fb, kb * kBK, n0);
+                    tma_load_2d_pair(sA + s * kABytes, rows, fb, kb * kBK, m0);
+                }
+                const int p1 = tile_pair[min(2 * mt + 2, halves)];
+                for (int pr = tile_pair[2 * mt]; pr < p1 && ok; ++pr) {
+                    const int a = pairs[pr].x;
+                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                        if (!(ok = free_stage(g))) break;
+                        const int s = g % NS;
+                        const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
+                        if (leader) mbar_arrive_expect_tx(&full[s], kStageTx);
+                        tma_load_2d_pair(sA + s * kABytes, &tm.s, fb, rb * kBK, m0);
+                        tma_load_3d_pair(sB + s * kBBytes, &tm.up, fb, rb * kBK, n0, a);
+                    }
+                }
+            }
+            if (leader) {   // leave none of the pair's loads in flight
+                for (int s = 0; s < NS; ++s)
+                    if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            constexpr uint32_t idesc = idesc_bf16(2 * kBM, BN);
+            grid_dep_wait();
+            int g = 0, t = 0;
+            auto ready = [&](int s) {
+                if (mbar_wait_cluster_bounded(&full[s], (g / NS) & 1, kWaitLimitNs)) return true;
+                raise(p.error, PK_DEV_TIMEOUT);
+                failed = 1;
+                return false;
+            };
+            for (int tile = pair; tile < tiles && !failed; tile += npairs, ++t) {
+                const int acc = t & 1, use = t >> 1, mt = tile % mtiles;
+                if (use >= 1 &&
+                    !mbar_wait_cluster_bounded(&tmem_empty[acc], (use - 1) & 1, kWaitLimitNs)) {
+                    raise(p.error, PK_DEV_TIMEOUT);
+                    failed = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem + acc * BN;
+                for (int kb = 0; kb < nk; ++kb, ++g) {
+                    const int s = g % NS;
+                    if (!ready(s)) break;
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 16; ++kk)
+                        umma_bf16_pair(d, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32), idesc,
+                                       (kb | kk) != 0);
+                    umma_commit_pair(&empty[s]);
+                }
+                for (int h = 2 * mt; h < min(2 * mt + 2, halves) && !failed; ++h) {
+                    const int p1 = tile_pair[h + 1];
+                    for (int pr = tile_pair[h]; pr < p1 && !failed; ++pr) {
+                        uint32_t off[8];
+                        lanes_off(h & 1 ? 0 : pairs[pr].y, off);
+                        lanes_off(h & 1 ? pairs[pr].y : 0, off + 4);
+                        for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                            const int s = g % NS;
+                            if (!ready(s)) break;
+                            tc_fence_after();
+                            const uint32_t a0 = smem_u32(sA + s * kABytes),
+                                           b0 = smem_u32(sB + s * kBBytes);
+                            const int steps = min(kBK, p.rank - rb * kBK);
+                            for (int kk = 0; kk * 16 < steps; ++kk)
+                                umma_bf16_pair_lanes(d, sw128_desc(a0 + kk * 32),
+                                                     sw128_desc(b0 + kk * 32), idesc, off);
+                            umma_commit_pair(&empty[s]);
+                        }
+                    }
+                }
+                if (failed) break;
+                umma_commit_pair(&tmem_full[acc]);
+            }
+        }
+    } else {
+        // epilogue warps 2..5 of each CTA: its own 128 rows
+        grid_dep_wait();
+        const int q = warp & 3;
+        const uint32_t empty0 = mapa_rank(smem_u32(&tmem_empty[0]), 0),
+                       empty1 = mapa_rank(smem_u32(&tmem_empty[1]), 0);
+        __nv_bfloat16 *C = static_cast<__nv_bfloat16 *>(p.C);
+        const __nv_bfloat16 *R = static_cast<const __nv_bfloat16 *>(p.R);
+        int t = 0;
+        uint4 rv[8], rn[8];
+        for (int tile = pair; tile < tiles; tile += npairs, ++t) {
+            const int acc = t & 1, use = t >> 1;
+            const int m0 = (tile % mtiles) * 2 * kBM + (int)rank * kBM, n0 = (tile / mtiles) * BN;
+            SortedRows rows;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int m = m0 < p.M ? order[m0 + q * 32 + i * 4 + (lane >> 3)] : p.M;
+                rows.row[i] = m < p.M ? m : -1;
+            }
+            if (is_residual(EPI)) load_residual64(rn, rows, n0, R, p.ldr);
+            const bool ok = __all_sync(0xffffffffu,
+                                       mbar_wait_bounded(&tmem_full[acc], use & 1, kWaitLimitNs));
+            if (!ok) {
+                if (lane == 0) raise(p.error, PK_DEV_TIMEOUT);
+                failed = 1;
+                break;
+            }
+            tc_fence_after();
+            if (tile + npairs >= tiles) grid_dep_launch();
+#pragma unroll 1
+            for (int c = 0; c < BN / 64; ++c) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) rv[i] = rn[i];
+                if (is_residual(EPI) && c + 1 < BN / 64)
+                    load_residual64(rn, rows, n0 + (c + 1) * 64, R, p.ldr);
+                epilogue_tile64<EPI>(tmem + acc * BN + ((uint32_t)(q * 32) << 16) + c * 64, rows,
+                                     n0 + c * 64, C, p.ldc, rv,
+                                     static_cast<const __nv_bfloat16 *>(p.bias), p.alpha, stage);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc ? empty1 : empty0);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 2 * BN);
+    }
+}
+
 template <int NT>
 cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
@@ -591,35 +790,59 @@ cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, adapter_shrink_kernel<NT>, p, cluster);
 }
 
-template <int BN, int NS, int EPI>
-int launch_product_t(const AdapterArgs &p, const CUtensorMap (&tm)[2], cudaStream_t s) {
+template <int BN, int NS, bool kPair, int EPI>
+int launch_product_t(const AdapterArgs &p, const AdapterMaps &tm, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr size_t smem = (size_t)NS * (kABytes + BN * kBK * 2) + 4 * kStageBytes + 1024;
-    cudaError_t e = allow_smem(adapter_gemm_kernel<BN, NS, EPI>, smem, done);
+    auto k = kPair ? adapter_gemm_pair_kernel<kPair ? BN : 256, kPair ? NS : 6, EPI>
+                   : adapter_gemm_kernel<kPair ? 64 : BN, kPair ? 6 : NS, EPI>;
+    constexpr size_t smem =
+        (size_t)NS * (kABytes + (kPair ? BN / 2 : BN) * kBK * 2) + 4 * kStageBytes + 1024;
+    cudaError_t e = allow_smem(k, smem, done);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(adapter gemm)");
-    const int tiles = ((p.M + kBM - 1) / kBM) * (p.N / BN), sms = current_sms();
-    e = launch_pdl(adapter_gemm_kernel<BN, NS, EPI>, dim3(tiles < sms ? tiles : sms),
-                   dim3(kAdThreads), smem, s, tm[0], tm[1], p);
-    return cuda_status(e, "adapter_gemm_kernel");
+    const int rows = kPair ? 2 * kBM : kBM, sms = current_sms();
+    const int tiles = ((p.M + rows - 1) / rows) * (p.N / BN);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = kPair ? dim3(2 * (tiles < sms / 2 ? tiles : sms / 2)) : dim3(tiles < sms ? tiles : sms);
+    cfg.blockDim = dim3(kAdThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = 2;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = kPair ? 2 : 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, k, tm, p), "adapter_gemm_kernel");
 }
 
-template <int BN, int NS>
+template <int BN, int NS, bool kPair = false>
 int launch_product(const AdapterArgs &p, cudaStream_t s) {
-    CUtensorMap tm[2];
+    AdapterMaps tm;
+    constexpr uint32_t box_n = kPair ? BN / 2 : BN;
+    const uint64_t padded = (uint64_t)((p.M + kBM - 1) / kBM * kBM), rb = (uint64_t)p.rank * 2;
+    const uint64_t xd[2] = {(uint64_t)p.K, (uint64_t)p.M}, xs[1] = {(uint64_t)p.ldx * 2};
+    const uint64_t pd[2] = {(uint64_t)p.K, padded}, ps[1] = {(uint64_t)p.K * 2};
     const uint64_t wd[2] = {(uint64_t)p.K, (uint64_t)p.N}, ws[1] = {(uint64_t)p.ldw * 2};
-    const uint64_t rb = (uint64_t)p.rank * 2;
+    const uint64_t sd[2] = {(uint64_t)p.rank, padded}, ss[1] = {rb};
     const uint64_t ud[3] = {(uint64_t)p.rank, (uint64_t)p.N, (uint64_t)p.adapters};
     const uint64_t us[2] = {rb, rb * p.N};
-    const uint32_t wbox[2] = {kBK, BN}, ubox[3] = {kBK, BN, 1};
-    int st = encode_tmap(&tm[0], PK_DTYPE_BF16, p.W, 2, wd, ws, wbox);
-    if (st == PK_OK) st = encode_tmap(&tm[1], PK_DTYPE_BF16, p.up, 3, ud, us, ubox);
+    const uint32_t abox[2] = {kBK, kBM}, wbox[2] = {kBK, box_n}, ubox[3] = {kBK, box_n, 1};
+    int st = encode_tmap(&tm.x, PK_DTYPE_BF16, p.x, 2, xd, xs, abox);
+    if (st == PK_OK) st = encode_tmap(&tm.xs, PK_DTYPE_BF16, p.xs, 2, pd, ps, abox);
+    if (st == PK_OK) st = encode_tmap(&tm.w, PK_DTYPE_BF16, p.W, 2, wd, ws, wbox);
+    if (st == PK_OK) st = encode_tmap(&tm.s, PK_DTYPE_BF16, p.s, 2, sd, ss, abox);
+    if (st == PK_OK) st = encode_tmap(&tm.up, PK_DTYPE_BF16, p.up, 3, ud, us, ubox);
     if (st != PK_OK) return st;
     switch (p.epilogue) {
-        case PK_GEMM_SILU: return launch_product_t<BN, NS, PK_GEMM_SILU>(p, tm, s);
-        case PK_GEMM_RESIDUAL: return launch_product_t<BN, NS, PK_GEMM_RESIDUAL>(p, tm, s);
-        case PK_GEMM_RESIDUAL_RELU: return launch_product_t<BN, NS, PK_GEMM_RESIDUAL_RELU>(p, tm, s);
-        case PK_GEMM_BIAS: return launch_product_t<BN, NS, PK_GEMM_BIAS>(p, tm, s);
-        default: return launch_product_t<BN, NS, PK_GEMM_STORE>(p, tm, s);
+        case PK_GEMM_SILU: return launch_product_t<BN, NS, kPair, PK_GEMM_SILU>(p, tm, s);
+        case PK_GEMM_RESIDUAL: return launch_product_t<BN, NS, kPair, PK_GEMM_RESIDUAL>(p, tm, s);
+        case PK_GEMM_RESIDUAL_RELU:
+            return launch_product_t<BN, NS, kPair, PK_GEMM_RESIDUAL_RELU>(p, tm, s);
+        case PK_GEMM_BIAS: return launch_product_t<BN, NS, kPair, PK_GEMM_BIAS>(p, tm, s);
+        default: return launch_product_t<BN, NS, kPair, PK_GEMM_STORE>(p, tm, s);
     }
 }
 
@@ -647,6 +870,13 @@ int launch_adapter_gemm(const AdapterArgs &a, cudaStream_t s) {
     // wide tiles where they still fill the GPU, narrow ones (more CTAs for the
     // weight stream) otherwise
     const int mtiles = (p.M + kBM - 1) / kBM, sms = current_sms();
+    // CTA pairs as in pk_gemm.cu: their tiles fill a wave of pairs, and the waves are
+    // at least 80 % full or K is long
+    const int mt2 = (mtiles + 1) / 2, halves = sms / 2;
+    const int t2 = p.N % 256 == 0 ? mt2 * (p.N / 256) : 0;
+    if (t2 >= halves &&
+        (p.K >= 2048 || 5 * t2 >= 4 * halves * ((t2 + halves - 1) / halves)))
+        return launch_product<256, 6, true>(p, s);
     if (p.N % 256 == 0 && mtiles * (p.N / 256) >= 2 * sms) return launch_product<256, 4>(p, s);
     if (p.N % 128 == 0 && mtiles * (p.N / 128) >= sms) return launch_product<128, 6>(p, s);
     return launch_product<64, 6>(p, s);

@@ -216,9 +216,10 @@ int pk_adapter_plan(const int32_t *ids, int32_t rows, int32_t num_adapters, int3
                                static_cast<cudaStream_t>(stream));
 }
 
-int64_t pk_adapter_workspace(int32_t rows, int32_t rank) {
-    if (rows < 0 || rows > PK_ADAPTER_MAX_ROWS || rank <= 0 || rank > PK_ADAPTER_MAX_RANK) return -1;
-    return ((int64_t)rows + 127) / 128 * 128 * rank * 2;
+int64_t pk_adapter_workspace(int32_t rows, int32_t K, int32_t rank) {
+    if (rows < 0 || rows > PK_ADAPTER_MAX_ROWS || K <= 0 || rank <= 0 || rank > PK_ADAPTER_MAX_RANK)
+        return -1;
+    return ((int64_t)rows + 127) / 128 * 128 * ((int64_t)K + rank) * 2;
 }
 
 int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int32_t M, int32_t N,
@@ -255,7 +256,8 @@ int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int3
     a.ldc = ldc;
     a.ldr = ldr;
     a.C = C;
-    a.s = workspace;
+    a.xs = workspace;   // padded rows of K, then of rank
+    a.s = static_cast<char *>(workspace) + ((int64_t)M + 127) / 128 * 128 * K * 2;
     a.M = M;
     a.N = N;
     a.K = K;

@@ -301,21 +301,22 @@ int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStre
 
 // pk_adapter.cu: plan block, int32 words
 struct AdapterLayout {
-    int64_t tile_pair, order, pairs, words;
+    int64_t tile_pair, order, sorted, pairs, words;
 };
 inline AdapterLayout adapter_layout(int rows, int adapters) {
     AdapterLayout l;
     const int64_t tiles = ((int64_t)rows + 127) / 128;
     l.order = 0;                         // sorted row -> row; `rows` past the last
     l.tile_pair = l.order + tiles * 128; // first pair of each tile
-    l.pairs = (l.tile_pair + tiles + 1 + 1) / 2 * 2;   // adapter, first | end << 16 row in the tile
+    l.sorted = l.tile_pair + tiles + 1;  // 1: the rows' own order is sorted
+    l.pairs = (l.sorted + 1 + 1) / 2 * 2;   // adapter, first | end << 16 row in the tile
     l.words = l.pairs + 2 * (tiles + (adapters < rows ? adapters : rows));
     return l;
 }
 struct AdapterArgs {
     const void *x, *W, *R, *bias, *down, *up;
     int64_t ldx, ldw, ldc, ldr;
-    void *C, *s;
+    void *C, *s, *xs;   // output; S and the rows' copy, sorted and padded to 128
     int M, N, K, epilogue, rank, adapters;
     float alpha;
     const float *scale;

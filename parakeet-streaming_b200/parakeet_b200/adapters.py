@@ -101,7 +101,7 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
                                or bias.dtype is not a.dtype or bias.device != dev):
         raise ValueError(f"the bias epilogue needs a contiguous bf16 bias of {N}")
     with _on(dev):
-        ws = torch.empty(max(lib().pk_adapter_workspace(M, rank), 0), dtype=torch.uint8, device=dev)
+        ws = torch.empty(max(lib().pk_adapter_workspace(M, K, rank), 0), dtype=torch.uint8, device=dev)
         check(lib().pk_adapter_gemm(
             a2.data_ptr(), a2.stride(0), weight.data_ptr(), weight.stride(0), M, N, K,
             out.data_ptr(), N, GEMM_EPILOGUES[epilogue], _ptr(r2),

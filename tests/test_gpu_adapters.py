@@ -80,7 +80,7 @@ def run(d, epilogue="store", alpha=1.0, scaled=True, plan=None, **kw):
     (1, 64, 64, 8, 1), (8, 512, 512, 8, 8), (7, 192, 128, 16, 3), (127, 64, 640, 24, 5),
     (128, 128, 64, 64, 2), (129, 128, 192, 72, 130), (300, 640, 512, 128, 7), (320, 2048, 512, 16, 32),
     (1000, 1024, 1024, 32, 64), (6720, 1024, 1024, 32, 64), (2500, 4096, 256, 16, 300),
-    (4096, 256, 320, 40, 1)])
+    (4096, 256, 320, 40, 1), (2500, 2048, 2048, 16, 40), (2305, 2048, 2048, 72, 5)])
 def test_store(M, N, K, rank, n):
     d = make(M, N, K, rank, n, M + N + K)
     check(run(d), reference(d, "store"))
@@ -88,7 +88,8 @@ def test_store(M, N, K, rank, n):
 
 @pytest.mark.parametrize("epilogue,alpha", [("silu", 1.0), ("residual", 0.5), ("residual_relu", -2.0),
                                             ("bias", 1.0)])
-@pytest.mark.parametrize("M,N,K", [(33, 192, 128), (700, 512, 512), (5000, 2048, 256)])
+@pytest.mark.parametrize("M,N,K", [(33, 192, 128), (700, 512, 512), (5000, 2048, 256),
+                                   (2400, 2048, 2048)])
 def test_epilogues(M, N, K, epilogue, alpha):
     d = make(M, N, K, 16, 9, M + len(epilogue))
     check(run(d, epilogue, alpha), reference(d, epilogue, alpha))
