@@ -41,17 +41,46 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
     for (int i = tid; i < bins; i += blockDim.x) s_bin[i] = 0;
     if (tid == 0) s_base = s_pairs = s_moved = 0;
     __syncthreads();
-    auto bin_of = [&](int r) {
+    // a thread's rows tid, tid + 1024, ...: the first kHeld of them are read once, all
+    // at a time
+    constexpr int kHeld = 8;
+    const int padded = (rows + 31) / 32 * 32;
+    auto bin_of = [&](int r) {   // -1 behind the last row
+        if (r >= rows) return -1;
         const int a = ids[r];
         return a >= 0 && a < adapters ? a : adapters;
     };
-    const int padded = (rows + 31) / 32 * 32;
-    for (int r = tid; r < padded; r += blockDim.x) {
-        const int a = r < rows ? bin_of(r) : -1;
+    int held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = bin_of(tid + i * 1024);
+    // one atomic for a warp whose rows agree, one a row otherwise (a match over the
+    // warp's ids costs more than the conflicts that it saves)
+    auto count = [&](int a) {
+        if (__all_sync(0xffffffffu, a == __shfl_sync(0xffffffffu, a, 0))) {
+            if (lane == 0 && a >= 0) atomicAdd(&s_bin[a], 32);
+        } else if (a >= 0) {
+            atomicAdd(&s_bin[a], 1);
+        }
+    };
+    bool moved = false;   // a row whose adapter is above the next one's
+    auto look = [&](int r, int a) {
+        int next = __shfl_down_sync(0xffffffffu, a, 1);
+        if (lane == 31) next = bin_of(r + 1);
+        moved |= r + 1 < rows && a > next;
         if (r < rows && (ids[r] < -1 || ids[r] >= adapters)) raise(error, PK_DEV_BAD_SLOT);
-        const unsigned same = __match_any_sync(0xffffffffu, a);
-        if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(&s_bin[a], __popc(same));
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (i * 1024 < rows) {
+            count(held[i]);
+            look(tid + i * 1024, held[i]);
+        }
+    for (int r = tid + kHeld * 1024; r < padded; r += 1024) {
+        const int a = bin_of(r);
+        count(a);
+        look(r, a);
     }
+    if (moved) s_moved = 1;
     __syncthreads();
     // each adapter's first sorted row and first pair (it has one for each tile that
     // its rows touch), 1024 adapters at a time
@@ -106,18 +135,24 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
     // tiles that no adapter's rows begin: past all of them
     for (int i = tid; i < tiles + 1; i += blockDim.x)
         if (plan[l.tile_pair + i] == 0x7fffffff) plan[l.tile_pair + i] = s_pairs;
-    for (int r = tid; r < padded; r += blockDim.x) {
-        const int a = r < rows ? bin_of(r) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, a);
-        const int lead = __ffs(same) - 1;
-        int at = 0;
-        if (a >= 0 && lane == lead) at = atomicAdd(&s_bin[a], __popc(same));
-        at = __shfl_sync(0xffffffffu, at, lead) + __popc(same & ((1u << lane) - 1u));
+    const bool resort = s_moved != 0;
+    auto place = [&](int r, int a) {
+        int at = r;
+        if (resort) {
+            if (__all_sync(0xffffffffu, a == __shfl_sync(0xffffffffu, a, 0))) {
+                if (lane == 0 && a >= 0) at = atomicAdd(&s_bin[a], 32);
+                at = __shfl_sync(0xffffffffu, at, 0) + lane;
+            } else if (a >= 0) {
+                at = atomicAdd(&s_bin[a], 1);
+            }
+        }
         if (a >= 0) plan[l.order + at] = r;
-        if (a >= 0 && at != r) s_moved = 1;
-    }
-    __syncthreads();
-    if (tid == 0) plan[l.sorted] = !s_moved;
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (i * 1024 < rows) place(tid + i * 1024, held[i]);
+    for (int r = tid + kHeld * 1024; r < padded; r += 1024) place(r, bin_of(r));
+    if (tid == 0) plan[l.sorted] = !resort;
     for (int r = rows + tid; r < tiles * kTileRows; r += blockDim.x) plan[l.order + r] = rows;
 }
 
@@ -125,8 +160,14 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
 // CTA (rank, tile): K blocks rank, rank + C, ... of the tile's 128 rows.  A stage
 // holds 64 columns of the rows and of the down rows of as many pairs as fit 128
 // columns of S; with more pairs the rows are streamed again for the next ones.
-constexpr int kShThreads = 256, kShStages = 3, kShCols = 128;
-constexpr int kShStage = kTileRows * 128 + kShCols * 128;
+constexpr int kShThreads = 256;
+template <int NT> struct ShrinkShape {
+    static constexpr int kCols = 128;
+    static constexpr int kStage = (kTileRows + kCols) * 128;
+    static constexpr int kStages = 96 * 1024 / kStage;   // two CTAs an SM
+    // the column tiles past a pair's rank read up to 8 NT columns behind the last
+    static constexpr int kSmem = kStages * kStage + NT * 1024 + 1024;
+};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool full) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
@@ -156,10 +197,13 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
 template <int NT>   // 8-column tiles of a pair: rank <= 8 NT
 __global__ void __launch_bounds__(kShThreads, 2)
     adapter_shrink_kernel(const AdapterArgs p, int cluster) {
+    using S = ShrinkShape<NT>;
+    constexpr int kShStage = S::kStage, kShStages = S::kStages, kShCols = S::kCols;
     extern __shared__ uint8_t sh_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(sh_raw) + 1023) & ~uintptr_t(1023));
     __shared__ int s_row[kTileRows];
+    __shared__ int2 s_pair[kTileRows];   // a tile's pairs: a row or more each
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     const int rank = (int)cluster_ctarank(), tile = blockIdx.y, m0 = tile * kTileRows;
     grid_dep_wait();
@@ -167,6 +211,7 @@ __global__ void __launch_bounds__(kShThreads, 2)
     const int32_t *plan = p.plan;
     if (tid < kTileRows) s_row[tid] = plan[p.l.order + m0 + tid];
     const int pair0 = plan[p.l.tile_pair + tile], pair1 = plan[p.l.tile_pair + tile + 1];
+    if (tid < pair1 - pair0) s_pair[tid] = reinterpret_cast<const int2 *>(plan + p.l.pairs)[pair0 + tid];
     const int r = p.rank, per = kShCols / r, nk = p.K / 64;
     const int mine = (nk - rank + cluster - 1) / cluster;   // K blocks of this CTA
     const int batches = max((pair1 - pair0 + per - 1) / per, 1);   // one for the copy at least
@@ -176,32 +221,49 @@ __global__ void __launch_bounds__(kShThreads, 2)
     char *copy = plan[p.l.sorted] ? nullptr : static_cast<char *>(p.xs);
     __syncthreads();
 
-    // this thread's shares of a stage: 4 row chunks
-    const char *src[4];
-    bool live[4];
+    // this thread's shares of a stage: 4 chunks of rows, 4 of down rows (those of the
+    // batch being loaded), at K block `rank`; a block further on is `step` bytes away
+    const char *src[4], *dsrc[4];
+    char *dst[4];
+    uint32_t live = 0, dlive = 0, soff[4];
+    const int64_t step = (int64_t)cluster * 128;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int c = tid + i * kShThreads, row = s_row[c >> 3];
-        live[i] = row < p.M;
-        src[i] = reinterpret_cast<const char *>(x + (int64_t)(live[i] ? row : 0) * p.ldx) +
+        const bool in = row < p.M;
+        live |= (uint32_t)in << i;
+        src[i] = reinterpret_cast<const char *>(x + (int64_t)(in ? row : 0) * p.ldx) + rank * 128 +
                  (c & 7) * 16;
+        dst[i] = copy + ((int64_t)(m0 + (c >> 3)) * p.K + rank * 64) * 2 + (c & 7) * 16;
+        soff[i] = sw128(c >> 3, (c & 7) * 16);
+        dsrc[i] = nullptr;
     }
-    auto load = [&](int it) {
-        const int b = it / mine, kb = rank + (it % mine) * cluster;
-        uint8_t *st = smem + (it % kShStages) * kShStage;
+    int lb = 0, lk = 0;   // batch and block of the next load
+    auto load = [&](int slot) {
+        if (lk == 0) {
+            const int np = min(per, pair1 - pair0 - lb * per);
+            dlive = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = tid + i * kShThreads, col = c >> 3, j = col / r;
+                if (j < np) {
+                    dlive |= 1u << i;
+                    dsrc[i] = reinterpret_cast<const char *>(
+                                  down + ((int64_t)s_pair[lb * per + j].x * r + col - j * r) * p.K) +
+                              rank * 128 + (c & 7) * 16;
+                }
+            }
+        }
+        const uint32_t st = smem_u32(smem + slot * kShStage);
+        const int64_t at = lk * step;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int c = tid + i * kShThreads;
-            cp_async16(smem_u32(st) + sw128(c >> 3, (c & 7) * 16), src[i] + (int64_t)kb * 128, live[i]);
+            cp_async16(st + soff[i], src[i] + at, live >> i & 1);
+            if (dlive >> i & 1) cp_async16(st + kTileRows * 128 + soff[i], dsrc[i] + at, true);
         }
-        const int np = min(per, pair1 - pair0 - b * per);
-        for (int c = tid; c < np * r * 8; c += kShThreads) {
-            const int col = c >> 3, j = col / r, q = col - j * r;
-            const int a = plan[p.l.pairs + 2 * (pair0 + b * per + j)];
-            cp_async16(smem_u32(st) + kTileRows * 128 + sw128(col, (c & 7) * 16),
-                       reinterpret_cast<const char *>(down + ((int64_t)a * r + q) * p.K) +
-                           (int64_t)kb * 128 + (c & 7) * 16,
-                       true);
+        if (++lk == mine) {
+            lk = 0;
+            ++lb;
         }
     };
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
@@ -211,49 +273,46 @@ __global__ void __launch_bounds__(kShThreads, 2)
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-    const int total = batches * max(mine, 0);
+    const int total = batches * mine;
     const int row_lo = warp * 16 + (lane >> 2);
     for (int it = 0; it < kShStages - 1; ++it) {
         if (it < total) load(it);
         commit();
     }
+    // ldmatrix offsets: every row index below is lane & 7 modulo 8
+    const uint32_t a_row = (warp * 16 + (lane & 15)) * 128, b_row = (lane & 7) * 128;
+    const uint32_t a_sw = (lane >> 4) ^ (lane & 7), b_sw = (lane >> 3) ^ (lane & 7);
+    int b = 0, kb = 0, slot = 0;
     for (int it = 0; it < total; ++it) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kShStages - 2) : "memory");
         __syncthreads();
-        if (it + kShStages - 1 < total) load(it + kShStages - 1);
+        if (it + kShStages - 1 < total) load(slot == 0 ? kShStages - 1 : slot - 1);
         commit();
-        const uint32_t sa = smem_u32(smem + (it % kShStages) * kShStage);
-        const uint32_t sb = sa + kTileRows * 128;
-        const int b = it / mine;
+        const uint8_t *st = smem + slot * kShStage;
+        const uint32_t sa = smem_u32(st), sb = sa + kTileRows * 128;
         if (copy && b == 0) {
-            const uint8_t *st = smem + (it % kShStages) * kShStage;
-            const int64_t kb = rank + it * cluster;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = tid + i * kShThreads, row = c >> 3;
-                *reinterpret_cast<uint4 *>(copy + ((int64_t)(m0 + row) * p.K + kb * 64) * 2 +
-                                           (c & 7) * 16) =
-                    *reinterpret_cast<const uint4 *>(st + sw128(row, (c & 7) * 16));
-            }
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4 *>(dst[i] + kb * step) =
+                    *reinterpret_cast<const uint4 *>(st + soff[i]);
         }
         const int np = min(per, pair1 - pair0 - b * per);
         uint32_t a[4][4];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-            ldsm4a(sa + sw128(warp * 16 + (lane & 15), ks * 32 + (lane >> 4) * 16), a[ks]);
+        for (int ks = 0; ks < 4; ++ks) ldsm4a(sa + a_row + ((a_sw ^ (ks * 2)) << 4), a[ks]);
         for (int j = 0; j < np; ++j) {
-            const int range = plan[p.l.pairs + 2 * (pair0 + b * per + j) + 1];
+            const int range = s_pair[b * per + j].y;
             const int lo = range & 0xffff, hi = range >> 16;
             if (hi <= warp * 16 || lo >= warp * 16 + 16) continue;
+            const uint32_t bj = sb + b_row + j * r * 128;
             const bool in0 = row_lo >= lo && row_lo < hi, in1 = row_lo + 8 >= lo && row_lo + 8 < hi;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                if (n * 8 >= r) break;
                 float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k2 = 0; k2 < 2; ++k2) {   // 32 columns of K: 4 matrices
                     uint32_t bm[4];
-                    ldsm4a(sb + sw128(j * r + n * 8 + (lane & 7), k2 * 64 + (lane >> 3) * 16), bm);
+                    ldsm4a(bj + n * 1024 + ((b_sw ^ (k2 * 4)) << 4), bm);
                     mma_16816(t, a[2 * k2], bm[0], bm[1]);
                     mma_16816(t, a[2 * k2 + 1], bm[2], bm[3]);
                 }
@@ -267,6 +326,11 @@ __global__ void __launch_bounds__(kShThreads, 2)
                     acc[n][3] += t[3];
                 }
             }
+        }
+        slot = slot + 1 == kShStages ? 0 : slot + 1;
+        if (++kb == mine) {
+            kb = 0;
+            ++b;
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -768,13 +832,15 @@ __global__ void __launch_bounds__(kAdThreads, 1)
 template <int NT>
 cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr size_t smem = kShStages * kShStage + 1024;
+    constexpr size_t smem = ShrinkShape<NT>::kSmem;
     cudaError_t e = allow_smem(adapter_shrink_kernel<NT>, smem, done);
     if (e != cudaSuccess) return e;
-    int cluster = 1;   // CTAs over K, a block of 64 or more each
-    while (cluster < 8 && 2 * cluster <= p.K / 64) cluster *= 2;
+    // CTAs over K, a block of 64 or more each, while the grid is below a wave
+    const int tiles = (p.M + kTileRows - 1) / kTileRows;
+    int cluster = 1;
+    while (cluster < 8 && 2 * cluster <= p.K / 64 && tiles * cluster < 2 * current_sms()) cluster *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster, (p.M + kTileRows - 1) / kTileRows);
+    cfg.gridDim = dim3(cluster, tiles);
     cfg.blockDim = dim3(kShThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
