@@ -53,6 +53,18 @@ def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
     return AdapterPlan(ids, rows, num_adapters, block)
 
 
+def _operand(t, shape, dtype, dev, name):
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be a contiguous {dtype} {shape} tensor on {dev}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _plain_rows(t):
+    """[rows, width] that ops._rows would leave as it is."""
+    return (t.dim() == 2 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+            and t.stride(0) >= t.shape[1])
+
+
 def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
                  plan: AdapterPlan, epilogue: str = "store", residual: torch.Tensor | None = None,
                  alpha: float = 1.0, bias: torch.Tensor | None = None,
@@ -64,51 +76,52 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     a [..., K], weight [N, K], down [num_adapters, rank, K], up [num_adapters, N,
     rank], bf16; K and N multiples of 64, rank a multiple of 8 up to 128; scale
     float32 [num_adapters] or None.  The plan's rows are those of ``a`` flattened."""
-    if not gemm_supported(a, weight):
-        raise ValueError("adapter_gemm needs bf16 CUDA operands, K and N multiples of 64, and an "
-                         "aligned weight")
     dev = a.device
+    if not gemm_supported(a, weight) or weight.device != dev:
+        raise ValueError("adapter_gemm needs bf16 operands on one CUDA device, K and N multiples "
+                         "of 64, and an aligned weight")
     N, K = weight.shape
-    n, rank = plan.num_adapters, down.shape[1] if down.dim() == 3 else 0
-    for t, shape, name in ((down, (n, rank, K), "down"), (up, (n, N, rank), "up")):
-        if t.shape != shape or t.dtype is not torch.bfloat16 or not t.is_contiguous() or \
-                t.device != dev:
-            raise ValueError(f"{name} must be a contiguous bf16 {shape} tensor on {dev}, got "
-                             f"{tuple(t.shape)} {t.dtype}")
-    if weight.device != dev or plan.ids.device != dev:
-        raise ValueError("operands on different devices")
-    if scale is not None and (scale.dtype is not torch.float32 or scale.shape != (n,)
-                              or not scale.is_contiguous() or scale.device != dev):
-        raise ValueError(f"scale must be a contiguous float32 [{n}] tensor on {dev}")
-    a2 = _rows(a, K)
+    n = plan.num_adapters
+    rank = down.shape[1] if down.dim() == 3 else 0
+    _operand(down, (n, rank, K), torch.bfloat16, dev, "down")
+    _operand(up, (n, N, rank), torch.bfloat16, dev, "up")
+    if scale is not None:
+        _operand(scale, (n,), torch.float32, dev, "scale")
+    a2 = a if _plain_rows(a) else _rows(a, K)
     M = a2.shape[0]
-    if plan.rows != M:
-        raise ValueError(f"the plan is for {plan.rows} rows, a has {M}")
+    if plan.rows != M or plan.ids.device != dev:
+        raise ValueError(f"the plan is for {plan.rows} rows on {plan.ids.device}, a has {M} on {dev}")
     if out is None:
-        out = torch.empty((M, N), dtype=a.dtype, device=dev)
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
     elif not out.is_contiguous() or out.numel() != M * N or out.dtype is not a.dtype or \
             out.device != dev:
         raise ValueError("out must be a contiguous [M, N] tensor of a's type and device")
-    if epilogue not in GEMM_EPILOGUES:
+    epi = GEMM_EPILOGUES.get(epilogue)
+    if epi is None:
         raise ValueError(f"epilogue {epilogue!r}: one of {sorted(GEMM_EPILOGUES)}")
-    r2 = None
-    if epilogue in ("residual", "residual_relu"):
+    r, ldr, b = None, 0, None
+    if epilogue == "residual" or epilogue == "residual_relu":
         if residual is None or residual.dtype is not a.dtype or residual.device != dev or \
                 residual.shape[-1] != N or residual.numel() != M * N:
             raise ValueError(f"the residual epilogue needs a bf16 residual of {M} x {N}")
-        r2 = _rows(residual, N)
-    if epilogue == "bias" and (bias is None or not bias.is_contiguous() or bias.shape != (N,)
-                               or bias.dtype is not a.dtype or bias.device != dev):
-        raise ValueError(f"the bias epilogue needs a contiguous bf16 bias of {N}")
+        r2 = residual if _plain_rows(residual) else _rows(residual, N)
+        r, ldr = r2.data_ptr(), r2.stride(0)
+    elif epilogue == "bias":
+        if bias is None:
+            raise ValueError("the bias epilogue needs a bias")
+        _operand(bias, (N,), a.dtype, dev, "bias")
+        b = bias.data_ptr()
     with _on(dev):
-        ws = torch.empty(max(lib().pk_adapter_workspace(M, K, rank), 0), dtype=torch.uint8, device=dev)
+        size = lib().pk_adapter_workspace(M, K, rank)
+        if size < 0:
+            raise ValueError(f"rank {rank}: a multiple of 8 up to 128")
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
         check(lib().pk_adapter_gemm(
             a2.data_ptr(), a2.stride(0), weight.data_ptr(), weight.stride(0), M, N, K,
-            out.data_ptr(), N, GEMM_EPILOGUES[epilogue], _ptr(r2),
-            r2.stride(0) if r2 is not None else 0, _ptr(bias), float(alpha), down.data_ptr(),
-            up.data_ptr(), rank, n, _ptr(scale), plan.ids.data_ptr(), plan.block.data_ptr(),
-            ws.data_ptr(), _error_word(dev).data_ptr(), _stream(dev)), "pk_adapter_gemm")
-    return out.reshape(*a.shape[:-1], N)
+            out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(), up.data_ptr(), rank, n,
+            _ptr(scale), plan.ids.data_ptr(), plan.block.data_ptr(), ws.data_ptr(),
+            _error_word(dev).data_ptr(), _stream(dev)), "pk_adapter_gemm")
+    return out if a.dim() == 2 and out.dim() == 2 else out.reshape(*a.shape[:-1], N)
 
 
 __all__ = ["AdapterPlan", "adapter_gemm", "adapter_plan"]

@@ -23,7 +23,10 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream as a raw handle (torch.cuda.current_stream
+    builds an object for it, 2 us of a call)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def layer_norm(x: torch.Tensor, ln, ln2=None):

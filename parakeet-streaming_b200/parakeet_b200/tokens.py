@@ -34,8 +34,11 @@ def _on(device):
     """The device's context where another one is current: launches and library
     attributes go by the current device."""
     if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 class TokenStep:
@@ -58,8 +61,7 @@ class TokenStep:
         self._at = at
 
     def _view(self, which, n):
-        a = self._at[which]
-        return self.block[a:a + n]
+        return self.block.narrow(0, self._at[which], n)
 
     @property
     def row_start(self):
@@ -153,11 +155,13 @@ class TokenKVPool:
 
     # ------------------------------------------------------------ checks
     def _i32(self, t, n, name):
+        """The length of an int32 vector, which has to be ``n`` where given."""
         if t.dtype is not torch.int32 or t.device != self.device:
             raise TypeError(f"{name}: expected int32 on {self.device}, got {t.dtype} on {t.device}")
         if t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
             raise ValueError(f"{name}: expected a contiguous [{'n' if n is None else n}] tensor, "
                              f"got {tuple(t.shape)}")
+        return t.shape[0]
 
     def _step(self, step, ending=False):
         if step.pool is not self:
@@ -171,13 +175,15 @@ class TokenKVPool:
         """t [..., rows, heads * head_dim] or [..., rows, heads, head_dim] as the latter."""
         if t.dtype is not self.dtype or t.device != self.device:
             raise TypeError(f"{name}: expected {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
-        if t.shape[-1] != self.head_dim or t.dim() < 3 or t.shape[-2] != heads:
-            if t.shape[-1] != heads * self.head_dim or t.dim() < 2:
+        shape = t.shape
+        if len(shape) < 3 or shape[-1] != self.head_dim or shape[-2] != heads:
+            if len(shape) < 2 or shape[-1] != heads * self.head_dim:
                 raise ValueError(f"{name}: expected [..., {rows}, {heads}, {self.head_dim}], got "
-                                 f"{tuple(t.shape)}")
+                                 f"{tuple(shape)}")
             t = t.unflatten(-1, (heads, self.head_dim))
-        if t.shape[-3] != rows:
-            raise ValueError(f"{name}: {t.shape[-3]} rows, the step has {rows}")
+            shape = t.shape
+        if shape[-3] != rows:
+            raise ValueError(f"{name}: {shape[-3]} rows, the step has {rows}")
         if t.stride(-1) != 1:
             raise ValueError(f"{name}: last dimension must be contiguous")
         return t
@@ -207,8 +213,7 @@ class TokenKVPool:
         A request that cannot be served (a slot out of range or named twice, a
         count out of range, no room or no pages left) sets its bit of ``error``
         and is left out: context -1, its rows not appended nor attended."""
-        self._i32(slots, None, "slots")
-        B = slots.shape[0]
+        B = self._i32(slots, None, "slots")
         self._i32(counts, B, "counts")
         trees = parents is not None
         if trees:
@@ -250,12 +255,11 @@ class TokenKVPool:
     def truncate(self, slots: torch.Tensor, lengths: torch.Tensor):
         """Cut requests to ``lengths[b]`` tokens (0 releases them); the pages
         past the end go back on the stack."""
-        self._i32(slots, None, "slots")
-        self._i32(lengths, slots.shape[0], "lengths")
+        n = self._i32(slots, None, "slots")
+        self._i32(lengths, n, "lengths")
         with _on(self.device):
-            check(lib().pk_token_truncate(self._h, slots.data_ptr(), lengths.data_ptr(),
-                                          slots.shape[0], _stream(self.device)),
-                  "pk_token_truncate")
+            check(lib().pk_token_truncate(self._h, slots.data_ptr(), lengths.data_ptr(), n,
+                                          _stream(self.device)), "pk_token_truncate")
 
     def read_error(self) -> int:
         return int(self.error.item())
@@ -267,15 +271,14 @@ class TokenKVPool:
         strides (slices of a fused projection)."""
         self._step(step)
         H = self.num_kv_heads
-        key, value = (self._rows(t, H, step.rows, n) for t, n in ((key, "key"), (value, "value")))
-        if key.dim() == 3:
-            key, value = key.unsqueeze(0), value.unsqueeze(0)
-        if key.dim() != 4 or value.shape != key.shape or value.stride() != key.stride():
+        key, value = self._rows(key, H, step.rows, "key"), self._rows(value, H, step.rows, "value")
+        strides = key.stride()
+        if len(strides) > 4 or value.shape != key.shape or value.stride() != strides:
             raise ValueError("key and value must have the same shape and strides")
+        nl, ls = (key.shape[0], strides[0]) if len(strides) == 4 else (1, 0)
         with _on(self.device):
-            check(lib().pk_token_append(self._h, layer, key.shape[0], key.data_ptr(),
-                                        value.data_ptr(), key.stride(0), key.stride(1),
-                                        key.stride(2), step.batch, step.rows, step.trees,
+            check(lib().pk_token_append(self._h, layer, nl, key.data_ptr(), value.data_ptr(), ls,
+                                        strides[-3], strides[-2], step.batch, step.rows, step.trees,
                                         step.block.data_ptr(), _stream(self.device)),
                   "pk_token_append")
 
@@ -292,17 +295,20 @@ class TokenKVPool:
             raise ValueError(f"query: one layer's rows, got {tuple(query.shape)}")
         if out is None:
             out = torch.empty(query.shape, dtype=self.dtype, device=self.device)
+            ors, ohs = self.num_heads * self.head_dim, self.head_dim
         elif out.shape != query.shape:
             raise ValueError(f"out: expected {tuple(query.shape)}, got {tuple(out.shape)}")
-        o = self._rows(out, self.num_heads, step.rows, "out")
+        else:
+            ors, ohs, _ = self._rows(out, self.num_heads, step.rows, "out").stride()
+        qrs, qhs, _ = q.stride()
         B, rows = step.batch, step.rows
         with _on(self.device):
             need = lib().pk_token_attention_workspace(self._h, B, rows)
             ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None
             check(lib().pk_token_attention(
-                self._h, layer, q.data_ptr(), q.stride(0), q.stride(1),
+                self._h, layer, q.data_ptr(), qrs, qhs,
                 self.head_dim ** -0.5 if scale is None else scale, B, rows, step.trees,
-                step.block.data_ptr(), o.data_ptr(), o.stride(0), o.stride(1), _ptr(ws),
+                step.block.data_ptr(), out.data_ptr(), ors, ohs, _ptr(ws),
                 _stream(self.device)), "pk_token_attention")
         return out
 
