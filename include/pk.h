@@ -517,20 +517,14 @@ int pk_token_reset(pk_token_kv *kv, const int32_t *init_order, void *stream);
  *   PK_TOK_SLOT_MAP   [rows]   page * page_size + row in the page, -1: none
  *   PK_TOK_MASK       [rows]   int64 bits of the row's ancestors and itself
  *                              (only with parents)
- * The other entries are the library's. */
+ * The rest of the block is the library's. */
 #define PK_TOK_ROW_START 0
 #define PK_TOK_CONTEXT 1
-#define PK_TOK_SLOT 2
-#define PK_TOK_UNIT_START 3
-#define PK_TOK_PART_START 4
-#define PK_TOK_TAKE 5
-#define PK_TOK_HELD 6
-#define PK_TOK_REQUEST 7
-#define PK_TOK_POSITION 8
-#define PK_TOK_SLOT_MAP 9
-#define PK_TOK_UNITS 10
-#define PK_TOK_MASK 11
-#define PK_TOK_OFFSETS 12
+#define PK_TOK_REQUEST 2
+#define PK_TOK_POSITION 3
+#define PK_TOK_SLOT_MAP 4
+#define PK_TOK_MASK 5
+#define PK_TOK_OFFSETS 6
 #define PK_TOK_MAX_TREE 64      /* most nodes of one tree                     */
 #define PK_TOK_MAX_BATCH 65536  /* most requests of one step                  */
 int64_t pk_token_step_words(const pk_token_kv *kv, int32_t batch, int32_t rows, int32_t trees,

@@ -54,13 +54,12 @@ int pk_token_kv_create(const pk_token_kv_desc *desc, pk_token_kv **out) {
     kv->esize = d.dtype == PK_DTYPE_BF16 ? 2 : 4;
     kv->group = d.num_heads / d.num_kv_heads;
     while ((1 << kv->ps_shift) < d.page_size) ++kv->ps_shift;
-    // two waves of two CTAs an SM
-    kv->target = (4 * (int64_t)current_sms() + d.num_kv_heads - 1) / d.num_kv_heads;
+    kv->sms = current_sms();
     if (d.dtype == PK_DTYPE_BF16) {
         const uint64_t row = (uint64_t)d.head_dim * 2;
         int st = encode_tmap_3d(&kv->kv_map, d.dtype, d.kv, d.head_dim, d.page_size,
                                 (uint64_t)planes, row, row * d.page_size, 64,
-                                d.page_size < kTokTile ? d.page_size : kTokTile, 1);
+                                d.page_size < 64 ? d.page_size : 64, 1);
         if (st != PK_OK) {
             free(kv);
             return st;
@@ -87,15 +86,9 @@ int64_t pk_token_step_words(const pk_token_kv *kv, int32_t batch, int32_t rows, 
     if (offsets) {
         offsets[PK_TOK_ROW_START] = l.row_start;
         offsets[PK_TOK_CONTEXT] = l.context;
-        offsets[PK_TOK_SLOT] = l.slot;
-        offsets[PK_TOK_UNIT_START] = l.unit_start;
-        offsets[PK_TOK_PART_START] = l.part_start;
-        offsets[PK_TOK_TAKE] = l.take;
-        offsets[PK_TOK_HELD] = l.held;
         offsets[PK_TOK_REQUEST] = l.request;
         offsets[PK_TOK_POSITION] = l.position;
         offsets[PK_TOK_SLOT_MAP] = l.slot_map;
-        offsets[PK_TOK_UNITS] = l.units;
         offsets[PK_TOK_MASK] = l.mask;
     }
     return l.words;

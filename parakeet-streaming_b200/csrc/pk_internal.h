@@ -214,41 +214,41 @@ struct pk_token_kv {
     CUtensorMap kv_map;  // bf16 pools: {head_dim, page_size, pages*layers*2*kv_heads}, boxes of
                          // 64 columns x min(page_size, 64) rows, 128B-swizzled
     int ps_shift, esize, group;
-    int64_t target;      // attention units per K/V head that a step aims at
+    int sms;
 };
 
 namespace pk {
 
-// Key tokens of one attention tile.
-constexpr int kTokTile = 64;
-
-// Step block, int32 words: header, then arrays at these offsets.
-enum TokHeader { kTokChunk = 0, kTokUnits, kTokRows, kTokFree, kTokHeaderWords = 16 };
-struct TokLayout {
-    int64_t row_start, context, slot, unit_start, part_start, take, held, request, position,
-        slot_map, units, mask, words;
+// How a step's rows are attended.  A row tile is up to `rows` query rows (token x
+// group) of one request and K/V head, a key tile `keys` of its keys; `ctas` CTAs
+// share the work.
+struct TokShape {
+    int rows, keys, ctas;
 };
-// One attention unit (a row tile of one request over a range of key tiles), 8
-// words, for every K/V head: slot, first row, tokens, context, row tile, first
-// and end key tile, partial (-1: the only range of its rows).
-constexpr int kTokUnitWords = 8;
-
-// Query rows (token x group) of one attention tile: the narrowest of 16, 32 and
-// 64 that holds an average request, since a tile's K/V is read once per row tile.
-inline int tok_tile_rows(const pk_token_kv *kv, int batch, int rows) {
-    if (kv->d.dtype == PK_DTYPE_F32) return 16;
+// bf16: the narrowest row tile that holds an average request, since a request's K/V
+// is read once per row tile - 16 or 32 rows by mma.sync (two CTAs an SM), 128 by
+// tcgen05 (one).  float32: 16.
+inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
-    return mean <= 16 ? 16 : (mean <= 32 ? 32 : 64);
+    if (kv->d.dtype == PK_DTYPE_F32 || mean <= 16) return {16, 64, 2 * kv->sms};
+    if (mean <= 32) return {32, 64, 2 * kv->sms};
+    return {128, 128, kv->sms};
 }
-// Most units of a step: the aimed-at number plus one for each row tile's last range.
-inline int64_t tok_max_units(const pk_token_kv *kv, int batch, int rows) {
-    const int bm = tok_tile_rows(kv, batch, rows);
-    return kv->target + ((int64_t)rows * kv->group) / bm + batch;
-}
-// Ranges of row tiles that have more than one: at most twice the aimed-at number.
-inline int64_t tok_max_parts(const pk_token_kv *kv) { return 2 * kv->target; }
-// Key tiles below which a range is not split.
-constexpr int kTokMinChunk = 8;
+// Keys that one CTA takes before a request's keys are split over several.
+constexpr int kTokMinKeys = 512;
+
+// Step block, int32 words: header, then arrays at these offsets.  The step's work
+// is a line of key tiles, request by request, K/V head by head, row tile by row
+// tile; CTA c takes tiles [c * share, (c + 1) * share), whatever they belong to, so
+// that every CTA has the same number however the lengths are spread (share 0: a
+// row tile each).
+enum TokHeader { kTokShare = 0, kTokRows, kTokFree, kTokHeaderWords = 16 };
+struct TokLayout {
+    // work: int64 first tile (share 0: row tile) of each request; first: the request
+    // that each CTA begins in (-1: no work); take: first new page; held: pages before
+    int64_t row_start, context, slot, work, first, take, held, request, position, slot_map, mask,
+        words;
+};
 inline TokLayout tok_layout(const pk_token_kv *kv, int batch, int rows, int trees) {
     TokLayout l;
     int64_t o = kTokHeaderWords;
@@ -257,19 +257,17 @@ inline TokLayout tok_layout(const pk_token_kv *kv, int batch, int rows, int tree
         o += n;
         return at;
     };
+    l.work = take(2 * ((int64_t)batch + 1));
+    l.mask = take(trees ? 2 * (int64_t)rows : 0);
     l.row_start = take(batch + 1);
     l.context = take(batch);
     l.slot = take(batch);
-    l.unit_start = take(batch + 1);
-    l.part_start = take(batch + 1);
+    l.first = take(2 * kv->sms);
     l.take = take(batch + 1);
     l.held = take(batch);
     l.request = take(rows);
     l.position = take(rows);
     l.slot_map = take(rows);
-    o = (o + 3) / 4 * 4;
-    l.units = take(tok_max_units(kv, batch, rows) * kTokUnitWords);
-    l.mask = take(trees ? 2 * (int64_t)rows : 0);
     l.words = o;
     return l;
 }
@@ -296,6 +294,23 @@ struct TreeAttnArgs {
     const int32_t *step;
     float *ws;
 };
+struct TreeParams {
+    const int32_t *step, *table;
+    TokLayout l;
+    TokShape shape;
+    int table_width, num_pages, num_layers, layer, kv_heads, group, ps_shift, trees;
+    int batch, rows, heads;
+    const void *q, *kv;
+    void *out;
+    int64_t q_rs, q_hs, o_rs, o_hs;
+    float scale_log2;
+    // partial results of row tiles that CTAs share, two a CTA: outputs [part][row][dim],
+    // (maximum, sum) pairs
+    float *ws_o, *ws_ml;
+    int32_t *error;
+};
+// pk_tree_attn_tc.cu: row tiles of 128
+cudaError_t launch_tree_tc(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s);
 int64_t tree_attn_workspace(const pk_token_kv *kv, int batch, int rows);
 int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStream_t s);
 

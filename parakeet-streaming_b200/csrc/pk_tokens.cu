@@ -7,9 +7,9 @@
 //   node j's cache row = table[(len + j) / page_size] * page_size + (len + j) % page_size
 //   mask(j) = bit j | mask(parent(j)),  position(j) = len + |ancestors of j|
 //
-// The prefix sums over the batch (rows, pages, attention units) need every
-// request, so one CTA makes them; what they place (rows, table entries, unit
-// records) is written by that CTA too while there is little of it, and by a grid
+// The prefix sums over the batch (rows, pages, attention tiles) need every
+// request, so one CTA makes them; what they place (rows, table entries, where each
+// attention CTA begins) is written by that CTA too while there is little of it, and by a grid
 // otherwise.  Masks come by doubling over the ancestors (mask |= mask[jump],
 // jump = jump[jump]): 6 rounds of warp shuffles for 64 nodes, whatever the depth.
 // Everything is integer work bound by latency: a few thousand rows are written
@@ -29,8 +29,8 @@ constexpr int kOneCtaRows = 2048;
 struct TokParams {
     pk_token_kv_desc d;
     TokLayout l;
-    int ps_shift, group, tile_rows, batch, rows;
-    int64_t target, max_units;
+    TokShape shape;
+    int ps_shift, group, kv_heads, batch, rows;
     const int32_t *slots, *counts, *parents;
     int32_t *step;
 };
@@ -96,12 +96,16 @@ __device__ __forceinline__ int page_of(const TokParams &p, int slot, int held, i
 __device__ void begin_plan(const TokParams &p) {
     __shared__ int64_t s_scan[33];
     __shared__ unsigned long long s_take;
+    __shared__ int s_longest;
     const pk_token_kv_desc &d = p.d;
     int32_t *st = p.step;
     const int nk = (p.batch + blockDim.x - 1) / blockDim.x;
     const int b0 = threadIdx.x * nk, b1 = min(b0 + nk, p.batch);
     const int free_n = *d.free_count;
-    if (threadIdx.x == 0) s_take = 0;
+    if (threadIdx.x == 0) {
+        s_take = 0;
+        s_longest = 0;
+    }
     mark_slots(d, p.slots, p.batch);
 
     // rows; which requests can be served but for their pages
@@ -145,57 +149,63 @@ __device__ void begin_plan(const TokParams &p) {
 
     // pages, in batch order: requests past the end of the stack are left out
     int64_t first = block_exclusive_sum64(takes, total, s_scan);
-    int64_t tiles = 0, taken = 0;
-    const int bm = p.tile_rows;
+    int64_t tiles = 0, items = 0, taken = 0;
+    int longest = 0;
+    auto shape_of = [&](int b, int &nr, int &kt) {   // row tiles and key tiles
+        const int ctx = st[p.l.context + b], n = max(p.counts[b], 0);
+        nr = ctx >= 0 ? (int)(((int64_t)n * p.group + p.shape.rows - 1) / p.shape.rows) : 0;
+        kt = nr ? (ctx + n + p.shape.keys - 1) / p.shape.keys : 0;
+    };
     for (int b = b0; b < b1; ++b) {
-        int ctx = st[p.l.context + b];
-        const int held = st[p.l.held + b], n = max(p.counts[b], 0);
+        const int ctx = st[p.l.context + b], held = st[p.l.held + b], n = max(p.counts[b], 0);
         const int take = ctx < 0 ? 0 : max(ceil_shift((int64_t)ctx + n, p.ps_shift) - held, 0);
         st[p.l.take + b] = (int)min(first, (int64_t)0x7fffffff);
         if (take > 0 && first + take > free_n) {
             raise(d.error, PK_DEV_POOL_EXHAUSTED);
-            st[p.l.context + b] = ctx = -1;
+            st[p.l.context + b] = -1;
         } else if (take > 0) {
             taken += take;
             d.held[st[p.l.slot + b]] = held + take;
         }
         first += take;
-        if (ctx >= 0 && n > 0)
-            tiles += ((int64_t)n * p.group + bm - 1) / bm *
-                     (((int64_t)ctx + n + kTokTile - 1) / kTokTile);
+        int nr, kt;
+        shape_of(b, nr, kt);
+        tiles += (int64_t)nr * kt;
+        items += nr;
+        longest = max(longest, kt);
     }
     if (taken) atomicAdd(&s_take, (unsigned long long)taken);
+    if (longest) atomicMax(&s_longest, longest);
 
-    // attention units: ranges of `chunk` key tiles, so that there are about
-    // `target` of them per K/V head
-    block_exclusive_sum64(tiles, total, s_scan);
-    const int chunk = (int)max((total + p.target - 1) / p.target, (int64_t)kTokMinChunk);
-    int64_t units = 0;
-    auto ranges = [&](int b, int64_t &rt, int64_t &ns) {
-        const int ctx = st[p.l.context + b], n = max(p.counts[b], 0);
-        rt = ctx >= 0 && n > 0 ? ((int64_t)n * p.group + bm - 1) / bm : 0;
-        ns = rt ? (((int64_t)ctx + n + kTokTile - 1) / kTokTile + chunk - 1) / chunk : 0;
-    };
-    for (int b = b0; b < b1; ++b) {
-        int64_t rt, ns;
-        ranges(b, rt, ns);
-        units += rt * ns + (ns > 1 ? (rt * ns) << 32 : 0);   // units low, partials high
+    // the attention's line of tiles: an equal share of it a CTA, but kTokMinKeys at
+    // least; a row tile each where there are no more of them than CTAs and none is
+    // longer than that
+    block_exclusive_sum64(items, total, s_scan);
+    const int64_t all_items = total * p.kv_heads;
+    int64_t before = block_exclusive_sum64(tiles, total, s_scan);
+    const int64_t all = total * p.kv_heads;
+    const int least = kTokMinKeys / p.shape.keys;
+    int64_t share = (all + p.shape.ctas - 1) / p.shape.ctas;
+    if (share < least) share = least;
+    if (all_items <= p.shape.ctas && s_longest <= least) {
+        share = 0;
+        before = block_exclusive_sum64(items, total, s_scan);
     }
-    int64_t u = block_exclusive_sum64(units, total, s_scan);
+    int64_t *work = reinterpret_cast<int64_t *>(st + p.l.work);
     for (int b = b0; b < b1; ++b) {
-        int64_t rt, ns;
-        ranges(b, rt, ns);
-        st[p.l.unit_start + b] = (int)(u & 0xffffffff);
-        st[p.l.part_start + b] = (int)(u >> 32);
-        u += rt * ns + (ns > 1 ? (rt * ns) << 32 : 0);
+        work[b] = before * p.kv_heads;
+        int nr, kt;
+        shape_of(b, nr, kt);
+        before += share ? (int64_t)nr * kt : nr;
     }
     if (threadIdx.x == 0) {
-        st[kTokChunk] = chunk;
-        st[kTokUnits] = (int)min(total & 0xffffffff, p.max_units);
-        st[p.l.unit_start + p.batch] = (int)(total & 0xffffffff);
-        st[p.l.part_start + p.batch] = (int)(total >> 32);
+        work[p.batch] = total * p.kv_heads;
+        st[kTokShare] = (int)min(share, (int64_t)0x7fffffff);
         *d.free_count = free_n - (int)s_take;
     }
+    // CTAs behind the last tile
+    const int64_t unit = share ? share : 1, used = (total * p.kv_heads + unit - 1) / unit;
+    for (int64_t c = used + threadIdx.x; c < p.shape.ctas; c += blockDim.x) st[p.l.first + c] = -1;
 }
 
 // One value of a 64-entry array held two entries a lane (j, j + 32).
@@ -276,12 +286,14 @@ __device__ void tree_rows(const TokParams &p, int b, int lane) {
 }
 
 // What the prefix sums place, by warps w of nw: the requests' new table entries,
-// unit records and tree rows a request at a time; chain rows and the rows behind
+// CTAs and tree rows a request at a time; chain rows and the rows behind
 // the last request a row at a time.
 __device__ void begin_fill(const TokParams &p, int w, int nw) {
     int32_t *st = p.step;
     const int lane = threadIdx.x & 31;
-    const int free_n = st[kTokFree], chunk = st[kTokChunk];
+    const int free_n = st[kTokFree];
+    const int64_t share = max(st[kTokShare], 1);
+    const int64_t *work = reinterpret_cast<const int64_t *>(st + p.l.work);
     for (int b = w; b < p.batch; b += nw) {
         const int ctx = st[p.l.context + b];
         if (ctx >= 0) {
@@ -291,23 +303,10 @@ __device__ void begin_fill(const TokParams &p, int w, int nw) {
             for (int i = held + lane; i < need; i += 32)
                 p.d.page_table[(int64_t)slot * p.d.table_width + i] =
                     p.d.free_pages[free_n - 1 - (first + i - held)];
-            const int u0 = st[p.l.unit_start + b], nu = st[p.l.unit_start + b + 1] - u0;
-            const int part0 = st[p.l.part_start + b];
-            const int nr = n > 0 ? (int)(((int64_t)n * p.group + p.tile_rows - 1) / p.tile_rows) : 1;
-            for (int i = lane; i < nu; i += 32) {
-                const int rt = i % nr, split = i / nr;
-                // keys that the tile's last row sees: for a chain, up to itself
-                const int64_t last = ((int64_t)(rt + 1) * p.tile_rows + p.group - 1) / p.group;
-                const int seen = ctx + (p.parents ? n : (int)min(last, (int64_t)n));
-                const int kt = (seen + kTokTile - 1) / kTokTile;
-                if (u0 + i < p.max_units) {
-                    int4 *rec = reinterpret_cast<int4 *>(st + p.l.units +
-                                                         (int64_t)(u0 + i) * kTokUnitWords);
-                    rec[0] = make_int4(slot, r0, n, ctx);
-                    rec[1] = make_int4(rt, min(split * chunk, kt), min((split + 1) * chunk, kt),
-                                       nu > nr ? part0 + i : -1);
-                }
-            }
+            // the CTAs that begin in this request
+            const int64_t w0 = work[b], w1 = work[b + 1];
+            for (int64_t c = (w0 + share - 1) / share + lane; c * share < w1; c += 32)
+                st[p.l.first + c] = b;
         }
         if (p.parents) tree_rows(p, b, lane);
     }
@@ -569,11 +568,10 @@ int launch_token_begin(const pk_token_kv *kv, const int32_t *slots, const int32_
     p.l = tok_layout(kv, batch, rows, parents != nullptr);
     p.ps_shift = kv->ps_shift;
     p.group = kv->group;
-    p.tile_rows = tok_tile_rows(kv, batch, rows);
+    p.shape = tok_shape(kv, batch, rows);
+    p.kv_heads = kv->d.num_kv_heads;
     p.batch = batch;
     p.rows = rows;
-    p.target = kv->target;
-    p.max_units = tok_max_units(kv, batch, rows);
     p.slots = slots;
     p.counts = counts;
     p.parents = parents;

@@ -6,60 +6,30 @@
 //
 // One pass over the keys in tiles of 64 with a running maximum and sum (fp32).
 // The rows of a K/V head are its group's query heads of every token, so a
-// request's pages are read once for up to 64 of them (a row tile).  The step
-// block lists units - a row tile over a range of key tiles - of about equal
-// length, some waves of them for the whole GPU however the lengths are spread;
-// a CTA walks its units and a second launch joins rows whose keys were split.
+// request's pages are read once for all of them that fit a row tile.  The step's
+// work is a line of (row tile, key tile) pairs that is cut into equal shares, one a
+// CTA, whatever the lengths; a second launch joins the row tiles that a cut went
+// through (two partial results a CTA at most).
 //
-// bf16: a producer warp brings each tile's pages (TMA boxes of a page's rows x
+// bf16, row tiles of 16 and 32: a producer warp brings each tile's pages (TMA boxes of a page's rows x
 // 64 columns, 128B swizzle) into a ring of K and V slots that runs ahead across
 // units; four warps hold 16-row fragments of the row tile and compute
-// S = Q K^T and O += P V with mma.sync m16n8k16.  With fewer than 64 rows the
-// warps share the keys of a tile instead (4 / (rows / 16) ways) and join through
-// shared memory at the end.  P is rounded to bf16 for the product, relative
+// S = Q K^T and O += P V with mma.sync m16n8k16.  The warps share the keys of a tile
+// (4 / (rows / 16) ways) and join through shared memory at the end.  P is rounded to bf16 for the product, relative
 // 2^-9 of each weight, below the rounding of the bf16 V that it multiplies; the
 // sum that normalises keeps fp32 weights.
 // Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
 // other waits return at once.
 #include <math.h>
 
-#include "pk_common.cuh"
-#include "pk_internal.h"
+#include "pk_tree.cuh"
 
 namespace pk {
 namespace {
 
-constexpr int kTile = kTokTile;
+constexpr int kTile = 64;
 constexpr int kConsumers = 128, kThreads = kConsumers + 32;
 
-struct TreeParams {
-    const int32_t *step, *table;
-    TokLayout l;
-    int table_width, num_pages, num_layers, layer, kv_heads, group, ps_shift, trees;
-    int rows, heads, tile_rows;
-    const void *q, *kv;
-    void *out;
-    int64_t q_rs, q_hs, o_rs, o_hs;
-    float scale_log2;
-    float *ws_o, *ws_ml;   // partial outputs [part][kv head][row of tile][dim], (m, l) pairs
-    int32_t *error;
-};
-
-struct Unit {
-    int slot, row0, count, ctx, rt, t0, t1, part;
-};
-__device__ __forceinline__ Unit load_unit(const TreeParams &p, int i) {
-    const int4 *r =
-        reinterpret_cast<const int4 *>(p.step + p.l.units + (int64_t)i * kTokUnitWords);
-    const int4 a = r[0], b = r[1];
-    return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -80,10 +50,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t *>(&v);
-}
 __device__ __forceinline__ void consumer_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory");
 }
@@ -100,33 +66,9 @@ __device__ __forceinline__ bool consumer_any(bool v) {
         : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void fence_async_proxy() {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
 // Whether row `node` sees the step's token `rel` (>= 0) of its request.
 __device__ __forceinline__ bool sees(int trees, uint64_t mask, int node, int rel) {
     return trees ? rel < PK_TOK_MAX_TREE && ((mask >> rel) & 1) : rel <= node;
-}
-
-// Bounded wait that gives up at once when another wait of the CTA already has.
-__device__ __forceinline__ void ring_wait(uint64_t *bar, uint32_t parity, volatile int *failed,
-                                          int32_t *error) {
-    if (mbar_try_wait(bar, parity)) return;
-    if (*failed) return;
-    const uint64_t t0 = globaltimer_ns();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*failed) return;
-        if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            *failed = 1;
-            raise(error, PK_DEV_TIMEOUT);
-            return;
-        }
-    }
 }
 
 template <int DH, int BM>
@@ -135,11 +77,11 @@ struct TreeShape {
     static constexpr int kBox = kTile * 128;                 // one column box of a tile
     static constexpr int kSlot = kCols * kBox;               // one tile of K or of V
     static constexpr int kWm = BM / 16, kWk = 4 / kWm;       // warps over rows, over keys
-    // 96 KB of tiles, or 64 KB beside the join buffer: two CTAs an SM
-    static constexpr int kSlots = (kWk > 1 ? 4 : 6) * (128 / DH);
+    // 64 KB of tiles beside the join buffer: two CTAs an SM
+    static constexpr int kSlots = 4 * (128 / DH);
     static constexpr int kKeys = kTile / kWk;                // keys of a tile per warp
     static constexpr int kPad = DH + 4;                      // join buffer row, floats
-    static constexpr int kJoin = kWk > 1 ? 4 * 16 * kPad * 4 + 4 * 16 * 8 : 0;
+    static constexpr int kJoin = 4 * 16 * kPad * 4 + 4 * 16 * 8;
     static constexpr int kSmem = kSlots * kSlot + kJoin + 1024;
 };
 
@@ -167,7 +109,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     grid_dep_wait();
     grid_dep_launch();
-    const int units = p.step[kTokUnits] * p.kv_heads;
 
     if (warp == 4) {
         // producer: lanes issue a tile's boxes, K then V
@@ -176,9 +117,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t bytes = rows_box * 128;
         int it = 0;   // ring use
         bool stop = false;   // the warp's, so that its lanes stay together
-        for (int u = blockIdx.x; u < units && !stop; u += gridDim.x) {
-            const Unit w = load_unit(p, u / p.kv_heads);
-            const int head = u % p.kv_heads;
+        Work work(p, blockIdx.x);
+        while (!stop && work.next()) {
+            const Unit &w = work.u;
+            const int head = w.head;
             const int32_t *table = p.table + (int64_t)w.slot * p.table_width;
             const int len = w.ctx + w.count;
             for (int t = w.t0; t < w.t1 && !stop; ++t) {
@@ -222,9 +164,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
     int it = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const Unit w = load_unit(p, u / p.kv_heads);
-        const int head = u % p.kv_heads;
+    Work work(p, blockIdx.x);
+    while (work.next()) {
+        const Unit &w = work.u;
+        const int head = w.head;
         const int m_rows = w.count * p.group;
         // this thread's two rows of the tile (fragment rows lane / 4 and + 8)
         uint32_t qf[DH / 16][4];
@@ -411,33 +354,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         }
-        const int64_t part = ((int64_t)w.part * p.kv_heads + head) * BM;
-        if (S::kWk == 1) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int rt = wm * 16 + (lane >> 2) + h * 8, r = w.rt * BM + rt;
-                if (r >= m_rows) continue;
-                if (w.part >= 0) {
-                    float *dst = p.ws_o + (part + rt) * DH + (lane & 3) * 2;
-#pragma unroll
-                    for (int n = 0; n < DH / 8; ++n)
-                        *reinterpret_cast<float2 *>(dst + n * 8) =
-                            make_float2(o[n][2 * h], o[n][2 * h + 1]);
-                    if ((lane & 3) == 0)
-                        *reinterpret_cast<float2 *>(p.ws_ml + (part + rt) * 2) =
-                            make_float2(__fmul_rn(m[h], p.scale_log2), l[h]);
-                } else {
-                    const float inv = 1.f / l[h];
-                    __nv_bfloat16 *dst = out + (int64_t)(w.row0 + node[h]) * p.o_rs +
-                                         (int64_t)(head * p.group + r - node[h] * p.group) * p.o_hs +
-                                         (lane & 3) * 2;
-#pragma unroll
-                    for (int n = 0; n < DH / 8; ++n)
-                        *reinterpret_cast<uint32_t *>(dst + n * 8) =
-                            pack2(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
-                }
-            }
-        } else {
+        const int64_t part = (int64_t)w.part * BM;
+        {
             // join the warps' shares of the keys: each writes its 16 rows, then every
             // thread sums 8 columns of a row over the shares
             float *ml = join + 4 * 16 * S::kPad;
@@ -520,12 +438,12 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
     grid_dep_wait();
     grid_dep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int units = p.step[kTokUnits] * p.kv_heads;
     const float *q = static_cast<const float *>(p.q), *kv = static_cast<const float *>(p.kv);
     float *out = static_cast<float *>(p.out);
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const Unit w = load_unit(p, u / p.kv_heads);
-        const int head = u % p.kv_heads, m_rows = w.count * p.group, len = w.ctx + w.count;
+    Work work(p, blockIdx.x);
+    while (work.next()) {
+        const Unit &w = work.u;
+        const int head = w.head, m_rows = w.count * p.group, len = w.ctx + w.count;
         __syncthreads();
         for (int c = threadIdx.x; c < kRowsF32 * DH / 4; c += 128) {
             const int rt = c / (DH / 4), e = c % (DH / 4), r = w.rt * kRowsF32 + rt;
@@ -639,7 +557,7 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
             for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
             if (r >= m_rows) continue;
             if (w.part >= 0) {
-                const int64_t part = ((int64_t)w.part * p.kv_heads + head) * kRowsF32 + rt;
+                const int64_t part = (int64_t)w.part * kRowsF32 + rt;
 #pragma unroll
                 for (int n = 0; n < NV; ++n) p.ws_o[part * DH + n * 32 + lane] = o[i][n];
                 if (lane == 0) {
@@ -658,16 +576,20 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
 }
 
 // ------------------------------------------------------------------ the join
-// A warp per (row, head): the row's ranges weighted by exp2(m - max m), in order
-// of the ranges, so that the result does not depend on which finished first.
+// A warp per (row, head): its row tile's partial results - of the CTAs whose shares
+// cut the tile's keys - weighted by exp2(m - max m), in order of the keys, so that
+// the result does not depend on which finished first.
 template <int DH, typename T>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     constexpr int NV = DH / 32;
     grid_dep_wait();
     grid_dep_launch();
+    const int64_t share = p.step[kTokShare];
+    if (share == 0) return;
     const int lane = threadIdx.x & 31;
     const int64_t n = (int64_t)p.rows * p.heads;
-    const int chunk = p.step[kTokChunk], bm = p.tile_rows;
+    const int bm = p.shape.rows;
+    const int64_t *work = reinterpret_cast<const int64_t *>(p.step + p.l.work);
     for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < n;
          i += ((int64_t)gridDim.x * blockDim.x) >> 5) {
         const int row = (int)(i / p.heads), qh = (int)(i - (int64_t)row * p.heads);
@@ -676,25 +598,26 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
         const int ctx = p.step[p.l.context + b];
         if (ctx < 0) continue;
         const int r0 = p.step[p.l.row_start + b], cnt = p.step[p.l.row_start + b + 1] - r0;
-        const int ns = ((ctx + cnt + kTile - 1) / kTile + chunk - 1) / chunk;
-        if (ns <= 1) continue;
         const int head = qh / p.group, r = (row - r0) * p.group + qh - head * p.group;
         const int nr = (cnt * p.group + bm - 1) / bm, rt = r / bm;
-        const int64_t base = p.step[p.l.part_start + b] + rt;
-        auto at = [&](int s) {
-            return ((base + (int64_t)s * nr) * p.kv_heads + head) * bm + (r - rt * bm);
+        const int64_t kt = (ctx + cnt + p.shape.keys - 1) / p.shape.keys;
+        const int64_t t0 = work[b] + ((int64_t)head * nr + rt) * kt, t1 = t0 + kt;
+        const int c0 = (int)(t0 / share), c1 = (int)((t1 - 1) / share);
+        if (c0 == c1) continue;
+        auto at = [&](int c) {   // the first CTA's last unit, the others' first
+            return ((int64_t)2 * c + (c == c0)) * bm + (r - rt * bm);
         };
         float top = -INFINITY;
-        for (int s = lane; s < ns; s += 32) top = fmaxf(top, p.ws_ml[at(s) * 2]);
+        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.ws_ml[at(c) * 2]);
 #pragma unroll
         for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
         if (top == -INFINITY) top = 0.f;
         float acc[NV] = {}, sum = 0.f;
-        for (int s = 0; s < ns; ++s) {
-            const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + at(s) * 2);
+        for (int c = c0; c <= c1; ++c) {
+            const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + at(c) * 2);
             const float f = exp2f(ml.x - top);
             sum += f * ml.y;
-            const float *src = p.ws_o + at(s) * DH + lane * NV;
+            const float *src = p.ws_o + at(c) * DH + lane * NV;
 #pragma unroll
             for (int e = 0; e < NV; ++e) acc[e] += f * src[e];
         }
@@ -706,54 +629,50 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
 }
 
 template <int DH, int BM>
-cudaError_t launch_bf16(const pk_token_kv *kv, const TreeParams &p, int64_t most, cudaStream_t s) {
+cudaError_t launch_bf16(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     constexpr int smem = TreeShape<DH, BM>::kSmem;
     cudaError_t e = allow_smem(tree_attn_kernel<DH, BM>, smem, done);
     if (e != cudaSuccess) return e;
-    // two CTAs an SM, which their shared memory allows
-    const int64_t ctas = 2 * current_sms();
-    return launch_pdl(tree_attn_kernel<DH, BM>, dim3((unsigned)(most < ctas ? most : ctas)),
-                      dim3(kThreads), smem, s, kv->kv_map, p);
+    return launch_pdl(tree_attn_kernel<DH, BM>, dim3(ctas), dim3(kThreads), smem, s, kv->kv_map, p);
 }
 template <int DH>
-cudaError_t launch_bm(const pk_token_kv *kv, const TreeParams &p, int64_t most, cudaStream_t s) {
-    switch (p.tile_rows) {
-        case 16: return launch_bf16<DH, 16>(kv, p, most, s);
-        case 32: return launch_bf16<DH, 32>(kv, p, most, s);
-        default: return launch_bf16<DH, 64>(kv, p, most, s);
-    }
-}
-template <int DH>
-cudaError_t launch_f32(const TreeParams &p, int64_t most, cudaStream_t s) {
+cudaError_t launch_dim(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
+    if (kv->d.dtype == PK_DTYPE_BF16)
+        return p.shape.rows == 16 ? launch_bf16<DH, 16>(kv, p, ctas, s)
+                                  : launch_bf16<DH, 32>(kv, p, ctas, s);
     static std::atomic<uint64_t> done{0};
     constexpr int smem = (kTile * (DH + 4) + kTile * DH + kRowsF32 * DH + kRowsF32 * kTile) * 4;
     cudaError_t e = allow_smem(tree_attn_f32_kernel<DH>, smem, done);
     if (e != cudaSuccess) return e;
-    const int64_t ctas = 2 * current_sms();
-    return launch_pdl(tree_attn_f32_kernel<DH>, dim3((unsigned)(most < ctas ? most : ctas)),
-                      dim3(128), smem, s, p);
+    return launch_pdl(tree_attn_f32_kernel<DH>, dim3(ctas), dim3(128), smem, s, p);
 }
 template <int DH>
-cudaError_t launch_join(const TreeParams &p, int dtype, cudaStream_t s) {
-    const int64_t ctas = ((int64_t)p.rows * p.heads + 7) / 8, lim = 8 * current_sms();
+cudaError_t launch_join(const TreeParams &p, int dtype, int sms, cudaStream_t s) {
+    const int64_t ctas = ((int64_t)p.rows * p.heads + 7) / 8, lim = 8 * (int64_t)sms;
     const dim3 grid((unsigned)(ctas < lim ? ctas : lim));
     return dtype == PK_DTYPE_BF16
                ? launch_pdl(tree_join_kernel<DH, __nv_bfloat16>, grid, dim3(256), 0, s, p)
                : launch_pdl(tree_join_kernel<DH, float>, grid, dim3(256), 0, s, p);
 }
 
-// No request of this pool can be long enough to be split.
-bool never_split(const pk_token_kv *kv) {
-    return (int64_t)kv->d.table_width << kv->ps_shift <= (int64_t)kTokMinChunk * kTile;
+// Most row tiles of a step.
+int64_t max_items(const pk_token_kv *kv, int batch, int rows, const TokShape &sh) {
+    return ((int64_t)rows * kv->group / sh.rows + batch) * kv->d.num_kv_heads;
+}
+// No row tile of such a step is shared by CTAs: as begin_plan decides, for the
+// longest request that the pool holds.
+bool never_shared(const pk_token_kv *kv, int batch, int rows, const TokShape &sh) {
+    return (int64_t)kv->d.table_width << kv->ps_shift <= kTokMinKeys &&
+           max_items(kv, batch, rows, sh) <= sh.ctas;
 }
 
 }  // namespace
 
 int64_t tree_attn_workspace(const pk_token_kv *kv, int batch, int rows) {
-    if (never_split(kv)) return 0;
-    return tok_max_parts(kv) * kv->d.num_kv_heads * tok_tile_rows(kv, batch, rows) *
-           (kv->d.head_dim + 2) * 4;
+    const TokShape sh = tok_shape(kv, batch, rows);
+    return never_shared(kv, batch, rows, sh) ? 0
+                                             : (int64_t)2 * sh.ctas * sh.rows * (kv->d.head_dim + 2) * 4;
 }
 
 int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStream_t s) {
@@ -762,6 +681,7 @@ int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStre
     p.step = a.step;
     p.table = d.page_table;
     p.l = tok_layout(kv, a.batch, a.rows, a.trees);
+    p.shape = tok_shape(kv, a.batch, a.rows);
     p.table_width = d.table_width;
     p.num_pages = d.num_pages;
     p.num_layers = d.num_layers;
@@ -770,9 +690,9 @@ int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStre
     p.group = kv->group;
     p.ps_shift = kv->ps_shift;
     p.trees = a.trees;
+    p.batch = a.batch;
     p.rows = a.rows;
     p.heads = d.num_heads;
-    p.tile_rows = tok_tile_rows(kv, a.batch, a.rows);
     p.q = a.q;
     p.kv = d.kv;
     p.out = a.out;
@@ -782,17 +702,19 @@ int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStre
     p.o_hs = a.o_hs;
     p.scale_log2 = a.scale * 1.44269504088896340736f;
     p.ws_o = a.ws;
-    p.ws_ml = a.ws ? a.ws + tok_max_parts(kv) * d.num_kv_heads * p.tile_rows * d.head_dim : nullptr;
+    p.ws_ml = a.ws ? a.ws + (int64_t)2 * p.shape.ctas * p.shape.rows * d.head_dim : nullptr;
     p.error = d.error;
-    const int64_t most = tok_max_units(kv, a.batch, a.rows) * d.num_kv_heads;
-    cudaError_t e;
-    if (d.dtype == PK_DTYPE_BF16)
-        e = d.head_dim == 64 ? launch_bm<64>(kv, p, most, s) : launch_bm<128>(kv, p, most, s);
-    else
-        e = d.head_dim == 64 ? launch_f32<64>(p, most, s) : launch_f32<128>(p, most, s);
+    const bool shared = !never_shared(kv, a.batch, a.rows, p.shape);
+    // without sharing a CTA has one row tile, so those behind the last have none
+    const int64_t items = max_items(kv, a.batch, a.rows, p.shape);
+    const int ctas = shared || items > p.shape.ctas ? p.shape.ctas : (int)items;
+    cudaError_t e = p.shape.rows == 128 ? launch_tree_tc(kv, p, ctas, s)
+                    : d.head_dim == 64  ? launch_dim<64>(kv, p, ctas, s)
+                                        : launch_dim<128>(kv, p, ctas, s);
     if (e != cudaSuccess) return cuda_status(e, "tree attention kernel");
-    if (never_split(kv)) return PK_OK;
-    e = d.head_dim == 64 ? launch_join<64>(p, d.dtype, s) : launch_join<128>(p, d.dtype, s);
+    if (!shared) return PK_OK;
+    e = d.head_dim == 64 ? launch_join<64>(p, d.dtype, kv->sms, s)
+                         : launch_join<128>(p, d.dtype, kv->sms, s);
     return cuda_status(e, "tree_join_kernel");
 }
 

@@ -1,0 +1,439 @@
+// Tree attention (see pk_tree_attn.cu) for row tiles of up to 128 query rows, bf16,
+// on the 5th-generation tensor cores.
+//
+// Bound by reading K and V as long as a request's rows fit one tile: 128 keys of a
+// 128-wide head are 64 KB, 2800 cycles of an SM's share of the memory rate, for
+// 1024 cycles of MMAs and about 1300 of exponentials.  So one CTA an SM with one
+// softmax warpgroup, and the scores of tile j + 1 made while tile j is weighted:
+//   warp 0      pages of K and V by TMA into a ring of slots (a slot: one tile of
+//               K or of V), running ahead over the CTA's units
+//   warp 1      one thread issues S_j = Q K_j^T (both from shared memory, fp32 in
+//               TMEM, two buffers) and O += P_j V_j (P from TMEM, V from shared
+//               memory as it lies: a row-major [keys][dim] tile is the MN-major
+//               operand), O in TMEM
+//   warps 2..5  a thread per row (TMEM lane): the row's scores without a shuffle,
+//               maximum, exp2, P as bf16 into TMEM, fp32 sum
+// The running maximum is raised, and O scaled for it, only when a row's scores pass
+// the one in use by more than 2^8: weights stay below 256, which the fp32 sums and
+// bf16's exponent hold, and most tiles touch O in the MMA alone.
+#include <math.h>
+
+#include "pk_tree.cuh"
+#include "pk_umma.cuh"
+
+namespace pk {
+namespace {
+
+constexpr int kRows = 128, kKeys = 128, kTcThreads = 192;
+constexpr float kRaise = 8.f;   // log2 of how far scores may pass the maximum in use
+
+template <int DH>
+struct TcShape {
+    static constexpr int kCols = DH / 64;              // 128-byte column boxes
+    static constexpr int kBox = kKeys * 128;           // a box: 128 rows of 128 bytes
+    static constexpr int kSlot = kCols * kBox;         // one tile of K, V or Q
+    static constexpr int kSlots = 5 * (128 / DH);      // 160 KB
+    static constexpr int kSmem = (kSlots + 1) * kSlot + 1024;
+    // TMEM columns: S and P twice each, O
+    static constexpr int kS = 0, kP = 2 * kKeys, kO = kP + kKeys, kTmem = 512;
+};
+
+// O += P V: A from TMEM (bf16 pairs), B MN-major
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
+                                             uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Descriptor of an MN-major operand: boxes of 64 (MN) x keys (K), 128B swizzle; LBO
+// between boxes, SBO between groups of 8 keys (1024 bytes).
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t box_bytes) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(box_bytes >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+        "%28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// barrier of the four softmax warps that also ORs a flag over them
+__device__ __forceinline__ bool softmax_any(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
+
+// Bits of keys rel0 .. rel0 + 31 of the step's own tokens that a row sees.
+__device__ __forceinline__ uint32_t seen_bits(int trees, uint64_t mask, int node, int rel0) {
+    if (rel0 <= -32) return 0xffffffffu;
+    if (!trees) {
+        const int n = node - rel0 + 1;   // keys up to the row's own
+        return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+    }
+    if (rel0 >= 64) return 0u;
+    if (rel0 >= 0) return (uint32_t)(mask >> rel0);
+    return (uint32_t)(mask << -rel0) | ((1u << -rel0) - 1u);
+}
+
+template <int DH>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeParams p) {
+    using S = TcShape<DH>;
+    constexpr int NS = S::kSlots;
+    extern __shared__ uint8_t tree_smem[];
+    uint8_t *sq = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
+    uint8_t *ring = sq + S::kSlot;
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], q_full, s_full[2], p_full[2], o_done, idle;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&q_full, 4);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+        }
+        mbar_init(&o_done, 1);
+        mbar_init(&idle, 1);
+        failed = 0;
+        fence_mbar_init();
+        prefetch_tmap(&kv_map);
+    }
+    if (warp == 0) {
+        tmem_alloc(&tmem_base, S::kTmem);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    grid_dep_wait();
+    grid_dep_launch();
+    Work work(p, blockIdx.x);
+
+    if (warp == 0) {
+        // producer: lanes issue a tile's boxes, K then V
+        const int ps = 1 << p.ps_shift, rows_box = min(ps, 64);
+        const int box_of = lane / S::kCols, col = lane % S::kCols;
+        const uint32_t bytes = rows_box * 128;
+        int it = 0;
+        bool stop = false;   // the warp's, so that its lanes stay together
+        while (!stop && work.next()) {
+            const Unit &w = work.u;
+            const int32_t *table = p.table + (int64_t)w.slot * p.table_width;
+            const int len = w.ctx + w.count;
+            for (int t = w.t0; t < w.t1 && !stop; ++t) {
+                const int k0 = t * kKeys, n = (min(kKeys, len - k0) + rows_box - 1) / rows_box;
+                int page = 0;
+                if (box_of < n) {
+                    page = table[(k0 + box_of * rows_box) >> p.ps_shift];
+                    if (page < 0 || page >= p.num_pages) {
+                        raise(p.error, PK_DEV_BAD_PAGE);
+                        page = 0;
+                    }
+                }
+                const int in_page = (k0 + box_of * rows_box) & (ps - 1);
+#pragma unroll
+                for (int v = 0; v < 2; ++v, ++it) {
+                    const int s = it % NS, use = it / NS;
+                    if (use) ring_wait(&empty[s], (use - 1) & 1, &failed, p.error);
+                    stop = __any_sync(0xffffffffu, failed != 0);
+                    if (stop) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * S::kCols * bytes);
+                    __syncwarp();
+                    if (box_of < n)
+                        tma_load_3d(ring + s * S::kSlot + col * S::kBox + box_of * bytes, &kv_map,
+                                    &full[s], col * 64, in_page,
+                                    ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
+                }
+            }
+        }
+        if (stop)   // leave no copy in flight
+            for (int s = 0; s < NS; ++s)
+                if (it > s) mbar_wait_bounded(&full[s], ((it - 1 - s) / NS) & 1, kWaitLimitNs);
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_bf16(kRows, kKeys);
+            constexpr uint32_t id_o = idesc_bf16(kRows, DH) | (1u << 16);   // B MN-major
+            const uint32_t q0 = smem_u32(sq);
+            int it = 0, j = 0, unit = 0;   // ring use, tile and unit of this CTA
+            // S_j of the tile whose K is ring use `use`
+            auto scores = [&](int use, int tile) {
+                const int s = use % NS;
+                ring_wait(&full[s], (use / NS) & 1, &failed, p.error);
+                tc_fence_after();
+                const uint32_t k0 = smem_u32(ring + s * S::kSlot);
+#pragma unroll
+                for (int kk = 0; kk < DH / 16; ++kk) {
+                    const uint32_t off = (kk / 4) * S::kBox + (kk % 4) * 32;
+                    umma_bf16(tmem + S::kS + (tile & 1) * kKeys, sw128_desc(q0 + off),
+                              sw128_desc(k0 + off), id_s, kk != 0);
+                }
+                umma_commit(&empty[s]);
+                umma_commit(&s_full[tile & 1]);
+            };
+            while (!failed && work.next()) {
+                const int n = work.u.t1 - work.u.t0;
+                if (n <= 0) continue;
+                ring_wait(&q_full, unit & 1, &failed, p.error);
+                ++unit;
+                tc_fence_after();
+                scores(it, j);
+                for (int i = 0; i < n && !failed; ++i, ++j, it += 2) {
+                    if (i + 1 < n) scores(it + 2, j + 1);
+                    const int s = (it + 1) % NS;
+                    ring_wait(&full[s], ((it + 1) / NS) & 1, &failed, p.error);
+                    ring_wait(&p_full[j & 1], (j >> 1) & 1, &failed, p.error);
+                    if (failed) break;
+                    tc_fence_after();
+                    const uint32_t v0 = smem_u32(ring + s * S::kSlot);
+#pragma unroll
+                    for (int kk = 0; kk < kKeys / 16; ++kk)
+                        umma_bf16_ts(tmem + S::kO, tmem + S::kP + (j & 1) * (kKeys / 2) + kk * 8,
+                                     mn_desc(v0 + kk * 2048, S::kBox), id_o, (i | kk) != 0);
+                    umma_commit(&empty[s]);
+                    umma_commit(&o_done);
+                }
+            }
+            umma_commit(&idle);   // no MMA is left when the CTA frees its TMEM
+            mbar_wait_bounded(&idle, 0, kWaitLimitNs);
+        }
+    } else {
+        // softmax: thread = row (TMEM lane) 32 (warp % 4) + lane of the tile
+        const int quad = warp & 3, rt = quad * 32 + lane;
+        const uint32_t mine = tmem + ((uint32_t)(quad * 32) << 16);
+        const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
+        __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
+        int it = 0, j = 0;
+        while (work.next()) {
+            const Unit &w = work.u;
+            const int r = w.rt * kRows + rt, n = w.t1 - w.t0, len = w.ctx + w.count;
+            const bool live = r < w.count * p.group;
+            const int node = live ? r / p.group : -1;
+            const int64_t row = w.row0 + (live ? node : 0);
+            const int64_t qh = (int64_t)w.head * p.group + (live ? r - node * p.group : 0);
+            uint64_t mask = 0;
+            if (live && p.trees) mask = reinterpret_cast<const uint64_t *>(p.step + p.l.mask)[row];
+            float m = -INFINITY, l = 0.f;   // the maximum in use (scaled), the sum
+            bool odd = false;               // a value that is not finite among the own rows
+            if (n > 0) {
+                // the tile's queries; the MMAs that read the last ones are done, since
+                // their scores have been read
+                const uint4 *src = reinterpret_cast<const uint4 *>(q + row * p.q_rs + qh * p.q_hs);
+#pragma unroll
+                for (int c = 0; c < DH / 8; ++c)
+                    *reinterpret_cast<uint4 *>(sq + (c / 8) * S::kBox + sw128(rt, (c % 8) * 16)) =
+                        live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                fence_async_proxy();
+                __syncwarp();
+                if (lane == 0) arrive(&q_full);
+            }
+            for (int i = 0; i < n; ++i, ++j, it += 2) {
+                const int k0 = (w.t0 + i) * kKeys;
+                const uint32_t st = mine + S::kS + (j & 1) * kKeys;
+                ring_wait(&s_full[j & 1], (j >> 1) & 1, &failed, p.error);
+                __syncwarp();
+                tc_fence_after();
+                float s[kKeys];
+#pragma unroll
+                for (int c = 0; c < kKeys / 32; ++c)
+                    tmem_ld32(st + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
+                const bool own = k0 + kKeys > w.ctx;
+                if (own) {
+                    const int sv = (it + 1) % NS;
+#pragma unroll
+                    for (int c = 0; c < kKeys / 32; ++c) {
+                        const uint32_t bits = seen_bits(p.trees, mask, node, k0 + c * 32 - w.ctx);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(bits >> e & 1)) s[c * 32 + e] = -INFINITY;
+                    }
+                    // V rows past the end hold what the page held before, and a token's
+                    // values may be inf or NaN: zero in the product, where a weight of
+                    // zero would not keep them out; the epilogue adds the latter to the
+                    // rows that see them
+                    ring_wait(&full[sv], ((it + 1) / NS) & 1, &failed, p.error);
+                    uint8_t *vs = ring + sv * S::kSlot;
+                    bool bad = false;
+                    for (int c = threadIdx.x - 64; c < kKeys * DH / 8; c += 128) {
+                        const int vr = c / (DH / 8), ch = c % (DH / 8), key = k0 + vr;
+                        if (key < w.ctx) continue;
+                        uint4 *at = reinterpret_cast<uint4 *>(vs + (ch / 8) * S::kBox +
+                                                              sw128(vr, (ch % 8) * 16));
+                        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                        if (key < len) {
+                            x = *at;
+                            uint32_t *e = &x.x;
+                            bool here = false;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                if ((e[k] & 0x7f80u) == 0x7f80u) {
+                                    e[k] &= 0xffff0000u;
+                                    here = true;
+                                }
+                                if ((e[k] & 0x7f800000u) == 0x7f800000u) {
+                                    e[k] &= 0x0000ffffu;
+                                    here = true;
+                                }
+                            }
+                            if (!here) continue;
+                            bad = true;
+                        }
+                        *at = x;
+                    }
+                    fence_async_proxy();
+                    odd |= softmax_any(bad);
+                }
+                float top = s[0];
+#pragma unroll
+                for (int e = 1; e < kKeys; ++e) top = fmaxf(top, s[e]);
+                top = top == -INFINITY ? top : __fmul_rn(top, p.scale_log2);
+                const bool raise_it = top > m + kRaise || (m == -INFINITY && top > m);
+                if (__any_sync(0xffffffffu, raise_it)) {
+                    const float keep = raise_it ? ex2(m - top) : 1.f;
+                    if (raise_it) m = top;
+                    l *= keep;
+                    if (i > 0) {   // O has the tiles before
+                        ring_wait(&o_done, (j - 1) & 1, &failed, p.error);
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < DH / 32; ++c) {
+                            float o[32];
+                            tmem_ld32(mine + S::kO + c * 32, o);
+                            uint32_t x[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(o[e] * keep);
+                            tmem_st32(mine + S::kO + c * 32, x);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : m;
+                float sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t x[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float a = ex2(s[c * 64 + 2 * e] * p.scale_log2 - base);
+                        const float b = ex2(s[c * 64 + 2 * e + 1] * p.scale_log2 - base);
+                        sum += a + b;
+                        x[e] = pack2(a, b);
+                    }
+                    tmem_st32(mine + S::kP + (j & 1) * (kKeys / 2) + c * 32, x);
+                }
+                l += sum;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(&p_full[j & 1]);
+            }
+            if (n > 0) {
+                ring_wait(&o_done, (j - 1) & 1, &failed, p.error);
+                __syncwarp();
+                tc_fence_after();
+            }
+            const float inv = 1.f / l;
+            float *dst = p.ws_o + ((int64_t)w.part * kRows + rt) * DH;
+            __nv_bfloat16 *o_row = out + row * p.o_rs + qh * p.o_hs;
+#pragma unroll 1
+            for (int c = 0; c < DH / 32; ++c) {
+                float o[32];
+                if (n > 0) {
+                    tmem_ld32(mine + S::kO + c * 32, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                }
+                if (!live) continue;
+                if (odd) {
+                    // the values that were kept out of the product, for the keys that
+                    // the row sees: they make the sum inf or NaN, whatever their weight
+#pragma unroll 1
+                    for (int key = max(w.ctx, w.t0 * kKeys); key < min(len, w.t1 * kKeys); ++key) {
+                        const int rel = key - w.ctx;
+                        if (!(seen_bits(p.trees, mask, node, rel) & 1)) continue;
+                        const int64_t page =
+                            p.table[(int64_t)w.slot * p.table_width + (key >> p.ps_shift)];
+                        const int64_t ps = 1 << p.ps_shift;
+                        const __nv_bfloat16 *v =
+                            static_cast<const __nv_bfloat16 *>(p.kv) +
+                            ((((page * p.num_layers + p.layer) * 2 + 1) * p.kv_heads + w.head) * ps +
+                             (key & (ps - 1))) * DH + c * 32;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float x = __bfloat162float(v[e]);
+                            if (!isfinite(x)) o[e] += x;
+                        }
+                    }
+                }
+                if (w.part >= 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        reinterpret_cast<float4 *>(dst + c * 32)[e] =
+                            make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        reinterpret_cast<uint4 *>(o_row + c * 32)[e] = make_uint4(
+                            pack2(o[8 * e] * inv, o[8 * e + 1] * inv),
+                            pack2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                            pack2(o[8 * e + 4] * inv, o[8 * e + 5] * inv),
+                            pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+                }
+            }
+            if (w.part >= 0 && live)
+                *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)w.part * kRows + rt) * 2) =
+                    make_float2(m, l);
+            tc_fence_before();   // O is read before the next unit's MMAs (by its q_full)
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, S::kTmem);
+    }
+}
+
+template <int DH>
+cudaError_t launch(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(tree_tc_kernel<DH>, TcShape<DH>::kSmem, done);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(tree_tc_kernel<DH>, dim3(ctas), dim3(kTcThreads), TcShape<DH>::kSmem, s,
+                      kv->kv_map, p);
+}
+
+}  // namespace
+
+cudaError_t launch_tree_tc(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
+    return kv->d.head_dim == 64 ? launch<64>(kv, p, ctas, s) : launch<128>(kv, p, ctas, s);
+}
+
+}  // namespace pk

@@ -21,8 +21,8 @@ PK_DEV_BAD_COUNT = 16
 PK_GEMM_STORE, PK_GEMM_SILU, PK_GEMM_RESIDUAL, PK_GEMM_RESIDUAL_RELU, PK_GEMM_BIAS = 0, 1, 2, 3, 4
 PK_FE_HIST, PK_FE_META_STRIDE, PK_FE_FIRST, PK_FE_FINAL = 512, 4, 1, 2
 PK_NOALLOC_SCRATCH_BYTES = 32 * 1024 * 1024   # pk_paged_attention_noalloc's static scratch
-PK_TOK_ROW_START, PK_TOK_CONTEXT, PK_TOK_REQUEST, PK_TOK_POSITION = 0, 1, 7, 8
-PK_TOK_SLOT_MAP, PK_TOK_MASK, PK_TOK_OFFSETS = 9, 11, 12
+PK_TOK_ROW_START, PK_TOK_CONTEXT, PK_TOK_REQUEST, PK_TOK_POSITION = 0, 1, 2, 3
+PK_TOK_SLOT_MAP, PK_TOK_MASK, PK_TOK_OFFSETS = 4, 5, 6
 PK_TOK_MAX_TREE, PK_TOK_MAX_BATCH = 64, 65536   # nodes of a tree, requests of a step
 PK_ADAPTER_MAX, PK_ADAPTER_MAX_RANK, PK_ADAPTER_MAX_ROWS = 8192, 128, 1048576
 META_FIRST, META_NEXT, META_WRITTEN, META_PROCESSED, META_CACHE_LEN = 0, 1, 2, 3, 4

@@ -61,7 +61,8 @@ class TokenStep:
         self._at = at
 
     def _view(self, which, n):
-        return self.block.narrow(0, self._at[which], n)
+        a = self._at[which]
+        return self.block[a:a + n]
 
     @property
     def row_start(self):

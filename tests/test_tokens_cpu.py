@@ -47,13 +47,13 @@ def test_step_block_layout(pool):
     at = (ctypes.c_int64 * _lib.PK_TOK_OFFSETS)()
     for batch, rows, trees in [(1, 1, 1), (3, 7, 1), (4, 1001, 0), (4, 0, 1)]:
         words = _lib.lib().pk_token_step_words(pool, batch, rows, trees, at)
-        o = list(at)
-        assert o == sorted(o) and o[0] >= 16
-        assert o[_lib.PK_TOK_CONTEXT] - o[_lib.PK_TOK_ROW_START] == batch + 1
-        assert o[_lib.PK_TOK_POSITION] - o[_lib.PK_TOK_REQUEST] == rows
-        assert o[_lib.PK_TOK_SLOT_MAP] - o[_lib.PK_TOK_POSITION] == rows
-        assert o[_lib.PK_TOK_MASK] % 2 == 0
-        assert words - o[_lib.PK_TOK_MASK] == (2 * rows if trees else 0)
+        n = {_lib.PK_TOK_ROW_START: batch + 1, _lib.PK_TOK_CONTEXT: batch, _lib.PK_TOK_REQUEST: rows,
+             _lib.PK_TOK_POSITION: rows, _lib.PK_TOK_SLOT_MAP: rows,
+             _lib.PK_TOK_MASK: 2 * rows if trees else 0}
+        spans = sorted((at[i], at[i] + k) for i, k in n.items() if k)
+        assert spans[0][0] >= 16 and spans[-1][1] <= words
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+        assert at[_lib.PK_TOK_MASK] % 2 == 0
     assert _lib.lib().pk_token_step_words(pool, -1, 1, 0, None) == -1
     assert _lib.lib().pk_token_step_words(pool, 1, -1, 0, None) == -1
 
