@@ -224,18 +224,18 @@ namespace pk {
 // share the work.
 struct TokShape {
     int rows, keys, ctas;
+    int least;   // key tiles that a CTA takes before a request's are split over several
 };
 // bf16: the narrowest row tile that holds an average request, since a request's K/V
 // is read once per row tile - 16 or 32 rows by mma.sync (two CTAs an SM), 128 by
 // tcgen05 (one).  float32: 16.
 inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
-    if (kv->d.dtype == PK_DTYPE_F32 || mean <= 16) return {16, 64, 2 * kv->sms};
-    if (mean <= 32) return {32, 64, 2 * kv->sms};
-    return {128, 128, kv->sms};
+    if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, 2 * kv->sms, 1};
+    if (mean <= 16) return {16, 64, 2 * kv->sms, 8};
+    if (mean <= 32) return {32, 64, 2 * kv->sms, 8};
+    return {128, 128, kv->sms, 4};
 }
-// Keys that one CTA takes before a request's keys are split over several.
-constexpr int kTokMinKeys = 512;
 
 // Step block, int32 words: header, then arrays at these offsets.  The step's work
 // is a line of key tiles, request by request, K/V head by head, row tile by row

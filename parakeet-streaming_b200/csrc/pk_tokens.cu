@@ -30,7 +30,7 @@ struct TokParams {
     pk_token_kv_desc d;
     TokLayout l;
     TokShape shape;
-    int ps_shift, group, kv_heads, batch, rows;
+    int ps_shift, row_shift, key_shift, group, kv_heads, batch, rows;
     const int32_t *slots, *counts, *parents;
     int32_t *step;
 };
@@ -62,22 +62,28 @@ __device__ int64_t block_exclusive_sum64(int64_t v, int64_t &total, int64_t *s_w
     return res;
 }
 
-// Marks every slot of the batch with the first request that names it; a slot
-// out of range is nobody's.  scratch[0 .. num_slots) is the mark.
-__device__ void mark_slots(const pk_token_kv_desc &d, const int32_t *slots, int batch) {
-    for (int b = threadIdx.x; b < batch; b += blockDim.x) {
-        const int s = slots[b];
-        if (s >= 0 && s < d.num_slots) d.scratch[s] = 0x7fffffff;
+// The requests of one thread of the planning CTA, b0 .. b0 + NK - 1: contiguous, so
+// that each prefix sum over the batch is one scan over the threads' sums, and in
+// registers, so that their loads overlap.
+//
+// A slot may be named once.  Every slot of the batch is marked with the first
+// request that names it (scratch[0 .. num_slots)); a slot out of range is nobody's.
+template <int NK>
+__device__ __forceinline__ void own_slots(const pk_token_kv_desc &d, const int32_t *slots, int batch,
+                                          int b0, int (&slot)[NK], bool (&own)[NK]) {
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        slot[k] = b0 + k < batch ? slots[b0 + k] : -1;
+        own[k] = slot[k] >= 0 && slot[k] < d.num_slots;
+        if (own[k]) d.scratch[slot[k]] = 0x7fffffff;
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < batch; b += blockDim.x) {
-        const int s = slots[b];
-        if (s >= 0 && s < d.num_slots) atomicMin(&d.scratch[s], b);
-    }
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+        if (own[k]) atomicMin(&d.scratch[slot[k]], b0 + k);
     __syncthreads();
-}
-__device__ bool owns_slot(const pk_token_kv_desc &d, int slot, int b) {
-    return slot >= 0 && slot < d.num_slots && d.scratch[slot] == b;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) own[k] = own[k] && d.scratch[slot[k]] == b0 + k;
 }
 
 __device__ __forceinline__ int ceil_shift(int64_t n, int shift) {
@@ -91,54 +97,56 @@ __device__ __forceinline__ int page_of(const TokParams &p, int slot, int held, i
                     : p.d.free_pages[free_n - 1 - (first + i - held)];
 }
 
-// The planning CTA.  Thread t owns the requests [t * nk, (t + 1) * nk), so that
-// each prefix sum is one scan over the threads' sums.
+template <int NK>
 __device__ void begin_plan(const TokParams &p) {
     __shared__ int64_t s_scan[33];
     __shared__ unsigned long long s_take;
     __shared__ int s_longest;
     const pk_token_kv_desc &d = p.d;
     int32_t *st = p.step;
-    const int nk = (p.batch + blockDim.x - 1) / blockDim.x;
-    const int b0 = threadIdx.x * nk, b1 = min(b0 + nk, p.batch);
+    const int b0 = threadIdx.x * NK;
     const int free_n = *d.free_count;
     if (threadIdx.x == 0) {
         s_take = 0;
         s_longest = 0;
     }
-    mark_slots(d, p.slots, p.batch);
+    int slot[NK], count[NK], ctx[NK], held[NK], take[NK];
+    bool own[NK];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) count[k] = b0 + k < p.batch ? p.counts[b0 + k] : 0;
+    own_slots<NK>(d, p.slots, p.batch, b0, slot, own);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        ctx[k] = own[k] ? d.lengths[slot[k]] : -1;
+        held[k] = own[k] ? d.held[slot[k]] : 0;
+    }
 
     // rows; which requests can be served but for their pages
     int64_t sum = 0, total;
-    for (int b = b0; b < b1; ++b) sum += max(p.counts[b], 0);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) sum += max(count[k], 0);
     int64_t at = block_exclusive_sum64(sum, total, s_scan);
     int64_t takes = 0;
-    for (int b = b0; b < b1; ++b) {
-        const int slot = p.slots[b], n = p.counts[b];
-        const int64_t end = at + max(n, 0);
-        int ctx = -1, held = 0, take = 0, err = 0;
-        if (!owns_slot(d, slot, b)) {
-            err = PK_DEV_BAD_SLOT;
-        } else if (n < 0 || end > p.rows || (p.parents && n > PK_TOK_MAX_TREE)) {
-            err = PK_DEV_BAD_COUNT;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        const int b = b0 + k, n = max(count[k], 0);
+        take[k] = 0;
+        if (b >= p.batch) continue;
+        const int64_t len = (int64_t)ctx[k] + n;
+        if (!own[k]) {
+            raise(d.error, PK_DEV_BAD_SLOT);
+        } else if (count[k] < 0 || at + n > p.rows || (p.parents && n > PK_TOK_MAX_TREE) ||
+                   len > (int64_t)d.table_width << p.ps_shift) {
+            raise(d.error, PK_DEV_BAD_COUNT);
+            ctx[k] = -1;
         } else {
-            const int len = d.lengths[slot];
-            const int need = ceil_shift((int64_t)len + n, p.ps_shift);
-            held = d.held[slot];
-            if (need > d.table_width || (int64_t)len + n > 0x7fffffff) {
-                err = PK_DEV_BAD_COUNT;
-            } else {
-                ctx = len;
-                take = max(need - held, 0);
-            }
+            take[k] = max(ceil_shift(len, p.ps_shift) - held[k], 0);
         }
-        if (err) raise(d.error, err);
         st[p.l.row_start + b] = (int)min(at, (int64_t)p.rows);
-        st[p.l.context + b] = ctx;
-        st[p.l.slot + b] = slot;
-        st[p.l.held + b] = held;
-        takes += take;
-        at = end;
+        st[p.l.slot + b] = slot[k];
+        st[p.l.held + b] = held[k];
+        takes += take[k];
+        at += n;
     }
     if (threadIdx.x == 0) {
         const int used = (int)min(total, (int64_t)p.rows);
@@ -149,62 +157,61 @@ __device__ void begin_plan(const TokParams &p) {
 
     // pages, in batch order: requests past the end of the stack are left out
     int64_t first = block_exclusive_sum64(takes, total, s_scan);
-    int64_t tiles = 0, items = 0, taken = 0;
-    int longest = 0;
-    auto shape_of = [&](int b, int &nr, int &kt) {   // row tiles and key tiles
-        const int ctx = st[p.l.context + b], n = max(p.counts[b], 0);
-        nr = ctx >= 0 ? (int)(((int64_t)n * p.group + p.shape.rows - 1) / p.shape.rows) : 0;
-        kt = nr ? (ctx + n + p.shape.keys - 1) / p.shape.keys : 0;
-    };
-    for (int b = b0; b < b1; ++b) {
-        const int ctx = st[p.l.context + b], held = st[p.l.held + b], n = max(p.counts[b], 0);
-        const int take = ctx < 0 ? 0 : max(ceil_shift((int64_t)ctx + n, p.ps_shift) - held, 0);
+    int64_t tiles = 0, taken = 0;
+    int items = 0, longest = 0, nr[NK], kt[NK];   // row tiles and key tiles
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        const int b = b0 + k;
+        nr[k] = kt[k] = 0;
+        if (b >= p.batch) continue;
         st[p.l.take + b] = (int)min(first, (int64_t)0x7fffffff);
-        if (take > 0 && first + take > free_n) {
+        if (take[k] > 0 && first + take[k] > free_n) {
             raise(d.error, PK_DEV_POOL_EXHAUSTED);
-            st[p.l.context + b] = -1;
-        } else if (take > 0) {
-            taken += take;
-            d.held[st[p.l.slot + b]] = held + take;
+            ctx[k] = -1;
+        } else if (take[k] > 0) {
+            taken += take[k];
+            d.held[slot[k]] = held[k] + take[k];
         }
-        first += take;
-        int nr, kt;
-        shape_of(b, nr, kt);
-        tiles += (int64_t)nr * kt;
-        items += nr;
-        longest = max(longest, kt);
+        first += take[k];
+        st[p.l.context + b] = ctx[k];
+        if (ctx[k] >= 0 && count[k] > 0) {
+            nr[k] = ceil_shift((int64_t)count[k] * p.group, p.row_shift);
+            kt[k] = ceil_shift((int64_t)ctx[k] + count[k], p.key_shift);
+        }
+        tiles += (int64_t)nr[k] * kt[k];
+        items += nr[k];
+        longest = max(longest, kt[k]);
     }
     if (taken) atomicAdd(&s_take, (unsigned long long)taken);
     if (longest) atomicMax(&s_longest, longest);
 
-    // the attention's line of tiles: an equal share of it a CTA, but kTokMinKeys at
-    // least; a row tile each where there are no more of them than CTAs and none is
+    // the attention's line of tiles: an equal share of it a CTA, but the shape's least
+    // at least; a row tile each where there are no more of them than CTAs and none is
     // longer than that
-    block_exclusive_sum64(items, total, s_scan);
+    const int64_t items_before = block_exclusive_sum64(items, total, s_scan);
     const int64_t all_items = total * p.kv_heads;
     int64_t before = block_exclusive_sum64(tiles, total, s_scan);
-    const int64_t all = total * p.kv_heads;
-    const int least = kTokMinKeys / p.shape.keys;
-    int64_t share = (all + p.shape.ctas - 1) / p.shape.ctas;
-    if (share < least) share = least;
-    if (all_items <= p.shape.ctas && s_longest <= least) {
+    int64_t all = total * p.kv_heads;
+    int64_t share = max((all + p.shape.ctas - 1) / p.shape.ctas, (int64_t)p.shape.least);
+    const bool whole = all_items <= p.shape.ctas && s_longest <= p.shape.least;
+    if (whole) {
         share = 0;
-        before = block_exclusive_sum64(items, total, s_scan);
+        before = items_before;
+        all = all_items;
     }
     int64_t *work = reinterpret_cast<int64_t *>(st + p.l.work);
-    for (int b = b0; b < b1; ++b) {
-        work[b] = before * p.kv_heads;
-        int nr, kt;
-        shape_of(b, nr, kt);
-        before += share ? (int64_t)nr * kt : nr;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        if (b0 + k < p.batch) work[b0 + k] = before * p.kv_heads;
+        before += whole ? nr[k] : (int64_t)nr[k] * kt[k];
     }
     if (threadIdx.x == 0) {
-        work[p.batch] = total * p.kv_heads;
+        work[p.batch] = all;
         st[kTokShare] = (int)min(share, (int64_t)0x7fffffff);
         *d.free_count = free_n - (int)s_take;
     }
     // CTAs behind the last tile
-    const int64_t unit = share ? share : 1, used = (total * p.kv_heads + unit - 1) / unit;
+    const int64_t used = whole ? all : (all + share - 1) / share;
     for (int64_t c = used + threadIdx.x; c < p.shape.ctas; c += blockDim.x) st[p.l.first + c] = -1;
 }
 
@@ -336,11 +343,11 @@ __device__ void begin_fill(const TokParams &p, int w, int nw) {
     }
 }
 
-template <bool kFill>
+template <int NK, bool kFill>
 __global__ void __launch_bounds__(kPlanThreads) token_begin_kernel(const TokParams p) {
     grid_dep_wait();
     grid_dep_launch();
-    begin_plan(p);
+    begin_plan<NK>(p);
     if (kFill) {
         __syncthreads();
         begin_fill(p, threadIdx.x >> 5, blockDim.x >> 5);
@@ -465,37 +472,49 @@ struct TokCut {
     const int32_t *slots, *lengths;
     int batch, ps_shift;
 };
+template <int NK>
 __device__ void cut_plan(const TokCut &p) {
     __shared__ int64_t s_scan[33];
     const pk_token_kv_desc &d = p.d;
     int32_t *head = d.scratch + d.num_slots, *tmp = head + 16;
     const int free_n = *d.free_count;
-    mark_slots(d, p.slots, p.batch);
-    const int nk = (p.batch + blockDim.x - 1) / blockDim.x;
-    const int b0 = threadIdx.x * nk, b1 = min(b0 + nk, p.batch);
+    const int b0 = threadIdx.x * NK;
+    int slot[NK], len[NK], have[NK], held[NK], give[NK];
+    bool own[NK];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) len[k] = b0 + k < p.batch ? p.lengths[b0 + k] : 0;
+    own_slots<NK>(d, p.slots, p.batch, b0, slot, own);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        have[k] = own[k] ? d.lengths[slot[k]] : 0;
+        held[k] = own[k] ? d.held[slot[k]] : 0;
+    }
     int64_t sum = 0, total;
-    for (int b = b0; b < b1; ++b) {
-        const int slot = p.slots[b], len = p.lengths[b];
-        int keep = 0, give = 0;
-        if (!owns_slot(d, slot, b)) {
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        const int b = b0 + k;
+        give[k] = 0;
+        if (b >= p.batch) continue;
+        int keep = 0;
+        if (!own[k]) {
             raise(d.error, PK_DEV_BAD_SLOT);
-        } else if (len < 0 || len > d.lengths[slot]) {
+        } else if (len[k] < 0 || len[k] > have[k]) {
             raise(d.error, PK_DEV_BAD_COUNT);
         } else {
-            const int held = d.held[slot];
-            keep = min(ceil_shift(len, p.ps_shift), held);
-            give = held - keep;
-            d.held[slot] = keep;
-            d.lengths[slot] = len;
+            keep = min(ceil_shift(len[k], p.ps_shift), held[k]);
+            give[k] = held[k] - keep;
+            d.held[slot[k]] = keep;
+            d.lengths[slot[k]] = len[k];
         }
         tmp[3 * b + 1] = keep;
-        tmp[3 * b + 2] = give;
-        sum += give;
+        tmp[3 * b + 2] = give[k];
+        sum += give[k];
     }
     int64_t first = block_exclusive_sum64(sum, total, s_scan);
-    for (int b = b0; b < b1; ++b) {
-        tmp[3 * b] = (int)first;
-        first += tmp[3 * b + 2];
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        if (b0 + k < p.batch) tmp[3 * (b0 + k)] = (int)first;
+        first += give[k];
     }
     if (threadIdx.x == 0) {
         head[0] = free_n + (int)total;
@@ -516,11 +535,11 @@ __device__ void cut_fill(const TokCut &p, int w, int nw) {
         }
     }
 }
-template <bool kFill>
+template <int NK, bool kFill>
 __global__ void __launch_bounds__(kPlanThreads) token_cut_kernel(const TokCut p) {
     grid_dep_wait();
     grid_dep_launch();
-    cut_plan(p);
+    cut_plan<NK>(p);
     if (kFill) {
         __syncthreads();
         cut_fill(p, threadIdx.x >> 5, blockDim.x >> 5);
@@ -530,6 +549,12 @@ __global__ void __launch_bounds__(256) token_cut_fill_kernel(const TokCut p) {
     grid_dep_wait();
     grid_dep_launch();
     cut_fill(p, (blockIdx.x * blockDim.x + threadIdx.x) >> 5, (gridDim.x * blockDim.x) >> 5);
+}
+
+// Threads of the planning CTA for a batch at NK requests each.
+int plan_threads(int batch, int nk) {
+    const int n = ((batch + nk - 1) / nk + 31) / 32 * 32;
+    return n < kPlanThreads ? n : kPlanThreads;
 }
 
 int grid_for(int64_t threads, int block) {
@@ -563,13 +588,15 @@ int launch_token_reset(const pk_token_kv *kv, const int32_t *init_order, cudaStr
 int launch_token_begin(const pk_token_kv *kv, const int32_t *slots, const int32_t *counts,
                        int batch, const int32_t *parents, int rows, int32_t *step,
                        cudaStream_t s) {
-    TokParams p;
+    TokParams p = {};
     p.d = kv->d;
     p.l = tok_layout(kv, batch, rows, parents != nullptr);
     p.ps_shift = kv->ps_shift;
     p.group = kv->group;
     p.shape = tok_shape(kv, batch, rows);
     p.kv_heads = kv->d.num_kv_heads;
+    while ((1 << p.row_shift) < p.shape.rows) ++p.row_shift;
+    while ((1 << p.key_shift) < p.shape.keys) ++p.key_shift;
     p.batch = batch;
     p.rows = rows;
     p.slots = slots;
@@ -577,9 +604,17 @@ int launch_token_begin(const pk_token_kv *kv, const int32_t *slots, const int32_
     p.parents = parents;
     p.step = step;
     if (batch <= 64 && rows <= kOneCtaRows)
-        return cuda_status(launch_pdl(token_begin_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, p),
+        return cuda_status(launch_pdl(token_begin_kernel<1, true>, dim3(1), dim3(kPlanThreads), 0, s, p),
                            "token_begin_kernel");
-    cudaError_t e = launch_pdl(token_begin_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, p);
+    // requests a thread: the fewest of 1, 2, 8 and 64 that the batch needs
+    cudaError_t e =
+        batch <= kPlanThreads
+            ? launch_pdl(token_begin_kernel<1, false>, dim3(1), dim3(plan_threads(batch, 1)), 0, s, p)
+        : batch <= 2 * kPlanThreads
+            ? launch_pdl(token_begin_kernel<2, false>, dim3(1), dim3(plan_threads(batch, 2)), 0, s, p)
+        : batch <= 8 * kPlanThreads
+            ? launch_pdl(token_begin_kernel<8, false>, dim3(1), dim3(plan_threads(batch, 8)), 0, s, p)
+            : launch_pdl(token_begin_kernel<64, false>, dim3(1), dim3(plan_threads(batch, 64)), 0, s, p);
     if (e != cudaSuccess) return cuda_status(e, "token_begin_kernel");
     const int64_t warps = parents ? (int64_t)batch : ((int64_t)rows + 31) / 32;
     return cuda_status(launch_pdl(token_fill_kernel,
@@ -615,9 +650,16 @@ int launch_token_truncate(const pk_token_kv *kv, const int32_t *slots, const int
     p.batch = batch;
     p.ps_shift = kv->ps_shift;
     if (batch <= 64 && (int64_t)batch * kv->d.table_width <= 2 * kOneCtaRows)
-        return cuda_status(launch_pdl(token_cut_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, p),
+        return cuda_status(launch_pdl(token_cut_kernel<1, true>, dim3(1), dim3(kPlanThreads), 0, s, p),
                            "token_cut_kernel");
-    cudaError_t e = launch_pdl(token_cut_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, p);
+    cudaError_t e =
+        batch <= kPlanThreads
+            ? launch_pdl(token_cut_kernel<1, false>, dim3(1), dim3(plan_threads(batch, 1)), 0, s, p)
+        : batch <= 2 * kPlanThreads
+            ? launch_pdl(token_cut_kernel<2, false>, dim3(1), dim3(plan_threads(batch, 2)), 0, s, p)
+        : batch <= 8 * kPlanThreads
+            ? launch_pdl(token_cut_kernel<8, false>, dim3(1), dim3(plan_threads(batch, 8)), 0, s, p)
+            : launch_pdl(token_cut_kernel<64, false>, dim3(1), dim3(plan_threads(batch, 64)), 0, s, p);
     if (e != cudaSuccess) return cuda_status(e, "token_cut_kernel");
     return cuda_status(launch_pdl(token_cut_fill_kernel, dim3(grid_for((int64_t)batch * 32, 256)),
                                   dim3(256), 0, s, p),

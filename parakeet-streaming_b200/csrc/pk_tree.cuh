@@ -50,60 +50,104 @@ struct Unit {
 // The units of one CTA, in order: a walk over its share of the line of tiles.
 struct Work {
     const TreeParams &p;
-    int cta, b, nr, kt;
-    int64_t at, end, base, next_base;
+    int cta, b, nr, kt;        // request, its row tiles and key tiles
+    int head, rt, t;           // the next unit's K/V head, row tile and first key tile
+    int64_t left;              // tiles (or row tiles) left to this CTA
     bool whole;
     Unit u;
 
     __device__ __forceinline__ Work(const TreeParams &params, int c) : p(params), cta(c) {
         b = p.step[p.l.first + c];
-        const int64_t share = p.step[kTokShare];
+        const int share = p.step[kTokShare];
         whole = share == 0;
-        at = whole ? c : c * share;
-        end = b < 0 ? at : at + (whole ? 1 : share);
-        if (b >= 0) load();
+        left = 0;
+        if (b < 0) return;
+        load();
+        const int64_t *work = reinterpret_cast<const int64_t *>(p.step + p.l.work);
+        const int64_t at = whole ? (int64_t)c : (int64_t)c * share, local = at - work[b];
+        left = min(whole ? (int64_t)1 : (int64_t)share, work[p.batch] - at);
+        int64_t item = local;
+        t = 0;
+        if (!whole) {
+            item = local / kt;
+            t = (int)(local - item * kt);
+        }
+        head = (int)(item / nr);
+        rt = (int)(item - (int64_t)head * nr);
     }
     __device__ __forceinline__ void load() {
-        const int64_t *work = reinterpret_cast<const int64_t *>(p.step + p.l.work);
-        base = work[b];
-        next_base = work[b + 1];
         u.ctx = p.step[p.l.context + b];
         u.slot = p.step[p.l.slot + b];
         u.row0 = p.step[p.l.row_start + b];
         u.count = p.step[p.l.row_start + b + 1] - u.row0;
-        nr = (int)(((int64_t)u.count * p.group + p.shape.rows - 1) / p.shape.rows);
+        nr = u.ctx < 0 ? 0 : (int)(((int64_t)u.count * p.group + p.shape.rows - 1) / p.shape.rows);
         kt = (u.ctx + u.count + p.shape.keys - 1) / p.shape.keys;
     }
     __device__ __forceinline__ bool next() {
-        if (at >= end) return false;
-        while (at >= next_base) {   // requests without work have no tiles
-            if (++b >= p.batch) return false;
-            load();
+        if (left <= 0) return false;
+        if (head == p.kv_heads) {   // the next request that has rows
+            do {
+                if (++b >= p.batch) return false;
+                load();
+            } while (nr == 0);
+            head = 0;
         }
-        const int64_t local = at - base;
-        int item;
+        u.head = head;
+        u.rt = rt;
+        u.t0 = t;
         if (whole) {
-            item = (int)local;
-            u.t0 = 0;
             u.t1 = kt;
             u.part = -1;
-            ++at;
+            --left;
         } else {
-            item = (int)(local / kt);
-            u.t0 = (int)(local - (int64_t)item * kt);
-            const int n = (int)min((int64_t)(kt - u.t0), end - at);
-            u.t1 = u.t0 + n;
-            u.part = n == kt ? -1 : (u.t0 == 0 ? 2 * cta + 1 : 2 * cta);
-            at += n;
+            const int n = (int)min((int64_t)(kt - t), left);
+            u.t1 = t + n;
+            u.part = n == kt ? -1 : (t == 0 ? 2 * cta + 1 : 2 * cta);
+            left -= n;
         }
-        u.head = item / nr;
-        u.rt = item - u.head * nr;
+        t = u.t1 == kt ? 0 : u.t1;
+        if (t == 0 && ++rt == nr) {
+            rt = 0;
+            ++head;
+        }
         if (!p.trees) {   // a chain's rows see no key past their own
             const int64_t last = ((int64_t)(u.rt + 1) * p.shape.rows + p.group - 1) / p.group;
             const int seen = u.ctx + (int)min(last, (int64_t)u.count);
             u.t1 = min(u.t1, (seen + p.shape.keys - 1) / p.shape.keys);
         }
         return true;
+    }
+};
+
+// Page ids of a unit's tiles, for the warp that issues their loads: 32 table entries
+// at a time, one in a lane, the next 32 requested ahead.  (A load of its own for each
+// tile puts its latency, as long as a tile's share of the memory rate, between the
+// tiles.)  The pages of a tile never cross a multiple of 32: a tile has a power of
+// two of them, or one.
+struct Pages {
+    const int32_t *table;
+    int width, block, ids, ahead;
+
+    __device__ __forceinline__ int fetch(int at) const {
+        const int i = at + (threadIdx.x & 31);
+        return i < width ? table[i] : -1;
+    }
+    // the first entries of a unit; used a unit before it begins
+    __device__ __forceinline__ void open(const TreeParams &p, const Unit &w) {
+        table = p.table + (int64_t)w.slot * p.table_width;
+        width = p.table_width;
+        block = ((w.t0 * p.shape.keys) >> p.ps_shift) & ~31;
+        ids = fetch(block);
+        ahead = fetch(block + 32);
+    }
+    // entry `at` of the caller's lane; uniform in at / 32
+    __device__ __forceinline__ int get(int at) {
+        while (at >= block + 32) {
+            ids = ahead;
+            block += 32;
+            ahead = fetch(block + 32);
+        }
+        return __shfl_sync(0xffffffffu, ids, at & 31);
     }
 };
 

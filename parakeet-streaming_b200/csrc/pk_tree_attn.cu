@@ -118,20 +118,21 @@ __global__ void __launch_bounds__(kThreads, 2)
         int it = 0;   // ring use
         bool stop = false;   // the warp's, so that its lanes stay together
         Work work(p, blockIdx.x);
-        while (!stop && work.next()) {
-            const Unit &w = work.u;
-            const int head = w.head;
-            const int32_t *table = p.table + (int64_t)w.slot * p.table_width;
+        Pages pages, then;
+        bool more = work.next();
+        Unit w = work.u;
+        if (more) pages.open(p, w);
+        while (more && !stop) {
+            more = work.next();
+            if (more) then.open(p, work.u);
             const int len = w.ctx + w.count;
             for (int t = w.t0; t < w.t1 && !stop; ++t) {
                 const int k0 = t * kTile, n = (min(kTile, len - k0) + rows_box - 1) / rows_box;
-                int page = 0;
-                if (box_of < n) {
-                    page = table[(k0 + box_of * rows_box) >> p.ps_shift];
-                    if (page < 0 || page >= p.num_pages) {
-                        raise(p.error, PK_DEV_BAD_PAGE);
-                        page = 0;
-                    }
+                // lanes without a box ask for the last one's page
+                int page = pages.get((k0 + min(box_of, n - 1) * rows_box) >> p.ps_shift);
+                if (page < 0 || page >= p.num_pages) {
+                    raise(p.error, PK_DEV_BAD_PAGE);
+                    page = 0;
                 }
                 const int in_page = (k0 + box_of * rows_box) & (ps - 1);
 #pragma unroll
@@ -145,9 +146,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                     if (box_of < n)
                         tma_load_3d(ring + s * S::kSlot + col * S::kBox + box_of * bytes, &kv_map,
                                     &full[s], col * 64, in_page,
-                                    ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + head);
+                                    ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
                 }
             }
+            w = work.u;
+            pages = then;
         }
         if (stop) {   // leave no copy in flight
             for (int s = 0; s < NS; ++s)
@@ -663,7 +666,7 @@ int64_t max_items(const pk_token_kv *kv, int batch, int rows, const TokShape &sh
 // No row tile of such a step is shared by CTAs: as begin_plan decides, for the
 // longest request that the pool holds.
 bool never_shared(const pk_token_kv *kv, int batch, int rows, const TokShape &sh) {
-    return (int64_t)kv->d.table_width << kv->ps_shift <= kTokMinKeys &&
+    return (int64_t)kv->d.table_width << kv->ps_shift <= (int64_t)sh.least * sh.keys &&
            max_items(kv, batch, rows, sh) <= sh.ctas;
 }
 

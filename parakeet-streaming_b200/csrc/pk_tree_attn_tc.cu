@@ -3,16 +3,18 @@
 //
 // Bound by reading K and V as long as a request's rows fit one tile: 128 keys of a
 // 128-wide head are 64 KB, 2800 cycles of an SM's share of the memory rate, for
-// 1024 cycles of MMAs and about 1300 of exponentials.  So one CTA an SM with one
-// softmax warpgroup, and the scores of tile j + 1 made while tile j is weighted:
+// 1024 cycles of MMAs and 1024 of exponentials, but some 2400 of a warpgroup's whole
+// softmax (loads from TMEM, maximum, sum, conversions).  So one CTA an SM, and two
+// softmax warpgroups that take every other tile:
 //   warp 0      pages of K and V by TMA into a ring of slots (a slot: one tile of
 //               K or of V), running ahead over the CTA's units
 //   warp 1      one thread issues S_j = Q K_j^T (both from shared memory, fp32 in
 //               TMEM, two buffers) and O += P_j V_j (P from TMEM, V from shared
 //               memory as it lies: a row-major [keys][dim] tile is the MN-major
-//               operand), O in TMEM
-//   warps 2..5  a thread per row (TMEM lane): the row's scores without a shuffle,
-//               maximum, exp2, P as bf16 into TMEM, fp32 sum
+//               operand), O in TMEM, one for the even tiles and one for the odd
+//   warps 4..11 a thread per row (TMEM lane), warps 4..7 for the even tiles: the row's
+//               scores without a shuffle, maximum, exp2, P as bf16 over the scores,
+//               fp32 sum; maxima, sums and O of the two meet at the end of a unit
 // The running maximum is raised, and O scaled for it, only when a row's scores pass
 // the one in use by more than 2^8: weights stay below 256, which the fp32 sums and
 // bf16's exponent hold, and most tiles touch O in the MMA alone.
@@ -24,7 +26,7 @@
 namespace pk {
 namespace {
 
-constexpr int kRows = 128, kKeys = 128, kTcThreads = 192;
+constexpr int kRows = 128, kKeys = 128, kTcThreads = 128 + 256;
 constexpr float kRaise = 8.f;   // log2 of how far scores may pass the maximum in use
 
 template <int DH>
@@ -34,8 +36,8 @@ struct TcShape {
     static constexpr int kSlot = kCols * kBox;         // one tile of K, V or Q
     static constexpr int kSlots = 5 * (128 / DH);      // 160 KB
     static constexpr int kSmem = (kSlots + 1) * kSlot + 1024;
-    // TMEM columns: S and P twice each, O
-    static constexpr int kS = 0, kP = 2 * kKeys, kO = kP + kKeys, kTmem = 512;
+    // TMEM columns: S twice (P over it), O twice
+    static constexpr int kS = 0, kO = 2 * kKeys, kTmem = 512;
 };
 
 // O += P V: A from TMEM (bf16 pairs), B MN-major
@@ -69,19 +71,21 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-// barrier of the four softmax warps that also ORs a flag over them
-__device__ __forceinline__ bool softmax_any(bool v) {
+// barrier of one softmax group (four warps) that also ORs a flag over them
+__device__ __forceinline__ bool group_any(int group, bool v) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.or.pred q, 1, 128, p;\n\t"
+        "bar.red.or.pred q, %2, 128, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"((uint32_t)v)
+        : "r"((uint32_t)v), "r"(2 + group)
         : "memory");
     return r != 0;
 }
+// barrier of both groups
+__device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Bits of keys rel0 .. rel0 + 31 of the step's own tokens that a row sees.
 __device__ __forceinline__ uint32_t seen_bits(int trees, uint64_t mask, int node, int rel0) {
@@ -104,7 +108,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t *sq = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = sq + S::kSlot;
-    __shared__ __align__(8) uint64_t full[NS], empty[NS], q_full, s_full[2], p_full[2], o_done, idle;
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], q_full, s_full[2], p_full[2], o_done[2],
+        idle;
+    __shared__ float s_max[2][kRows], s_sum[2][kRows];
+    __shared__ int s_odd[2];
     __shared__ uint32_t tmem_base;
     __shared__ volatile int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -113,12 +120,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(&q_full, 4);
+        mbar_init(&q_full, 8);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
         }
-        mbar_init(&o_done, 1);
         mbar_init(&idle, 1);
         failed = 0;
         fence_mbar_init();
@@ -134,28 +141,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = tmem_base;
     grid_dep_wait();
     grid_dep_launch();
-    Work work(p, blockIdx.x);
-
-    if (warp == 0) {
+    auto produce = [&]() {
         // producer: lanes issue a tile's boxes, K then V
         const int ps = 1 << p.ps_shift, rows_box = min(ps, 64);
         const int box_of = lane / S::kCols, col = lane % S::kCols;
         const uint32_t bytes = rows_box * 128;
         int it = 0;
         bool stop = false;   // the warp's, so that its lanes stay together
-        while (!stop && work.next()) {
-            const Unit &w = work.u;
-            const int32_t *table = p.table + (int64_t)w.slot * p.table_width;
+        Work work(p, blockIdx.x);
+        Pages pages, then;
+        bool more = work.next();
+        Unit w = work.u;
+        if (more) pages.open(p, w);
+        while (more && !stop) {
+            more = work.next();
+            if (more) then.open(p, work.u);
             const int len = w.ctx + w.count;
             for (int t = w.t0; t < w.t1 && !stop; ++t) {
                 const int k0 = t * kKeys, n = (min(kKeys, len - k0) + rows_box - 1) / rows_box;
-                int page = 0;
-                if (box_of < n) {
-                    page = table[(k0 + box_of * rows_box) >> p.ps_shift];
-                    if (page < 0 || page >= p.num_pages) {
-                        raise(p.error, PK_DEV_BAD_PAGE);
-                        page = 0;
-                    }
+                // lanes without a box ask for the last one's page
+                int page = pages.get((k0 + min(box_of, n - 1) * rows_box) >> p.ps_shift);
+                if (page < 0 || page >= p.num_pages) {
+                    raise(p.error, PK_DEV_BAD_PAGE);
+                    page = 0;
                 }
                 const int in_page = (k0 + box_of * rows_box) & (ps - 1);
 #pragma unroll
@@ -172,64 +180,82 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                     ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
                 }
             }
+            w = work.u;
+            pages = then;
         }
         if (stop)   // leave no copy in flight
             for (int s = 0; s < NS; ++s)
                 if (it > s) mbar_wait_bounded(&full[s], ((it - 1 - s) / NS) & 1, kWaitLimitNs);
-    } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc_bf16(kRows, kKeys);
-            constexpr uint32_t id_o = idesc_bf16(kRows, DH) | (1u << 16);   // B MN-major
-            const uint32_t q0 = smem_u32(sq);
-            int it = 0, j = 0, unit = 0;   // ring use, tile and unit of this CTA
-            // S_j of the tile whose K is ring use `use`
-            auto scores = [&](int use, int tile) {
-                const int s = use % NS;
-                ring_wait(&full[s], (use / NS) & 1, &failed, p.error);
-                tc_fence_after();
-                const uint32_t k0 = smem_u32(ring + s * S::kSlot);
+    };
+    auto multiply = [&]() {
+        Work work(p, blockIdx.x);
+        constexpr uint32_t id_s = idesc_bf16(kRows, kKeys);
+        constexpr uint32_t id_o = idesc_bf16(kRows, DH) | (1u << 16);   // B MN-major
+        const uint32_t q0 = smem_u32(sq);
+        int it = 0, j = 0, unit = 0;   // ring use, tile and unit of this CTA
+        // S of a tile whose K is ring use `use`, over the P of the tile two before, whose
+        // product has to be done with it
+        auto scores = [&](int use, int tile) {
+            const int s = use % NS;
+            if (tile >= 2) ring_wait(&o_done[tile & 1], ((tile >> 1) - 1) & 1, &failed, p.error);
+            ring_wait(&full[s], (use / NS) & 1, &failed, p.error);
+            tc_fence_after();
+            const uint32_t k0 = smem_u32(ring + s * S::kSlot);
 #pragma unroll
-                for (int kk = 0; kk < DH / 16; ++kk) {
-                    const uint32_t off = (kk / 4) * S::kBox + (kk % 4) * 32;
-                    umma_bf16(tmem + S::kS + (tile & 1) * kKeys, sw128_desc(q0 + off),
-                              sw128_desc(k0 + off), id_s, kk != 0);
-                }
-                umma_commit(&empty[s]);
-                umma_commit(&s_full[tile & 1]);
-            };
-            while (!failed && work.next()) {
-                const int n = work.u.t1 - work.u.t0;
-                if (n <= 0) continue;
-                ring_wait(&q_full, unit & 1, &failed, p.error);
-                ++unit;
-                tc_fence_after();
-                scores(it, j);
-                for (int i = 0; i < n && !failed; ++i, ++j, it += 2) {
-                    if (i + 1 < n) scores(it + 2, j + 1);
-                    const int s = (it + 1) % NS;
-                    ring_wait(&full[s], ((it + 1) / NS) & 1, &failed, p.error);
-                    ring_wait(&p_full[j & 1], (j >> 1) & 1, &failed, p.error);
-                    if (failed) break;
-                    tc_fence_after();
-                    const uint32_t v0 = smem_u32(ring + s * S::kSlot);
-#pragma unroll
-                    for (int kk = 0; kk < kKeys / 16; ++kk)
-                        umma_bf16_ts(tmem + S::kO, tmem + S::kP + (j & 1) * (kKeys / 2) + kk * 8,
-                                     mn_desc(v0 + kk * 2048, S::kBox), id_o, (i | kk) != 0);
-                    umma_commit(&empty[s]);
-                    umma_commit(&o_done);
-                }
+            for (int kk = 0; kk < DH / 16; ++kk) {
+                const uint32_t off = (kk / 4) * S::kBox + (kk % 4) * 32;
+                umma_bf16(tmem + S::kS + (tile & 1) * kKeys, sw128_desc(q0 + off),
+                          sw128_desc(k0 + off), id_s, kk != 0);
             }
-            umma_commit(&idle);   // no MMA is left when the CTA frees its TMEM
-            mbar_wait_bounded(&idle, 0, kWaitLimitNs);
+            umma_commit(&empty[s]);
+            umma_commit(&s_full[tile & 1]);
+        };
+        while (!failed && work.next()) {
+            const int n = work.u.t1 - work.u.t0;
+            if (n <= 0) continue;
+            ring_wait(&q_full, unit & 1, &failed, p.error);
+            ++unit;
+            tc_fence_after();
+            scores(it, j);
+            for (int i = 0; i < n && !failed; ++i, ++j, it += 2) {
+                if (i + 1 < n) scores(it + 2, j + 1);
+                const int s = (it + 1) % NS;
+                ring_wait(&full[s], ((it + 1) / NS) & 1, &failed, p.error);
+                ring_wait(&p_full[j & 1], (j >> 1) & 1, &failed, p.error);
+                if (failed) break;
+                tc_fence_after();
+                const uint32_t v0 = smem_u32(ring + s * S::kSlot);
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                    umma_bf16_ts(tmem + S::kO + (j & 1) * DH,
+                                 tmem + S::kS + (j & 1) * kKeys + kk * 8,
+                                 mn_desc(v0 + kk * 2048, S::kBox), id_o, (i > 1) | (kk != 0));
+                umma_commit(&empty[s]);
+                umma_commit(&o_done[j & 1]);
+            }
         }
+        umma_commit(&idle);   // no MMA is left when the CTA frees its TMEM
+        mbar_wait_bounded(&idle, 0, kWaitLimitNs);
+    };
+
+    // a row's scores take 128 registers: 208 for the softmax warps out of the launch's
+    // 168 x 384, 88 for the other warpgroup (128 x 88 + 256 x 208 = 64512)
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 0) produce();
+        else if (warp == 1 && lane == 0) multiply();
     } else {
-        // softmax: thread = row (TMEM lane) 32 (warp % 4) + lane of the tile
-        const int quad = warp & 3, rt = quad * 32 + lane;
-        const uint32_t mine = tmem + ((uint32_t)(quad * 32) << 16);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        Work work(p, blockIdx.x);
+        // softmax group g takes the CTA's tiles j with j % 2 == g; thread = row (TMEM
+        // lane) 32 (warp % 4) + lane of the tile
+        const int g = (warp >> 2) - 1, quad = warp & 3, rt = quad * 32 + lane;
+        const int gt = threadIdx.x & 127;   // thread in the group
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const uint32_t st = tmem + lanes + S::kS + g * kKeys, ot = tmem + lanes + S::kO + g * DH;
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
         __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
-        int it = 0, j = 0;
+        int it = 0, j = 0;   // ring use and tile of the unit's first tile
         while (work.next()) {
             const Unit &w = work.u;
             const int r = w.rt * kRows + rt, n = w.t1 - w.t0, len = w.ctx + w.count;
@@ -242,30 +268,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float m = -INFINITY, l = 0.f;   // the maximum in use (scaled), the sum
             bool odd = false;               // a value that is not finite among the own rows
             if (n > 0) {
-                // the tile's queries; the MMAs that read the last ones are done, since
-                // their scores have been read
+                // the tile's queries, half a group; the MMAs that read the last ones are
+                // done, since both groups have read their scores
                 const uint4 *src = reinterpret_cast<const uint4 *>(q + row * p.q_rs + qh * p.q_hs);
 #pragma unroll
-                for (int c = 0; c < DH / 8; ++c)
+                for (int i = 0; i < DH / 16; ++i) {
+                    const int c = g * (DH / 16) + i;
                     *reinterpret_cast<uint4 *>(sq + (c / 8) * S::kBox + sw128(rt, (c % 8) * 16)) =
                         live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+                }
                 fence_async_proxy();
                 __syncwarp();
                 if (lane == 0) arrive(&q_full);
             }
-            for (int i = 0; i < n; ++i, ++j, it += 2) {
+            int mine = 0;   // tiles of this group in the unit
+            for (int i = (g ^ j) & 1; i < n; i += 2, ++mine) {
+                const int tile = j + i, use = it + 2 * i;
                 const int k0 = (w.t0 + i) * kKeys;
-                const uint32_t st = mine + S::kS + (j & 1) * kKeys;
-                ring_wait(&s_full[j & 1], (j >> 1) & 1, &failed, p.error);
+                ring_wait(&s_full[g], (tile >> 1) & 1, &failed, p.error);
                 __syncwarp();
                 tc_fence_after();
                 float s[kKeys];
 #pragma unroll
                 for (int c = 0; c < kKeys / 32; ++c)
                     tmem_ld32(st + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
-                const bool own = k0 + kKeys > w.ctx;
-                if (own) {
-                    const int sv = (it + 1) % NS;
+                if (k0 + kKeys > w.ctx) {   // some of the step's own tokens, or the end
+                    const int sv = (use + 1) % NS;
 #pragma unroll
                     for (int c = 0; c < kKeys / 32; ++c) {
                         const uint32_t bits = seen_bits(p.trees, mask, node, k0 + c * 32 - w.ctx);
@@ -277,10 +305,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     // values may be inf or NaN: zero in the product, where a weight of
                     // zero would not keep them out; the epilogue adds the latter to the
                     // rows that see them
-                    ring_wait(&full[sv], ((it + 1) / NS) & 1, &failed, p.error);
+                    ring_wait(&full[sv], ((use + 1) / NS) & 1, &failed, p.error);
                     uint8_t *vs = ring + sv * S::kSlot;
                     bool bad = false;
-                    for (int c = threadIdx.x - 64; c < kKeys * DH / 8; c += 128) {
+                    for (int c = gt; c < kKeys * DH / 8; c += 128) {
                         const int vr = c / (DH / 8), ch = c % (DH / 8), key = k0 + vr;
                         if (key < w.ctx) continue;
                         uint4 *at = reinterpret_cast<uint4 *>(vs + (ch / 8) * S::kBox +
@@ -307,34 +335,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         *at = x;
                     }
                     fence_async_proxy();
-                    odd |= softmax_any(bad);
+                    odd |= group_any(g, bad);
                 }
-                float top = s[0];
+                float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int e = 1; e < kKeys; ++e) top = fmaxf(top, s[e]);
+                for (int e = 4; e < kKeys; ++e) tops[e & 3] = fmaxf(tops[e & 3], s[e]);
+                float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 top = top == -INFINITY ? top : __fmul_rn(top, p.scale_log2);
                 const bool raise_it = top > m + kRaise || (m == -INFINITY && top > m);
                 if (__any_sync(0xffffffffu, raise_it)) {
                     const float keep = raise_it ? ex2(m - top) : 1.f;
                     if (raise_it) m = top;
                     l *= keep;
-                    if (i > 0) {   // O has the tiles before
-                        ring_wait(&o_done, (j - 1) & 1, &failed, p.error);
+                    if (mine > 0) {   // O has the group's tiles before
+                        ring_wait(&o_done[g], ((tile >> 1) - 1) & 1, &failed, p.error);
                         __syncwarp();
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DH / 32; ++c) {
                             float o[32];
-                            tmem_ld32(mine + S::kO + c * 32, o);
+                            tmem_ld32(ot + c * 32, o);
                             uint32_t x[32];
 #pragma unroll
                             for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(o[e] * keep);
-                            tmem_st32(mine + S::kO + c * 32, x);
+                            tmem_st32(ot + c * 32, x);
                         }
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : m;
-                float sum = 0.f;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t x[32];
@@ -342,33 +371,60 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int e = 0; e < 32; ++e) {
                         const float a = ex2(s[c * 64 + 2 * e] * p.scale_log2 - base);
                         const float b = ex2(s[c * 64 + 2 * e + 1] * p.scale_log2 - base);
-                        sum += a + b;
+                        sum[(2 * e) & 3] += a;
+                        sum[(2 * e + 1) & 3] += b;
                         x[e] = pack2(a, b);
                     }
-                    tmem_st32(mine + S::kP + (j & 1) * (kKeys / 2) + c * 32, x);
+                    tmem_st32(st + c * 32, x);   // P over the scores, all of them read
                 }
-                l += sum;
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(&p_full[j & 1]);
+                if (lane == 0) arrive(&p_full[g]);
             }
+            // the last tile of each group in O, and the groups' maxima and sums
+            const int last = j + n - 1;   // the CTA's last tile; the other group's is the one before
             if (n > 0) {
-                ring_wait(&o_done, (j - 1) & 1, &failed, p.error);
+                if (n > 1 || (last & 1) == 0)
+                    ring_wait(&o_done[0], ((last & 1 ? last - 1 : last) >> 1) & 1, &failed, p.error);
+                if (n > 1 || (last & 1) == 1)
+                    ring_wait(&o_done[1], ((last & 1 ? last : last - 1) >> 1) & 1, &failed, p.error);
                 __syncwarp();
                 tc_fence_after();
             }
-            const float inv = 1.f / l;
+            j += n > 0 ? n : 0;
+            it += n > 0 ? 2 * n : 0;
+            s_max[g][rt] = m;
+            s_sum[g][rt] = l;
+            if (gt == 0) s_odd[g] = odd;
+            groups_sync();
+            odd = s_odd[0] | s_odd[1];
+            // a group without a tile has O that was never written: a factor of 0 and no
+            // product with it
+            const float ma = s_max[0][rt], mb = s_max[1][rt], mm = fmaxf(ma, mb);
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            const float fa = ex2(ma - ref), fb = ex2(mb - ref);
+            const float ls = fa * s_sum[0][rt] + fb * s_sum[1][rt];
+            const bool has_a = n > 1 || (n == 1 && (last & 1) == 0),
+                       has_b = n > 1 || (n == 1 && (last & 1) == 1);
+            const float inv = 1.f / ls;
             float *dst = p.ws_o + ((int64_t)w.part * kRows + rt) * DH;
             __nv_bfloat16 *o_row = out + row * p.o_rs + qh * p.o_hs;
 #pragma unroll 1
-            for (int c = 0; c < DH / 32; ++c) {
-                float o[32];
-                if (n > 0) {
-                    tmem_ld32(mine + S::kO + c * 32, o);
-                } else {
+            for (int c = g * (DH / 64); c < (g + 1) * (DH / 64); ++c) {   // half the columns each
+                float o[32], x[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                if (has_a) {
+                    tmem_ld32(tmem + lanes + S::kO + c * 32, x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = fa * x[e];
+                }
+                if (has_b) {
+                    tmem_ld32(tmem + lanes + S::kO + DH + c * 32, x);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] += fb * x[e];
                 }
                 if (!live) continue;
                 if (odd) {
@@ -387,8 +443,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                              (key & (ps - 1))) * DH + c * 32;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            const float x = __bfloat162float(v[e]);
-                            if (!isfinite(x)) o[e] += x;
+                            const float y = __bfloat162float(v[e]);
+                            if (!isfinite(y)) o[e] += y;
                         }
                     }
                 }
@@ -407,10 +463,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
                 }
             }
-            if (w.part >= 0 && live)
+            if (g == 0 && w.part >= 0 && live)
                 *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)w.part * kRows + rt) * 2) =
-                    make_float2(m, l);
-            tc_fence_before();   // O is read before the next unit's MMAs (by its q_full)
+                    make_float2(mm, ls);
+            tc_fence_before();
+            groups_sync();   // O and the exchange are free again
         }
     }
     tc_fence_before();
