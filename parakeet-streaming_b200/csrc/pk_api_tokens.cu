@@ -56,10 +56,14 @@ int pk_token_kv_create(const pk_token_kv_desc *desc, pk_token_kv **out) {
     while ((1 << kv->ps_shift) < d.page_size) ++kv->ps_shift;
     kv->sms = current_sms();
     if (d.dtype == PK_DTYPE_BF16) {
-        const uint64_t row = (uint64_t)d.head_dim * 2;
-        int st = encode_tmap_3d(&kv->kv_map, d.dtype, d.kv, d.head_dim, d.page_size,
-                                (uint64_t)planes, row, row * d.page_size, 64,
-                                d.page_size < 64 ? d.page_size : 64, 1);
+        // a page's rows of one head in one copy, laid out in groups of 8 rows of 128
+        // bytes (a swizzle atom), the 64-column blocks of a group beside each other
+        const uint64_t row = (uint64_t)d.head_dim * 2, blocks = d.head_dim / 64;
+        const uint64_t dims[5] = {64, 8, blocks, (uint64_t)d.page_size / 8, (uint64_t)planes};
+        const uint64_t strides[4] = {row, 128, 8 * row, row * d.page_size};
+        const uint32_t groups = (d.page_size < 64 ? d.page_size : 64) / 8;
+        const uint32_t box[5] = {64, 8, (uint32_t)blocks, groups, 1};
+        int st = encode_tmap(&kv->kv_map, d.dtype, d.kv, 5, dims, strides, box);
         if (st != PK_OK) {
             free(kv);
             return st;

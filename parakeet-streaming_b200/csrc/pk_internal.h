@@ -211,8 +211,8 @@ int launch_features(const FeArgs &a, cudaStream_t s);
 
 struct pk_token_kv {
     pk_token_kv_desc d;
-    CUtensorMap kv_map;  // bf16 pools: {head_dim, page_size, pages*layers*2*kv_heads}, boxes of
-                         // 64 columns x min(page_size, 64) rows, 128B-swizzled
+    CUtensorMap kv_map;  // bf16 pools: {64, 8, head_dim / 64, page_size / 8, pages*layers*2*
+                         // kv_heads}, boxes of min(page_size, 64) rows, 128B-swizzled
     int ps_shift, esize, group;
     int sms;
 };

@@ -40,6 +40,24 @@ __device__ __forceinline__ void ring_wait(uint64_t *bar, uint32_t parity, volati
     }
 }
 
+// kv_map's copy of a page's rows from `row` on (a multiple of 8): groups of 8 rows, in
+// each the 64-column blocks, 1024 bytes a block.
+__device__ __forceinline__ void tma_load_rows(void *dst, const CUtensorMap *map, uint64_t *bar,
+                                              int32_t row, int32_t plane) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(0), "r"(0), "r"(row >> 3), "r"(plane),
+        "r"(smem_u32(bar))
+        : "memory");
+}
+// Byte of a tile laid out so: row, 16-byte chunk of the row (8 a column block).
+template <int DH>
+__device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t chunk) {
+    return (row >> 3) * (DH / 64 * 1024) + (chunk >> 3) * 1024 + (row & 7) * 128 +
+           (((chunk ^ row) & 7) << 4);
+}
+
 // A row tile of one request and K/V head over key tiles [t0, t1).
 struct Unit {
     int slot, row0, count, ctx;   // the request: table row, first row, tokens, context

@@ -11,8 +11,8 @@
 // CTA, whatever the lengths; a second launch joins the row tiles that a cut went
 // through (two partial results a CTA at most).
 //
-// bf16, row tiles of 16 and 32: a producer warp brings each tile's pages (TMA boxes of a page's rows x
-// 64 columns, 128B swizzle) into a ring of K and V slots that runs ahead across
+// bf16, row tiles of 16 and 32: a producer warp brings each tile's pages (one TMA copy a page, 128B
+// swizzle) into a ring of K and V slots that runs ahead across
 // units; four warps hold 16-row fragments of the row tile and compute
 // S = Q K^T and O += P V with mma.sync m16n8k16.  The warps share the keys of a tile
 // (4 / (rows / 16) ways) and join through shared memory at the end.  P is rounded to bf16 for the product, relative
@@ -73,9 +73,7 @@ __device__ __forceinline__ bool sees(int trees, uint64_t mask, int node, int rel
 
 template <int DH, int BM>
 struct TreeShape {
-    static constexpr int kCols = DH / 64;                    // 128-byte column boxes of a row
-    static constexpr int kBox = kTile * 128;                 // one column box of a tile
-    static constexpr int kSlot = kCols * kBox;               // one tile of K or of V
+    static constexpr int kSlot = kTile * DH * 2;             // one tile of K or of V
     static constexpr int kWm = BM / 16, kWk = 4 / kWm;       // warps over rows, over keys
     // 64 KB of tiles beside the join buffer: two CTAs an SM
     static constexpr int kSlots = 4 * (128 / DH);
@@ -113,8 +111,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp == 4) {
         // producer: lanes issue a tile's boxes, K then V
         const int ps = 1 << p.ps_shift, rows_box = min(ps, kTile);
-        const int box_of = lane / S::kCols, col = lane % S::kCols;
-        const uint32_t bytes = rows_box * 128;
+        const int box_of = lane;
+        const uint32_t bytes = rows_box * DH * 2;
         int it = 0;   // ring use
         bool stop = false;   // the warp's, so that its lanes stay together
         Work work(p, blockIdx.x);
@@ -141,12 +139,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                     if (use) ring_wait(&empty[s], (use - 1) & 1, &failed, p.error);
                     stop = __any_sync(0xffffffffu, failed != 0);
                     if (stop) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * S::kCols * bytes);
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * bytes);
                     __syncwarp();
                     if (box_of < n)
-                        tma_load_3d(ring + s * S::kSlot + col * S::kBox + box_of * bytes, &kv_map,
-                                    &full[s], col * 64, in_page,
-                                    ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
+                        tma_load_rows(ring + s * S::kSlot + box_of * bytes, &kv_map, &full[s], in_page,
+                                      ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
                 }
             }
             w = work.u;
@@ -221,8 +218,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int nb = 0; nb < S::kKeys / 16; ++nb) {
                     uint32_t b[4];
                     const uint32_t row = key0 + nb * 16 + ((lane >> 4) << 3) + (lane & 7);
-                    ldsm4(kb + (ks / 4) * S::kBox +
-                              sw128(row, (ks % 4) * 32 + ((lane >> 3) & 1) * 16), b);
+                    ldsm4(kb + tile_at<DH>(row, ks * 2 + ((lane >> 3) & 1)), b);
                     mma16816(s[2 * nb], qf[ks], b[0], b[1]);
                     mma16816(s[2 * nb + 1], qf[ks], b[2], b[3]);
                 }
@@ -284,8 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 bool bad = false;
                 for (int c = threadIdx.x; c < kTile * DH / 8; c += kConsumers) {
                     const int row = c / (DH / 8), ch = c % (DH / 8);
-                    uint4 *at = reinterpret_cast<uint4 *>(
-                        vs + (ch / 8) * S::kBox + sw128(row, (ch % 8) * 16));
+                    uint4 *at = reinterpret_cast<uint4 *>(vs + tile_at<DH>(row, ch));
                     const int key = k0 + row;
                     if (key >= len) {
                         *at = make_uint4(0u, 0u, 0u, 0u);
@@ -311,8 +306,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     for (int nb = 0; nb < DH / 16; ++nb) {
                         uint32_t b[4];
                         const uint32_t row = key0 + kk * 16 + (lane & 15);
-                        ldsm4_t(vb + (nb / 4) * S::kBox +
-                                    sw128(row, (nb % 4) * 32 + (lane >> 4) * 16), b);
+                        ldsm4_t(vb + tile_at<DH>(row, nb * 2 + (lane >> 4)), b);
                         mma16816(o[2 * nb], a, b[0], b[1]);
                         mma16816(o[2 * nb + 1], a, b[2], b[3]);
                     }
@@ -334,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                         for (int n = 0; n < DH / 8; ++n) {
                             const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(
-                                vs + (n / 8) * S::kBox + sw128(row, (n % 8) * 16 + (lane & 3) * 4));
+                                vs + tile_at<DH>(row, n) + (lane & 3) * 4);
                             const float2 f = __bfloat1622float2(v);
                             if (w0 != 0.f) {
                                 o[n][0] += w0 * f.x;

@@ -31,9 +31,8 @@ constexpr float kRaise = 8.f;   // log2 of how far scores may pass the maximum i
 
 template <int DH>
 struct TcShape {
-    static constexpr int kCols = DH / 64;              // 128-byte column boxes
-    static constexpr int kBox = kKeys * 128;           // a box: 128 rows of 128 bytes
-    static constexpr int kSlot = kCols * kBox;         // one tile of K, V or Q
+    static constexpr int kSlot = kKeys * DH * 2;       // one tile of K, V or Q
+    static constexpr int kGroup = DH / 64 * 1024;      // 8 rows of one
     static constexpr int kSlots = 5 * (128 / DH);      // 160 KB
     static constexpr int kSmem = (kSlots + 1) * kSlot + 1024;
     // TMEM columns: S twice (P over it), O twice
@@ -50,11 +49,12 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
         "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Descriptor of an MN-major operand: boxes of 64 (MN) x keys (K), 128B swizzle; LBO
-// between boxes, SBO between groups of 8 keys (1024 bytes).
-__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t box_bytes) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(box_bytes >> 4) << 16) |
-           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Descriptor of a tile of tma_load_rows: 128B swizzle, `group` bytes between groups of
+// 8 rows (SBO).  As a K-major operand (rows x 64 columns of the dim) the LBO is unused;
+// as an MN-major one (the dim x keys) it is the 1024 bytes between 64-column blocks.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t group) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(1024 >> 4) << 16) |
+           ((uint64_t)(group >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     auto produce = [&]() {
         // producer: lanes issue a tile's boxes, K then V
         const int ps = 1 << p.ps_shift, rows_box = min(ps, 64);
-        const int box_of = lane / S::kCols, col = lane % S::kCols;
-        const uint32_t bytes = rows_box * 128;
+        const int box_of = lane;
+        const uint32_t bytes = rows_box * DH * 2;
         int it = 0;
         bool stop = false;   // the warp's, so that its lanes stay together
         Work work(p, blockIdx.x);
@@ -172,12 +172,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (use) ring_wait(&empty[s], (use - 1) & 1, &failed, p.error);
                     stop = __any_sync(0xffffffffu, failed != 0);
                     if (stop) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * S::kCols * bytes);
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * bytes);
                     __syncwarp();
                     if (box_of < n)
-                        tma_load_3d(ring + s * S::kSlot + col * S::kBox + box_of * bytes, &kv_map,
-                                    &full[s], col * 64, in_page,
-                                    ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
+                        tma_load_rows(ring + s * S::kSlot + box_of * bytes, &kv_map, &full[s], in_page,
+                                      ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
                 }
             }
             w = work.u;
@@ -203,9 +202,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t k0 = smem_u32(ring + s * S::kSlot);
 #pragma unroll
             for (int kk = 0; kk < DH / 16; ++kk) {
-                const uint32_t off = (kk / 4) * S::kBox + (kk % 4) * 32;
-                umma_bf16(tmem + S::kS + (tile & 1) * kKeys, sw128_desc(q0 + off),
-                          sw128_desc(k0 + off), id_s, kk != 0);
+                const uint32_t off = (kk / 4) * 1024 + (kk % 4) * 32;
+                umma_bf16(tmem + S::kS + (tile & 1) * kKeys, tile_desc(q0 + off, S::kGroup),
+                          tile_desc(k0 + off, S::kGroup), id_s, kk != 0);
             }
             umma_commit(&empty[s]);
             umma_commit(&s_full[tile & 1]);
@@ -229,7 +228,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int kk = 0; kk < kKeys / 16; ++kk)
                     umma_bf16_ts(tmem + S::kO + (j & 1) * DH,
                                  tmem + S::kS + (j & 1) * kKeys + kk * 8,
-                                 mn_desc(v0 + kk * 2048, S::kBox), id_o, (i > 1) | (kk != 0));
+                                 tile_desc(v0 + kk * 2 * S::kGroup, S::kGroup), id_o, (i > 1) | (kk != 0));
                 umma_commit(&empty[s]);
                 umma_commit(&o_done[j & 1]);
             }
@@ -274,7 +273,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                 for (int i = 0; i < DH / 16; ++i) {
                     const int c = g * (DH / 16) + i;
-                    *reinterpret_cast<uint4 *>(sq + (c / 8) * S::kBox + sw128(rt, (c % 8) * 16)) =
+                    *reinterpret_cast<uint4 *>(sq + tile_at<DH>(rt, c)) =
                         live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
                 }
                 fence_async_proxy();
@@ -311,8 +310,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int c = gt; c < kKeys * DH / 8; c += 128) {
                         const int vr = c / (DH / 8), ch = c % (DH / 8), key = k0 + vr;
                         if (key < w.ctx) continue;
-                        uint4 *at = reinterpret_cast<uint4 *>(vs + (ch / 8) * S::kBox +
-                                                              sw128(vr, (ch % 8) * 16));
+                        uint4 *at = reinterpret_cast<uint4 *>(vs + tile_at<DH>(vr, ch));
                         uint4 x = make_uint4(0u, 0u, 0u, 0u);
                         if (key < len) {
                             x = *at;
