@@ -100,14 +100,13 @@ __device__ __forceinline__ int page_of(const TokParams &p, int slot, int held, i
 template <int NK>
 __device__ void begin_plan(const TokParams &p) {
     __shared__ int64_t s_scan[33];
-    __shared__ unsigned long long s_take;
-    __shared__ int s_longest;
+    __shared__ int s_taken, s_longest;
     const pk_token_kv_desc &d = p.d;
     int32_t *st = p.step;
     const int b0 = threadIdx.x * NK;
     const int free_n = *d.free_count;
     if (threadIdx.x == 0) {
-        s_take = 0;
+        s_taken = free_n;
         s_longest = 0;
     }
     int slot[NK], count[NK], ctx[NK], held[NK], take[NK];
@@ -157,7 +156,8 @@ __device__ void begin_plan(const TokParams &p) {
 
     // pages, in batch order: requests past the end of the stack are left out
     int64_t first = block_exclusive_sum64(takes, total, s_scan);
-    int64_t tiles = 0, taken = 0;
+    const int64_t all_takes = total;
+    int64_t tiles = 0;
     int items = 0, longest = 0, nr[NK], kt[NK];   // row tiles and key tiles
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
@@ -167,9 +167,9 @@ __device__ void begin_plan(const TokParams &p) {
         st[p.l.take + b] = (int)min(first, (int64_t)0x7fffffff);
         if (take[k] > 0 && first + take[k] > free_n) {
             raise(d.error, PK_DEV_POOL_EXHAUSTED);
+            atomicMin(&s_taken, (int)min(first, (int64_t)free_n));   // the pages before it
             ctx[k] = -1;
         } else if (take[k] > 0) {
-            taken += take[k];
             d.held[slot[k]] = held[k] + take[k];
         }
         first += take[k];
@@ -182,8 +182,8 @@ __device__ void begin_plan(const TokParams &p) {
         items += nr[k];
         longest = max(longest, kt[k]);
     }
-    if (taken) atomicAdd(&s_take, (unsigned long long)taken);
-    if (longest) atomicMax(&s_longest, longest);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if ((threadIdx.x & 31) == 0 && longest) atomicMax(&s_longest, longest);
 
     // the attention's line of tiles: an equal share of it a CTA, but the shape's least
     // at least; a row tile each where there are no more of them than CTAs and none is
@@ -208,7 +208,7 @@ __device__ void begin_plan(const TokParams &p) {
     if (threadIdx.x == 0) {
         work[p.batch] = all;
         st[kTokShare] = (int)min(share, (int64_t)0x7fffffff);
-        *d.free_count = free_n - (int)s_take;
+        *d.free_count = free_n - (int)min(all_takes, (int64_t)s_taken);
     }
     // CTAs behind the last tile
     const int64_t used = whole ? all : (all + share - 1) / share;

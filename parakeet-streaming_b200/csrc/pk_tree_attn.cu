@@ -610,6 +610,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
         for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
         if (top == -INFINITY) top = 0.f;
         float acc[NV] = {}, sum = 0.f;
+#pragma unroll 4
         for (int c = c0; c <= c1; ++c) {
             const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + at(c) * 2);
             const float f = exp2f(ml.x - top);
