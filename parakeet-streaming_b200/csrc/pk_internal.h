@@ -225,16 +225,17 @@ namespace pk {
 struct TokShape {
     int rows, keys, ctas;
     int least;   // key tiles that a CTA takes before a request's are split over several
+    int lead;    // what beginning a row tile costs, in key tiles
 };
 // bf16: the narrowest row tile that holds an average request, since a request's K/V
 // is read once per row tile - 16 or 32 rows by mma.sync (two CTAs an SM), 128 by
 // tcgen05 (one).  float32: 16.
 inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
-    if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, 2 * kv->sms, 1};
-    if (mean <= 16) return {16, 64, 2 * kv->sms, 8};
-    if (mean <= 32) return {32, 64, 2 * kv->sms, 8};
-    return {128, 128, kv->sms, 4};
+    if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, 2 * kv->sms, 1, 1};
+    if (mean <= 16) return {16, 64, (kv->d.head_dim == 64 ? 4 : 2) * kv->sms, 8, 2};
+    if (mean <= 32) return {32, 64, 2 * kv->sms, 8, 2};
+    return {128, 128, kv->sms, 4, 2};
 }
 
 // Step block, int32 words: header, then arrays at these offsets.  The step's work
@@ -244,7 +245,7 @@ inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
 // row tile each).
 enum TokHeader { kTokShare = 0, kTokRows, kTokFree, kTokHeaderWords = 16 };
 struct TokLayout {
-    // work: int64 first tile (share 0: row tile) of each request; first: the request
+    // work: int64 first place (share 0: row tile) of each request; first: the request
     // that each CTA begins in (-1: no work); take: first new page; held: pages before
     int64_t row_start, context, slot, work, first, take, held, request, position, slot_map, mask,
         words;
@@ -262,7 +263,7 @@ inline TokLayout tok_layout(const pk_token_kv *kv, int batch, int rows, int tree
     l.row_start = take(batch + 1);
     l.context = take(batch);
     l.slot = take(batch);
-    l.first = take(2 * kv->sms);
+    l.first = take(4 * kv->sms);
     l.take = take(batch + 1);
     l.held = take(batch);
     l.request = take(rows);

@@ -178,7 +178,7 @@ __device__ void begin_plan(const TokParams &p) {
             nr[k] = ceil_shift((int64_t)count[k] * p.group, p.row_shift);
             kt[k] = ceil_shift((int64_t)ctx[k] + count[k], p.key_shift);
         }
-        tiles += (int64_t)nr[k] * kt[k];
+        tiles += (int64_t)nr[k] * (kt[k] + p.shape.lead);
         items += nr[k];
         longest = max(longest, kt[k]);
     }
@@ -192,7 +192,7 @@ __device__ void begin_plan(const TokParams &p) {
     const int64_t all_items = total * p.kv_heads;
     int64_t before = block_exclusive_sum64(tiles, total, s_scan);
     int64_t all = total * p.kv_heads;
-    int64_t share = max((all + p.shape.ctas - 1) / p.shape.ctas, (int64_t)p.shape.least);
+    int64_t share = max((all + p.shape.ctas - 1) / p.shape.ctas, (int64_t)(p.shape.least + p.shape.lead));
     const bool whole = all_items <= p.shape.ctas && s_longest <= p.shape.least;
     if (whole) {
         share = 0;
@@ -203,7 +203,7 @@ __device__ void begin_plan(const TokParams &p) {
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
         if (b0 + k < p.batch) work[b0 + k] = before * p.kv_heads;
-        before += whole ? nr[k] : (int64_t)nr[k] * kt[k];
+        before += whole ? nr[k] : (int64_t)nr[k] * (kt[k] + p.shape.lead);
     }
     if (threadIdx.x == 0) {
         work[p.batch] = all;

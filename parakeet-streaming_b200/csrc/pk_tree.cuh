@@ -68,9 +68,9 @@ struct Unit {
 // The units of one CTA, in order: a walk over its share of the line of tiles.
 struct Work {
     const TreeParams &p;
-    int cta, b, nr, kt;        // request, its row tiles and key tiles
-    int head, rt, t;           // the next unit's K/V head, row tile and first key tile
-    int64_t left;              // tiles (or row tiles) left to this CTA
+    int cta, b, nr, kt;   // request, its row tiles and key tiles
+    int head, rt, at;     // the next unit's K/V head, row tile and place in it
+    int64_t left;         // places (or row tiles) left to this CTA
     bool whole;
     Unit u;
 
@@ -82,13 +82,14 @@ struct Work {
         if (b < 0) return;
         load();
         const int64_t *work = reinterpret_cast<const int64_t *>(p.step + p.l.work);
-        const int64_t at = whole ? (int64_t)c : (int64_t)c * share, local = at - work[b];
-        left = min(whole ? (int64_t)1 : (int64_t)share, work[p.batch] - at);
+        const int64_t from = whole ? (int64_t)c : (int64_t)c * share, local = from - work[b];
+        left = min(whole ? (int64_t)1 : (int64_t)share, work[p.batch] - from);
         int64_t item = local;
-        t = 0;
+        at = 0;
         if (!whole) {
-            item = local / kt;
-            t = (int)(local - item * kt);
+            const int places = kt + p.shape.lead;
+            item = local / places;
+            at = (int)(local - item * places);
         }
         head = (int)(item / nr);
         rt = (int)(item - (int64_t)head * nr);
@@ -102,32 +103,36 @@ struct Work {
         kt = (u.ctx + u.count + p.shape.keys - 1) / p.shape.keys;
     }
     __device__ __forceinline__ bool next() {
-        if (left <= 0) return false;
-        if (head == p.kv_heads) {   // the next request that has rows
-            do {
-                if (++b >= p.batch) return false;
-                load();
-            } while (nr == 0);
-            head = 0;
-        }
-        u.head = head;
-        u.rt = rt;
-        u.t0 = t;
-        if (whole) {
-            u.t1 = kt;
-            u.part = -1;
-            --left;
-        } else {
-            const int n = (int)min((int64_t)(kt - t), left);
-            u.t1 = t + n;
-            u.part = n == kt ? -1 : (t == 0 ? 2 * cta + 1 : 2 * cta);
-            left -= n;
-        }
-        t = u.t1 == kt ? 0 : u.t1;
-        if (t == 0 && ++rt == nr) {
-            rt = 0;
-            ++head;
-        }
+        do {
+            if (left <= 0) return false;
+            if (head == p.kv_heads) {   // the next request that has rows
+                do {
+                    if (++b >= p.batch) return false;
+                    load();
+                } while (nr == 0);
+                head = 0;
+            }
+            u.head = head;
+            u.rt = rt;
+            if (whole) {
+                u.t0 = 0;
+                u.t1 = kt;
+                u.part = -1;
+                --left;
+                at = 0;
+            } else {
+                const int lead = p.shape.lead, n = (int)min((int64_t)(kt + lead - at), left);
+                u.t0 = max(at - lead, 0);
+                u.t1 = max(at + n - lead, 0);
+                u.part = u.t1 - u.t0 == kt ? -1 : (u.t0 == 0 ? 2 * cta + 1 : 2 * cta);
+                left -= n;
+                at = at + n == kt + lead ? 0 : at + n;
+            }
+            if (at == 0 && ++rt == nr) {
+                rt = 0;
+                ++head;
+            }
+        } while (u.t0 == u.t1);   // empty places alone
         if (!p.trees) {   // a chain's rows see no key past their own
             const int64_t last = ((int64_t)(u.rt + 1) * p.shape.rows + p.group - 1) / p.group;
             const int seen = u.ctx + (int)min(last, (int64_t)u.count);
@@ -136,6 +141,14 @@ struct Work {
         return true;
     }
 };
+
+// Whether a row tile whose places begin at `from` is shared by CTAs c0 .. c1.
+__device__ __forceinline__ bool shared_by(const TreeParams &p, int64_t from, int kt, int64_t share,
+                                          int &c0, int &c1) {
+    c0 = (int)((from + p.shape.lead) / share);
+    c1 = (int)((from + p.shape.lead + kt - 1) / share);
+    return c0 != c1;
+}
 
 // Page ids of a unit's tiles, for the warp that issues their loads: 32 table entries
 // at a time, one in a lane, the next 32 requested ahead.  (A load of its own for each

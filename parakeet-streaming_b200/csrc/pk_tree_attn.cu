@@ -75,8 +75,9 @@ template <int DH, int BM>
 struct TreeShape {
     static constexpr int kSlot = kTile * DH * 2;             // one tile of K or of V
     static constexpr int kWm = BM / 16, kWk = 4 / kWm;       // warps over rows, over keys
-    // 64 KB of tiles beside the join buffer: two CTAs an SM
-    static constexpr int kSlots = 4 * (128 / DH);
+    // CTAs an SM, and what the tiles get beside the join buffer
+    static constexpr int kCtas = BM == 16 && DH == 64 ? 4 : 2;
+    static constexpr int kSlots = 4 * (128 / DH) / (kCtas / 2);
     static constexpr int kKeys = kTile / kWk;                // keys of a tile per warp
     static constexpr int kPad = DH + 4;                      // join buffer row, floats
     static constexpr int kJoin = 4 * 16 * kPad * 4 + 4 * 16 * 8;
@@ -84,7 +85,7 @@ struct TreeShape {
 };
 
 template <int DH, int BM>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
     tree_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const TreeParams p) {
     using S = TreeShape<DH, BM>;
     constexpr int NS = S::kSlots;
@@ -165,10 +166,25 @@ __global__ void __launch_bounds__(kThreads, 2)
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
     int it = 0;
     Work work(p, blockIdx.x);
-    while (work.next()) {
-        const Unit &w = work.u;
+    bool more = work.next();
+    while (more) {
+        const Unit w = work.u;
         const int head = w.head;
         const int m_rows = w.count * p.group;
+        // the next unit's queries towards L1 while this one is computed: a row a lane
+        more = work.next();
+        if (more) {
+            const Unit &x = work.u;
+            const int r = x.rt * BM + wm * 16 + (lane & 15);
+            if (r < x.count * p.group) {
+                const int nd = r / p.group;
+                const char *at = reinterpret_cast<const char *>(
+                    q + (int64_t)(x.row0 + nd) * p.q_rs +
+                    (int64_t)(x.head * p.group + r - nd * p.group) * p.q_hs);
+                if (lane < 16 || DH == 128)
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(at + (lane >> 4) * 128));
+            }
+        }
         // this thread's two rows of the tile (fragment rows lane / 4 and + 8)
         uint32_t qf[DH / 16][4];
         uint64_t mask[2];
@@ -597,10 +613,10 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
         const int r0 = p.step[p.l.row_start + b], cnt = p.step[p.l.row_start + b + 1] - r0;
         const int head = qh / p.group, r = (row - r0) * p.group + qh - head * p.group;
         const int nr = (cnt * p.group + bm - 1) / bm, rt = r / bm;
-        const int64_t kt = (ctx + cnt + p.shape.keys - 1) / p.shape.keys;
-        const int64_t t0 = work[b] + ((int64_t)head * nr + rt) * kt, t1 = t0 + kt;
-        const int c0 = (int)(t0 / share), c1 = (int)((t1 - 1) / share);
-        if (c0 == c1) continue;
+        const int kt = (ctx + cnt + p.shape.keys - 1) / p.shape.keys;
+        int c0, c1;
+        if (!shared_by(p, work[b] + ((int64_t)head * nr + rt) * (kt + p.shape.lead), kt, share, c0, c1))
+            continue;
         auto at = [&](int c) {   // the first CTA's last unit, the others' first
             return ((int64_t)2 * c + (c == c0)) * bm + (r - rt * bm);
         };
