@@ -212,7 +212,7 @@ int launch_features(const FeArgs &a, cudaStream_t s);
 struct pk_token_kv {
     pk_token_kv_desc d;
     CUtensorMap kv_map;  // bf16 pools: {64, 8, head_dim / 64, page_size / 8, pages*layers*2*
-                         // kv_heads}, boxes of min(page_size, 64) rows, 128B-swizzled
+                         // kv_heads}, boxes of min(page_size, tree_tile_keys) rows, 128B-swizzled
     int ps_shift, esize, group;
     int sms;
 };
@@ -227,14 +227,18 @@ struct TokShape {
     int least;   // key tiles that a CTA takes before a request's are split over several
     int lead;    // what beginning a row tile costs, in key tiles
 };
+// Keys of a tile of the mma.sync kernels, and most rows of a page that one TMA copy
+// brings: 8 KB.
+constexpr int tree_tile_keys(int head_dim) { return head_dim == 64 ? 64 : 32; }
 // bf16: the narrowest row tile that holds an average request, since a request's K/V
 // is read once per row tile - 16 or 32 rows by mma.sync (two CTAs an SM), 128 by
 // tcgen05 (one).  float32: 16.
 inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
     if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, 2 * kv->sms, 1, 1};
-    if (mean <= 16) return {16, 64, (kv->d.head_dim == 64 ? 4 : 2) * kv->sms, 8, 2};
-    if (mean <= 32) return {32, 64, 2 * kv->sms, 8, 2};
+    const int keys = tree_tile_keys(kv->d.head_dim);
+    if (mean <= 16) return {16, keys, 2 * kv->sms, 512 / keys, 128 / keys};
+    if (mean <= 32) return {32, keys, 2 * kv->sms, 512 / keys, 128 / keys};
     return {128, 128, kv->sms, 4, 2};
 }
 
@@ -263,7 +267,7 @@ inline TokLayout tok_layout(const pk_token_kv *kv, int batch, int rows, int tree
     l.row_start = take(batch + 1);
     l.context = take(batch);
     l.slot = take(batch);
-    l.first = take(4 * kv->sms);
+    l.first = take(2 * kv->sms);
     l.take = take(batch + 1);
     l.held = take(batch);
     l.request = take(rows);

@@ -14,8 +14,10 @@
 // bf16, row tiles of 16 and 32: a producer warp brings each tile's pages (one TMA copy a page, 128B
 // swizzle) into a ring of K and V slots that runs ahead across
 // units; four warps hold 16-row fragments of the row tile and compute
-// S = Q K^T and O += P V with mma.sync m16n8k16.  The warps share the keys of a tile
-// (4 / (rows / 16) ways) and join through shared memory at the end.  P is rounded to bf16 for the product, relative
+// S = Q K^T and O += P V with mma.sync m16n8k16.  The warps take the tiles in
+// turn (a warp, or a pair for 32 rows, a whole tile: one chain of maximum, exponential
+// and sum for 64 keys; sharing a tile's keys had that chain for 16 and took 900 cycles
+// a tile) and join through shared memory at the end of a row tile.  P is rounded to bf16 for the product, relative
 // 2^-9 of each weight, below the rounding of the bf16 V that it multiplies; the
 // sum that normalises keeps fp32 weights.
 // Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
@@ -27,7 +29,6 @@
 namespace pk {
 namespace {
 
-constexpr int kTile = 64;
 constexpr int kConsumers = 128, kThreads = kConsumers + 32;
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -53,42 +54,68 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void consumer_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory");
 }
-// barrier that also ORs a flag over the consumer warps
-__device__ __forceinline__ bool consumer_any(bool v) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.or.pred q, 1, %2, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"((uint32_t)v), "n"(kConsumers)
-        : "memory");
-    return r != 0;
-}
 // Whether row `node` sees the step's token `rel` (>= 0) of its request.
 __device__ __forceinline__ bool sees(int trees, uint64_t mask, int node, int rel) {
     return trees ? rel < PK_TOK_MAX_TREE && ((mask >> rel) & 1) : rel <= node;
 }
 
+// Bit j: whether a row sees key rel0 + j, counted from the step's first token.
+__device__ __forceinline__ uint64_t seen_keys(int trees, uint64_t mask, int node, int rel0) {
+    if (rel0 <= -64) return ~0ull;
+    if (!trees) {
+        const int n = node - rel0 + 1;   // keys up to the row's own
+        return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1ull);
+    }
+    if (rel0 >= PK_TOK_MAX_TREE) return 0ull;
+    return rel0 >= 0 ? mask >> rel0 : (mask << -rel0) | ((1ull << -rel0) - 1ull);
+}
+
+// V rows past the end hold what the page held before: zero for the product (0 x inf
+// would reach every row).  Returns whether a token of the step's own has a value that
+// is not finite, which must not reach the rows that do not see it.  By one warp; the
+// warps of a tile write the same zeros.
+template <int DH>
+__device__ __forceinline__ bool clean_values(uint8_t *vs, int k0, int ctx, int len) {
+    constexpr int kTile = tree_tile_keys(DH);
+    bool odd = false;
+    for (int c = max(ctx - k0, 0) * (DH / 8) + (threadIdx.x & 31); c < kTile * DH / 8; c += 32) {
+        const int row = c / (DH / 8), ch = c % (DH / 8);
+        uint4 *at = reinterpret_cast<uint4 *>(vs + tile_at<DH>(row, ch));
+        if (k0 + row >= len) {
+            *at = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            const uint4 x = *at;
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                odd |= (e[k] & 0x7f80u) == 0x7f80u || (e[k] & 0x7f800000u) == 0x7f800000u;
+        }
+    }
+    fence_async_proxy();   // the slot's next TMA load comes after these writes
+    return __any_sync(0xffffffffu, odd);
+}
+
 template <int DH, int BM>
 struct TreeShape {
+    // keys of a tile, and of one chain of maximum, exponential and sum: 8 KB of K
+    static constexpr int kTile = tree_tile_keys(DH);
     static constexpr int kSlot = kTile * DH * 2;             // one tile of K or of V
-    static constexpr int kWm = BM / 16, kWk = 4 / kWm;       // warps over rows, over keys
-    // CTAs an SM, and what the tiles get beside the join buffer
-    static constexpr int kCtas = BM == 16 && DH == 64 ? 4 : 2;
-    static constexpr int kSlots = 4 * (128 / DH) / (kCtas / 2);
-    static constexpr int kKeys = kTile / kWk;                // keys of a tile per warp
+    static constexpr int kWm = BM / 16, kWk = 4 / kWm;       // warps over rows, over tiles
     static constexpr int kPad = DH + 4;                      // join buffer row, floats
-    static constexpr int kJoin = 4 * 16 * kPad * 4 + 4 * 16 * 8;
+    static constexpr int kJoin = 4 * 16 * (kPad + 2) * 4;    // every warp's rows
+    static constexpr int kCtas = 2;                          // an SM
+    // K and V slots of the ring: two for each warp over tiles (or a multiple), so that a
+    // slot is always the same warps' - a wait tells two phases apart, no more
+    static constexpr int kSlots = 8;
+    static_assert(kSlots % (2 * kWk) == 0, "slots per warp");
     static constexpr int kSmem = kSlots * kSlot + kJoin + 1024;
 };
 
 template <int DH, int BM>
 __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
-    tree_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const TreeParams p) {
+    tree_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeParams p) {
     using S = TreeShape<DH, BM>;
-    constexpr int NS = S::kSlots;
+    constexpr int NS = S::kSlots, kTile = S::kTile;
     extern __shared__ uint8_t tree_smem[];
     uint8_t *ring = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
@@ -99,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 4);
+            mbar_init(&empty[s], S::kWm);   // the warps of a tile
         }
         failed = 0;
         fence_mbar_init();
@@ -110,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
     grid_dep_launch();
 
     if (warp == 4) {
-        // producer: lanes issue a tile's boxes, K then V
+        // producer: lanes issue a tile's pages, K then V
         const int ps = 1 << p.ps_shift, rows_box = min(ps, kTile);
         const int box_of = lane;
         const uint32_t bytes = rows_box * DH * 2;
@@ -160,31 +187,16 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
         return;
     }
 
+    // a warp: rows 16 wm .. of the row tile, every kWk-th of the CTA's tiles
     const int wm = warp % S::kWm, wk = warp / S::kWm;
-    const int key0 = wk * S::kKeys;
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
-    int it = 0;
+    int first = 0;   // tiles of the CTA before the unit
     Work work(p, blockIdx.x);
     bool more = work.next();
     while (more) {
         const Unit w = work.u;
-        const int head = w.head;
         const int m_rows = w.count * p.group;
-        // the next unit's queries towards L1 while this one is computed: a row a lane
-        more = work.next();
-        if (more) {
-            const Unit &x = work.u;
-            const int r = x.rt * BM + wm * 16 + (lane & 15);
-            if (r < x.count * p.group) {
-                const int nd = r / p.group;
-                const char *at = reinterpret_cast<const char *>(
-                    q + (int64_t)(x.row0 + nd) * p.q_rs +
-                    (int64_t)(x.head * p.group + r - nd * p.group) * p.q_hs);
-                if (lane < 16 || DH == 128)
-                    asm volatile("prefetch.global.L1 [%0];" ::"l"(at + (lane >> 4) * 128));
-            }
-        }
         // this thread's two rows of the tile (fragment rows lane / 4 and + 8)
         uint32_t qf[DH / 16][4];
         uint64_t mask[2];
@@ -200,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
                 const int64_t row = w.row0 + node[h];
                 if (p.trees)
                     mask[h] = reinterpret_cast<const uint64_t *>(p.step + p.l.mask)[row];
-                src = q + row * p.q_rs + (int64_t)(head * p.group + r - node[h] * p.group) * p.q_hs +
-                      (lane & 3) * 2;
+                src = q + row * p.q_rs +
+                      (int64_t)(w.head * p.group + r - node[h] * p.group) * p.q_hs + (lane & 3) * 2;
             }
 #pragma unroll
             for (int ks = 0; ks < DH / 16; ++ks) {
@@ -209,31 +221,47 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
                 qf[ks][h + 2] = src ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8) : 0u;
             }
         }
+        // the next unit, and its queries towards L1 while this one is computed
+        more = work.next();
+        if (more) {
+            const Unit &x = work.u;
+            const int r = x.rt * BM + wm * 16 + (lane & 15);
+            if (r < x.count * p.group && (lane < 16 || DH == 128)) {
+                const int nd = r / p.group;
+                const char *at = reinterpret_cast<const char *>(
+                    q + (int64_t)(x.row0 + nd) * p.q_rs +
+                    (int64_t)(x.head * p.group + r - nd * p.group) * p.q_hs);
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(at + (lane >> 4) * 128));
+            }
+        }
         float o[DH / 8][4];
 #pragma unroll
         for (int i = 0; i < DH / 8; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        const int len = w.ctx + w.count;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // maxima scaled
+        const int len = w.ctx + w.count, tiles = max(w.t1 - w.t0, 0);
 
-        for (int t = w.t0; t < w.t1; ++t, it += 2) {
-            const int sk = it % NS, sv = (it + 1) % NS;
-            const int k0 = t * kTile;
-            const uint32_t kb = smem_u32(ring + sk * S::kSlot), vb = smem_u32(ring + sv * S::kSlot);
-            float s[S::kKeys / 8][4];
-#pragma unroll
-            for (int i = 0; i < S::kKeys / 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+        for (int i = (wk - first) & (S::kWk - 1); i < tiles; i += S::kWk) {
+            const int it = 2 * (first + i), sk = it % NS, sv = (it + 1) % NS;
+            const int k0 = (w.t0 + i) * kTile;
+            uint8_t *vs = ring + sv * S::kSlot;
+            const uint32_t kb = smem_u32(ring + sk * S::kSlot), vb = smem_u32(vs);
+            const bool own = k0 + kTile > w.ctx;   // some of the step's own tokens, or the end
             ring_wait(&full[sk], (it / NS) & 1, &failed, p.error);
             __syncwarp();
+            constexpr int kN = kTile / 8;
+            float s[kN][4];
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < DH / 16; ++ks) {
 #pragma unroll
-                for (int nb = 0; nb < S::kKeys / 16; ++nb) {
+                for (int nb = 0; nb < kN / 2; ++nb) {
                     uint32_t b[4];
-                    const uint32_t row = key0 + nb * 16 + ((lane >> 4) << 3) + (lane & 7);
+                    const uint32_t row = nb * 16 + ((lane >> 4) << 3) + (lane & 7);
                     ldsm4(kb + tile_at<DH>(row, ks * 2 + ((lane >> 3) & 1)), b);
                     mma16816(s[2 * nb], qf[ks], b[0], b[1]);
                     mma16816(s[2 * nb + 1], qf[ks], b[2], b[3]);
@@ -241,79 +269,60 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
             }
             __syncwarp();
             if (lane == 0) arrive(&empty[sk]);
-            const bool own = k0 + kTile > w.ctx;   // some of the step's own tokens, or the end
             if (own) {
 #pragma unroll
-                for (int i = 0; i < S::kKeys / 8; ++i)
+                for (int h = 0; h < 2; ++h) {
+                    // bit j: key j of this thread's (no row sees a key past the end)
+                    const uint64_t bits =
+                        seen_keys(p.trees, mask[h], node[h], k0 - w.ctx) >> ((lane & 3) * 2);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = k0 + key0 + i * 8 + (lane & 3) * 2 + (e & 1), h = e >> 1;
-                        const int rel = key - w.ctx;
-                        if (key >= len || (rel >= 0 && !sees(p.trees, mask[h], node[h], rel)))
-                            s[i][e] = -INFINITY;
-                    }
+                    for (int n = 0; n < kN; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (!(bits >> (n * 8 + e) & 1)) s[n][2 * h + e] = -INFINITY;
+                }
             }
             float keep[2], base[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float top = m[h];
+                float top = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
 #pragma unroll
-                for (int i = 0; i < S::kKeys / 8; ++i)
-                    top = fmaxf(top, fmaxf(s[i][2 * h], s[i][2 * h + 1]));
+                for (int n = 1; n < kN; ++n)
+                    top = fmaxf(top, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // (-inf stays so; a product rounded alike keeps an unchanged
+                // maximum's factor at 1)
+                top = fmaxf(m[h], top == -INFINITY ? top : __fmul_rn(top, p.scale_log2));
                 // nothing seen yet: weights and factor are exp2(-inf) = 0
-                base[h] = top == -INFINITY ? 0.f : __fmul_rn(top, p.scale_log2);
-                // both products rounded alike: an unchanged maximum keeps a factor of 1
-                keep[h] = ex2(__fmul_rn(m[h], p.scale_log2) - base[h]);
+                base[h] = top == -INFINITY ? 0.f : top;
+                keep[h] = ex2(m[h] - base[h]);
                 m[h] = top;
                 float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < S::kKeys / 8; ++i)
+                for (int n = 0; n < kN; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float w2 = ex2(s[i][2 * h + e] * p.scale_log2 - base[h]);
-                        s[i][2 * h + e] = w2;
-                        sum += w2;
+                        const float x = ex2(s[n][2 * h + e] * p.scale_log2 - base[h]);
+                        s[n][2 * h + e] = x;
+                        sum += x;
                     }
                 l[h] = l[h] * keep[h] + sum;
             }
 #pragma unroll
-            for (int i = 0; i < DH / 8; ++i) {
-                o[i][0] *= keep[0];
-                o[i][1] *= keep[0];
-                o[i][2] *= keep[1];
-                o[i][3] *= keep[1];
+            for (int n = 0; n < DH / 8; ++n) {
+                o[n][0] *= keep[0];
+                o[n][1] *= keep[0];
+                o[n][2] *= keep[1];
+                o[n][3] *= keep[1];
             }
             ring_wait(&full[sv], ((it + 1) / NS) & 1, &failed, p.error);
             __syncwarp();
-            bool odd = false;   // a value that is not finite among the step's own rows
-            if (own) {
-                // rows past the end hold what the page held before: zero for the
-                // product; a non-finite value of a token that some rows do not see
-                // must not reach them as 0 x inf
-                uint8_t *vs = ring + sv * S::kSlot;
-                bool bad = false;
-                for (int c = threadIdx.x; c < kTile * DH / 8; c += kConsumers) {
-                    const int row = c / (DH / 8), ch = c % (DH / 8);
-                    uint4 *at = reinterpret_cast<uint4 *>(vs + tile_at<DH>(row, ch));
-                    const int key = k0 + row;
-                    if (key >= len) {
-                        *at = make_uint4(0u, 0u, 0u, 0u);
-                    } else if (key >= w.ctx) {
-                        const uint4 x = *at;
-                        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            bad |= (e[i] & 0x7f80u) == 0x7f80u || (e[i] & 0x7f800000u) == 0x7f800000u;
-                    }
-                }
-                odd = consumer_any(bad);
-                fence_async_proxy();   // the slot's next TMA load comes after these writes
-            }
+            // a value that is not finite among the step's own rows
+            const bool odd = own && clean_values<DH>(vs, k0, w.ctx, len);
             if (!odd) {
 #pragma unroll
-                for (int kk = 0; kk < S::kKeys / 16; ++kk) {
+                for (int kk = 0; kk < kN / 2; ++kk) {
                     const uint32_t a[4] = {
                         pack2(s[2 * kk][0], s[2 * kk][1]), pack2(s[2 * kk][2], s[2 * kk][3]),
                         pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]),
@@ -321,38 +330,35 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
 #pragma unroll
                     for (int nb = 0; nb < DH / 16; ++nb) {
                         uint32_t b[4];
-                        const uint32_t row = key0 + kk * 16 + (lane & 15);
-                        ldsm4_t(vb + tile_at<DH>(row, nb * 2 + (lane >> 4)), b);
+                        ldsm4_t(vb + tile_at<DH>(kk * 16 + (lane & 15), nb * 2 + (lane >> 4)), b);
                         mma16816(o[2 * nb], a, b[0], b[1]);
                         mma16816(o[2 * nb + 1], a, b[2], b[3]);
                     }
                 }
             } else {
                 // the same product a key at a time, keys of weight zero left out
-                const uint8_t *vs = ring + sv * S::kSlot;
 #pragma unroll
-                for (int i = 0; i < S::kKeys / 8; ++i) {
+                for (int n = 0; n < kN; ++n) {
 #pragma unroll 1
                     for (int x = 0; x < 8; ++x) {
                         const int from = (lane & ~3) | (x >> 1);
-                        const float w0a = __shfl_sync(0xffffffffu, s[i][0], from);
-                        const float w0b = __shfl_sync(0xffffffffu, s[i][1], from);
-                        const float w1a = __shfl_sync(0xffffffffu, s[i][2], from);
-                        const float w1b = __shfl_sync(0xffffffffu, s[i][3], from);
+                        const float w0a = __shfl_sync(0xffffffffu, s[n][0], from);
+                        const float w0b = __shfl_sync(0xffffffffu, s[n][1], from);
+                        const float w1a = __shfl_sync(0xffffffffu, s[n][2], from);
+                        const float w1b = __shfl_sync(0xffffffffu, s[n][3], from);
                         const float w0 = x & 1 ? w0b : w0a, w1 = x & 1 ? w1b : w1a;
-                        const int row = key0 + i * 8 + x;
 #pragma unroll
-                        for (int n = 0; n < DH / 8; ++n) {
+                        for (int d = 0; d < DH / 8; ++d) {
                             const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(
-                                vs + tile_at<DH>(row, n) + (lane & 3) * 4);
+                                vs + tile_at<DH>(n * 8 + x, d) + (lane & 3) * 4);
                             const float2 f = __bfloat1622float2(v);
                             if (w0 != 0.f) {
-                                o[n][0] += w0 * f.x;
-                                o[n][1] += w0 * f.y;
+                                o[d][0] += w0 * f.x;
+                                o[d][1] += w0 * f.y;
                             }
                             if (w1 != 0.f) {
-                                o[n][2] += w1 * f.x;
-                                o[n][3] += w1 * f.y;
+                                o[d][2] += w1 * f.x;
+                                o[d][3] += w1 * f.y;
                             }
                         }
                     }
@@ -361,76 +367,73 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
             __syncwarp();
             if (lane == 0) arrive(&empty[sv]);
         }
+        first += tiles;
         // row sums over the quad's lanes
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
         }
-        const int64_t part = (int64_t)w.part * BM;
-        {
-            // join the warps' shares of the keys: each writes its 16 rows, then every
-            // thread sums 8 columns of a row over the shares
-            float *ml = join + 4 * 16 * S::kPad;
-            const int base = warp * 16;
+        // join the warps' shares of the tiles: each leaves its 16 rows, then every thread
+        // sums 8 columns of a row over the shares
+        float *ml = join + 4 * 16 * S::kPad;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float *dst = join + (base + (lane >> 2) + h * 8) * S::kPad + (lane & 3) * 2;
+        for (int h = 0; h < 2; ++h) {
+            const int at = warp * 16 + (lane >> 2) + h * 8;
+            float *dst = join + at * S::kPad + (lane & 3) * 2;
 #pragma unroll
-                for (int n = 0; n < DH / 8; ++n)
-                    *reinterpret_cast<float2 *>(dst + n * 8) =
-                        make_float2(o[n][2 * h], o[n][2 * h + 1]);
-                if ((lane & 3) == 0) {
-                    ml[2 * (base + (lane >> 2) + h * 8)] = __fmul_rn(m[h], p.scale_log2);
-                    ml[2 * (base + (lane >> 2) + h * 8) + 1] = l[h];
-                }
-            }
-            consumer_sync();
-            for (int c = threadIdx.x; c < BM * DH / 8; c += kConsumers) {
-                const int rt = c / (DH / 8), ch = c % (DH / 8), r = w.rt * BM + rt;
-                if (r >= m_rows) continue;
-                float top = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < S::kWk; ++k)   // share k of row rt: warp k * kWm + rt / 16
-                    top = fmaxf(top, ml[2 * (k * BM + rt)]);
-                const float ref = top == -INFINITY ? 0.f : top;
-                float acc[8] = {}, sum = 0.f;
-#pragma unroll
-                for (int k = 0; k < S::kWk; ++k) {
-                    const float f = ex2(ml[2 * (k * BM + rt)] - ref);
-                    sum += f * ml[2 * (k * BM + rt) + 1];
-                    const float4 *src = reinterpret_cast<const float4 *>(
-                        join + (k * BM + rt) * S::kPad + ch * 8);
-                    const float4 a = src[0], b = src[1];
-                    acc[0] += f * a.x;
-                    acc[1] += f * a.y;
-                    acc[2] += f * a.z;
-                    acc[3] += f * a.w;
-                    acc[4] += f * b.x;
-                    acc[5] += f * b.y;
-                    acc[6] += f * b.z;
-                    acc[7] += f * b.w;
-                }
-                if (w.part >= 0) {
-                    float4 *dst = reinterpret_cast<float4 *>(p.ws_o + (part + rt) * DH + ch * 8);
-                    dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                    dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                    if (ch == 0)
-                        *reinterpret_cast<float2 *>(p.ws_ml + (part + rt) * 2) =
-                            make_float2(top, sum);
-                } else {
-                    const float inv = 1.f / sum;
-                    const int nd = r / p.group;
-                    __nv_bfloat16 *dst = out + (int64_t)(w.row0 + nd) * p.o_rs +
-                                         (int64_t)(head * p.group + r - nd * p.group) * p.o_hs +
-                                         ch * 8;
-                    *reinterpret_cast<uint4 *>(dst) =
-                        make_uint4(pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv),
-                                   pack2(acc[4] * inv, acc[5] * inv), pack2(acc[6] * inv, acc[7] * inv));
-                }
-            }
-            consumer_sync();   // the buffer is free again
+            for (int n = 0; n < DH / 8; ++n)
+                *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+            if ((lane & 3) == 0)
+                *reinterpret_cast<float2 *>(ml + 2 * at) = make_float2(m[h], l[h]);
         }
+        consumer_sync();
+        for (int c = threadIdx.x; c < BM * DH / 8; c += kConsumers) {
+            const int rt = c / (DH / 8), ch = c % (DH / 8), r = w.rt * BM + rt;
+            if (r >= m_rows) continue;
+            float2 x[S::kWk];
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < S::kWk; ++k) {   // share k of row rt: warp k * kWm + rt / 16
+                x[k] = *reinterpret_cast<const float2 *>(ml + 2 * (k * BM + rt));
+                top = fmaxf(top, x[k].x);
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+            float acc[8] = {}, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < S::kWk; ++k) {
+                const float f = ex2(x[k].x - ref);
+                sum += f * x[k].y;
+                const float4 *src =
+                    reinterpret_cast<const float4 *>(join + (k * BM + rt) * S::kPad + ch * 8);
+                const float4 a = src[0], b = src[1];
+                acc[0] += f * a.x;
+                acc[1] += f * a.y;
+                acc[2] += f * a.z;
+                acc[3] += f * a.w;
+                acc[4] += f * b.x;
+                acc[5] += f * b.y;
+                acc[6] += f * b.z;
+                acc[7] += f * b.w;
+            }
+            if (w.part >= 0) {
+                const int64_t at = (int64_t)w.part * BM + rt;
+                float4 *dst = reinterpret_cast<float4 *>(p.ws_o + at * DH + ch * 8);
+                dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                if (ch == 0)
+                    *reinterpret_cast<float2 *>(p.ws_ml + at * 2) = make_float2(top, sum);
+            } else {
+                const float inv = 1.f / sum;
+                const int nd = r / p.group;
+                __nv_bfloat16 *dst = out + (int64_t)(w.row0 + nd) * p.o_rs +
+                                     (int64_t)(w.head * p.group + r - nd * p.group) * p.o_hs + ch * 8;
+                *reinterpret_cast<uint4 *>(dst) =
+                    make_uint4(pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv),
+                               pack2(acc[4] * inv, acc[5] * inv), pack2(acc[6] * inv, acc[7] * inv));
+            }
+        }
+        consumer_sync();   // the buffer is free again
     }
 }
 
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
 // 16-row tile; K rows are padded so that a lane per key reads without bank
 // conflicts; a warp computes the scores of its four rows (two keys a lane), then
 // their outputs (DH / 32 columns a lane).
-constexpr int kRowsF32 = 16;
+constexpr int kRowsF32 = 16, kTile = 64;
 template <int DH>
 __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) {
     constexpr int kKp = DH + 4, NV = DH / 32;
