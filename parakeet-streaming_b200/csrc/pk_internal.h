@@ -220,25 +220,24 @@ struct pk_token_kv {
 namespace pk {
 
 // How a step's rows are attended.  A row tile is up to `rows` query rows (token x
-// group) of one request and K/V head, a key tile `keys` of its keys; `ctas` CTAs
-// share the work.
+// group) of one request and K/V head, a key tile `keys` of its keys; `ctas` workers
+// (CTAs, or warps) share the work.
 struct TokShape {
     int rows, keys, ctas;
-    int least;   // key tiles that a CTA takes before a request's are split over several
+    int least;   // key tiles that a worker takes before a request's are split over several
     int lead;    // what beginning a row tile costs, in key tiles
 };
-// Keys of a tile of the mma.sync kernels, and most rows of a page that one TMA copy
+// Keys of a tile of the 16-row kernel, and most rows of a page that one TMA copy
 // brings: 8 KB.
 constexpr int tree_tile_keys(int head_dim) { return head_dim == 64 ? 64 : 32; }
-// bf16: the narrowest row tile that holds an average request, since a request's K/V
-// is read once per row tile - 16 or 32 rows by mma.sync (two CTAs an SM), 128 by
-// tcgen05 (one).  float32: 16.
+constexpr int kTokWorkers = 12;   // most workers an SM
+// bf16: row tiles of 16 by mma.sync, a warp a worker, where they hold an average
+// request (its K/V is read once per row tile); of 128 by tcgen05, a CTA a worker,
+// otherwise.  float32: 16.
 inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
     if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, 2 * kv->sms, 1, 1};
-    const int keys = tree_tile_keys(kv->d.head_dim);
-    if (mean <= 16) return {16, keys, 2 * kv->sms, 512 / keys, 128 / keys};
-    if (mean <= 32) return {32, keys, 2 * kv->sms, 512 / keys, 128 / keys};
+    if (mean <= 16) return {16, tree_tile_keys(kv->d.head_dim), kTokWorkers * kv->sms, 8, 1};
     return {128, 128, kv->sms, 4, 2};
 }
 
@@ -250,7 +249,7 @@ inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
 enum TokHeader { kTokShare = 0, kTokRows, kTokFree, kTokHeaderWords = 16 };
 struct TokLayout {
     // work: int64 first place (share 0: row tile) of each request; first: the request
-    // that each CTA begins in (-1: no work); take: first new page; held: pages before
+    // that each worker begins in (-1: no work); take: first new page; held: pages before
     int64_t row_start, context, slot, work, first, take, held, request, position, slot_map, mask,
         words;
 };
@@ -267,7 +266,7 @@ inline TokLayout tok_layout(const pk_token_kv *kv, int batch, int rows, int tree
     l.row_start = take(batch + 1);
     l.context = take(batch);
     l.slot = take(batch);
-    l.first = take(2 * kv->sms);
+    l.first = take(kTokWorkers * kv->sms);
     l.take = take(batch + 1);
     l.held = take(batch);
     l.request = take(rows);

@@ -171,6 +171,11 @@ struct Pages {
         ids = fetch(block);
         ahead = fetch(block + 32);
     }
+    // back to the unit's first entries
+    __device__ __forceinline__ void rewind(const TreeParams &p, const Unit &w) {
+        const int first = ((w.t0 * p.shape.keys) >> p.ps_shift) & ~31;
+        if (block != first) open(p, w);
+    }
     // entry `at` of the caller's lane; uniform in at / 32
     __device__ __forceinline__ int get(int at) {
         while (at >= block + 32) {

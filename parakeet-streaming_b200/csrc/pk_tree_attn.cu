@@ -8,19 +8,20 @@
 // The rows of a K/V head are its group's query heads of every token, so a
 // request's pages are read once for all of them that fit a row tile.  The step's
 // work is a line of (row tile, key tile) pairs that is cut into equal shares, one a
-// CTA, whatever the lengths; a second launch joins the row tiles that a cut went
-// through (two partial results a CTA at most).
+// worker, whatever the lengths; a second launch joins the row tiles that a cut went
+// through (two partial results a worker at most).
 //
-// bf16, row tiles of 16 and 32: a producer warp brings each tile's pages (one TMA copy a page, 128B
-// swizzle) into a ring of K and V slots that runs ahead across
-// units; four warps hold 16-row fragments of the row tile and compute
-// S = Q K^T and O += P V with mma.sync m16n8k16.  The warps take the tiles in
-// turn (a warp, or a pair for 32 rows, a whole tile: one chain of maximum, exponential
-// and sum for 64 keys; sharing a tile's keys had that chain for 16 and took 900 cycles
-// a tile) and join through shared memory at the end of a row tile.  P is rounded to bf16 for the product, relative
-// 2^-9 of each weight, below the rounding of the bf16 V that it multiplies; the
-// sum that normalises keeps fp32 weights.
-// Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
+// bf16, row tiles of 16: every warp is a worker of its own, with a share of the line and
+// two 8 KB slots of shared memory, one for a tile of K and one for its V (TMA, a page a
+// copy, 128B swizzle).  It requests the next K as soon as it has read one and the next
+// V likewise, across its units, computes S = Q K^T and O += P V with mma.sync m16n8k16
+// and waits for nobody: 12 such chains an SM (a tile takes a warp some 2600 cycles, 700
+// is an SM's share of the memory rate) hide each other's latencies.  Warps that shared
+// a row tile met in a barrier at its end and cost 5000 cycles a row tile, however short
+// (160 requests of up to 500 tokens, 8 heads: 41 us).
+// P is rounded to bf16 for the product, relative 2^-9 of each weight, below the
+// rounding of the bf16 V that it multiplies; the sum that normalises keeps fp32
+// weights.  Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
 // other waits return at once.
 #include <math.h>
 
@@ -29,7 +30,7 @@
 namespace pk {
 namespace {
 
-constexpr int kConsumers = 128, kThreads = kConsumers + 32;
+constexpr int kWarps = 4;   // workers of a CTA
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -50,9 +51,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void consumer_sync() {
-    asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory");
 }
 // Whether row `node` sees the step's token `rel` (>= 0) of its request.
 __device__ __forceinline__ bool sees(int trees, uint64_t mask, int node, int rel) {
@@ -95,38 +93,24 @@ __device__ __forceinline__ bool clean_values(uint8_t *vs, int k0, int ctx, int l
     return __any_sync(0xffffffffu, odd);
 }
 
-template <int DH, int BM>
-struct TreeShape {
-    // keys of a tile, and of one chain of maximum, exponential and sum: 8 KB of K
-    static constexpr int kTile = tree_tile_keys(DH);
-    static constexpr int kSlot = kTile * DH * 2;             // one tile of K or of V
-    static constexpr int kWm = BM / 16, kWk = 4 / kWm;       // warps over rows, over tiles
-    static constexpr int kPad = DH + 4;                      // join buffer row, floats
-    static constexpr int kJoin = 4 * 16 * (kPad + 2) * 4;    // every warp's rows
-    static constexpr int kCtas = 2;                          // an SM
-    // K and V slots of the ring: two for each warp over tiles (or a multiple), so that a
-    // slot is always the same warps' - a wait tells two phases apart, no more
-    static constexpr int kSlots = 8;
-    static_assert(kSlots % (2 * kWk) == 0, "slots per warp");
-    static constexpr int kSmem = kSlots * kSlot + kJoin + 1024;
-};
-
-template <int DH, int BM>
-__global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
+template <int DH>
+__global__ void __launch_bounds__(kWarps * 32, 3)
     tree_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeParams p) {
-    using S = TreeShape<DH, BM>;
-    constexpr int NS = S::kSlots, kTile = S::kTile;
+    // keys of a tile, and of one chain of maximum, exponential and sum: 8 KB of K
+    constexpr int kTile = tree_tile_keys(DH), kSlot = kTile * DH * 2, kN = kTile / 8;
     extern __shared__ uint8_t tree_smem[];
-    uint8_t *ring = reinterpret_cast<uint8_t *>(
-        (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
-    float *join = reinterpret_cast<float *>(ring + NS * S::kSlot);
-    __shared__ __align__(8) uint64_t full[NS], empty[NS];
+    __shared__ __align__(8) uint64_t full[kWarps][2];
     __shared__ volatile int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t *ks = reinterpret_cast<uint8_t *>(
+                      (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023)) +
+                  warp * 2 * kSlot;
+    uint8_t *vs = ks + kSlot;
+    const uint32_t kb = smem_u32(ks), vb = smem_u32(vs);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < NS; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], S::kWm);   // the warps of a tile
+        for (int w = 0; w < kWarps; ++w) {
+            mbar_init(&full[w][0], 1);
+            mbar_init(&full[w][1], 1);
         }
         failed = 0;
         fence_mbar_init();
@@ -136,74 +120,59 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
     grid_dep_wait();
     grid_dep_launch();
 
-    if (warp == 4) {
-        // producer: lanes issue a tile's pages, K then V
-        const int ps = 1 << p.ps_shift, rows_box = min(ps, kTile);
-        const int box_of = lane;
+    const int ps = 1 << p.ps_shift, rows_box = min(ps, kTile);
+    // request K (v = 0) or V (1) of tile t of a unit: a page a lane
+    auto request = [&](const Unit &w, Pages &pages, int t, int v) {
+        const int k0 = t * kTile;
+        const int n = (min(kTile, w.ctx + w.count - k0) + rows_box - 1) / rows_box;
+        // lanes without a box ask for the last one's page
+        int page = pages.get((k0 + min(lane, n - 1) * rows_box) >> p.ps_shift);
+        if (page < 0 || page >= p.num_pages) {
+            raise(p.error, PK_DEV_BAD_PAGE);
+            page = 0;
+        }
         const uint32_t bytes = rows_box * DH * 2;
-        int it = 0;   // ring use
-        bool stop = false;   // the warp's, so that its lanes stay together
-        Work work(p, blockIdx.x);
-        Pages pages, then;
-        bool more = work.next();
-        Unit w = work.u;
-        if (more) pages.open(p, w);
-        while (more && !stop) {
-            more = work.next();
-            if (more) then.open(p, work.u);
-            const int len = w.ctx + w.count;
-            for (int t = w.t0; t < w.t1 && !stop; ++t) {
-                const int k0 = t * kTile, n = (min(kTile, len - k0) + rows_box - 1) / rows_box;
-                // lanes without a box ask for the last one's page
-                int page = pages.get((k0 + min(box_of, n - 1) * rows_box) >> p.ps_shift);
-                if (page < 0 || page >= p.num_pages) {
-                    raise(p.error, PK_DEV_BAD_PAGE);
-                    page = 0;
-                }
-                const int in_page = (k0 + box_of * rows_box) & (ps - 1);
-#pragma unroll
-                for (int v = 0; v < 2; ++v, ++it) {
-                    const int s = it % NS, use = it / NS;
-                    if (use) ring_wait(&empty[s], (use - 1) & 1, &failed, p.error);
-                    stop = __any_sync(0xffffffffu, failed != 0);
-                    if (stop) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n * bytes);
-                    __syncwarp();
-                    if (box_of < n)
-                        tma_load_rows(ring + s * S::kSlot + box_of * bytes, &kv_map, &full[s], in_page,
-                                      ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
-                }
-            }
-            w = work.u;
-            pages = then;
-        }
-        if (stop) {   // leave no copy in flight
-            for (int s = 0; s < NS; ++s)
-                if (it > s) {
-                    const int lastu = (it - 1 - s) / NS;
-                    mbar_wait_bounded(&full[s], lastu & 1, kWaitLimitNs);
-                }
-        }
-        return;
-    }
+        if (lane == 0) mbar_arrive_expect_tx(&full[warp][v], n * bytes);
+        __syncwarp();
+        if (lane < n)
+            tma_load_rows((v ? vs : ks) + lane * bytes, &kv_map, &full[warp][v],
+                          (k0 + lane * rows_box) & (ps - 1),
+                          ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
+    };
 
-    // a warp: rows 16 wm .. of the row tile, every kWk-th of the CTA's tiles
-    const int wm = warp % S::kWm, wk = warp / S::kWm;
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
-    int first = 0;   // tiles of the CTA before the unit
-    Work work(p, blockIdx.x);
-    bool more = work.next();
+    // neighbouring shares on different SMs
+    Work work(p, warp * gridDim.x + blockIdx.x);
+    // units that have tiles (a chain's rows may see none of a share's)
+    auto advance = [&]() {
+        while (work.next()) {
+            if (work.u.t0 < work.u.t1) return true;
+            if (work.u.part >= 0 && lane < 16)   // nothing seen: no weight in the join
+                *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)work.u.part * 16 + lane) * 2) =
+                    make_float2(-INFINITY, 0.f);
+        }
+        return false;
+    };
+    bool more = advance();
+    Unit w = work.u;
+    Pages pages, vpages, then;   // K and V walk the pages a tile apart
+    if (more) {
+        pages.open(p, w);
+        vpages = pages;
+        request(w, pages, w.t0, 0);
+        request(w, vpages, w.t0, 1);
+    }
+    uint32_t phase = 0;   // of both barriers: one use a tile
     while (more) {
-        const Unit w = work.u;
-        const int m_rows = w.count * p.group;
+        const int m_rows = w.count * p.group, len = w.ctx + w.count;
         // this thread's two rows of the tile (fragment rows lane / 4 and + 8)
         uint32_t qf[DH / 16][4];
         uint64_t mask[2];
         int node[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int r = w.rt * BM + wm * 16 + (lane >> 2) + h * 8;
+            const int r = w.rt * 16 + (lane >> 2) + h * 8;
             node[h] = -1;
             mask[h] = 0;
             const __nv_bfloat16 *src = nullptr;
@@ -216,59 +185,45 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
                       (int64_t)(w.head * p.group + r - node[h] * p.group) * p.q_hs + (lane & 3) * 2;
             }
 #pragma unroll
-            for (int ks = 0; ks < DH / 16; ++ks) {
-                qf[ks][h] = src ? *reinterpret_cast<const uint32_t *>(src + ks * 16) : 0u;
-                qf[ks][h + 2] = src ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + 8) : 0u;
+            for (int c = 0; c < DH / 16; ++c) {
+                qf[c][h] = src ? *reinterpret_cast<const uint32_t *>(src + c * 16) : 0u;
+                qf[c][h + 2] = src ? *reinterpret_cast<const uint32_t *>(src + c * 16 + 8) : 0u;
             }
         }
-        // the next unit, and its queries towards L1 while this one is computed
-        more = work.next();
-        if (more) {
-            const Unit &x = work.u;
-            const int r = x.rt * BM + wm * 16 + (lane & 15);
-            if (r < x.count * p.group && (lane < 16 || DH == 128)) {
-                const int nd = r / p.group;
-                const char *at = reinterpret_cast<const char *>(
-                    q + (int64_t)(x.row0 + nd) * p.q_rs +
-                    (int64_t)(x.head * p.group + r - nd * p.group) * p.q_hs);
-                asm volatile("prefetch.global.L1 [%0];" ::"l"(at + (lane >> 4) * 128));
-            }
-        }
+        // the next unit is known before this one is computed
+        more = advance();
+        if (more) then.open(p, work.u);
         float o[DH / 8][4];
 #pragma unroll
         for (int i = 0; i < DH / 8; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // maxima scaled
-        const int len = w.ctx + w.count, tiles = max(w.t1 - w.t0, 0);
 
-        for (int i = (wk - first) & (S::kWk - 1); i < tiles; i += S::kWk) {
-            const int it = 2 * (first + i), sk = it % NS, sv = (it + 1) % NS;
-            const int k0 = (w.t0 + i) * kTile;
-            uint8_t *vs = ring + sv * S::kSlot;
-            const uint32_t kb = smem_u32(ring + sk * S::kSlot), vb = smem_u32(vs);
+        for (int t = w.t0; t < w.t1; ++t, phase ^= 1) {
+            const int k0 = t * kTile;
             const bool own = k0 + kTile > w.ctx;   // some of the step's own tokens, or the end
-            ring_wait(&full[sk], (it / NS) & 1, &failed, p.error);
+            ring_wait(&full[warp][0], phase, &failed, p.error);
             __syncwarp();
-            constexpr int kN = kTile / 8;
             float s[kN][4];
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < DH / 16; ++ks) {
+            for (int c = 0; c < DH / 16; ++c) {
 #pragma unroll
                 for (int nb = 0; nb < kN / 2; ++nb) {
                     uint32_t b[4];
                     const uint32_t row = nb * 16 + ((lane >> 4) << 3) + (lane & 7);
-                    ldsm4(kb + tile_at<DH>(row, ks * 2 + ((lane >> 3) & 1)), b);
-                    mma16816(s[2 * nb], qf[ks], b[0], b[1]);
-                    mma16816(s[2 * nb + 1], qf[ks], b[2], b[3]);
+                    ldsm4(kb + tile_at<DH>(row, c * 2 + ((lane >> 3) & 1)), b);
+                    mma16816(s[2 * nb], qf[c], b[0], b[1]);
+                    mma16816(s[2 * nb + 1], qf[c], b[2], b[3]);
                 }
             }
             __syncwarp();
-            if (lane == 0) arrive(&empty[sk]);
+            if (t + 1 < w.t1) request(w, pages, t + 1, 0);
+            else if (more) request(work.u, then, work.u.t0, 0);
             if (own) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -291,8 +246,8 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
                     top = fmaxf(top, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // (-inf stays so; a product rounded alike keeps an unchanged
-                // maximum's factor at 1)
+                // (-inf stays so; a product rounded alike keeps an unchanged maximum's
+                // factor at 1)
                 top = fmaxf(m[h], top == -INFINITY ? top : __fmul_rn(top, p.scale_log2));
                 // nothing seen yet: weights and factor are exp2(-inf) = 0
                 base[h] = top == -INFINITY ? 0.f : top;
@@ -316,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
                 o[n][2] *= keep[1];
                 o[n][3] *= keep[1];
             }
-            ring_wait(&full[sv], ((it + 1) / NS) & 1, &failed, p.error);
+            ring_wait(&full[warp][1], phase, &failed, p.error);
             __syncwarp();
             // a value that is not finite among the step's own rows
             const bool odd = own && clean_values<DH>(vs, k0, w.ctx, len);
@@ -365,75 +320,46 @@ __global__ void __launch_bounds__(kThreads, TreeShape<DH, BM>::kCtas)
                 }
             }
             __syncwarp();
-            if (lane == 0) arrive(&empty[sv]);
+            if (t + 1 < w.t1) {
+                request(w, vpages, t + 1, 1);
+            } else if (more) {
+                vpages = then;
+                vpages.rewind(p, work.u);
+                request(work.u, vpages, work.u.t0, 1);
+            }
         }
-        first += tiles;
         // row sums over the quad's lanes
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        }
-        // join the warps' shares of the tiles: each leaves its 16 rows, then every thread
-        // sums 8 columns of a row over the shares
-        float *ml = join + 4 * 16 * S::kPad;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int at = warp * 16 + (lane >> 2) + h * 8;
-            float *dst = join + at * S::kPad + (lane & 3) * 2;
-#pragma unroll
-            for (int n = 0; n < DH / 8; ++n)
-                *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-            if ((lane & 3) == 0)
-                *reinterpret_cast<float2 *>(ml + 2 * at) = make_float2(m[h], l[h]);
-        }
-        consumer_sync();
-        for (int c = threadIdx.x; c < BM * DH / 8; c += kConsumers) {
-            const int rt = c / (DH / 8), ch = c % (DH / 8), r = w.rt * BM + rt;
+            const int rt = (lane >> 2) + h * 8, r = w.rt * 16 + rt;
             if (r >= m_rows) continue;
-            float2 x[S::kWk];
-            float top = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < S::kWk; ++k) {   // share k of row rt: warp k * kWm + rt / 16
-                x[k] = *reinterpret_cast<const float2 *>(ml + 2 * (k * BM + rt));
-                top = fmaxf(top, x[k].x);
-            }
-            const float ref = top == -INFINITY ? 0.f : top;
-            float acc[8] = {}, sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < S::kWk; ++k) {
-                const float f = ex2(x[k].x - ref);
-                sum += f * x[k].y;
-                const float4 *src =
-                    reinterpret_cast<const float4 *>(join + (k * BM + rt) * S::kPad + ch * 8);
-                const float4 a = src[0], b = src[1];
-                acc[0] += f * a.x;
-                acc[1] += f * a.y;
-                acc[2] += f * a.z;
-                acc[3] += f * a.w;
-                acc[4] += f * b.x;
-                acc[5] += f * b.y;
-                acc[6] += f * b.z;
-                acc[7] += f * b.w;
-            }
             if (w.part >= 0) {
-                const int64_t at = (int64_t)w.part * BM + rt;
-                float4 *dst = reinterpret_cast<float4 *>(p.ws_o + at * DH + ch * 8);
-                dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                if (ch == 0)
-                    *reinterpret_cast<float2 *>(p.ws_ml + at * 2) = make_float2(top, sum);
+                const int64_t at = (int64_t)w.part * 16 + rt;
+                float *dst = p.ws_o + at * DH + (lane & 3) * 2;
+#pragma unroll
+                for (int n = 0; n < DH / 8; ++n)
+                    *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                if ((lane & 3) == 0)
+                    *reinterpret_cast<float2 *>(p.ws_ml + at * 2) = make_float2(m[h], l[h]);
             } else {
-                const float inv = 1.f / sum;
-                const int nd = r / p.group;
-                __nv_bfloat16 *dst = out + (int64_t)(w.row0 + nd) * p.o_rs +
-                                     (int64_t)(w.head * p.group + r - nd * p.group) * p.o_hs + ch * 8;
-                *reinterpret_cast<uint4 *>(dst) =
-                    make_uint4(pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv),
-                               pack2(acc[4] * inv, acc[5] * inv), pack2(acc[6] * inv, acc[7] * inv));
+                const float inv = 1.f / l[h];
+                __nv_bfloat16 *dst =
+                    out + (int64_t)(w.row0 + node[h]) * p.o_rs +
+                    (int64_t)(w.head * p.group + r - node[h] * p.group) * p.o_hs + (lane & 3) * 2;
+#pragma unroll
+                for (int n = 0; n < DH / 8; ++n)
+                    *reinterpret_cast<uint32_t *>(dst + n * 8) =
+                        pack2(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
             }
         }
-        consumer_sync();   // the buffer is free again
+        w = work.u;
+        pages = then;
+    }
+    if (failed) {   // leave no copy in flight
+        mbar_wait_bounded(&full[warp][0], phase ^ 1, kWaitLimitNs);
+        mbar_wait_bounded(&full[warp][1], phase ^ 1, kWaitLimitNs);
     }
 }
 
@@ -592,72 +518,128 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
 }
 
 // ------------------------------------------------------------------ the join
-// A warp per (row, head): its row tile's partial results - of the CTAs whose shares
-// cut the tile's keys - weighted by exp2(m - max m), in order of the keys, so that
-// the result does not depend on which finished first.
+// A warp per (row, head): its row tile's partial results - of the workers whose shares
+// cut the tile's keys - weighted by exp2(m - max m).  Rows with more than kAlone
+// partials (a long request's) are summed by the block's eight warps together.  The
+// order is that of the keys in both, so that the result does not depend on which
+// worker finished first.
+constexpr int kAlone = 16;
 template <int DH, typename T>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     constexpr int NV = DH / 32;
+    __shared__ float s_acc[8][DH], s_sum[8];
+    __shared__ int s_many;
     grid_dep_wait();
     grid_dep_launch();
     const int64_t share = p.step[kTokShare];
     if (share == 0) return;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t n = (int64_t)p.rows * p.heads;
     const int bm = p.shape.rows;
     const int64_t *work = reinterpret_cast<const int64_t *>(p.step + p.l.work);
-    for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < n;
-         i += ((int64_t)gridDim.x * blockDim.x) >> 5) {
+    // the workers of entry i, and where the first one's partial of its row lies
+    auto find = [&](int64_t i, int &c0, int &c1, int &in_tile) {
+        if (i >= n) return false;
         const int row = (int)(i / p.heads), qh = (int)(i - (int64_t)row * p.heads);
         const int b = p.step[p.l.request + row];
-        if (b < 0) continue;
+        if (b < 0) return false;
         const int ctx = p.step[p.l.context + b];
-        if (ctx < 0) continue;
+        if (ctx < 0) return false;
         const int r0 = p.step[p.l.row_start + b], cnt = p.step[p.l.row_start + b + 1] - r0;
         const int head = qh / p.group, r = (row - r0) * p.group + qh - head * p.group;
         const int nr = (cnt * p.group + bm - 1) / bm, rt = r / bm;
         const int kt = (ctx + cnt + p.shape.keys - 1) / p.shape.keys;
-        int c0, c1;
-        if (!shared_by(p, work[b] + ((int64_t)head * nr + rt) * (kt + p.shape.lead), kt, share, c0, c1))
-            continue;
-        auto at = [&](int c) {   // the first CTA's last unit, the others' first
-            return ((int64_t)2 * c + (c == c0)) * bm + (r - rt * bm);
-        };
-        float top = -INFINITY;
-        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.ws_ml[at(c) * 2]);
-#pragma unroll
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        if (top == -INFINITY) top = 0.f;
-        float acc[NV] = {}, sum = 0.f;
+        in_tile = r - rt * bm;
+        return shared_by(p, work[b] + ((int64_t)head * nr + rt) * (kt + p.shape.lead), kt, share, c0,
+                         c1);
+    };
+    auto at = [&](int c, int c0, int in_tile) {   // the first worker's last unit, the others' first
+        return ((int64_t)2 * c + (c == c0)) * bm + in_tile;
+    };
+    // sums workers c0 + w0, + step, ..: outputs and the sum, relative to exp2(top)
+    auto add = [&](int c0, int c1, int in_tile, float top, int w0, int step, float (&acc)[NV]) {
+        float sum = 0.f;
 #pragma unroll 4
-        for (int c = c0; c <= c1; ++c) {
-            const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + at(c) * 2);
+        for (int c = c0 + w0; c <= c1; c += step) {
+            const int64_t k = at(c, c0, in_tile);
+            const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + k * 2);
             const float f = exp2f(ml.x - top);
             sum += f * ml.y;
-            const float *src = p.ws_o + at(c) * DH + lane * NV;
+            if (f == 0.f) continue;   // (a part that saw nothing has no outputs)
+            const float *src = p.ws_o + k * DH + lane * NV;
 #pragma unroll
             for (int e = 0; e < NV; ++e) acc[e] += f * src[e];
         }
+        return sum;
+    };
+    auto highest = [&](int c0, int c1, int in_tile) {
+        float top = -INFINITY;
+        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, p.ws_ml[at(c, c0, in_tile) * 2]);
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        return top == -INFINITY ? 0.f : top;
+    };
+    auto store = [&](int64_t i, const float (&acc)[NV], float sum) {
+        const int64_t row = i / p.heads, qh = i - row * p.heads;
+        T *dst = static_cast<T *>(p.out) + row * p.o_rs + qh * p.o_hs + lane * NV;
         const float inv = 1.f / sum;
-        T *dst = static_cast<T *>(p.out) + (int64_t)row * p.o_rs + (int64_t)qh * p.o_hs + lane * NV;
 #pragma unroll
         for (int e = 0; e < NV; ++e) dst[e] = Elem<T>::from_f(acc[e] * inv);
+    };
+    for (int64_t i0 = (int64_t)blockIdx.x * 8; i0 < n; i0 += (int64_t)gridDim.x * 8) {
+        if (threadIdx.x == 0) s_many = 0;
+        __syncthreads();
+        int c0, c1, in_tile;
+        if (find(i0 + warp, c0, c1, in_tile)) {
+            if (c1 - c0 < kAlone) {
+                float acc[NV] = {};
+                const float top = highest(c0, c1, in_tile);
+                const float sum = add(c0, c1, in_tile, top, 0, 1, acc);
+                store(i0 + warp, acc, sum);
+            } else if (lane == 0) {
+                atomicOr(&s_many, 1 << warp);
+            }
+        }
+        __syncthreads();
+        for (int many = s_many; many; many &= many - 1) {
+            const int64_t i = i0 + __ffs(many) - 1;
+            find(i, c0, c1, in_tile);
+            float acc[NV] = {};
+            const float top = highest(c0, c1, in_tile);
+            const float sum = add(c0, c1, in_tile, top, warp, 8, acc);
+#pragma unroll
+            for (int e = 0; e < NV; ++e) s_acc[warp][lane * NV + e] = acc[e];
+            if (lane == 0) s_sum[warp] = sum;
+            __syncthreads();
+            if (warp == 0) {
+                float total = 0.f;
+#pragma unroll
+                for (int e = 0; e < NV; ++e) acc[e] = 0.f;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    total += s_sum[x];
+#pragma unroll
+                    for (int e = 0; e < NV; ++e) acc[e] += s_acc[x][lane * NV + e];
+                }
+                store(i, acc, total);
+            }
+            __syncthreads();
+        }
     }
 }
 
-template <int DH, int BM>
-cudaError_t launch_bf16(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
-    static std::atomic<uint64_t> done{0};
-    constexpr int smem = TreeShape<DH, BM>::kSmem;
-    cudaError_t e = allow_smem(tree_attn_kernel<DH, BM>, smem, done);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(tree_attn_kernel<DH, BM>, dim3(ctas), dim3(kThreads), smem, s, kv->kv_map, p);
-}
 template <int DH>
-cudaError_t launch_dim(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
-    if (kv->d.dtype == PK_DTYPE_BF16)
-        return p.shape.rows == 16 ? launch_bf16<DH, 16>(kv, p, ctas, s)
-                                  : launch_bf16<DH, 32>(kv, p, ctas, s);
+cudaError_t launch_dim(const pk_token_kv *kv, const TreeParams &p, int workers, cudaStream_t s) {
+    if (kv->d.dtype == PK_DTYPE_BF16) {
+        static std::atomic<uint64_t> done{0};
+        constexpr int smem = kWarps * 2 * tree_tile_keys(DH) * DH * 2 + 1024;
+        cudaError_t e = allow_smem(tree_attn_kernel<DH>, smem, done);
+        if (e != cudaSuccess) return e;
+        // few workers: one a CTA, on an SM of its own
+        const int ctas = workers <= kv->sms ? workers : (workers + kWarps - 1) / kWarps;
+        return launch_pdl(tree_attn_kernel<DH>, dim3(ctas), dim3(kWarps * 32), smem, s, kv->kv_map, p);
+    }
+    const int ctas = workers;
     static std::atomic<uint64_t> done{0};
     constexpr int smem = (kTile * (DH + 4) + kTile * DH + kRowsF32 * DH + kRowsF32 * kTile) * 4;
     cudaError_t e = allow_smem(tree_attn_f32_kernel<DH>, smem, done);
