@@ -61,8 +61,7 @@ int pk_token_kv_create(const pk_token_kv_desc *desc, pk_token_kv **out) {
         const uint64_t row = (uint64_t)d.head_dim * 2, blocks = d.head_dim / 64;
         const uint64_t dims[5] = {64, 8, blocks, (uint64_t)d.page_size / 8, (uint64_t)planes};
         const uint64_t strides[4] = {row, 128, 8 * row, row * d.page_size};
-        const int most = tree_tile_keys(d.head_dim);
-        const uint32_t groups = (d.page_size < most ? d.page_size : most) / 8;
+        const uint32_t groups = (d.page_size < kTokRowsBox ? d.page_size : kTokRowsBox) / 8;
         const uint32_t box[5] = {64, 8, (uint32_t)blocks, groups, 1};
         int st = encode_tmap(&kv->kv_map, d.dtype, d.kv, 5, dims, strides, box);
         if (st != PK_OK) {

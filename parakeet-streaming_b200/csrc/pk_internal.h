@@ -212,7 +212,7 @@ int launch_features(const FeArgs &a, cudaStream_t s);
 struct pk_token_kv {
     pk_token_kv_desc d;
     CUtensorMap kv_map;  // bf16 pools: {64, 8, head_dim / 64, page_size / 8, pages*layers*2*
-                         // kv_heads}, boxes of min(page_size, tree_tile_keys) rows, 128B-swizzled
+                         // kv_heads}, boxes of min(page_size, kTokRowsBox) rows, 128B-swizzled
     int ps_shift, esize, group;
     int sms;
 };
@@ -227,17 +227,18 @@ struct TokShape {
     int least;   // key tiles that a worker takes before a request's are split over several
     int lead;    // what beginning a row tile costs, in key tiles
 };
-// Keys of a tile of the 16-row kernel, and most rows of a page that one TMA copy
-// brings: 8 KB.
-constexpr int tree_tile_keys(int head_dim) { return head_dim == 64 ? 64 : 32; }
-constexpr int kTokWorkers = 12;   // most workers an SM
+// Most rows of a page that one TMA copy brings, and keys of a tile of the 16-row
+// kernel; its workers an SM, with two tiles of shared memory each (8 KB, or 16 for
+// 128-wide heads).
+constexpr int kTokRowsBox = 64;
+constexpr int tok_workers(int head_dim) { return head_dim == 64 ? 12 : 6; }
 // bf16: row tiles of 16 by mma.sync, a warp a worker, where they hold an average
 // request (its K/V is read once per row tile); of 128 by tcgen05, a CTA a worker,
 // otherwise.  float32: 16.
 inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
     if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, 2 * kv->sms, 1, 1};
-    if (mean <= 16) return {16, tree_tile_keys(kv->d.head_dim), kTokWorkers * kv->sms, 8, 1};
+    if (mean <= 16) return {16, kTokRowsBox, tok_workers(kv->d.head_dim) * kv->sms, 8, 1};
     return {128, 128, kv->sms, 4, 2};
 }
 
@@ -266,7 +267,7 @@ inline TokLayout tok_layout(const pk_token_kv *kv, int batch, int rows, int tree
     l.row_start = take(batch + 1);
     l.context = take(batch);
     l.slot = take(batch);
-    l.first = take(kTokWorkers * kv->sms);
+    l.first = take(tok_workers(64) * kv->sms);
     l.take = take(batch + 1);
     l.held = take(batch);
     l.request = take(rows);

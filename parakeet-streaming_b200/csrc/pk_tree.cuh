@@ -70,7 +70,7 @@ struct Work {
     const TreeParams &p;
     int cta, b, nr, kt;   // request, its row tiles and key tiles
     int head, rt, at;     // the next unit's K/V head, row tile and place in it
-    int64_t left;         // places (or row tiles) left to this CTA
+    int left;             // places (or row tiles) left to this worker
     bool whole;
     Unit u;
 
@@ -83,7 +83,7 @@ struct Work {
         load();
         const int64_t *work = reinterpret_cast<const int64_t *>(p.step + p.l.work);
         const int64_t from = whole ? (int64_t)c : (int64_t)c * share, local = from - work[b];
-        left = min(whole ? (int64_t)1 : (int64_t)share, work[p.batch] - from);
+        left = (int)min(whole ? (int64_t)1 : (int64_t)share, work[p.batch] - from);
         int64_t item = local;
         at = 0;
         if (!whole) {
@@ -121,7 +121,7 @@ struct Work {
                 --left;
                 at = 0;
             } else {
-                const int lead = p.shape.lead, n = (int)min((int64_t)(kt + lead - at), left);
+                const int lead = p.shape.lead, n = min(kt + lead - at, left);
                 u.t0 = max(at - lead, 0);
                 u.t1 = max(at + n - lead, 0);
                 u.part = u.t1 - u.t0 == kt ? -1 : (u.t0 == 0 ? 2 * cta + 1 : 2 * cta);
@@ -170,11 +170,6 @@ struct Pages {
         block = ((w.t0 * p.shape.keys) >> p.ps_shift) & ~31;
         ids = fetch(block);
         ahead = fetch(block + 32);
-    }
-    // back to the unit's first entries
-    __device__ __forceinline__ void rewind(const TreeParams &p, const Unit &w) {
-        const int first = ((w.t0 * p.shape.keys) >> p.ps_shift) & ~31;
-        if (block != first) open(p, w);
     }
     // entry `at` of the caller's lane; uniform in at / 32
     __device__ __forceinline__ int get(int at) {

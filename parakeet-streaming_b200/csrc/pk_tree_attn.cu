@@ -12,11 +12,12 @@
 // through (two partial results a worker at most).
 //
 // bf16, row tiles of 16: every warp is a worker of its own, with a share of the line and
-// two 8 KB slots of shared memory, one for a tile of K and one for its V (TMA, a page a
+// two slots of shared memory, one for a tile of 64 keys and one for its V (TMA, a page a
 // copy, 128B swizzle).  It requests the next K as soon as it has read one and the next
 // V likewise, across its units, computes S = Q K^T and O += P V with mma.sync m16n8k16
-// and waits for nobody: 12 such chains an SM (a tile takes a warp some 2600 cycles, 700
-// is an SM's share of the memory rate) hide each other's latencies.  Warps that shared
+// and waits for nobody: 12 such chains an SM for 64-wide heads, 6 for 128 (a tile takes
+// a warp some 2600 cycles; its 16 KB are 700 of an SM's share of the memory rate) hide
+// each other's latencies.  Warps that shared
 // a row tile met in a barrier at its end and cost 5000 cycles a row tile, however short
 // (160 requests of up to 500 tokens, 8 heads: 41 us).
 // P is rounded to bf16 for the product, relative 2^-9 of each weight, below the
@@ -30,7 +31,14 @@
 namespace pk {
 namespace {
 
-constexpr int kWarps = 4;   // workers of a CTA
+constexpr int kTile = kTokRowsBox;   // keys
+// Workers (warps) of a CTA and CTAs an SM: what registers and shared memory hold.
+template <int DH> struct TreeShape {
+    static constexpr int kWarps = DH == 64 ? 4 : 6, kCtas = DH == 64 ? 3 : 1;
+    static_assert(kWarps * kCtas == tok_workers(DH), "workers");
+    static constexpr int kSlot = kTile * DH * 2;   // a tile of K or of V
+    static constexpr int kSmem = kWarps * 2 * kSlot + 1024;
+};
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -74,7 +82,6 @@ __device__ __forceinline__ uint64_t seen_keys(int trees, uint64_t mask, int node
 // warps of a tile write the same zeros.
 template <int DH>
 __device__ __forceinline__ bool clean_values(uint8_t *vs, int k0, int ctx, int len) {
-    constexpr int kTile = tree_tile_keys(DH);
     bool odd = false;
     for (int c = max(ctx - k0, 0) * (DH / 8) + (threadIdx.x & 31); c < kTile * DH / 8; c += 32) {
         const int row = c / (DH / 8), ch = c % (DH / 8);
@@ -93,61 +100,60 @@ __device__ __forceinline__ bool clean_values(uint8_t *vs, int k0, int ctx, int l
     return __any_sync(0xffffffffu, odd);
 }
 
-template <int DH>
-__global__ void __launch_bounds__(kWarps * 32, 3)
-    tree_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeParams p) {
-    // keys of a tile, and of one chain of maximum, exponential and sum: 8 KB of K
-    constexpr int kTile = tree_tile_keys(DH), kSlot = kTile * DH * 2, kN = kTile / 8;
-    extern __shared__ uint8_t tree_smem[];
-    __shared__ __align__(8) uint64_t full[kWarps][2];
-    __shared__ volatile int failed;
+template <int kWarps> struct TreeShared {
+    uint64_t full[kWarps][2];   // K and V of each worker
+    float2 ml[kWarps][16];
+    int failed;
+};
+
+// One worker's share; or, kTeam, one warp's part of the CTA's row tile: every kWarps-th
+// key tile, the warps meeting at the end.
+template <int DH, bool kTeam>
+__device__ __forceinline__ void attend(const CUtensorMap &kv_map, const TreeParams &p, uint8_t *smem,
+                                       TreeShared<TreeShape<DH>::kWarps> &sh) {
+    constexpr int kWarps = TreeShape<DH>::kWarps, kSlot = TreeShape<DH>::kSlot, kN = kTile / 8;
+    constexpr int kStride = kTeam ? kWarps : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint8_t *ks = reinterpret_cast<uint8_t *>(
-                      (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023)) +
-                  warp * 2 * kSlot;
-    uint8_t *vs = ks + kSlot;
+    uint8_t *ks = smem + warp * 2 * kSlot, *vs = ks + kSlot;
     const uint32_t kb = smem_u32(ks), vb = smem_u32(vs);
-    if (threadIdx.x == 0) {
-        for (int w = 0; w < kWarps; ++w) {
-            mbar_init(&full[w][0], 1);
-            mbar_init(&full[w][1], 1);
-        }
-        failed = 0;
-        fence_mbar_init();
-        prefetch_tmap(&kv_map);
-    }
-    __syncthreads();
-    grid_dep_wait();
-    grid_dep_launch();
+    uint64_t *full = sh.full[warp];
+    volatile int *failed = &sh.failed;
 
     const int ps = 1 << p.ps_shift, rows_box = min(ps, kTile);
-    // request K (v = 0) or V (1) of tile t of a unit: a page a lane
-    auto request = [&](const Unit &w, Pages &pages, int t, int v) {
+    int page = 0;   // of this lane's rows of the tile requested last
+    // request V of tile t of a unit, whose K has been; K of one: a page a lane
+    auto request_rows = [&](const Unit &w, int t, int v) {
         const int k0 = t * kTile;
         const int n = (min(kTile, w.ctx + w.count - k0) + rows_box - 1) / rows_box;
-        // lanes without a box ask for the last one's page
-        int page = pages.get((k0 + min(lane, n - 1) * rows_box) >> p.ps_shift);
+        const uint32_t bytes = rows_box * DH * 2;
+        if (lane == 0) mbar_arrive_expect_tx(&full[v], n * bytes);
+        __syncwarp();
+        if (lane < n)
+            tma_load_rows((v ? vs : ks) + lane * bytes, &kv_map, &full[v],
+                          (k0 + lane * rows_box) & (ps - 1),
+                          ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
+    };
+    auto request_keys = [&](const Unit &w, Pages &pages, int t) {
+        const int k0 = t * kTile;
+        const int last = (min(kTile, w.ctx + w.count - k0) - 1) / rows_box;
+        // lanes without rows ask for the last page
+        page = pages.get((k0 + min(lane, last) * rows_box) >> p.ps_shift);
         if (page < 0 || page >= p.num_pages) {
             raise(p.error, PK_DEV_BAD_PAGE);
             page = 0;
         }
-        const uint32_t bytes = rows_box * DH * 2;
-        if (lane == 0) mbar_arrive_expect_tx(&full[warp][v], n * bytes);
-        __syncwarp();
-        if (lane < n)
-            tma_load_rows((v ? vs : ks) + lane * bytes, &kv_map, &full[warp][v],
-                          (k0 + lane * rows_box) & (ps - 1),
-                          ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
+        request_rows(w, t, 0);
     };
 
     const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
     // neighbouring shares on different SMs
-    Work work(p, warp * gridDim.x + blockIdx.x);
+    Work work(p, kTeam ? blockIdx.x : warp * gridDim.x + blockIdx.x);
     // units that have tiles (a chain's rows may see none of a share's)
     auto advance = [&]() {
         while (work.next()) {
-            if (work.u.t0 < work.u.t1) return true;
+            if (kTeam) work.u.t0 += warp;
+            if (work.u.t0 < work.u.t1 || kTeam) return true;
             if (work.u.part >= 0 && lane < 16)   // nothing seen: no weight in the join
                 *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)work.u.part * 16 + lane) * 2) =
                     make_float2(-INFINITY, 0.f);
@@ -156,12 +162,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
     };
     bool more = advance();
     Unit w = work.u;
-    Pages pages, vpages, then;   // K and V walk the pages a tile apart
-    if (more) {
+    Pages pages, then;
+    if (more && w.t0 < w.t1) {
         pages.open(p, w);
-        vpages = pages;
-        request(w, pages, w.t0, 0);
-        request(w, vpages, w.t0, 1);
+        request_keys(w, pages, w.t0);
+        request_rows(w, w.t0, 1);
     }
     uint32_t phase = 0;   // of both barriers: one use a tile
     while (more) {
@@ -200,10 +205,10 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
             for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // maxima scaled
 
-        for (int t = w.t0; t < w.t1; ++t, phase ^= 1) {
+        for (int t = w.t0; t < w.t1; t += kStride, phase ^= 1) {
             const int k0 = t * kTile;
             const bool own = k0 + kTile > w.ctx;   // some of the step's own tokens, or the end
-            ring_wait(&full[warp][0], phase, &failed, p.error);
+            ring_wait(&full[0], phase, failed, p.error);
             __syncwarp();
             float s[kN][4];
 #pragma unroll
@@ -222,8 +227,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
                 }
             }
             __syncwarp();
-            if (t + 1 < w.t1) request(w, pages, t + 1, 0);
-            else if (more) request(work.u, then, work.u.t0, 0);
+            const bool here = t + kStride < w.t1;   // the next tile is this unit's
+            if (here) request_keys(w, pages, t + kStride);
+            else if (more) request_keys(work.u, then, work.u.t0);
             if (own) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -271,7 +277,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
                 o[n][2] *= keep[1];
                 o[n][3] *= keep[1];
             }
-            ring_wait(&full[warp][1], phase, &failed, p.error);
+            ring_wait(&full[1], phase, failed, p.error);
             __syncwarp();
             // a value that is not finite among the step's own rows
             const bool odd = own && clean_values<DH>(vs, k0, w.ctx, len);
@@ -320,47 +326,112 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
                 }
             }
             __syncwarp();
-            if (t + 1 < w.t1) {
-                request(w, vpages, t + 1, 1);
-            } else if (more) {
-                vpages = then;
-                vpages.rewind(p, work.u);
-                request(work.u, vpages, work.u.t0, 1);
-            }
+            if (here) request_rows(w, t + kStride, 1);
+            else if (more) request_rows(work.u, work.u.t0, 1);
         }
         // row sums over the quad's lanes
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            const int rt = (lane >> 2) + h * 8, r = w.rt * 16 + rt;
-            if (r >= m_rows) continue;
-            if (w.part >= 0) {
-                const int64_t at = (int64_t)w.part * 16 + rt;
-                float *dst = p.ws_o + at * DH + (lane & 3) * 2;
+        }
+        if (kTeam) {
+            // the warps' rows in their slots (all copies have been waited for)
+            float *mine = reinterpret_cast<float *>(ks);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int rt = (lane >> 2) + h * 8;
 #pragma unroll
                 for (int n = 0; n < DH / 8; ++n)
-                    *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-                if ((lane & 3) == 0)
-                    *reinterpret_cast<float2 *>(p.ws_ml + at * 2) = make_float2(m[h], l[h]);
-            } else {
-                const float inv = 1.f / l[h];
-                __nv_bfloat16 *dst =
-                    out + (int64_t)(w.row0 + node[h]) * p.o_rs +
-                    (int64_t)(w.head * p.group + r - node[h] * p.group) * p.o_hs + (lane & 3) * 2;
+                    *reinterpret_cast<float2 *>(mine + rt * DH + n * 8 + (lane & 3) * 2) =
+                        make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                if ((lane & 3) == 0) sh.ml[warp][rt] = make_float2(m[h], l[h]);
+            }
+            __syncthreads();
+            const float *all = reinterpret_cast<const float *>(smem);
+            for (int c = threadIdx.x; c < 16 * DH / 2; c += kWarps * 32) {
+                const int rt = c / (DH / 2), col = c % (DH / 2) * 2, r = w.rt * 16 + rt;
+                if (r >= m_rows) continue;
+                float top = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < DH / 8; ++n)
-                    *reinterpret_cast<uint32_t *>(dst + n * 8) =
-                        pack2(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+                for (int k = 0; k < kWarps; ++k) top = fmaxf(top, sh.ml[k][rt].x);
+                const float ref = top == -INFINITY ? 0.f : top;
+                float x = 0.f, y = 0.f, sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < kWarps; ++k) {
+                    const float f = ex2(sh.ml[k][rt].x - ref);
+                    const float2 v = *reinterpret_cast<const float2 *>(
+                        all + k * (2 * kSlot / 4) + rt * DH + col);
+                    sum += f * sh.ml[k][rt].y;
+                    x += f * v.x;
+                    y += f * v.y;
+                }
+                const int nd = r / p.group;
+                *reinterpret_cast<uint32_t *>(
+                    out + (int64_t)(w.row0 + nd) * p.o_rs +
+                    (int64_t)(w.head * p.group + r - nd * p.group) * p.o_hs + col) =
+                    pack2(x / sum, y / sum);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int rt = (lane >> 2) + h * 8, r = w.rt * 16 + rt;
+                if (r >= m_rows) continue;
+                if (w.part >= 0) {
+                    const int64_t at = (int64_t)w.part * 16 + rt;
+                    float *dst = p.ws_o + at * DH + (lane & 3) * 2;
+#pragma unroll
+                    for (int n = 0; n < DH / 8; ++n)
+                        *reinterpret_cast<float2 *>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                    if ((lane & 3) == 0)
+                        *reinterpret_cast<float2 *>(p.ws_ml + at * 2) = make_float2(m[h], l[h]);
+                } else {
+                    const float inv = 1.f / l[h];
+                    __nv_bfloat16 *dst =
+                        out + (int64_t)(w.row0 + node[h]) * p.o_rs +
+                        (int64_t)(w.head * p.group + r - node[h] * p.group) * p.o_hs + (lane & 3) * 2;
+#pragma unroll
+                    for (int n = 0; n < DH / 8; ++n)
+                        *reinterpret_cast<uint32_t *>(dst + n * 8) =
+                            pack2(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+                }
             }
         }
         w = work.u;
         pages = then;
     }
-    if (failed) {   // leave no copy in flight
-        mbar_wait_bounded(&full[warp][0], phase ^ 1, kWaitLimitNs);
-        mbar_wait_bounded(&full[warp][1], phase ^ 1, kWaitLimitNs);
+    if (*failed) {   // leave no copy in flight
+        mbar_wait_bounded(&full[0], phase ^ 1, kWaitLimitNs);
+        mbar_wait_bounded(&full[1], phase ^ 1, kWaitLimitNs);
     }
+}
+
+template <int DH>
+__global__ void __launch_bounds__(TreeShape<DH>::kWarps * 32, TreeShape<DH>::kCtas)
+    tree_attn_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeParams p) {
+    extern __shared__ uint8_t tree_smem[];
+    constexpr int kWarps = TreeShape<DH>::kWarps;
+    __shared__ __align__(8) TreeShared<kWarps> sh;
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < kWarps; ++w) {
+            mbar_init(&sh.full[w][0], 1);
+            mbar_init(&sh.full[w][1], 1);
+        }
+        sh.failed = 0;
+        fence_mbar_init();
+        prefetch_tmap(&kv_map);
+    }
+    __syncthreads();
+    grid_dep_wait();
+    grid_dep_launch();
+    // a CTA for every row tile (short requests, few of them): its warps are a team
+    if (p.step[kTokShare] == 0 &&
+        reinterpret_cast<const int64_t *>(p.step + p.l.work)[p.batch] <= gridDim.x)
+        attend<DH, true>(kv_map, p, smem, sh);
+    else
+        attend<DH, false>(kv_map, p, smem, sh);
 }
 
 // ------------------------------------------------------------------ float32
@@ -368,7 +439,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
 // 16-row tile; K rows are padded so that a lane per key reads without bank
 // conflicts; a warp computes the scores of its four rows (two keys a lane), then
 // their outputs (DH / 32 columns a lane).
-constexpr int kRowsF32 = 16, kTile = 64;
+constexpr int kRowsF32 = 16;
 template <int DH>
 __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) {
     constexpr int kKp = DH + 4, NV = DH / 32;
@@ -518,17 +589,14 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
 }
 
 // ------------------------------------------------------------------ the join
-// A warp per (row, head): its row tile's partial results - of the workers whose shares
-// cut the tile's keys - weighted by exp2(m - max m).  Rows with more than kAlone
-// partials (a long request's) are summed by the block's eight warps together.  The
-// order is that of the keys in both, so that the result does not depend on which
-// worker finished first.
-constexpr int kAlone = 16;
-template <int DH, typename T>
+// For every (row, head) its row tile's partial results - of the workers whose shares
+// cut the tile's keys - weighted by exp2(m - max m), in order of the keys, so that the
+// result does not depend on which worker finished first.  A warp an entry, or, with few
+// entries (kTeam), a block: each warp every eighth partial, then the warps' sums.
+template <int DH, typename T, bool kTeam>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     constexpr int NV = DH / 32;
     __shared__ float s_acc[8][DH], s_sum[8];
-    __shared__ int s_many;
     grid_dep_wait();
     grid_dep_launch();
     const int64_t share = p.step[kTokShare];
@@ -559,16 +627,18 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     // sums workers c0 + w0, + step, ..: outputs and the sum, relative to exp2(top)
     auto add = [&](int c0, int c1, int in_tile, float top, int w0, int step, float (&acc)[NV]) {
         float sum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int c = c0 + w0; c <= c1; c += step) {
             const int64_t k = at(c, c0, in_tile);
             const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + k * 2);
             const float f = exp2f(ml.x - top);
             sum += f * ml.y;
-            if (f == 0.f) continue;   // (a part that saw nothing has no outputs)
             const float *src = p.ws_o + k * DH + lane * NV;
 #pragma unroll
-            for (int e = 0; e < NV; ++e) acc[e] += f * src[e];
+            for (int e = 0; e < NV; ++e) {
+                const float x = src[e];
+                acc[e] += f == 0.f ? 0.f : f * x;   // a part that saw nothing wrote no outputs
+            }
         }
         return sum;
     };
@@ -586,27 +656,15 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
 #pragma unroll
         for (int e = 0; e < NV; ++e) dst[e] = Elem<T>::from_f(acc[e] * inv);
     };
-    for (int64_t i0 = (int64_t)blockIdx.x * 8; i0 < n; i0 += (int64_t)gridDim.x * 8) {
-        if (threadIdx.x == 0) s_many = 0;
-        __syncthreads();
+    const int step = kTeam ? 8 : 1, first = kTeam ? warp : 0;
+    for (int64_t i = kTeam ? blockIdx.x : (int64_t)blockIdx.x * 8 + warp; i < n;
+         i += (int64_t)gridDim.x * (kTeam ? 1 : 8)) {
         int c0, c1, in_tile;
-        if (find(i0 + warp, c0, c1, in_tile)) {
-            if (c1 - c0 < kAlone) {
-                float acc[NV] = {};
-                const float top = highest(c0, c1, in_tile);
-                const float sum = add(c0, c1, in_tile, top, 0, 1, acc);
-                store(i0 + warp, acc, sum);
-            } else if (lane == 0) {
-                atomicOr(&s_many, 1 << warp);
-            }
-        }
-        __syncthreads();
-        for (int many = s_many; many; many &= many - 1) {
-            const int64_t i = i0 + __ffs(many) - 1;
-            find(i, c0, c1, in_tile);
-            float acc[NV] = {};
-            const float top = highest(c0, c1, in_tile);
-            const float sum = add(c0, c1, in_tile, top, warp, 8, acc);
+        if (!find(i, c0, c1, in_tile)) continue;
+        float acc[NV] = {};
+        const float top = highest(c0, c1, in_tile);
+        const float sum = add(c0, c1, in_tile, top, first, step, acc);
+        if (kTeam) {
 #pragma unroll
             for (int e = 0; e < NV; ++e) s_acc[warp][lane * NV + e] = acc[e];
             if (lane == 0) s_sum[warp] = sum;
@@ -624,6 +682,8 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
                 store(i, acc, total);
             }
             __syncthreads();
+        } else {
+            store(i, acc, sum);
         }
     }
 }
@@ -632,12 +692,13 @@ template <int DH>
 cudaError_t launch_dim(const pk_token_kv *kv, const TreeParams &p, int workers, cudaStream_t s) {
     if (kv->d.dtype == PK_DTYPE_BF16) {
         static std::atomic<uint64_t> done{0};
-        constexpr int smem = kWarps * 2 * tree_tile_keys(DH) * DH * 2 + 1024;
+        using S = TreeShape<DH>;
+        constexpr int smem = S::kSmem;
         cudaError_t e = allow_smem(tree_attn_kernel<DH>, smem, done);
         if (e != cudaSuccess) return e;
         // few workers: one a CTA, on an SM of its own
-        const int ctas = workers <= kv->sms ? workers : (workers + kWarps - 1) / kWarps;
-        return launch_pdl(tree_attn_kernel<DH>, dim3(ctas), dim3(kWarps * 32), smem, s, kv->kv_map, p);
+        const int most = S::kCtas * kv->sms, ctas = workers < most ? workers : most;
+        return launch_pdl(tree_attn_kernel<DH>, dim3(ctas), dim3(S::kWarps * 32), smem, s, kv->kv_map, p);
     }
     const int ctas = workers;
     static std::atomic<uint64_t> done{0};
@@ -646,13 +707,14 @@ cudaError_t launch_dim(const pk_token_kv *kv, const TreeParams &p, int workers, 
     if (e != cudaSuccess) return e;
     return launch_pdl(tree_attn_f32_kernel<DH>, dim3(ctas), dim3(128), smem, s, p);
 }
-template <int DH>
-cudaError_t launch_join(const TreeParams &p, int dtype, int sms, cudaStream_t s) {
-    const int64_t ctas = ((int64_t)p.rows * p.heads + 7) / 8, lim = 8 * (int64_t)sms;
-    const dim3 grid((unsigned)(ctas < lim ? ctas : lim));
-    return dtype == PK_DTYPE_BF16
-               ? launch_pdl(tree_join_kernel<DH, __nv_bfloat16>, grid, dim3(256), 0, s, p)
-               : launch_pdl(tree_join_kernel<DH, float>, grid, dim3(256), 0, s, p);
+template <int DH, typename T>
+cudaError_t launch_join(const TreeParams &p, int sms, cudaStream_t s) {
+    const int64_t n = (int64_t)p.rows * p.heads, most = 8 * (int64_t)sms;
+    if (n <= most)
+        return launch_pdl(tree_join_kernel<DH, T, true>, dim3((unsigned)n), dim3(256), 0, s, p);
+    const int64_t ctas = (n + 7) / 8;
+    return launch_pdl(tree_join_kernel<DH, T, false>, dim3((unsigned)(ctas < most ? ctas : most)),
+                      dim3(256), 0, s, p);
 }
 
 // Most row tiles of a step.
@@ -712,8 +774,12 @@ int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStre
                                         : launch_dim<128>(kv, p, ctas, s);
     if (e != cudaSuccess) return cuda_status(e, "tree attention kernel");
     if (!shared) return PK_OK;
-    e = d.head_dim == 64 ? launch_join<64>(p, d.dtype, kv->sms, s)
-                         : launch_join<128>(p, d.dtype, kv->sms, s);
+    if (d.dtype == PK_DTYPE_BF16)
+        e = d.head_dim == 64 ? launch_join<64, __nv_bfloat16>(p, kv->sms, s)
+                             : launch_join<128, __nv_bfloat16>(p, kv->sms, s);
+    else
+        e = d.head_dim == 64 ? launch_join<64, float>(p, kv->sms, s)
+                             : launch_join<128, float>(p, kv->sms, s);
     return cuda_status(e, "tree_join_kernel");
 }
 

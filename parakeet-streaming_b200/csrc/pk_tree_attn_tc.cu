@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     grid_dep_launch();
     auto produce = [&]() {
         // producer: lanes issue a tile's boxes, K then V
-        const int ps = 1 << p.ps_shift, rows_box = min(ps, tree_tile_keys(DH));
+        const int ps = 1 << p.ps_shift, rows_box = min(ps, kTokRowsBox);
         const int box_of = lane;
         const uint32_t bytes = rows_box * DH * 2;
         int it = 0;
