@@ -7,14 +7,12 @@
 //  1. the plan (once per step: every projection of a model uses the same ids)
 //     sorts the rows by adapter, so that a 128-row tile meets few adapters, and
 //     lists each tile's (adapter, rows) pairs;
-//  2. S in bf16, by sorted row.  Bound by reading x: a tile's K is cut over a
-//     cluster of CTAs, whose sums meet in distributed shared memory;
-//  3. the product on the tcgen05 tensor cores.  The A operand's rows are fetched
-//     in sorted order; after the K blocks of x W^T each pair of the
-//     tile adds one K block S up[a]^T into the same accumulator, with the lanes of
-//     other rows disabled in the MMA: they get no zero products, so one adapter's
-//     weights, whatever they hold, do not reach another's rows.  The epilogue
-//     writes the rows back to their own places.
+//  2. S in bf16 and the rows' sorted copy, bound by reading and writing them;
+//  3. the product on the tcgen05 tensor cores, over the sorted rows; after the K
+//     blocks of x W^T each pair of the tile adds one K block S up[a]^T into the same
+//     accumulator, with the lanes of other rows disabled in the MMA: they get no zero
+//     products, so one adapter's weights, whatever they hold, do not reach another's
+//     rows.  The epilogue writes the rows back to their own places.
 //
 // S is rounded to bf16 because the tensor cores take it so: relative 2^-9 of each
 // of its terms, half of what rounding the sum to the bf16 result costs.  Sums are
@@ -157,211 +155,147 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
 }
 
 // --------------------------------------------------------------------- S
-// CTA (rank, tile): K blocks rank, rank + C, ... of the tile's 128 rows.  A stage
-// holds 64 columns of the rows and of the down rows of as many pairs as fit 128
-// columns of S; with more pairs the rows are streamed again for the next ones.
-constexpr int kShThreads = 256;
-template <int NT> struct ShrinkShape {
-    static constexpr int kCols = 128;
-    static constexpr int kStage = (kTileRows + kCols) * 128;
-    static constexpr int kStages = 96 * 1024 / kStage;   // two CTAs an SM
-    // the column tiles past a pair's rank read up to 8 NT columns behind the last
-    static constexpr int kSmem = kStages * kStage + NT * 1024 + 1024;
-};
+// S[m] = scale[a] * x[m] down[a]^T for 16 sorted rows (one m16n8k16 row tile) a CTA,
+// the K blocks of 64 dealt out to its eight warps.  Operands go from global memory to
+// fragments directly: the contraction may take its terms in any order, so a lane's
+// share of a row's 32 columns can be 8 neighbouring ones (16 bytes), for rows of x and
+// of down alike, and needs no shared memory, no barrier and no ldmatrix.  Rows whose
+// order is not the sorted one are written to their sorted copy on the way.
+//
+// A group of rows with several adapters takes a pass for each, and a pass keeps the
+// sums of its own rows only, so no product of another adapter's weights reaches a row;
+// with few groups the passes are CTAs of their own (blockIdx.y).
+//
+// Reading x and writing its copy bound it: 6720 x 4096, rank 32, 64 adapters, 110 MB.
+// Tiles staged in shared memory with a barrier a stage took 46 us.
+constexpr int kShWarps = 8, kShRows = 16;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool full) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                 "r"(full ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void ldsm4a(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                          uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
         "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NT>   // 8-column tiles of a pair: rank <= 8 NT
-__global__ void __launch_bounds__(kShThreads, 2)
-    adapter_shrink_kernel(const AdapterArgs p, int cluster) {
-    using S = ShrinkShape<NT>;
-    constexpr int kShStage = S::kStage, kShStages = S::kStages, kShCols = S::kCols;
-    extern __shared__ uint8_t sh_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>(
-        (reinterpret_cast<uintptr_t>(sh_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ int s_row[kTileRows];
-    __shared__ int2 s_pair[kTileRows];   // a tile's pairs: a row or more each
+template <int NT>   // 8-column tiles of S: rank <= 8 NT
+__global__ void __launch_bounds__(kShWarps * 32, NT <= 4 ? 3 : 2)
+    adapter_shrink_kernel(const AdapterArgs p) {
+    extern __shared__ float sh_part[];   // [warp][row][rank]
+    __shared__ int2 s_pair[kShRows];     // the group's pairs: adapter, first | end << 16
+    __shared__ int s_n;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-    const int rank = (int)cluster_ctarank(), tile = blockIdx.y, m0 = tile * kTileRows;
     grid_dep_wait();
     grid_dep_launch();
     const int32_t *plan = p.plan;
-    if (tid < kTileRows) s_row[tid] = plan[p.l.order + m0 + tid];
-    const int pair0 = plan[p.l.tile_pair + tile], pair1 = plan[p.l.tile_pair + tile + 1];
-    if (tid < pair1 - pair0) s_pair[tid] = reinterpret_cast<const int2 *>(plan + p.l.pairs)[pair0 + tid];
-    const int r = p.rank, per = kShCols / r, nk = p.K / 64;
-    const int mine = (nk - rank + cluster - 1) / cluster;   // K blocks of this CTA
-    const int batches = max((pair1 - pair0 + per - 1) / per, 1);   // one for the copy at least
-    const __nv_bfloat16 *x = static_cast<const __nv_bfloat16 *>(p.x);
-    const __nv_bfloat16 *down = static_cast<const __nv_bfloat16 *>(p.down);
-    // the rows' sorted copy is made on the way, where their order is another
-    char *copy = plan[p.l.sorted] ? nullptr : static_cast<char *>(p.xs);
-    __syncthreads();
-
-    // this thread's shares of a stage: 4 chunks of rows, 4 of down rows (those of the
-    // batch being loaded), at K block `rank`; a block further on is `step` bytes away
-    const char *src[4], *dsrc[4];
-    char *dst[4];
-    uint32_t live = 0, dlive = 0, soff[4];
-    const int64_t step = (int64_t)cluster * 128;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = tid + i * kShThreads, row = s_row[c >> 3];
-        const bool in = row < p.M;
-        live |= (uint32_t)in << i;
-        src[i] = reinterpret_cast<const char *>(x + (int64_t)(in ? row : 0) * p.ldx) + rank * 128 +
-                 (c & 7) * 16;
-        dst[i] = copy + ((int64_t)(m0 + (c >> 3)) * p.K + rank * 64) * 2 + (c & 7) * 16;
-        soff[i] = sw128(c >> 3, (c & 7) * 16);
-        dsrc[i] = nullptr;
+    const int tile = blockIdx.x / (kTileRows / kShRows);
+    const int g0 = blockIdx.x % (kTileRows / kShRows) * kShRows;   // first row in the tile
+    const int64_t m0 = (int64_t)tile * kTileRows + g0;
+    // the pairs of the tile that have rows of the group
+    if (warp == 0) {
+        const int pair0 = plan[p.l.tile_pair + tile], pair1 = plan[p.l.tile_pair + tile + 1];
+        int n = 0;
+        for (int q = pair0; q < pair1; q += 32) {
+            int2 pr = make_int2(0, 0);
+            if (q + lane < pair1) pr = reinterpret_cast<const int2 *>(plan + p.l.pairs)[q + lane];
+            const int lo = max((pr.y & 0xffff) - g0, 0), hi = min((pr.y >> 16) - g0, kShRows);
+            const unsigned has = __ballot_sync(0xffffffffu, lo < hi);
+            if (lo < hi) s_pair[n + __popc(has & ((1u << lane) - 1u))] = make_int2(pr.x, lo | hi << 16);
+            n += __popc(has);
+        }
+        if (lane == 0) s_n = n;
     }
-    int lb = 0, lk = 0;   // batch and block of the next load
-    auto load = [&](int slot) {
-        if (lk == 0) {
-            const int np = min(per, pair1 - pair0 - lb * per);
-            dlive = 0;
+    __syncthreads();
+    const int n_pairs = s_n, r = p.rank, nk = p.K / 64;
+    const int first = blockIdx.y, step = gridDim.y;
+    if (first > 0 && first >= n_pairs) return;
+    // this lane's rows of x: fragment rows lane / 4 and + 8
+    const int fr = lane >> 2, fc = (lane & 3) * 8;
+    const int r0 = plan[p.l.order + m0 + fr], r1 = plan[p.l.order + m0 + fr + 8];
+    const bool in0 = r0 < p.M, in1 = r1 < p.M;
+    const __nv_bfloat16 *x0 = static_cast<const __nv_bfloat16 *>(p.x) + (in0 ? (int64_t)r0 * p.ldx : 0) + fc;
+    const __nv_bfloat16 *x1 = static_cast<const __nv_bfloat16 *>(p.x) + (in1 ? (int64_t)r1 * p.ldx : 0) + fc;
+    const bool copying = first == 0 && !plan[p.l.sorted];
+    __nv_bfloat16 *copy = static_cast<__nv_bfloat16 *>(p.xs) + (m0 + fr) * p.K + fc;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    const int warps = min(kShWarps, nk);
+
+    for (int j = first; j < max(n_pairs, 1); j += step) {
+        const bool any = j < n_pairs;
+        const int2 pr = any ? s_pair[j] : make_int2(0, 0);
+        const int lo = pr.y & 0xffff, hi = pr.y >> 16;
+        const __nv_bfloat16 *down =
+            static_cast<const __nv_bfloat16 *>(p.down) + ((int64_t)pr.x * r + fr) * p.K + fc;
+        float acc[NT][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = tid + i * kShThreads, col = c >> 3, j = col / r;
-                if (j < np) {
-                    dlive |= 1u << i;
-                    dsrc[i] = reinterpret_cast<const char *>(
-                                  down + ((int64_t)s_pair[lb * per + j].x * r + col - j * r) * p.K) +
-                              rank * 128 + (c & 7) * 16;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+        for (int kb = warp; kb < nk; kb += kShWarps) {
+            uint4 a[2][2];   // columns fc .. + 7 of both halves of the block
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                a[h][0] = in0 ? *reinterpret_cast<const uint4 *>(x0 + kb * 64 + h * 32) : zero;
+                a[h][1] = in1 ? *reinterpret_cast<const uint4 *>(x1 + kb * 64 + h * 32) : zero;
+            }
+            constexpr int kAtOnce = NT < 8 ? NT : 8;   // tiles of S whose rows are in registers
+#pragma unroll
+            for (int n0 = 0; n0 < NT; n0 += kAtOnce) {
+                uint4 b[kAtOnce][2];
+#pragma unroll
+                for (int n = 0; n < kAtOnce; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        b[n][h] = any && (n0 + n) * 8 < r
+                                      ? __ldg(reinterpret_cast<const uint4 *>(
+                                            down + (int64_t)(n0 + n) * 8 * p.K + kb * 64 + h * 32))
+                                      : zero;
+                if (copying && j == 0 && n0 == 0) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        *reinterpret_cast<uint4 *>(copy + kb * 64 + h * 32) = a[h][0];
+                        *reinterpret_cast<uint4 *>(copy + (int64_t)8 * p.K + kb * 64 + h * 32) = a[h][1];
+                    }
+                }
+                if (any) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int n = 0; n < kAtOnce; ++n) {
+                            mma_16816(acc[n0 + n], a[h][0].x, a[h][1].x, a[h][0].y, a[h][1].y,
+                                      b[n][h].x, b[n][h].y);
+                            mma_16816(acc[n0 + n], a[h][0].z, a[h][1].z, a[h][0].w, a[h][1].w,
+                                      b[n][h].z, b[n][h].w);
+                        }
                 }
             }
         }
-        const uint32_t st = smem_u32(smem + slot * kShStage);
-        const int64_t at = lk * step;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cp_async16(st + soff[i], src[i] + at, live >> i & 1);
-            if (dlive >> i & 1) cp_async16(st + kTileRows * 128 + soff[i], dsrc[i] + at, true);
-        }
-        if (++lk == mine) {
-            lk = 0;
-            ++lb;
-        }
-    };
-    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-
-    float acc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-    const int total = batches * mine;
-    const int row_lo = warp * 16 + (lane >> 2);
-    for (int it = 0; it < kShStages - 1; ++it) {
-        if (it < total) load(it);
-        commit();
-    }
-    // ldmatrix offsets: every row index below is lane & 7 modulo 8
-    const uint32_t a_row = (warp * 16 + (lane & 15)) * 128, b_row = (lane & 7) * 128;
-    const uint32_t a_sw = (lane >> 4) ^ (lane & 7), b_sw = (lane >> 3) ^ (lane & 7);
-    int b = 0, kb = 0, slot = 0;
-    for (int it = 0; it < total; ++it) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kShStages - 2) : "memory");
-        __syncthreads();
-        if (it + kShStages - 1 < total) load(slot == 0 ? kShStages - 1 : slot - 1);
-        commit();
-        const uint8_t *st = smem + slot * kShStage;
-        const uint32_t sa = smem_u32(st), sb = sa + kTileRows * 128;
-        if (copy && b == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint4 *>(dst[i] + kb * step) =
-                    *reinterpret_cast<const uint4 *>(st + soff[i]);
-        }
-        const int np = min(per, pair1 - pair0 - b * per);
-        uint32_t a[4][4];
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) ldsm4a(sa + a_row + ((a_sw ^ (ks * 2)) << 4), a[ks]);
-        for (int j = 0; j < np; ++j) {
-            const int range = s_pair[b * per + j].y;
-            const int lo = range & 0xffff, hi = range >> 16;
-            if (hi <= warp * 16 || lo >= warp * 16 + 16) continue;
-            const uint32_t bj = sb + b_row + j * r * 128;
-            const bool in0 = row_lo >= lo && row_lo < hi, in1 = row_lo + 8 >= lo && row_lo + 8 < hi;
+        // the warps' sums, in order (rows without an adapter have no S: their lanes are
+        // off in every product)
+        if (warp < warps) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float t[4] = {0.f, 0.f, 0.f, 0.f};
+                if (n * 8 >= r) break;
 #pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {   // 32 columns of K: 4 matrices
-                    uint32_t bm[4];
-                    ldsm4a(bj + n * 1024 + ((b_sw ^ (k2 * 4)) << 4), bm);
-                    mma_16816(t, a[2 * k2], bm[0], bm[1]);
-                    mma_16816(t, a[2 * k2 + 1], bm[2], bm[3]);
-                }
-                // rows of other adapters keep what they have: no product of theirs
-                if (in0) {
-                    acc[n][0] += t[0];
-                    acc[n][1] += t[1];
-                }
-                if (in1) {
-                    acc[n][2] += t[2];
-                    acc[n][3] += t[3];
-                }
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<float2 *>(sh_part + (warp * kShRows + fr + 8 * h) * r + n * 8 +
+                                                (lane & 3) * 2) =
+                        make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
             }
         }
-        slot = slot + 1 == kShStages ? 0 : slot + 1;
-        if (++kb == mine) {
-            kb = 0;
-            ++b;
+        __syncthreads();
+        const float scale = any && p.scale ? p.scale[pr.x] : 1.f;
+        __nv_bfloat16 *s = static_cast<__nv_bfloat16 *>(p.s) + m0 * r;
+        for (int c = tid; c < kShRows * r; c += kShWarps * 32) {
+            const int row = c / r;
+            if (row < lo || row >= hi) continue;
+            float v = 0.f;
+            for (int w = 0; w < warps; ++w) v += sh_part[w * kShRows * r + c];
+            s[c] = __float2bfloat16_rn(v * scale);
         }
+        __syncthreads();
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
-    // partial sums [row][r] of this CTA, then rows rank * share .. summed over the
-    // cluster in rank order
-    float *part = reinterpret_cast<float *>(smem);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        if (n * 8 >= r) break;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<float2 *>(part + (row_lo + 8 * h) * r + n * 8 + (lane & 3) * 2) =
-                make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
-    }
-    cluster_sync_all();
-    const int share = kTileRows / cluster;
-    __nv_bfloat16 *s = static_cast<__nv_bfloat16 *>(p.s);
-    for (int c = tid; c < share * r; c += kShThreads) {
-        const int row = rank * share + c / r, col = c % r;
-        const uint32_t at = smem_u32(part + row * r + col);
-        float v = 0.f;
-        for (int q = 0; q < cluster; ++q) v += ld_cluster(mapa_rank(at, q));
-        const int m = s_row[row];
-        if (p.scale && m < p.M) {
-            const int a = p.ids[m];
-            if (a >= 0 && a < p.adapters) v *= p.scale[a];
-        }
-        s[(int64_t)(m0 + row) * r + col] = __float2bfloat16_rn(v);
-    }
-    cluster_sync_all();   // no CTA leaves while its sums are read
 }
 
 // ------------------------------------------------------------------ the product
@@ -832,28 +766,14 @@ __global__ void __launch_bounds__(kAdThreads, 1)
 template <int NT>
 cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    constexpr size_t smem = ShrinkShape<NT>::kSmem;
-    cudaError_t e = allow_smem(adapter_shrink_kernel<NT>, smem, done);
+    cudaError_t e = allow_smem(adapter_shrink_kernel<NT>, kShWarps * kShRows * NT * 8 * 4, done);
     if (e != cudaSuccess) return e;
-    // CTAs over K, a block of 64 or more each, while the grid is below a wave
-    const int tiles = (p.M + kTileRows - 1) / kTileRows;
-    int cluster = 1;
-    while (cluster < 8 && 2 * cluster <= p.K / 64 && tiles * cluster < 2 * current_sms()) cluster *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster, tiles);
-    cfg.blockDim = dim3(kShThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attrs[2];
-    attrs[0].id = cudaLaunchAttributeClusterDimension;
-    attrs[0].val.clusterDim.x = cluster;
-    attrs[0].val.clusterDim.y = 1;
-    attrs[0].val.clusterDim.z = 1;
-    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attrs;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, adapter_shrink_kernel<NT>, p, cluster);
+    const int groups = (p.M + kTileRows - 1) / kTileRows * (kTileRows / kShRows);
+    // a CTA for every adapter that a group can have while there are SMs for them; two
+    // otherwise, since a border between two adapters would take its group twice as long
+    const int passes = groups * kShRows <= 2 * current_sms() ? kShRows : 2;
+    return launch_pdl(adapter_shrink_kernel<NT>, dim3(groups, passes), dim3(kShWarps * 32),
+                      kShWarps * kShRows * p.rank * 4, s, p);
 }
 
 template <int BN, int NS, bool kPair, int EPI>
