@@ -13,9 +13,11 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import check, lib
-from .ops import GEMM_EPILOGUES, _gemm_error, _ptr, _rows, _stream, gemm_supported
-from .tokens import _on
+from ._lib import PK_ADAPTER_MAX_RANK, lib
+from .ops import GEMM_EPILOGUES, _gemm_error, _launch, _rows, _stream
+
+
+_BF16 = torch.bfloat16
 
 
 def _error_word(device):
@@ -41,15 +43,13 @@ def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
     change while it is in use."""
     if ids.dtype is not torch.int32 or not ids.is_cuda or ids.dim() != 1 or not ids.is_contiguous():
         raise ValueError("ids must be a contiguous int32 [M] CUDA tensor")
-    rows = ids.shape[0]
+    rows, dev = ids.shape[0], ids.device
     words = lib().pk_adapter_plan_words(rows, num_adapters)
     if words < 0:
         raise ValueError(f"{rows} rows or {num_adapters} adapters: out of range")
-    block = torch.empty(words, dtype=torch.int32, device=ids.device)
-    with _on(ids.device):
-        check(lib().pk_adapter_plan(ids.data_ptr(), rows, num_adapters, block.data_ptr(),
-                                    _error_word(ids.device).data_ptr(), _stream(ids.device)),
-              "pk_adapter_plan")
+    block = torch.empty(words, dtype=torch.int32, device=dev)
+    _launch(dev, lib().pk_adapter_plan, ids.data_ptr(), rows, num_adapters, block.data_ptr(),
+            _error_word(dev).data_ptr(), _stream(dev))
     return AdapterPlan(ids, rows, num_adapters, block)
 
 
@@ -61,8 +61,8 @@ def _operand(t, shape, dtype, dev, name):
 
 def _plain_rows(t):
     """[rows, width] that ops._rows would leave as it is."""
-    return (t.dim() == 2 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-            and t.stride(0) >= t.shape[1])
+    row, col = t.stride()
+    return col == 1 and row % 8 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0
 
 
 def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
@@ -77,23 +77,28 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     rank], bf16; K and N multiples of 64, rank a multiple of 8 up to 128; scale
     float32 [num_adapters] or None.  The plan's rows are those of ``a`` flattened."""
     dev = a.device
-    if not gemm_supported(a, weight) or weight.device != dev:
-        raise ValueError("adapter_gemm needs bf16 operands on one CUDA device, K and N multiples "
-                         "of 64, and an aligned weight")
+    if a.dtype is not _BF16 or weight.dtype is not _BF16 or dev.type != "cuda" or \
+            weight.device != dev or weight.dim() != 2 or a.shape[-1] != weight.shape[1] or \
+            weight.stride(1) != 1:
+        raise ValueError("adapter_gemm needs bf16 operands a [..., K] and weight [N, K], rows "
+                         "contiguous, on one CUDA device")
     N, K = weight.shape
     n = plan.num_adapters
     rank = down.shape[1] if down.dim() == 3 else 0
-    _operand(down, (n, rank, K), torch.bfloat16, dev, "down")
-    _operand(up, (n, N, rank), torch.bfloat16, dev, "up")
+    _operand(down, (n, rank, K), _BF16, dev, "down")
+    _operand(up, (n, N, rank), _BF16, dev, "up")
+    sc = None
     if scale is not None:
         _operand(scale, (n,), torch.float32, dev, "scale")
-    a2 = a if _plain_rows(a) else _rows(a, K)
+        sc = scale.data_ptr()
+    flat = a.dim() == 2
+    a2 = a if flat and _plain_rows(a) else _rows(a, K)
     M = a2.shape[0]
     if plan.rows != M or plan.ids.device != dev:
         raise ValueError(f"the plan is for {plan.rows} rows on {plan.ids.device}, a has {M} on {dev}")
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
-    elif not out.is_contiguous() or out.numel() != M * N or out.dtype is not a.dtype or \
+        out = torch.empty((M, N), dtype=_BF16, device=dev)
+    elif not out.is_contiguous() or out.numel() != M * N or out.dtype is not _BF16 or \
             out.device != dev:
         raise ValueError("out must be a contiguous [M, N] tensor of a's type and device")
     epi = GEMM_EPILOGUES.get(epilogue)
@@ -101,27 +106,25 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
         raise ValueError(f"epilogue {epilogue!r}: one of {sorted(GEMM_EPILOGUES)}")
     r, ldr, b = None, 0, None
     if epilogue == "residual" or epilogue == "residual_relu":
-        if residual is None or residual.dtype is not a.dtype or residual.device != dev or \
+        if residual is None or residual.dtype is not _BF16 or residual.device != dev or \
                 residual.shape[-1] != N or residual.numel() != M * N:
             raise ValueError(f"the residual epilogue needs a bf16 residual of {M} x {N}")
-        r2 = residual if _plain_rows(residual) else _rows(residual, N)
+        r2 = residual if residual.dim() == 2 and _plain_rows(residual) else _rows(residual, N)
         r, ldr = r2.data_ptr(), r2.stride(0)
     elif epilogue == "bias":
         if bias is None:
             raise ValueError("the bias epilogue needs a bias")
-        _operand(bias, (N,), a.dtype, dev, "bias")
+        _operand(bias, (N,), _BF16, dev, "bias")
         b = bias.data_ptr()
-    with _on(dev):
-        size = lib().pk_adapter_workspace(M, K, rank)
-        if size < 0:
-            raise ValueError(f"rank {rank}: a multiple of 8 up to 128")
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        check(lib().pk_adapter_gemm(
-            a2.data_ptr(), a2.stride(0), weight.data_ptr(), weight.stride(0), M, N, K,
-            out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(), up.data_ptr(), rank, n,
-            _ptr(scale), plan.ids.data_ptr(), plan.block.data_ptr(), ws.data_ptr(),
-            _error_word(dev).data_ptr(), _stream(dev)), "pk_adapter_gemm")
-    return out if a.dim() == 2 and out.dim() == 2 else out.reshape(*a.shape[:-1], N)
+    if rank == 0 or rank > PK_ADAPTER_MAX_RANK:
+        raise ValueError(f"rank {rank}: a multiple of 8 up to {PK_ADAPTER_MAX_RANK}")
+    # (rows padded to 128 of K and of rank; a buffer of this call's own)
+    ws = torch.empty((M + 127) // 128 * 256 * (K + rank), dtype=torch.uint8, device=dev)
+    _launch(dev, lib().pk_adapter_gemm, a2.data_ptr(), a2.stride(0), weight.data_ptr(),
+            weight.stride(0), M, N, K, out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(),
+            up.data_ptr(), rank, n, sc, plan.ids.data_ptr(), plan.block.data_ptr(), ws.data_ptr(),
+            _error_word(dev).data_ptr(), _stream(dev))
+    return out if flat and out.dim() == 2 else out.reshape(*a.shape[:-1], N)
 
 
 __all__ = ["AdapterPlan", "adapter_gemm", "adapter_plan"]

@@ -29,6 +29,21 @@ def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
+_current_device = torch._C._cuda_getDevice
+
+
+def _launch(device, fn, *args) -> None:
+    """One library call on ``device``: launches and per-device attributes go by the
+    current device, which is switched for the call where it is another."""
+    if device.index == _current_device():
+        status = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args)
+    if status:
+        check(status, fn.__name__)
+
+
 def layer_norm(x: torch.Tensor, ln, ln2=None):
     """nn.LayerNorm ``ln`` over the last dim of ``x`` (one libpk launch); with
     ``ln2`` also ``ln2(ln(x))`` from the same launch, returned as a pair.

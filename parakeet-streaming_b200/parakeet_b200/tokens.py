@@ -20,25 +20,13 @@ same request are not begun at once.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
 
 from . import _lib
-from ._lib import check, lib
-from .ops import DTYPES, _ptr, _stream
-
-
-def _on(device):
-    """The device's context where another one is current: launches and library
-    attributes go by the current device."""
-    if device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
-
-
-_HERE = contextlib.nullcontext()
+from ._lib import lib
+from .ops import DTYPES, _launch, _ptr, _stream
 
 
 class TokenStep:
@@ -53,16 +41,15 @@ class TokenStep:
     masks       int64 [rows]   bits of a node's ancestors and itself (trees; else None)
     """
 
-    __slots__ = ("pool", "block", "batch", "rows", "trees", "open", "_at")
+    __slots__ = ("pool", "block", "batch", "rows", "trees", "open", "_at", "_workspace")
 
-    def __init__(self, pool, block, batch, rows, trees, at):
+    def __init__(self, pool, block, batch, rows, trees, at, workspace):
         self.pool, self.block, self.batch, self.rows, self.trees = pool, block, batch, rows, trees
         self.open = True     # until end_step
-        self._at = at
+        self._at, self._workspace = at, workspace
 
     def _view(self, which, n):
-        a = self._at[which]
-        return self.block[a:a + n]
+        return self.block.as_strided((n,), (1,), self._at[which])
 
     @property
     def row_start(self):
@@ -139,10 +126,11 @@ class TokenKVPool:
             num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim,
             page_size=page_size, table_width=self.table_width, dtype=DTYPES[dtype])
         h = ctypes.c_void_p()
-        with _on(dev):
-            check(lib().pk_token_kv_create(ctypes.byref(d), ctypes.byref(h)), "pk_token_kv_create")
+        self._lib = lib()
+        _launch(dev, self._lib.pk_token_kv_create, ctypes.byref(d), ctypes.byref(h))
         self._h = h
-        self._sizes: dict = {}   # (batch, rows, trees): the step block's words and offsets
+        # (batch, rows, trees): a step block's words and offsets, attention's workspace
+        self._sizes: dict = {}
         self.reset(page_order)
 
     def __del__(self):
@@ -199,8 +187,7 @@ class TokenKVPool:
             if order.numel() != self.num_pages:
                 raise ValueError("page_order must list every page once")
         self._order = order
-        with _on(self.device):
-            check(lib().pk_token_reset(self._h, _ptr(order), _stream(self.device)), "pk_token_reset")
+        _launch(self.device, self._lib.pk_token_reset, self._h, _ptr(order), _stream(self.device))
 
     def begin_step(self, slots: torch.Tensor, counts: torch.Tensor, rows: int,
                    parents: torch.Tensor | None = None) -> TokenStep:
@@ -223,18 +210,18 @@ class TokenKVPool:
         size = self._sizes.get(key)
         if size is None:
             at = (ctypes.c_int64 * _lib.PK_TOK_OFFSETS)()
-            words = lib().pk_token_step_words(self._h, B, rows, trees, at)
+            words = self._lib.pk_token_step_words(self._h, B, rows, trees, at)
             if words < 0:
                 raise ValueError(f"rows must not be negative, got {rows}")
             if len(self._sizes) >= 64:
                 self._sizes.clear()
-            size = self._sizes[key] = (words, tuple(at))
-        block = torch.empty(size[0], dtype=torch.int32, device=self.device)
-        with _on(self.device):
-            check(lib().pk_token_begin_step(self._h, slots.data_ptr(), counts.data_ptr(), B,
-                                            _ptr(parents), rows, block.data_ptr(),
-                                            _stream(self.device)), "pk_token_begin_step")
-        step = TokenStep(self, block, B, rows, trees, size[1])
+            size = self._sizes[key] = (words, tuple(at),
+                                       self._lib.pk_token_attention_workspace(self._h, B, rows))
+        dev = self.device
+        block = torch.empty(size[0], dtype=torch.int32, device=dev)
+        _launch(dev, self._lib.pk_token_begin_step, self._h, slots.data_ptr(), counts.data_ptr(), B,
+                parents.data_ptr() if trees else None, rows, block.data_ptr(), _stream(dev))
+        step = TokenStep(self, block, B, rows, trees, size[1], size[2])
         if B == 0:   # nothing was launched: no rows, no units
             block.zero_()
             step.row_request.fill_(-1)
@@ -248,19 +235,16 @@ class TokenKVPool:
         the request."""
         self._i32(last, step.batch, "last")
         self._step(step, ending=True)
-        with _on(self.device):
-            check(lib().pk_token_end_step(self._h, last.data_ptr(), step.batch, step.rows,
-                                          step.trees, step.block.data_ptr(),
-                                          _stream(self.device)), "pk_token_end_step")
+        _launch(self.device, self._lib.pk_token_end_step, self._h, last.data_ptr(), step.batch,
+                step.rows, step.trees, step.block.data_ptr(), _stream(self.device))
 
     def truncate(self, slots: torch.Tensor, lengths: torch.Tensor):
         """Cut requests to ``lengths[b]`` tokens (0 releases them); the pages
         past the end go back on the stack."""
         n = self._i32(slots, None, "slots")
         self._i32(lengths, n, "lengths")
-        with _on(self.device):
-            check(lib().pk_token_truncate(self._h, slots.data_ptr(), lengths.data_ptr(), n,
-                                          _stream(self.device)), "pk_token_truncate")
+        _launch(self.device, self._lib.pk_token_truncate, self._h, slots.data_ptr(),
+                lengths.data_ptr(), n, _stream(self.device))
 
     def read_error(self) -> int:
         return int(self.error.item())
@@ -277,11 +261,9 @@ class TokenKVPool:
         if len(strides) > 4 or value.shape != key.shape or value.stride() != strides:
             raise ValueError("key and value must have the same shape and strides")
         nl, ls = (key.shape[0], strides[0]) if len(strides) == 4 else (1, 0)
-        with _on(self.device):
-            check(lib().pk_token_append(self._h, layer, nl, key.data_ptr(), value.data_ptr(), ls,
-                                        strides[-3], strides[-2], step.batch, step.rows, step.trees,
-                                        step.block.data_ptr(), _stream(self.device)),
-                  "pk_token_append")
+        _launch(self.device, self._lib.pk_token_append, self._h, layer, nl, key.data_ptr(),
+                value.data_ptr(), ls, strides[-3], strides[-2], step.batch, step.rows, step.trees,
+                step.block.data_ptr(), _stream(self.device))
 
     def attention(self, layer: int, query: torch.Tensor, step: TokenStep,
                   scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -302,15 +284,12 @@ class TokenKVPool:
         else:
             ors, ohs, _ = self._rows(out, self.num_heads, step.rows, "out").stride()
         qrs, qhs, _ = q.stride()
-        B, rows = step.batch, step.rows
-        with _on(self.device):
-            need = lib().pk_token_attention_workspace(self._h, B, rows)
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need > 0 else None
-            check(lib().pk_token_attention(
-                self._h, layer, q.data_ptr(), qrs, qhs,
-                self.head_dim ** -0.5 if scale is None else scale, B, rows, step.trees,
-                step.block.data_ptr(), out.data_ptr(), ors, ohs, _ptr(ws),
-                _stream(self.device)), "pk_token_attention")
+        dev, need, ws = self.device, step._workspace, None
+        if need:   # a buffer of this call's own: the steps' layers may run side by side
+            ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr()
+        _launch(dev, self._lib.pk_token_attention, self._h, layer, q.data_ptr(), qrs, qhs,
+                self.head_dim ** -0.5 if scale is None else scale, step.batch, step.rows, step.trees,
+                step.block.data_ptr(), out.data_ptr(), ors, ohs, ws, _stream(dev))
         return out
 
 
