@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(TreeShape<DH>::kWarps * 32, TreeShape<DH>::kCt
 // their outputs (DH / 32 columns a lane).
 constexpr int kRowsF32 = 16;
 template <int DH>
-__global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) {
+__global__ void __launch_bounds__(128, 3) tree_attn_f32_kernel(const TreeParams p) {
     constexpr int kKp = DH + 4, NV = DH / 32;
     extern __shared__ uint8_t tree_smem[];
     float *sk = reinterpret_cast<float *>(tree_smem);   // [kTile][kKp]
@@ -470,11 +470,13 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
             reinterpret_cast<float4 *>(sq)[c] = x;
         }
         float o[4][NV] = {}, m[4], l[4];
+        // the warp's rows are warp, warp + 4, ..: as many as are live
+        const int rows = (min(m_rows - w.rt * kRowsF32, kRowsF32) + 3 - warp) >> 2;
         uint64_t mask[4];
         int node[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = w.rt * kRowsF32 + warp * 4 + i;
+            const int r = w.rt * kRowsF32 + i * 4 + warp;
             m[i] = -INFINITY;
             l[i] = 0.f;
             node[i] = r < m_rows ? r / p.group : -1;
@@ -485,24 +487,41 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
         for (int t = w.t0; t < w.t1; ++t) {
             const int k0 = t * kTile;
             __syncthreads();   // the previous tile is done with
-            for (int c = threadIdx.x; c < kTile * DH / 4; c += 128) {
-                const int row = c / (DH / 4), e = c % (DH / 4), key = k0 + row;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-                if (key < len) {
-                    int page = p.table[(int64_t)w.slot * p.table_width + (key >> p.ps_shift)];
-                    if (page < 0 || page >= p.num_pages) {
-                        raise(p.error, PK_DEV_BAD_PAGE);
-                        page = 0;
-                    }
-                    const int64_t ps = 1 << p.ps_shift, off = key & (ps - 1);
-                    const int64_t plane =
-                        (((int64_t)page * p.num_layers + p.layer) * 2) * p.kv_heads + head;
-                    const float *src = kv + (plane * ps + off) * DH + e * 4;
-                    a = *reinterpret_cast<const float4 *>(src);
-                    b = *reinterpret_cast<const float4 *>(src + p.kv_heads * ps * DH);
+            // eight chunks at a time, so that their table entries and then their rows are
+            // requested together
+            for (int c0 = threadIdx.x; c0 < kTile * DH / 4; c0 += 8 * 128) {
+                int page[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = k0 + (c0 + i * 128) / (DH / 4);
+                    page[i] = 0;
+                    if (key < len)
+                        page[i] = p.table[(int64_t)w.slot * p.table_width + (key >> p.ps_shift)];
                 }
-                *reinterpret_cast<float4 *>(sk + row * kKp + e * 4) = a;
-                reinterpret_cast<float4 *>(sv)[c] = b;
+                float4 a[8], b[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int c = c0 + i * 128, e = c % (DH / 4), key = k0 + c / (DH / 4);
+                    a[i] = b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (page[i] < 0 || page[i] >= p.num_pages) {
+                        raise(p.error, PK_DEV_BAD_PAGE);
+                        page[i] = 0;
+                    }
+                    if (key < len) {
+                        const int64_t ps = 1 << p.ps_shift, off = key & (ps - 1);
+                        const int64_t plane =
+                            (((int64_t)page[i] * p.num_layers + p.layer) * 2) * p.kv_heads + head;
+                        const float *src = kv + (plane * ps + off) * DH + e * 4;
+                        a[i] = *reinterpret_cast<const float4 *>(src);
+                        b[i] = *reinterpret_cast<const float4 *>(src + p.kv_heads * ps * DH);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int c = c0 + i * 128, row = c / (DH / 4), e = c % (DH / 4);
+                    *reinterpret_cast<float4 *>(sk + row * kKp + e * 4) = a[i];
+                    reinterpret_cast<float4 *>(sv)[c] = b[i];
+                }
             }
             __syncthreads();
             float s[4][2] = {};
@@ -512,8 +531,9 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
                 const float4 b = *reinterpret_cast<const float4 *>(sk + (lane + 32) * kKp + e * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    if (i >= rows) break;
                     const float4 x =
-                        *reinterpret_cast<const float4 *>(sq + (warp * 4 + i) * DH + e * 4);
+                        *reinterpret_cast<const float4 *>(sq + (i * 4 + warp) * DH + e * 4);
                     s[i][0] += x.x * a.x + x.y * a.y + x.z * a.z + x.w * a.w;
                     s[i][1] += x.x * b.x + x.y * b.y + x.z * b.z + x.w * b.w;
                 }
@@ -521,6 +541,7 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
             const bool own = k0 + kTile > w.ctx;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                if (i >= rows) break;
                 float top = m[i];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -541,34 +562,40 @@ __global__ void __launch_bounds__(128) tree_attn_f32_kernel(const TreeParams p) 
                 l[i] = l[i] * keep + a + b;
 #pragma unroll
                 for (int n = 0; n < NV; ++n) o[i][n] *= keep;
-                sp[(warp * 4 + i) * kTile + lane] = a;
-                sp[(warp * 4 + i) * kTile + lane + 32] = b;
+                sp[(i * 4 + warp) * kTile + lane] = a;
+                sp[(i * 4 + warp) * kTile + lane + 32] = b;
             }
             __syncwarp();
-            const int end = min(kTile, len - k0);
-#pragma unroll 1
-            for (int j = 0; j < end; ++j) {
-                float v[NV];
+            // (rows past the end were staged as zeros, their weights are zero)
+#pragma unroll 2
+            for (int j = 0; j < kTile; j += 4) {
+                float v[4][NV];
+                float4 x[4];   // the four rows' weights of the four keys
 #pragma unroll
-                for (int n = 0; n < NV; ++n) v[n] = sv[j * DH + n * 32 + lane];
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int n = 0; n < NV; ++n) v[k][n] = sv[(j + k) * DH + n * 32 + lane];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = sp[(warp * 4 + i) * kTile + j];
-                    if (x != 0.f) {   // a key that the row does not see has no part, even inf
+                    if (i >= rows) break;
+                    x[i] = *reinterpret_cast<const float4 *>(sp + (i * 4 + warp) * kTile + j);
+                    const float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-                        for (int n = 0; n < NV; ++n) o[i][n] += x * v[n];
-                    }
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int n = 0; n < NV; ++n)   // a key that the row does not see has no
+                            o[i][n] += y[k] != 0.f ? y[k] * v[k][n] : 0.f;   // part, even inf
                 }
             }
             __syncwarp();
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int rt = warp * 4 + i, r = w.rt * kRowsF32 + rt;
+            const int rt = i * 4 + warp, r = w.rt * kRowsF32 + rt;
+            if (i >= rows) break;
             float sum = l[i];
 #pragma unroll
             for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            if (r >= m_rows) continue;
             if (w.part >= 0) {
                 const int64_t part = (int64_t)w.part * kRowsF32 + rt;
 #pragma unroll

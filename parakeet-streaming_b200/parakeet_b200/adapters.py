@@ -47,7 +47,7 @@ def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
     words = lib().pk_adapter_plan_words(rows, num_adapters)
     if words < 0:
         raise ValueError(f"{rows} rows or {num_adapters} adapters: out of range")
-    block = torch.empty(words, dtype=torch.int32, device=dev)
+    block = ids.new_empty(words)
     _launch(dev, lib().pk_adapter_plan, ids.data_ptr(), rows, num_adapters, block.data_ptr(),
             _error_word(dev).data_ptr(), _stream(dev))
     return AdapterPlan(ids, rows, num_adapters, block)
@@ -97,7 +97,7 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     if plan.rows != M or plan.ids.device != dev:
         raise ValueError(f"the plan is for {plan.rows} rows on {plan.ids.device}, a has {M} on {dev}")
     if out is None:
-        out = torch.empty((M, N), dtype=_BF16, device=dev)
+        out = a.new_empty((M, N))
     elif not out.is_contiguous() or out.numel() != M * N or out.dtype is not _BF16 or \
             out.device != dev:
         raise ValueError("out must be a contiguous [M, N] tensor of a's type and device")
@@ -119,7 +119,7 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     if rank == 0 or rank > PK_ADAPTER_MAX_RANK:
         raise ValueError(f"rank {rank}: a multiple of 8 up to {PK_ADAPTER_MAX_RANK}")
     # (rows padded to 128 of K and of rank; a buffer of this call's own)
-    ws = torch.empty((M + 127) // 128 * 256 * (K + rank), dtype=torch.uint8, device=dev)
+    ws = a.new_empty((M + 127) // 128 * 128 * (K + rank))
     _launch(dev, lib().pk_adapter_gemm, a2.data_ptr(), a2.stride(0), weight.data_ptr(),
             weight.stride(0), M, N, K, out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(),
             up.data_ptr(), rank, n, sc, plan.ids.data_ptr(), plan.block.data_ptr(), ws.data_ptr(),

@@ -218,7 +218,7 @@ class TokenKVPool:
             size = self._sizes[key] = (words, tuple(at),
                                        self._lib.pk_token_attention_workspace(self._h, B, rows))
         dev = self.device
-        block = torch.empty(size[0], dtype=torch.int32, device=dev)
+        block = slots.new_empty(size[0])
         _launch(dev, self._lib.pk_token_begin_step, self._h, slots.data_ptr(), counts.data_ptr(), B,
                 parents.data_ptr() if trees else None, rows, block.data_ptr(), _stream(dev))
         step = TokenStep(self, block, B, rows, trees, size[1], size[2])
@@ -277,7 +277,7 @@ class TokenKVPool:
         if q.dim() != 3:
             raise ValueError(f"query: one layer's rows, got {tuple(query.shape)}")
         if out is None:
-            out = torch.empty(query.shape, dtype=self.dtype, device=self.device)
+            out = query.new_empty(query.shape)
             ors, ohs = self.num_heads * self.head_dim, self.head_dim
         elif out.shape != query.shape:
             raise ValueError(f"out: expected {tuple(query.shape)}, got {tuple(out.shape)}")
@@ -286,7 +286,7 @@ class TokenKVPool:
         qrs, qhs, _ = q.stride()
         dev, need, ws = self.device, step._workspace, None
         if need:   # a buffer of this call's own: the steps' layers may run side by side
-            ws = torch.empty(need, dtype=torch.uint8, device=dev).data_ptr()
+            ws = step.block.new_empty(need // 4).data_ptr()
         _launch(dev, self._lib.pk_token_attention, self._h, layer, q.data_ptr(), qrs, qhs,
                 self.head_dim ** -0.5 if scale is None else scale, step.batch, step.rows, step.trees,
                 step.block.data_ptr(), out.data_ptr(), ors, ohs, ws, _stream(dev))
