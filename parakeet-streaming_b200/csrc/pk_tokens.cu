@@ -393,6 +393,10 @@ __global__ void __launch_bounds__(256)
         const int c = (int)(i - r * per_row), h = c / per_head, e = c - h * per_head;
         const int map = a.step[slot_map + r];
         if (map < 0) continue;
+        if (map >> ps_shift >= d.num_pages) {   // a table that names no page of the pool
+            raise(d.error, PK_DEV_BAD_PAGE);
+            continue;
+        }
         const int64_t src = (layer * a.ls + r * a.rs + h * a.hs) * esize + e * 16;
         const uint4 k = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.key) + src);
         const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.value) + src);
@@ -437,8 +441,14 @@ __global__ void __launch_bounds__(256)
     if (threadIdx.x < PK_TOK_MAX_TREE && (path >> threadIdx.x & 1) &&
         (int)threadIdx.x >= in_place) {
         const int rank = __popcll(path & ((1ull << threadIdx.x) - 1ull));
-        s_src[rank - in_place] = step[l.slot_map + r0 + threadIdx.x];
-        s_dst[rank - in_place] = step[l.slot_map + r0 + rank];
+        int src = step[l.slot_map + r0 + threadIdx.x], dst = step[l.slot_map + r0 + rank];
+        if ((unsigned)src >> ps_shift >= (unsigned)d.num_pages ||
+            (unsigned)dst >> ps_shift >= (unsigned)d.num_pages) {
+            raise(d.error, PK_DEV_BAD_PAGE);
+            src = dst = 0;
+        }
+        s_src[rank - in_place] = src;
+        s_dst[rank - in_place] = dst;
     }
     if (threadIdx.x == 0) s_n = kept - in_place;
     __syncthreads();

@@ -182,5 +182,16 @@ struct Pages {
     }
 };
 
+// The V row of a unit's key in its page (bf16).
+template <int DH>
+__device__ __forceinline__ const __nv_bfloat16 *value_row(const TreeParams &p, const Unit &w,
+                                                          int key) {
+    int64_t page = p.table[(int64_t)w.slot * p.table_width + (key >> p.ps_shift)];
+    if (page < 0 || page >= p.num_pages) page = 0;   // (the loads have reported it)
+    const int64_t plane = ((page * p.num_layers + p.layer) * 2 + 1) * p.kv_heads + w.head;
+    const int64_t row = (plane << p.ps_shift) + (key & ((1 << p.ps_shift) - 1));
+    return static_cast<const __nv_bfloat16 *>(p.kv) + row * DH;
+}
+
 }  // namespace
 }  // namespace pk

@@ -76,28 +76,40 @@ __device__ __forceinline__ uint64_t seen_keys(int trees, uint64_t mask, int node
     return rel0 >= 0 ? mask >> rel0 : (mask << -rel0) | ((1ull << -rel0) - 1ull);
 }
 
-// V rows past the end hold what the page held before: zero for the product (0 x inf
-// would reach every row).  Returns whether a token of the step's own has a value that
-// is not finite, which must not reach the rows that do not see it.  By one warp; the
-// warps of a tile write the same zeros.
+// V rows past the end hold what the page held before, and a token's values may be inf or
+// NaN: zero in the product, where a weight of zero would not keep them from the rows
+// that do not see them.  Returns whether there were any of the latter.  By one warp.
 template <int DH>
 __device__ __forceinline__ bool clean_values(uint8_t *vs, int k0, int ctx, int len) {
     bool odd = false;
     for (int c = max(ctx - k0, 0) * (DH / 8) + (threadIdx.x & 31); c < kTile * DH / 8; c += 32) {
         const int row = c / (DH / 8), ch = c % (DH / 8);
         uint4 *at = reinterpret_cast<uint4 *>(vs + tile_at<DH>(row, ch));
-        if (k0 + row >= len) {
-            *at = make_uint4(0u, 0u, 0u, 0u);
-        } else {
-            const uint4 x = *at;
-            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (k0 + row < len) {
+            x = *at;
+            uint32_t *e = &x.x;
+            bool here = false;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                odd |= (e[k] & 0x7f80u) == 0x7f80u || (e[k] & 0x7f800000u) == 0x7f800000u;
+            for (int k = 0; k < 4; ++k) {
+                if ((e[k] & 0x7f80u) == 0x7f80u) {
+                    e[k] &= 0xffff0000u;
+                    here = true;
+                }
+                if ((e[k] & 0x7f800000u) == 0x7f800000u) {
+                    e[k] &= 0x0000ffffu;
+                    here = true;
+                }
+            }
+            if (!here) continue;
+            odd = true;
         }
+        *at = x;
     }
     fence_async_proxy();   // the slot's next TMA load comes after these writes
-    return __any_sync(0xffffffffu, odd);
+    const bool any = __any_sync(0xffffffffu, odd);   // (and the warp's writes before its reads)
+    __syncwarp();
+    return any;
 }
 
 template <int kWarps> struct TreeShared {
@@ -279,49 +291,38 @@ __device__ __forceinline__ void attend(const CUtensorMap &kv_map, const TreePara
             }
             ring_wait(&full[1], phase, failed, p.error);
             __syncwarp();
-            // a value that is not finite among the step's own rows
+            // values that are not finite among the step's own rows
             const bool odd = own && clean_values<DH>(vs, k0, w.ctx, len);
-            if (!odd) {
 #pragma unroll
-                for (int kk = 0; kk < kN / 2; ++kk) {
-                    const uint32_t a[4] = {
-                        pack2(s[2 * kk][0], s[2 * kk][1]), pack2(s[2 * kk][2], s[2 * kk][3]),
-                        pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]),
-                        pack2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+            for (int kk = 0; kk < kN / 2; ++kk) {
+                const uint32_t a[4] = {
+                    pack2(s[2 * kk][0], s[2 * kk][1]), pack2(s[2 * kk][2], s[2 * kk][3]),
+                    pack2(s[2 * kk + 1][0], s[2 * kk + 1][1]),
+                    pack2(s[2 * kk + 1][2], s[2 * kk + 1][3])};
 #pragma unroll
-                    for (int nb = 0; nb < DH / 16; ++nb) {
-                        uint32_t b[4];
-                        ldsm4_t(vb + tile_at<DH>(kk * 16 + (lane & 15), nb * 2 + (lane >> 4)), b);
-                        mma16816(o[2 * nb], a, b[0], b[1]);
-                        mma16816(o[2 * nb + 1], a, b[2], b[3]);
-                    }
+                for (int nb = 0; nb < DH / 16; ++nb) {
+                    uint32_t b[4];
+                    ldsm4_t(vb + tile_at<DH>(kk * 16 + (lane & 15), nb * 2 + (lane >> 4)), b);
+                    mma16816(o[2 * nb], a, b[0], b[1]);
+                    mma16816(o[2 * nb + 1], a, b[2], b[3]);
                 }
-            } else {
-                // the same product a key at a time, keys of weight zero left out
-#pragma unroll
-                for (int n = 0; n < kN; ++n) {
+            }
+            if (odd) {
+                // the values kept out of the product, to the rows that see their keys:
+                // they make the sum inf or NaN, whatever their weight
 #pragma unroll 1
-                    for (int x = 0; x < 8; ++x) {
-                        const int from = (lane & ~3) | (x >> 1);
-                        const float w0a = __shfl_sync(0xffffffffu, s[n][0], from);
-                        const float w0b = __shfl_sync(0xffffffffu, s[n][1], from);
-                        const float w1a = __shfl_sync(0xffffffffu, s[n][2], from);
-                        const float w1b = __shfl_sync(0xffffffffu, s[n][3], from);
-                        const float w0 = x & 1 ? w0b : w0a, w1 = x & 1 ? w1b : w1a;
+                for (int key = max(w.ctx, k0); key < min(len, k0 + kTile); ++key) {
+                    const __nv_bfloat16 *v = value_row<DH>(p, w, key) + (lane & 3) * 2;
 #pragma unroll
-                        for (int d = 0; d < DH / 8; ++d) {
-                            const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(
-                                vs + tile_at<DH>(n * 8 + x, d) + (lane & 3) * 4);
-                            const float2 f = __bfloat1622float2(v);
-                            if (w0 != 0.f) {
-                                o[d][0] += w0 * f.x;
-                                o[d][1] += w0 * f.y;
+                    for (int h = 0; h < 2; ++h) {
+                        if (!(seen_keys(p.trees, mask[h], node[h], key - w.ctx) & 1)) continue;
+#pragma unroll
+                        for (int n = 0; n < DH / 8; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float x = __bfloat162float(v[n * 8 + e]);
+                                if (!isfinite(x)) o[n][2 * h + e] += x;
                             }
-                            if (w1 != 0.f) {
-                                o[d][2] += w1 * f.x;
-                                o[d][3] += w1 * f.y;
-                            }
-                        }
                     }
                 }
             }

@@ -432,13 +432,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int key = max(w.ctx, w.t0 * kKeys); key < min(len, w.t1 * kKeys); ++key) {
                         const int rel = key - w.ctx;
                         if (!(seen_bits(p.trees, mask, node, rel) & 1)) continue;
-                        const int64_t page =
-                            p.table[(int64_t)w.slot * p.table_width + (key >> p.ps_shift)];
-                        const int64_t ps = 1 << p.ps_shift;
-                        const __nv_bfloat16 *v =
-                            static_cast<const __nv_bfloat16 *>(p.kv) +
-                            ((((page * p.num_layers + p.layer) * 2 + 1) * p.kv_heads + w.head) * ps +
-                             (key & (ps - 1))) * DH + c * 32;
+                        const __nv_bfloat16 *v = value_row<DH>(p, w, key) + c * 32;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             const float y = __bfloat162float(v[e]);

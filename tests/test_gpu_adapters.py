@@ -203,3 +203,59 @@ def test_refusals():
         adapter_plan(d["ids"].long(), 3)
     with pytest.raises(ValueError):
         adapter_plan(d["ids"], 0)
+
+
+@pytest.mark.parametrize("kind", ["random", "sorted", "one"])
+def test_more_rows_than_the_plan_holds_in_registers(kind):
+    """9,000 rows: the plan's loop past 8 rows a thread, with and without resorting."""
+    d = make(9000, 128, 64, 8, 40, 17)
+    if kind == "sorted":
+        d["ids"] = torch.where(d["ids"] < 0, 40, d["ids"]).sort().values.int()
+        d["ids"][d["ids"] == 40] = -1
+    elif kind == "one":
+        d["ids"][:] = 3
+    check(run(d), reference(d, "store"))
+
+
+def test_two_streams_at_once():
+    """The same plan under two products on two streams, eager and captured."""
+    d = [make(300, 256, 512, 16, 5, s) for s in (1, 2)]
+    d[1]["ids"] = d[0]["ids"]
+    plan = adapter_plan(d[0]["ids"], 5)
+    want = [run(x, plan=plan).clone() for x in d]
+    streams = [torch.cuda.Stream() for _ in d]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x, s in zip(d, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+            outs.append(run(x, plan=plan))
+        graphs.append(g)
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    got = []
+    for x, s in zip(d, streams):
+        with torch.cuda.stream(s):
+            got.append(run(x, plan=plan))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_empty_rows():
+    d = make(4, 64, 64, 8, 3, 1)
+    plan = adapter_plan(d["ids"][:0], 3)
+    out = adapter_gemm(d["x"][:0], d["w"], d["down"], d["up"], plan)
+    assert out.shape == (0, 64)
+
+
+def test_same_bits_every_time():
+    for M, N, K in ((8, 512, 512), (700, 512, 512), (2400, 2048, 2048)):
+        d = make(M, N, K, 16, 9, M)
+        plan = adapter_plan(d["ids"], 9)
+        first = run(d, plan=plan)
+        for _ in range(3):
+            assert torch.equal(run(d, plan=adapter_plan(d["ids"], 9)), first)

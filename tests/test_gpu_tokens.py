@@ -216,3 +216,372 @@ def test_attention(case, dtype):
     used = sum(new)
     bound(got[:used], want[:used], mean_abs[:used], reach[:used], dtype, max_tokens, dh)
     assert (got[used:] == 7.0).all()                        # rows behind the last request
+
+
+def filled(rng, page, H, Hkv, dh, ctx, new, dtype, tree=True, num_pages=None, order=None, layers=1):
+    """A pool whose requests have ``ctx`` tokens of random K and V, and a step of
+    ``new`` more, all in place; the model and the step's arrays beside them."""
+    B = len(ctx)
+    most = max(c + n for c, n in zip(ctx, new))
+    pages = num_pages or sum(-(-(c + n) // page) for c, n in zip(ctx, new)) + 1
+    pool = TokenKVPool(layers, H, Hkv, dh, B, most, num_pages=pages, page_size=page, dtype=dtype,
+                       device=DEV, page_order=order)
+    model = TokenPoolModel(B, most, pages, page, order)
+    slots = np.arange(B, dtype=np.int32)
+    grow(pool, model, slots, np.asarray(ctx))
+    rows = int(sum(new))
+    parents = random_tree(rng, new, rows) if tree else None
+    step = pool.begin_step(i32(slots), i32(new), rows, i32(parents) if tree else None)
+    ref = model.begin_step(slots, new, rows, parents)
+    if num_pages is None:
+        pool.kv.copy_(torch.randn(pool.kv.shape, device=DEV).to(dtype))
+    q = torch.randn(rows, H, dh, device=DEV).to(dtype)
+    return pool, model, step, ref, parents, q
+
+
+def reference(pool, model, ref, parents, q, layer=0, scale=None):
+    dh = q.shape[-1]
+    return tree_attention(q.double().cpu().numpy(), pool.kv.double().cpu().numpy(), layer, model, ref,
+                          parents, scale or dh ** -0.5)
+
+
+# one shape for each kernel: fp32, 16-row tiles (a team of warps, workers with cut row
+# tiles), 128-row tiles
+KERNELS = [(torch.float32, 8, 2, 64, [90, 700, 3], [6, 9, 12]),
+           (torch.bfloat16, 4, 4, 64, [90, 130, 3], [6, 9, 12]),
+           (torch.bfloat16, 2, 2, 128, [3000, 700, 3], [6, 9, 12]),
+           (torch.bfloat16, 8, 2, 128, [90, 700, 3], [40, 9, 12]),
+           (torch.bfloat16, 8, 1, 64, [2000, 61, 0], [20, 64, 5])]
+
+
+@pytest.mark.parametrize("kernel", range(len(KERNELS)))
+@pytest.mark.parametrize("what", ["nan key", "inf value", "nan value", "inf key"])
+def test_a_tokens_bad_values_stay_with_the_rows_that_see_it(kernel, what):
+    """An inf or NaN in a drafted token's K or V reaches the rows that descend from
+    it; every other row is bit for bit what it is without it."""
+    dtype, H, Hkv, dh, ctx, new = KERNELS[kernel]
+    rng = np.random.default_rng(7 + kernel)
+    pool, model, step, ref, parents, q = filled(rng, 16, H, Hkv, dh, ctx, new, dtype)
+    clean = pool.attention(0, q, step).clone()
+    victims = [(0, 2), (1, 0), (2, 3)]                    # (request, node)
+    bad = float("nan") if "nan" in what else float("inf")
+    for b, j in victims:
+        at = int(ref["slot_map"][ref["row_start"][b] + j])
+        pool.kv[at // 16, 0, 0 if "key" in what else 1, :, at % 16, 5::7] = bad
+    out = pool.attention(0, q, step)
+    masks = ref["masks"].view(np.uint64)
+    seen = np.zeros(len(masks), bool)
+    for b, j in victims:
+        r0, r1 = ref["row_start"][b], ref["row_start"][b + 1]
+        seen[r0:r1] |= (masks[r0:r1] >> np.uint64(j) & np.uint64(1)).astype(bool)
+    assert seen.any() and not seen.all()
+    keep = torch.tensor(~seen, device=DEV)
+    assert torch.equal(out[keep], clean[keep])
+    if "key" not in what:      # (an inf key may also give a row a weight of zero)
+        assert not bool(out[~keep][..., 5::7].isfinite().any())
+        others = [c for c in range(dh) if c % 7 != 5]
+        assert torch.equal(out[~keep][..., others], clean[~keep][..., others])
+    elif bad != bad:
+        assert not bool(out[~keep].isfinite().any())
+    assert pool.read_error() == 0
+
+
+@pytest.mark.parametrize("kernel", range(len(KERNELS)))
+def test_large_scores_scale_strides_and_repeatability(kernel):
+    """Scores of hundreds (weights of 1 and 0), a given scale, queries out of a
+    wider buffer, a strided output, and the same bits every time."""
+    dtype, H, Hkv, dh, ctx, new = KERNELS[kernel]
+    rng = np.random.default_rng(kernel)
+    pool, model, step, ref, parents, _ = filled(rng, 8, H, Hkv, dh, ctx, new, dtype)
+    rows = step.rows
+    wide = (16 * torch.randn(rows, 3, H, dh, device=DEV)).to(dtype)
+    q = wide[:, 1]
+    buf = torch.full((rows, H, 2, dh), 3.0, dtype=dtype, device=DEV)
+    out = pool.attention(0, q, step, scale=0.25, out=buf[:, :, 1])
+    want, mean_abs, reach = reference(pool, model, ref, parents, q, scale=0.25)
+    bound(out.double().cpu().numpy(), want, mean_abs, reach, dtype, max(ctx) + 64, dh)
+    assert bool((buf[:, :, 0] == 3.0).all())
+    for _ in range(3):
+        assert torch.equal(pool.attention(0, q, step, scale=0.25), out)
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^31 elements whose requests hold its last pages."""
+    page, Hkv, dh = 16, 8, 128
+    pages = 2 ** 31 // (2 * Hkv * page * dh) + 70
+    rng = np.random.default_rng(0)
+    order = np.concatenate([np.arange(pages - 60), rng.permutation(np.arange(pages - 60, pages))])
+    for H, ctx, new in ((8, [200, 77], [5, 7]), (32, [300, 77], [30, 64])):
+        pool, model, step, ref, parents, q = filled(rng, page, H, Hkv, dh, ctx, new, torch.bfloat16,
+                                                    num_pages=pages, order=order)
+        assert pool.kv.numel() > 2 ** 31
+        tail = torch.randn(pool.kv[-60:].shape, device=DEV).to(torch.bfloat16)
+        pool.kv[-60:] = tail
+        k = torch.randn(step.rows, Hkv, dh, device=DEV).to(torch.bfloat16)
+        v = torch.randn_like(k)
+        pool.append(0, k, v, step)
+        at = step.slot_map.long()
+        assert torch.equal(pool.kv[at // page, 0, 0, :, at % page], k)
+        assert torch.equal(pool.kv[at // page, 0, 1, :, at % page], v)
+        out = pool.attention(0, q, step)
+        small = pool.kv[-60:].double().cpu().numpy()
+        shifted = TokenPoolModel(1, 1, 1, page)
+        shifted.table = np.where(model.table >= 0, model.table - (pages - 60), -1)
+        want, mean_abs, reach = tree_attention(q.double().cpu().numpy(), small, 0, shifted, ref,
+                                               parents, dh ** -0.5)
+        bound(out.double().cpu().numpy(), want, mean_abs, reach, torch.bfloat16, 400, dh)
+        last = np.array([n - 1 for n in new])
+        pool.end_step(step, i32(last))
+        kept = [int(((int(ref["masks"][ref["row_start"][b] + last[b]])) & (2 ** 64 - 1)).bit_count())
+                for b in range(2)]
+        assert pool.lengths.tolist() == [c + k for c, k in zip(ctx, kept)]
+        assert pool.read_error() == 0
+        del pool, tail, step
+
+
+@pytest.mark.parametrize("batch", [3000, 9000])
+def test_tables_of_many_requests(batch):
+    """More requests than the planning CTA has threads, and than eight times that."""
+    rng = np.random.default_rng(batch)
+    n = rng.integers(0, 6, batch).astype(np.int32)
+    pages = int((-(-n // 8)).sum()) - 5          # a few requests find none left
+    pool = TokenKVPool(1, 1, 1, 64, batch, 16, num_pages=pages, page_size=8, dtype=torch.float32,
+                       device=DEV)
+    model = TokenPoolModel(batch, 16, pages, 8)
+    slots = rng.permutation(batch).astype(np.int32)
+    rows = int(n.sum())
+    parents = random_tree(rng, n, rows)
+    step = pool.begin_step(i32(slots), i32(n), rows, i32(parents))
+    ref = model.begin_step(slots, n, rows, parents)
+    check_step(step, ref)
+    last = np.where(n > 0, n - 1, -1)
+    pool.end_step(step, i32(last))
+    model.end_step(ref, last)
+    check_tables(pool, model)
+    cut = np.where(rng.random(batch) < 0.5, 0, model.lengths[slots]).astype(np.int32)
+    pool.truncate(i32(slots), i32(cut))
+    model.truncate(slots, cut)
+    check_tables(pool, model)
+    q = torch.randn(rows, 1, 64, device=DEV)
+    step = pool.begin_step(i32(slots), i32(np.zeros(batch)), rows)   # rows of nobody
+    out = torch.full_like(q, 5.0)
+    pool.attention(0, q, step, out=out)
+    assert bool((out == 5.0).all())
+
+
+def test_empty_calls():
+    pool = TokenKVPool(2, 4, 2, 64, 3, 100, page_size=16, device=DEV)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    step = pool.begin_step(none, none, 4)
+    assert step.row_start.tolist() == [0] and step.row_request.tolist() == [-1] * 4
+    assert step.slot_map.tolist() == [-1] * 4
+    kv = torch.ones(4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    pool.append(0, kv, kv, step)
+    out = torch.full((4, 4, 64), 2.0, dtype=torch.bfloat16, device=DEV)
+    pool.attention(0, torch.ones_like(out), step, out=out)
+    pool.end_step(step, none)
+    pool.truncate(none, none)
+    assert bool((out == 2.0).all()) and not bool(pool.kv.any()) and pool.read_error() == 0
+    step = pool.begin_step(i32([1]), i32([0]), 0)
+    assert step.context.tolist() == [0]
+    pool.end_step(step, i32([-1]))
+    assert pool.lengths.tolist() == [0, 0, 0] and int(pool.free_count) == pool.num_pages
+
+
+@pytest.mark.parametrize("dtype,H,Hkv,dh", [(torch.float32, 4, 2, 64), (torch.bfloat16, 4, 4, 64),
+                                            (torch.bfloat16, 8, 2, 128)])
+def test_bad_table_entries_are_reported(dtype, H, Hkv, dh):
+    """A page id outside the pool is an error bit, and the others' rows are right."""
+    rng = np.random.default_rng(1)
+    ctx, new = [40, 70], [12, 3]
+    pool, model, step, ref, parents, q = filled(rng, 16, H, Hkv, dh, ctx, new, dtype)
+    want = pool.attention(0, q, step).clone()
+    for bad in (pool.num_pages, 2 ** 30, -5):
+        held = pool.page_table.clone()
+        pool.page_table[0, 1] = bad
+        out = pool.attention(0, q, step)
+        r0, r1 = int(ref["row_start"][1]), int(ref["row_start"][2])
+        assert torch.equal(out[r0:r1], want[r0:r1])
+        assert pool.read_error() == _lib.PK_DEV_BAD_PAGE
+        pool.error.zero_()
+        pool.page_table[0, 2] = min(bad, 2 ** 26)       # where request 0's new rows are
+        again = pool.begin_step(i32([0, 1]), i32(new), sum(new), i32(parents))
+        before = pool.kv.clone()
+        k = torch.ones(sum(new), Hkv, dh, dtype=dtype, device=DEV)
+        pool.append(0, k, k, again)
+        pool.end_step(again, i32([n - 1 for n in new]))
+        torch.cuda.synchronize()
+        assert bad < 0 or pool.read_error() == _lib.PK_DEV_BAD_PAGE
+        changed = (pool.kv != before).flatten(1).any(1).nonzero()[:, 0].tolist()
+        assert set(changed) <= {0, *model.table[1].tolist(), *model.table[0].tolist()}
+        pool.kv.copy_(before)
+        pool.page_table.copy_(held)
+        pool.lengths.copy_(i32(ctx))
+        pool.error.zero_()
+
+
+def test_a_whole_decode_captured_and_replayed():
+    """Steps of drafting, attention, acceptance and cutting, captured once and
+    replayed with other requests, counts, trees and acceptances: lengths and page
+    tables live on the device.  The second layer reads the first one's output, as
+    a model's would."""
+    rng = np.random.default_rng(3)
+    slots_n, B, rows, L, H, Hkv, dh, page = 7, 4, 40, 2, 4, 2, 64, 16
+    pages, most = 60, 400
+    order = rng.permutation(pages)
+    pool = TokenKVPool(L, H, Hkv, dh, slots_n, most, num_pages=pages, page_size=page, device=DEV,
+                       page_order=order)
+    model = TokenPoolModel(slots_n, most, pages, page, order,
+                           kv=np.zeros((pages, L, 2, Hkv, page, dh), np.float32))
+    buf = dict(slots=i32(np.arange(B)), counts=i32(np.ones(B)), parents=i32(np.full(rows, -1)),
+               last=i32(np.zeros(B)), cut=i32(np.zeros(B)),
+               x=torch.zeros(rows, H * dh, dtype=torch.bfloat16, device=DEV))
+    w = [(torch.randn(2 * Hkv * dh, H * dh, device=DEV) / 16).to(torch.bfloat16) for _ in range(L)]
+
+    def decode():
+        step = pool.begin_step(buf["slots"], buf["counts"], rows, buf["parents"])
+        x = buf["x"]
+        outs = []
+        for layer in range(L):
+            kv = x @ w[layer].t()
+            pool.append(layer, kv[:, :Hkv * dh], kv[:, Hkv * dh:], step)
+            x = pool.attention(layer, x, step, out=torch.zeros_like(x))
+            outs.append((kv, x))
+        pool.end_step(step, buf["last"])
+        return step, outs
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        decode()
+    torch.cuda.current_stream().wait_stream(side)
+    pool.reset(order)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        step, outs = decode()
+    torch.cuda.synchronize()
+    pool.reset(order)
+    pool.kv.zero_()
+    for it in range(12):
+        slots = rng.permutation(slots_n)[:B].astype(np.int32)
+        n = rng.integers(0, 11, B).astype(np.int32)
+        parents = random_tree(rng, n, rows)
+        last = np.array([rng.integers(-1, k) for k in n], np.int32)
+        for key, v in (("slots", slots), ("counts", n), ("parents", parents), ("last", last)):
+            buf[key].copy_(i32(v))
+        buf["x"].copy_(torch.randn(rows, H * dh, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = model.begin_step(slots, n, rows, parents)
+        check_step(step, ref)
+        used = int(n.sum())
+        x = buf["x"]
+        for layer, (kv, got) in enumerate(outs):
+            rows_np = kv.float().cpu().numpy().reshape(rows, 2, Hkv, dh)
+            model.append(layer, rows_np[:, 0], rows_np[:, 1], ref)
+            want, mean_abs, reach = tree_attention(x.double().cpu().numpy().reshape(rows, H, dh),
+                                                   model.kv, layer, model, ref, parents, dh ** -0.5)
+            bound(got.double().cpu().numpy().reshape(rows, H, dh)[:used], want[:used], mean_abs[:used],
+                  reach[:used], torch.bfloat16, most, dh)
+            assert not bool(got[used:].any())
+            x = got
+        model.end_step(ref, last)
+        check_tables(pool, model)
+        assert np.array_equal(pool.kv.float().cpu().numpy(), model.kv)
+        if it % 4 == 3:
+            who = rng.permutation(slots_n)[:3].astype(np.int32)
+            keep = (model.lengths[who] // 2).astype(np.int32)
+            pool.truncate(i32(who), i32(keep))
+            model.truncate(who, keep)
+            check_tables(pool, model)
+
+
+def test_layers_on_two_streams_at_once():
+    """The attention of two layers of one step, in two captured graphs replayed
+    side by side and on two streams: each call has a workspace of its own."""
+    rng = np.random.default_rng(5)
+    for dtype, H, Hkv, dh, ctx, new in KERNELS[2:]:
+        pool, model, step, ref, parents, q = filled(rng, 16, H, Hkv, dh, ctx, new, dtype, layers=2)
+        want = [pool.attention(layer, q, step).clone() for layer in (0, 1)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        graphs, outs = [], []
+        torch.cuda.synchronize()
+        for layer, s in enumerate(streams):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+                outs.append(pool.attention(layer, q, step))
+            graphs.append(g)
+        for _ in range(20):
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        got = []
+        for layer, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(pool.attention(layer, q, step))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_python_refusals():
+    pool = TokenKVPool(2, 4, 2, 64, 3, 100, page_size=16, device=DEV)
+    other = TokenKVPool(2, 4, 2, 64, 3, 100, page_size=16, device=DEV)
+    s, n = i32([0, 1]), i32([2, 3])
+    with pytest.raises(TypeError):
+        pool.begin_step(s.long(), n, 5)
+    with pytest.raises(TypeError):
+        pool.begin_step(s.cpu(), n, 5)
+    with pytest.raises(ValueError):
+        pool.begin_step(s, n[:1], 5)
+    with pytest.raises(ValueError):
+        pool.begin_step(s, n, -1)
+    with pytest.raises(ValueError):
+        pool.begin_step(s, n, 5, i32([0, 0]))
+    with pytest.raises(ValueError):
+        pool.begin_step(i32([[0, 1]]), n, 5)
+    with pytest.raises(_lib.PKError):
+        pool.begin_step(i32([0, 1, 2, 3]), i32([1, 1, 1, 1]), 4)       # more than the slots
+    step = pool.begin_step(s, n, 5)
+    kv = torch.zeros(5, 2, 64, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(5, 4, 64, dtype=torch.bfloat16, device=DEV)
+    for bad in (kv.float(), kv[:4], kv[:, :1], kv[..., :32], kv.transpose(1, 2)):
+        with pytest.raises((TypeError, ValueError)):
+            pool.append(0, bad, bad, step)
+    with pytest.raises(ValueError):
+        pool.append(0, kv, kv.repeat(1, 2, 1)[:, :2], step)            # other strides
+    with pytest.raises(_lib.PKError):
+        pool.append(2, kv, kv, step)
+    with pytest.raises(_lib.PKError):
+        pool.append(1, kv[None].repeat(2, 1, 1, 1), kv[None].repeat(2, 1, 1, 1), step)
+    with pytest.raises((TypeError, ValueError)):
+        pool.attention(0, q.half(), step)
+    with pytest.raises(ValueError):
+        pool.attention(0, q, step, out=q[:4])
+    with pytest.raises(_lib.PKError):
+        pool.attention(0, q, step, scale=0.0)
+    with pytest.raises(_lib.PKError):
+        pool.attention(-1, q, step)
+    with pytest.raises(_lib.PKError):   # rows that are not 16-byte aligned
+        pool.attention(0, torch.zeros(5 * 4 * 64 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(5, 4, 64),
+                       step)
+    with pytest.raises(ValueError):
+        other.attention(0, q, step)
+    with pytest.raises(ValueError):
+        other.end_step(step, n - 1)
+    pool.end_step(step, n - 1)
+    for call in (lambda: pool.append(0, kv, kv, step), lambda: pool.attention(0, q, step),
+                 lambda: pool.end_step(step, n - 1)):
+        with pytest.raises(ValueError):
+            call()
+    assert pool.lengths.tolist() == [2, 3, 0]
+    for bad in (dict(dtype=torch.float16), dict(head_dim=96), dict(page_size=12), dict(num_heads=3),
+                dict(device="cpu"), dict(max_tokens=0)):
+        args = dict(num_layers=1, num_heads=4, num_kv_heads=2, head_dim=64, num_slots=2, max_tokens=64,
+                    device=DEV)
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            TokenKVPool(**{**args, **bad})
