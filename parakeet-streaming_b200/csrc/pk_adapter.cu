@@ -335,6 +335,34 @@ __device__ __forceinline__ void lanes_off(int range, uint32_t *off) {
     }
 }
 
+// The pairs p0 .. p1 of a tile, read eight at a time: the first eight when the tile
+// begins, so that the reads' latency (one a pair took 0.4 us of a pair's turn) is
+// under the K blocks before them.
+struct TilePairs {
+    const int2 *pairs;
+    int p0, p1;
+    int2 ahead[8];
+    __device__ __forceinline__ TilePairs(const int2 *all, int from, int to)
+        : pairs(all), p0(from), p1(to) {
+        fetch();
+    }
+    __device__ __forceinline__ void fetch() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            ahead[i] = p0 + i < p1 ? pairs[p0 + i] : make_int2(0, 0);
+    }
+    // fn(pair) for each, while it returns true
+    template <typename F> __device__ __forceinline__ void each(F fn) {
+        while (p0 < p1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (p0 + i < p1 && !fn(ahead[i])) return;
+            p0 += 8;
+            fetch();
+        }
+    }
+};
+
 // A warp's rows of C and R in sorted order: the eight that this lane's pieces touch.
 struct SortedRows {
     int row[8];
@@ -422,6 +450,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             bool ok = true;
             for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
                 const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
+                TilePairs of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     const int s = g % NS;
                     if (g >= pre) {
@@ -431,17 +460,16 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     }
                     tma_load_2d(sA + s * kABytes, rows, &full[s], kb * kBK, m0);
                 }
-                const int p1 = tile_pair[mt + 1];
-                for (int pr = tile_pair[mt]; pr < p1 && ok; ++pr) {
-                    const int a = pairs[pr].x;
-                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                of_tile.each([&](int2 pr) {
+                    for (int rb = 0; rb < rblocks && ok; ++rb, ++g) {
                         const int s = g % NS;
                         if (!(ok = free_stage(g))) break;
                         mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
                         tma_load_2d(sA + s * kABytes, &tm.s, &full[s], rb * kBK, m0);
-                        tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, a);
+                        tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, pr.x);
                     }
-                }
+                    return ok;
+                });
             }
             if (!ok)   // leave no copy in flight
                 for (int s = 0; s < NS; ++s)
@@ -467,6 +495,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
+                TilePairs of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     const int s = g % NS;
                     if (!ready(s)) break;
@@ -478,14 +507,13 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                                   (kb | kk) != 0);
                     umma_commit(&empty[s]);
                 }
-                const int p1 = tile_pair[mt + 1];
-                for (int pr = tile_pair[mt]; pr < p1 && !failed; ++pr) {
+                of_tile.each([&](int2 pr) {
                     uint32_t off[4];
-                    lanes_off(pairs[pr].y, off);
+                    lanes_off(pr.y, off);
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         const int s = g % NS;
-                        if (!ready(s)) break;
-                            tc_fence_after();
+                        if (failed || !ready(s)) return false;
+                        tc_fence_after();
                         const uint32_t a0 = smem_u32(sA + s * kABytes),
                                        b0 = smem_u32(sB + s * kBBytes);
                         const int steps = min(kBK, p.rank - rb * kBK);
@@ -494,7 +522,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                                             idesc, off);
                         umma_commit(&empty[s]);
                     }
-                }
+                    return true;
+                });
                 umma_commit(&tmem_full[acc]);
             }
         }
@@ -628,6 +657,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             for (int tile = pair; tile < tiles && ok; tile += npairs) {
                 const int mt = tile % mtiles, m0 = mt * 2 * kBM + (int)rank * kBM;
                 const int n0 = (tile / mtiles) * BN + (int)rank * kHalfB;
+                TilePairs of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     if (!(ok = free_stage(g))) break;
                     const int s = g % NS;
@@ -636,18 +666,18 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     tma_load_2d_pair(sB + s * kBBytes, &tm.w, fb, kb * kBK, n0);
                     tma_load_2d_pair(sA + s * kABytes, rows, fb, kb * kBK, m0);
                 }
-                const int p1 = tile_pair[min(2 * mt + 2, halves)];
-                for (int pr = tile_pair[2 * mt]; pr < p1 && ok; ++pr) {
-                    const int a = pairs[pr].x;
+                if (!ok) break;
+                of_tile.each([&](int2 pr) {
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
-                        if (!(ok = free_stage(g))) break;
+                        if (!(ok = free_stage(g))) return false;
                         const int s = g % NS;
                         const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
                         if (leader) mbar_arrive_expect_tx(&full[s], kStageTx);
                         tma_load_2d_pair(sA + s * kABytes, &tm.s, fb, rb * kBK, m0);
-                        tma_load_3d_pair(sB + s * kBBytes, &tm.up, fb, rb * kBK, n0, a);
+                        tma_load_3d_pair(sB + s * kBBytes, &tm.up, fb, rb * kBK, n0, pr.x);
                     }
-                }
+                    return true;
+                });
             }
             if (leader) {   // leave none of the pair's loads in flight
                 for (int s = 0; s < NS; ++s)
@@ -675,6 +705,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
+                const int border = tile_pair[min(2 * mt + 1, halves)];   // of the two halves
+                TilePairs of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     const int s = g % NS;
                     if (!ready(s)) break;
@@ -686,26 +718,25 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                                        (kb | kk) != 0);
                     umma_commit_pair(&empty[s]);
                 }
-                for (int h = 2 * mt; h < min(2 * mt + 2, halves) && !failed; ++h) {
-                    const int p1 = tile_pair[h + 1];
-                    for (int pr = tile_pair[h]; pr < p1 && !failed; ++pr) {
-                        uint32_t off[8];
-                        lanes_off(h & 1 ? 0 : pairs[pr].y, off);
-                        lanes_off(h & 1 ? pairs[pr].y : 0, off + 4);
-                        for (int rb = 0; rb < rblocks; ++rb, ++g) {
-                            const int s = g % NS;
-                            if (!ready(s)) break;
-                            tc_fence_after();
-                            const uint32_t a0 = smem_u32(sA + s * kABytes),
-                                           b0 = smem_u32(sB + s * kBBytes);
-                            const int steps = min(kBK, p.rank - rb * kBK);
-                            for (int kk = 0; kk * 16 < steps; ++kk)
-                                umma_bf16_pair_lanes(d, sw128_desc(a0 + kk * 32),
-                                                     sw128_desc(b0 + kk * 32), idesc, off);
-                            umma_commit_pair(&empty[s]);
-                        }
+                int pr_at = tile_pair[2 * mt];
+                of_tile.each([&](int2 pr) {
+                    const bool odd = pr_at++ >= border;   // the second half's
+                    uint32_t off[8];
+                    lanes_off(odd ? 0 : pr.y, off);
+                    lanes_off(odd ? pr.y : 0, off + 4);
+                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
+                        const int s = g % NS;
+                        if (failed || !ready(s)) return false;
+                        tc_fence_after();
+                        const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
+                        const int steps = min(kBK, p.rank - rb * kBK);
+                        for (int kk = 0; kk * 16 < steps; ++kk)
+                            umma_bf16_pair_lanes(d, sw128_desc(a0 + kk * 32),
+                                                 sw128_desc(b0 + kk * 32), idesc, off);
+                        umma_commit_pair(&empty[s]);
                     }
-                }
+                    return true;
+                });
                 if (failed) break;
                 umma_commit_pair(&tmem_full[acc]);
             }
@@ -769,9 +800,11 @@ cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
     cudaError_t e = allow_smem(adapter_shrink_kernel<NT>, kShWarps * kShRows * NT * 8 * 4, done);
     if (e != cudaSuccess) return e;
     const int groups = (p.M + kTileRows - 1) / kTileRows * (kTileRows / kShRows);
-    // a CTA for every adapter that a group can have while there are SMs for them; two
-    // otherwise, since a border between two adapters would take its group twice as long
-    const int passes = groups * kShRows <= 2 * current_sms() ? kShRows : 2;
+    // a CTA for every adapter that a group can have while there is room for them on the
+    // GPU; two otherwise, since a border between two adapters would take its group
+    // twice as long
+    const int room = 8 * current_sms() / groups;
+    const int passes = room < 2 ? 2 : (room < kShRows ? room : kShRows);
     return launch_pdl(adapter_shrink_kernel<NT>, dim3(groups, passes), dim3(kShWarps * 32),
                       kShWarps * kShRows * p.rank * 4, s, p);
 }

@@ -20,11 +20,15 @@ from .ops import GEMM_EPILOGUES, _gemm_error, _launch, _rows, _stream
 _BF16 = torch.bfloat16
 
 
-def _error_word(device):
+_plan_words: dict = {}   # (rows, adapters): a plan's size
+
+
+def _error_word(device) -> int:
+    """Address of the device's error word, which the GEMMs share."""
     err = _gemm_error.get(device)
     if err is None:
         err = _gemm_error[device] = torch.zeros(1, dtype=torch.int32, device=device)
-    return err
+    return err.data_ptr()
 
 
 class AdapterPlan:
@@ -43,13 +47,18 @@ def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
     change while it is in use."""
     if ids.dtype is not torch.int32 or not ids.is_cuda or ids.dim() != 1 or not ids.is_contiguous():
         raise ValueError("ids must be a contiguous int32 [M] CUDA tensor")
-    rows, dev = ids.shape[0], ids.device
-    words = lib().pk_adapter_plan_words(rows, num_adapters)
-    if words < 0:
-        raise ValueError(f"{rows} rows or {num_adapters} adapters: out of range")
+    rows, dev, L = ids.shape[0], ids.device, lib()
+    words = _plan_words.get((rows, num_adapters))
+    if words is None:
+        words = L.pk_adapter_plan_words(rows, num_adapters)
+        if words < 0:
+            raise ValueError(f"{rows} rows or {num_adapters} adapters: out of range")
+        if len(_plan_words) >= 256:
+            _plan_words.clear()
+        _plan_words[rows, num_adapters] = words
     block = ids.new_empty(words)
-    _launch(dev, lib().pk_adapter_plan, ids.data_ptr(), rows, num_adapters, block.data_ptr(),
-            _error_word(dev).data_ptr(), _stream(dev))
+    _launch(dev, L.pk_adapter_plan, ids.data_ptr(), rows, num_adapters, block.data_ptr(),
+            _error_word(dev), _stream(dev))
     return AdapterPlan(ids, rows, num_adapters, block)
 
 
@@ -76,13 +85,12 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     a [..., K], weight [N, K], down [num_adapters, rank, K], up [num_adapters, N,
     rank], bf16; K and N multiples of 64, rank a multiple of 8 up to 128; scale
     float32 [num_adapters] or None.  The plan's rows are those of ``a`` flattened."""
-    dev = a.device
-    if a.dtype is not _BF16 or weight.dtype is not _BF16 or dev.type != "cuda" or \
-            weight.device != dev or weight.dim() != 2 or a.shape[-1] != weight.shape[1] or \
-            weight.stride(1) != 1:
+    dev, shape = a.device, a.shape
+    N, K = weight.shape if weight.dim() == 2 else (0, 0)
+    if a.dtype is not _BF16 or weight.dtype is not _BF16 or not a.is_cuda or weight.device != dev \
+            or shape[-1] != K or weight.stride(1) != 1:
         raise ValueError("adapter_gemm needs bf16 operands a [..., K] and weight [N, K], rows "
                          "contiguous, on one CUDA device")
-    N, K = weight.shape
     n = plan.num_adapters
     rank = down.shape[1] if down.dim() == 3 else 0
     _operand(down, (n, rank, K), _BF16, dev, "down")
@@ -91,8 +99,13 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     if scale is not None:
         _operand(scale, (n,), torch.float32, dev, "scale")
         sc = scale.data_ptr()
-    flat = a.dim() == 2
-    a2 = a if flat and _plain_rows(a) else _rows(a, K)
+    flat = len(shape) == 2
+    a2 = a
+    lda, col = a.stride() if flat else (0, 0)
+    ap = a.data_ptr()
+    if col != 1 or lda % 8 or lda < K or ap % 16:
+        a2 = _rows(a, K)
+        ap, lda = a2.data_ptr(), a2.stride(0)
     M = a2.shape[0]
     if plan.rows != M or plan.ids.device != dev:
         raise ValueError(f"the plan is for {plan.rows} rows on {plan.ids.device}, a has {M} on {dev}")
@@ -120,10 +133,9 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
         raise ValueError(f"rank {rank}: a multiple of 8 up to {PK_ADAPTER_MAX_RANK}")
     # (rows padded to 128 of K and of rank; a buffer of this call's own)
     ws = a.new_empty((M + 127) // 128 * 128 * (K + rank))
-    _launch(dev, lib().pk_adapter_gemm, a2.data_ptr(), a2.stride(0), weight.data_ptr(),
-            weight.stride(0), M, N, K, out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(),
-            up.data_ptr(), rank, n, sc, plan.ids.data_ptr(), plan.block.data_ptr(), ws.data_ptr(),
-            _error_word(dev).data_ptr(), _stream(dev))
+    _launch(dev, lib().pk_adapter_gemm, ap, lda, weight.data_ptr(), weight.stride(0), M, N, K,
+            out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(), up.data_ptr(), rank, n, sc,
+            plan.ids.data_ptr(), plan.block.data_ptr(), ws.data_ptr(), _error_word(dev), _stream(dev))
     return out if flat and out.dim() == 2 else out.reshape(*a.shape[:-1], N)
 
 
