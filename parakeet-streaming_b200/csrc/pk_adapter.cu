@@ -389,15 +389,15 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     extern __shared__ uint8_t gemm_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *sA = smem, *sB = smem + NS * kABytes;
-    __shared__ __align__(8) uint64_t full[NS], empty[NS], tmem_full[2], tmem_empty[2];
+    uint8_t *sA = smem, *sB = smem + NS * kABytes, *sS = sB + NS * kBBytes;
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], tmem_full[2], tmem_empty[2], s_full, s_empty;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int failed;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    uint8_t *stage = sB + NS * kBBytes + (warp & 3) * kStageBytes;
     const int mtiles = (p.M + kBM - 1) / kBM, tiles = mtiles * (p.N / BN), nk = p.K / kBK;
     const int rblocks = (p.rank + kBK - 1) / kBK;
+    uint8_t *stage = sS + rblocks * kABytes + (warp & 3) * kStageBytes;
     const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order,
                   *sorted = p.plan + p.l.sorted;
     const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
@@ -410,6 +410,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             mbar_init(&tmem_full[a], 1);
             mbar_init(&tmem_empty[a], 4);
         }
+        mbar_init(&s_full, 1);
+        mbar_init(&s_empty, 1);
         failed = 0;
         fence_mbar_init();
         prefetch_tmap(&tm.w);
@@ -446,7 +448,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             }
             grid_dep_wait();
             const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
-            int g = 0;
+            int g = 0, with_s = 0;   // ring uses; tiles that had an S
             bool ok = true;
             for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
                 const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
@@ -460,32 +462,47 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     }
                     tma_load_2d(sA + s * kABytes, rows, &full[s], kb * kBK, m0);
                 }
+                if (!ok || of_tile.p0 == of_tile.p1) continue;
+                // S once a tile (a copy for each pair made every CTA of a row tile ask for
+                // the same few lines again and again: 0.65 us a pair)
+                if (with_s >= 1 && !mbar_wait_bounded(&s_empty, (with_s - 1) & 1, kWaitLimitNs)) {
+                    raise(p.error, PK_DEV_TIMEOUT);
+                    failed = 1;
+                    ok = false;
+                    break;
+                }
+                ++with_s;
+                mbar_arrive_expect_tx(&s_full, rblocks * kABytes);
+                for (int rb = 0; rb < rblocks; ++rb)
+                    tma_load_2d(sS + rb * kABytes, &tm.s, &s_full, rb * kBK, m0);
                 of_tile.each([&](int2 pr) {
-                    for (int rb = 0; rb < rblocks && ok; ++rb, ++g) {
+                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         const int s = g % NS;
-                        if (!(ok = free_stage(g))) break;
-                        mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
-                        tma_load_2d(sA + s * kABytes, &tm.s, &full[s], rb * kBK, m0);
+                        if (!(ok = free_stage(g))) return false;
+                        mbar_arrive_expect_tx(&full[s], kBBytes);
                         tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, pr.x);
                     }
-                    return ok;
+                    return true;
                 });
             }
-            if (!ok)   // leave no copy in flight
+            if (!ok) {   // leave no copy in flight
                 for (int s = 0; s < NS; ++s)
                     if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
+                if (with_s) mbar_wait_bounded(&s_full, (with_s - 1) & 1, kWaitLimitNs);
+            }
         }
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = idesc_bf16(kBM, BN);
             grid_dep_wait();   // the plan
-            int g = 0, t = 0;
-            auto ready = [&](int s) {
-                if (mbar_wait_bounded(&full[s], (g / NS) & 1, kWaitLimitNs)) return true;
+            int g = 0, t = 0, with_s = 0;
+            auto done = [&](uint64_t *bar, uint32_t parity) {
+                if (mbar_wait_bounded(bar, parity, kWaitLimitNs)) return true;
                 raise(p.error, PK_DEV_TIMEOUT);
                 failed = 1;
                 return false;
             };
+            auto ready = [&](int s) { return done(&full[s], (g / NS) & 1); };
             for (int tile = blockIdx.x; tile < tiles && !failed; tile += gridDim.x, ++t) {
                 const int acc = t & 1, use = t >> 1, mt = tile % mtiles;
                 if (use >= 1 && !mbar_wait_bounded(&tmem_empty[acc], (use - 1) & 1, kWaitLimitNs)) {
@@ -507,6 +524,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                                   (kb | kk) != 0);
                     umma_commit(&empty[s]);
                 }
+                const bool any = of_tile.p0 < of_tile.p1;
+                if (any && !failed) done(&s_full, with_s++ & 1);
                 of_tile.each([&](int2 pr) {
                     uint32_t off[4];
                     lanes_off(pr.y, off);
@@ -514,7 +533,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                         const int s = g % NS;
                         if (failed || !ready(s)) return false;
                         tc_fence_after();
-                        const uint32_t a0 = smem_u32(sA + s * kABytes),
+                        const uint32_t a0 = smem_u32(sS + rb * kABytes),
                                        b0 = smem_u32(sB + s * kBBytes);
                         const int steps = min(kBK, p.rank - rb * kBK);
                         for (int kk = 0; kk * 16 < steps; ++kk)
@@ -524,6 +543,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     }
                     return true;
                 });
+                if (any) umma_commit(&s_empty);
                 umma_commit(&tmem_full[acc]);
             }
         }
@@ -600,19 +620,19 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     extern __shared__ uint8_t gemm_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *sA = smem, *sB = smem + NS * kABytes;
-    __shared__ __align__(8) uint64_t full[NS], empty[NS], tmem_full[2], tmem_empty[2];
+    uint8_t *sA = smem, *sB = smem + NS * kABytes, *sS = sB + NS * kBBytes;
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], tmem_full[2], tmem_empty[2], s_full, s_empty;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int failed;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    uint8_t *stage = sB + NS * kBBytes + (warp & 3) * kStageBytes;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const int pair = blockIdx.x / 2, npairs = gridDim.x / 2;
     const int halves = (p.M + kBM - 1) / kBM, mtiles = (halves + 1) / 2;
     const int tiles = mtiles * (p.N / BN), nk = p.K / kBK;
     const int rblocks = (p.rank + kBK - 1) / kBK;
+    uint8_t *stage = sS + rblocks * kABytes + (warp & 3) * kStageBytes;
     const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order,
                   *sorted = p.plan + p.l.sorted;
     const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
@@ -625,6 +645,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             mbar_init(&tmem_full[a], 1);
             mbar_init(&tmem_empty[a], 8);
         }
+        mbar_init(&s_full, 1);
+        mbar_init(&s_empty, 1);
         failed = 0;
         fence_mbar_init();
         prefetch_tmap(&tm.w);
@@ -652,8 +674,9 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         if (lane == 0) {
             grid_dep_wait();
             const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
-            int g = 0;
+            int g = 0, with_s = 0;   // ring uses; tiles that had an S
             bool ok = true;
+            const uint32_t sb = mapa_rank(smem_u32(&s_full), 0);
             for (int tile = pair; tile < tiles && ok; tile += npairs) {
                 const int mt = tile % mtiles, m0 = mt * 2 * kBM + (int)rank * kBM;
                 const int n0 = (tile / mtiles) * BN + (int)rank * kHalfB;
@@ -666,14 +689,23 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     tma_load_2d_pair(sB + s * kBBytes, &tm.w, fb, kb * kBK, n0);
                     tma_load_2d_pair(sA + s * kABytes, rows, fb, kb * kBK, m0);
                 }
-                if (!ok) break;
+                if (!ok || of_tile.p0 == of_tile.p1) continue;
+                if (with_s >= 1 && !mbar_wait_bounded(&s_empty, (with_s - 1) & 1, kWaitLimitNs)) {
+                    raise(p.error, PK_DEV_TIMEOUT);
+                    failed = 1;
+                    ok = false;
+                    break;
+                }
+                ++with_s;
+                if (leader) mbar_arrive_expect_tx(&s_full, 2 * rblocks * kABytes);
+                for (int rb = 0; rb < rblocks; ++rb)
+                    tma_load_2d_pair(sS + rb * kABytes, &tm.s, sb, rb * kBK, m0);
                 of_tile.each([&](int2 pr) {
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         if (!(ok = free_stage(g))) return false;
                         const int s = g % NS;
                         const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
-                        if (leader) mbar_arrive_expect_tx(&full[s], kStageTx);
-                        tma_load_2d_pair(sA + s * kABytes, &tm.s, fb, rb * kBK, m0);
+                        if (leader) mbar_arrive_expect_tx(&full[s], 2 * kBBytes);
                         tma_load_3d_pair(sB + s * kBBytes, &tm.up, fb, rb * kBK, n0, pr.x);
                     }
                     return true;
@@ -682,19 +714,21 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             if (leader) {   // leave none of the pair's loads in flight
                 for (int s = 0; s < NS; ++s)
                     if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
+                if (with_s) mbar_wait_bounded(&s_full, (with_s - 1) & 1, kWaitLimitNs);
             }
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
             constexpr uint32_t idesc = idesc_bf16(2 * kBM, BN);
             grid_dep_wait();
-            int g = 0, t = 0;
-            auto ready = [&](int s) {
-                if (mbar_wait_cluster_bounded(&full[s], (g / NS) & 1, kWaitLimitNs)) return true;
+            int g = 0, t = 0, with_s = 0;
+            auto done = [&](uint64_t *bar, uint32_t parity) {
+                if (mbar_wait_cluster_bounded(bar, parity, kWaitLimitNs)) return true;
                 raise(p.error, PK_DEV_TIMEOUT);
                 failed = 1;
                 return false;
             };
+            auto ready = [&](int s) { return done(&full[s], (g / NS) & 1); };
             for (int tile = pair; tile < tiles && !failed; tile += npairs, ++t) {
                 const int acc = t & 1, use = t >> 1, mt = tile % mtiles;
                 if (use >= 1 &&
@@ -718,7 +752,9 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                                        (kb | kk) != 0);
                     umma_commit_pair(&empty[s]);
                 }
-                int pr_at = tile_pair[2 * mt];
+                int pr_at = of_tile.p0;
+                const bool any = of_tile.p0 < of_tile.p1;
+                if (any && !failed) done(&s_full, with_s++ & 1);
                 of_tile.each([&](int2 pr) {
                     const bool odd = pr_at++ >= border;   // the second half's
                     uint32_t off[8];
@@ -728,7 +764,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                         const int s = g % NS;
                         if (failed || !ready(s)) return false;
                         tc_fence_after();
-                        const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
+                        const uint32_t a0 = smem_u32(sS + rb * kABytes), b0 = smem_u32(sB + s * kBBytes);
                         const int steps = min(kBK, p.rank - rb * kBK);
                         for (int kk = 0; kk * 16 < steps; ++kk)
                             umma_bf16_pair_lanes(d, sw128_desc(a0 + kk * 32),
@@ -738,6 +774,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     return true;
                 });
                 if (failed) break;
+                if (any) umma_commit_pair(&s_empty);
                 umma_commit_pair(&tmem_full[acc]);
             }
         }
@@ -812,11 +849,13 @@ cudaError_t launch_shrink(const AdapterArgs &p, cudaStream_t s) {
 template <int BN, int NS, bool kPair, int EPI>
 int launch_product_t(const AdapterArgs &p, const AdapterMaps &tm, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
-    auto k = kPair ? adapter_gemm_pair_kernel<kPair ? BN : 256, kPair ? NS : 6, EPI>
+    auto k = kPair ? adapter_gemm_pair_kernel<kPair ? BN : 256, kPair ? NS : 5, EPI>
                    : adapter_gemm_kernel<kPair ? 64 : BN, kPair ? 6 : NS, EPI>;
-    constexpr size_t smem =
+    constexpr size_t ring =
         (size_t)NS * (kABytes + (kPair ? BN / 2 : BN) * kBK * 2) + 4 * kStageBytes + 1024;
-    cudaError_t e = allow_smem(k, smem, done);
+    static_assert(ring + 2 * kABytes <= 226 * 1024, "shared memory");
+    const size_t smem = ring + (p.rank + kBK - 1) / kBK * kABytes;   // and a tile's S
+    cudaError_t e = allow_smem(k, ring + 2 * kABytes, done);
     if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(adapter gemm)");
     const int rows = kPair ? 2 * kBM : kBM, sms = current_sms();
     const int tiles = ((p.M + rows - 1) / rows) * (p.N / BN);
@@ -895,9 +934,9 @@ int launch_adapter_gemm(const AdapterArgs &a, cudaStream_t s) {
     const int t2 = p.N % 256 == 0 ? mt2 * (p.N / 256) : 0;
     if (t2 >= halves &&
         (p.K >= 2048 || 5 * t2 >= 4 * halves * ((t2 + halves - 1) / halves)))
-        return launch_product<256, 6, true>(p, s);
-    if (p.N % 256 == 0 && mtiles * (p.N / 256) >= 2 * sms) return launch_product<256, 4>(p, s);
-    if (p.N % 128 == 0 && mtiles * (p.N / 128) >= sms) return launch_product<128, 6>(p, s);
+        return launch_product<256, 5, true>(p, s);
+    if (p.N % 256 == 0 && mtiles * (p.N / 256) >= 2 * sms) return launch_product<256, 3>(p, s);
+    if (p.N % 128 == 0 && mtiles * (p.N / 128) >= sms) return launch_product<128, 5>(p, s);
     return launch_product<64, 6>(p, s);
 }
 
