@@ -15,8 +15,11 @@ a host read and can be captured in a CUDA graph::
     pool.end_step(step, last)                              # keep the path to node last[b]
     pool.truncate(slots, lengths)                          # cut back, or release (0)
 
-Calls on one pool are ordered by the stream they are made on; two steps of the
-same request are not begun at once.
+Calls on one pool are ordered by the stream they are made on; only ``attention``
+calls, and ``append`` and ``attention`` of different layers, may run side by side.
+Two steps of the same request are not begun at once, and a step's tables hold until
+its requests are truncated or the pool is reset.  A step's block belongs to the
+stream that it was begun on, as any tensor does.
 """
 from __future__ import annotations
 
@@ -165,14 +168,16 @@ class TokenKVPool:
         if t.dtype is not self.dtype or t.device != self.device:
             raise TypeError(f"{name}: expected {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
         shape = t.shape
-        if len(shape) < 3 or shape[-1] != self.head_dim or shape[-2] != heads:
+        # (one row of one 64-wide head in several layers fits the former but for its rows)
+        if len(shape) < 3 or shape[-3:] != (rows, heads, self.head_dim):
             if len(shape) < 2 or shape[-1] != heads * self.head_dim:
                 raise ValueError(f"{name}: expected [..., {rows}, {heads}, {self.head_dim}], got "
                                  f"{tuple(shape)}")
             t = t.unflatten(-1, (heads, self.head_dim))
             shape = t.shape
-        if shape[-3] != rows:
-            raise ValueError(f"{name}: {shape[-3]} rows, the step has {rows}")
+        if len(shape) < 3 or shape[-3] != rows:
+            raise ValueError(f"{name}: expected [..., {rows}, {heads}, {self.head_dim}], got "
+                             f"{tuple(shape)}")
         if t.stride(-1) != 1:
             raise ValueError(f"{name}: last dimension must be contiguous")
         return t
@@ -222,7 +227,7 @@ class TokenKVPool:
         _launch(dev, self._lib.pk_token_begin_step, self._h, slots.data_ptr(), counts.data_ptr(), B,
                 parents.data_ptr() if trees else None, rows, block.data_ptr(), _stream(dev))
         step = TokenStep(self, block, B, rows, trees, size[1], size[2])
-        if B == 0:   # nothing was launched: no rows, no units
+        if B == 0:   # nothing was launched
             block.zero_()
             step.row_request.fill_(-1)
             step.slot_map.fill_(-1)
@@ -270,7 +275,8 @@ class TokenKVPool:
         """Attention of the step's rows over their request's context and, of the
         step's own tokens, their ancestors and themselves (without ``parents``:
         the rows before and themselves).  query [rows, H, dh] (or [rows, H * dh]);
-        ``scale`` defaults to dh ** -0.5; returns ``out`` in the query's shape.
+        ``scale`` defaults to dh ** -0.5; returns ``out`` in the query's shape (it may
+        be the query itself).
         Rows of no request, and of refused ones, are left as they were."""
         self._step(step)
         q = self._rows(query, self.num_heads, step.rows, "query")

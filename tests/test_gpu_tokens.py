@@ -528,6 +528,42 @@ def test_layers_on_two_streams_at_once():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("nl", [1, 3])
+def test_one_token_of_one_kv_head(dh, nl):
+    """[nl, 1, dh] may be one row of nl layers or nl rows of one head: the step's
+    rows say which."""
+    pool = TokenKVPool(nl, 2, 1, dh, 2, 40, num_pages=4, page_size=8, device=DEV)
+    k = torch.randn(nl, 1, dh, device=DEV).to(torch.bfloat16)
+    v = torch.randn_like(k)
+    step = pool.begin_step(i32([1]), i32([1]), 1)
+    pool.append(0, k, v, step)
+    page = pool.page_table.tolist()[1][0]
+    assert torch.equal(pool.kv[page, :, 0, 0, 0], k[:, 0])
+    assert torch.equal(pool.kv[page, :, 1, 0, 0], v[:, 0])
+    out = pool.attention(nl - 1, torch.randn(1, 2 * dh, device=DEV).to(torch.bfloat16), step)
+    assert torch.equal(out, v[nl - 1].repeat(1, 2))    # one key: its value
+    pool.end_step(step, i32([0]))
+    step = pool.begin_step(i32([1]), i32([3]), 3)
+    rows = torch.randn(3, 1, dh, device=DEV).to(torch.bfloat16)
+    pool.append(0, rows, rows, step)
+    assert torch.equal(pool.kv[page, 0, 0, 0, 1:4], rows[:, 0])
+    assert pool.read_error() == 0
+
+
+@pytest.mark.parametrize("kernel", range(len(KERNELS)))
+def test_out_may_be_the_query(kernel):
+    dtype, H, Hkv, dh, ctx, new = KERNELS[kernel]
+    rng = np.random.default_rng(31 + kernel)
+    pool, model, step, ref, parents, q = filled(rng, 16, H, Hkv, dh, ctx, new, dtype)
+    want = pool.attention(0, q, step).clone()
+    got = pool.attention(0, q, step, out=q)
+    assert got.data_ptr() == q.data_ptr()
+    for row, req in enumerate(step.row_request.tolist()):
+        if req >= 0:
+            assert torch.equal(got[row], want[row])
+
+
 def test_python_refusals():
     pool = TokenKVPool(2, 4, 2, 64, 3, 100, page_size=16, device=DEV)
     other = TokenKVPool(2, 4, 2, 64, 3, 100, page_size=16, device=DEV)
