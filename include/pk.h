@@ -598,15 +598,15 @@ int64_t pk_adapter_plan_words(int32_t rows, int32_t num_adapters);
 int pk_adapter_plan(const int32_t *ids, int32_t rows, int32_t num_adapters, int32_t *plan,
                     int32_t *error, void *stream);
 
-/* Arguments as pk_gemm_bf16's; ids and plan as given to and made by
- * pk_adapter_plan (rows = M); workspace: pk_adapter_workspace() bytes, 16-byte
+/* Arguments as pk_gemm_bf16's; plan as made by pk_adapter_plan (rows = M);
+ * workspace: pk_adapter_workspace() bytes, 16-byte
  * aligned, for this call alone. */
 int64_t pk_adapter_workspace(int32_t rows, int32_t K, int32_t rank);
 int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int32_t M, int32_t N,
                     int32_t K, void *C, int64_t ldc, int32_t epilogue, const void *R, int64_t ldr,
                     const void *bias, float alpha, const void *down, const void *up, int32_t rank,
-                    int32_t num_adapters, const float *scale, const int32_t *ids,
-                    const int32_t *plan, void *workspace, int32_t *error, void *stream);
+                    int32_t num_adapters, const float *scale, const int32_t *plan,
+                    void *workspace, int32_t *error, void *stream);
 
 /* Self-test of the failure path of every TMA pipeline here: the bounded
  * mbarrier wait that gives up after a time limit and records PK_DEV_TIMEOUT in

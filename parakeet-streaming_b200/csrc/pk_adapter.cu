@@ -14,8 +14,8 @@
 //     products, so one adapter's weights, whatever they hold, do not reach another's
 //     rows.  The epilogue writes the rows back to their own places.
 //
-// S is rounded to bf16 because the tensor cores take it so: relative 2^-9 of each
-// of its terms, half of what rounding the sum to the bf16 result costs.  Sums are
+// S is rounded to bf16 because the tensor cores take it so: off by 2^-8 of each of
+// its terms at most, as the bf16 result is of their sum.  Sums are
 // fp32 throughout and in a fixed order.
 #include "pk_common.cuh"
 #include "pk_internal.h"

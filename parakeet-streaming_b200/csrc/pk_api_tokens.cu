@@ -222,17 +222,19 @@ int64_t pk_adapter_workspace(int32_t rows, int32_t K, int32_t rank) {
 int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int32_t M, int32_t N,
                     int32_t K, void *C, int64_t ldc, int32_t epilogue, const void *R, int64_t ldr,
                     const void *bias, float alpha, const void *down, const void *up, int32_t rank,
-                    int32_t num_adapters, const float *scale, const int32_t *ids,
-                    const int32_t *plan, void *workspace, int32_t *error, void *stream) {
+                    int32_t num_adapters, const float *scale, const int32_t *plan,
+                    void *workspace, int32_t *error, void *stream) {
     PK_CHECK(M >= 0 && M <= PK_ADAPTER_MAX_ROWS && N > 0 && K > 0, "bad shape %d x %d x %d", M, N, K);
     PK_CHECK(num_adapters > 0 && num_adapters <= PK_ADAPTER_MAX, "num_adapters %d outside [1, %d]",
              num_adapters, PK_ADAPTER_MAX);
     PK_CHECK(rank > 0 && rank % 8 == 0 && rank <= PK_ADAPTER_MAX_RANK,
              "rank %d: a multiple of 8 up to %d", rank, PK_ADAPTER_MAX_RANK);
+    PK_CHECK((int64_t)num_adapters * N <= 0x7fffffff, "%d adapters of %d rows: more than 32 bits count",
+             num_adapters, N);
     if (M == 0) return PK_OK;
     PK_CHECK(K % 64 == 0 && N % 64 == 0, "K (%d) and N (%d) must be multiples of 64", K, N);
     PK_CHECK(epilogue >= PK_GEMM_STORE && epilogue <= PK_GEMM_BIAS, "bad epilogue %d", epilogue);
-    PK_CHECK(A && W && C && down && up && ids && plan && workspace && error, "null pointer");
+    PK_CHECK(A && W && C && down && up && plan && workspace && error, "null pointer");
     PK_CHECK(aligned16(A) && aligned16(W) && aligned16(C) && aligned16(down) && aligned16(up) &&
                  aligned16(plan) && aligned16(workspace),
              "operands must be 16-byte aligned");
@@ -263,7 +265,6 @@ int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int3
     a.adapters = num_adapters;
     a.alpha = alpha;
     a.scale = scale;
-    a.ids = ids;
     a.plan = plan;
     a.error = error;
     return launch_adapter_gemm(a, static_cast<cudaStream_t>(stream));

@@ -223,7 +223,8 @@ namespace pk {
 // group) of one request and K/V head, a key tile `keys` of its keys; `ctas` workers
 // (CTAs, or warps) share the work.
 struct TokShape {
-    int rows, keys, ctas;
+    int rows, keys;
+    int ctas;    // workers: CTAs, or warps of the 16-row bf16 kernel
     int least;   // key tiles that a worker takes before a request's are split over several
     int lead;    // what beginning a row tile costs, in key tiles
 };
@@ -244,8 +245,8 @@ inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
 
 // Step block, int32 words: header, then arrays at these offsets.  The step's work
 // is a line of key tiles, request by request, K/V head by head, row tile by row
-// tile; CTA c takes tiles [c * share, (c + 1) * share), whatever they belong to, so
-// that every CTA has the same number however the lengths are spread (share 0: a
+// tile; worker c takes tiles [c * share, (c + 1) * share), whatever they belong to, so
+// that every worker has the same number however the lengths are spread (share 0: a
 // row tile each).
 enum TokHeader { kTokShare = 0, kTokRows, kTokFree, kTokHeaderWords = 16 };
 struct TokLayout {
@@ -340,7 +341,7 @@ struct AdapterArgs {
     int M, N, K, epilogue, rank, adapters;
     float alpha;
     const float *scale;
-    const int32_t *ids, *plan;
+    const int32_t *plan;
     int32_t *error;
     AdapterLayout l;
 };

@@ -156,7 +156,7 @@ SIGNATURES = {
     "pk_adapter_plan": [_P, _I32, _I32, _P, _P, _P],
     "pk_adapter_workspace": [_I32, _I32, _I32],
     "pk_adapter_gemm": [_P, _I64, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _I64, _P,
-                        ctypes.c_float, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _P],
+                        ctypes.c_float, _P, _P, _I32, _I32, _P, _P, _P, _P, _P],
     "pk_selftest_bounded_wait": [_P, _I32, _I64, _P, _P],
     "pk_last_error": [],
 }

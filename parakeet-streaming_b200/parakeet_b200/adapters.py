@@ -27,6 +27,8 @@ def _error_word(device) -> int:
     """Address of the device's error word, which the GEMMs share."""
     err = _gemm_error.get(device)
     if err is None:
+        if torch.cuda.is_current_stream_capturing():   # a replay would clear it again
+            raise RuntimeError("a device's first adapter call cannot be captured: make one before")
         err = _gemm_error[device] = torch.zeros(1, dtype=torch.int32, device=device)
     return err.data_ptr()
 
@@ -34,17 +36,16 @@ def _error_word(device) -> int:
 class AdapterPlan:
     """The rows of a step sorted by adapter (``adapter_plan``)."""
 
-    __slots__ = ("ids", "rows", "num_adapters", "block")
+    __slots__ = ("rows", "num_adapters", "block")
 
-    def __init__(self, ids, rows, num_adapters, block):
-        self.ids, self.rows, self.num_adapters, self.block = ids, rows, num_adapters, block
+    def __init__(self, rows, num_adapters, block):
+        self.rows, self.num_adapters, self.block = rows, num_adapters, block
 
 
 def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
     """ids int32 [M] on the device: each row's adapter in [0, num_adapters), or
-    -1.  An id out of range counts as -1 and sets PK_DEV_BAD_SLOT in the GEMMs'
-    error word (``ops.gemm_error_word``).  The plan keeps ``ids``; they must not
-    change while it is in use."""
+    -1 (``num_adapters`` is 1 at least).  An id out of range counts as -1 and sets PK_DEV_BAD_SLOT in the GEMMs'
+    error word (``ops.gemm_error_word``)."""
     if ids.dtype is not torch.int32 or not ids.is_cuda or ids.dim() != 1 or not ids.is_contiguous():
         raise ValueError("ids must be a contiguous int32 [M] CUDA tensor")
     rows, dev, L = ids.shape[0], ids.device, lib()
@@ -59,7 +60,7 @@ def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
     block = ids.new_empty(words)
     _launch(dev, L.pk_adapter_plan, ids.data_ptr(), rows, num_adapters, block.data_ptr(),
             _error_word(dev), _stream(dev))
-    return AdapterPlan(ids, rows, num_adapters, block)
+    return AdapterPlan(rows, num_adapters, block)
 
 
 def _operand(t, shape, dtype, dev, name):
@@ -107,8 +108,8 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
         a2 = _rows(a, K)
         ap, lda = a2.data_ptr(), a2.stride(0)
     M = a2.shape[0]
-    if plan.rows != M or plan.ids.device != dev:
-        raise ValueError(f"the plan is for {plan.rows} rows on {plan.ids.device}, a has {M} on {dev}")
+    if plan.rows != M or plan.block.device != dev:
+        raise ValueError(f"the plan is for {plan.rows} rows on {plan.block.device}, a has {M} on {dev}")
     if out is None:
         out = a.new_empty((M, N))
     elif not out.is_contiguous() or out.numel() != M * N or out.dtype is not _BF16 or \
@@ -135,7 +136,7 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     ws = a.new_empty((M + 127) // 128 * 128 * (K + rank))
     _launch(dev, lib().pk_adapter_gemm, ap, lda, weight.data_ptr(), weight.stride(0), M, N, K,
             out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(), up.data_ptr(), rank, n, sc,
-            plan.ids.data_ptr(), plan.block.data_ptr(), ws.data_ptr(), _error_word(dev), _stream(dev))
+            plan.block.data_ptr(), ws.data_ptr(), _error_word(dev), _stream(dev))
     return out if flat and out.dim() == 2 else out.reshape(*a.shape[:-1], N)
 
 

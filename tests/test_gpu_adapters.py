@@ -169,6 +169,32 @@ def test_graph_replay_with_other_ids():
         check(out, reference(d, "silu"))
 
 
+def test_a_devices_first_call_is_not_captured():
+    """The GEMMs' error word is made by the first call; made under capture, each
+    replay would clear it."""
+    from parakeet_b200 import ops
+    d = make(20, 64, 64, 8, 3, 4)
+    want = run(d)
+    word = ops._gemm_error.pop(d["x"].device)
+    try:
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="first"):
+            with torch.cuda.graph(g):
+                run(d)
+    finally:
+        ops._gemm_error[d["x"].device] = word
+    torch.cuda.synchronize()
+    assert torch.equal(run(d), want)
+
+
+def test_the_ids_may_change_after_the_plan():
+    d = make(300, 128, 128, 16, 6, 8)
+    plan = adapter_plan(d["ids"], 6)
+    want = reference(d, "store")
+    d["ids"].fill_(1 << 30)
+    check(run(d, plan=plan), want)
+
+
 def test_bad_ids_are_reported_and_left_without():
     from parakeet_b200 import _lib, ops
     d = make(50, 64, 64, 8, 3, 2)
