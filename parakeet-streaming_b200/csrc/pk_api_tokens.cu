@@ -229,8 +229,6 @@ int pk_adapter_gemm(const void *A, int64_t lda, const void *W, int64_t ldw, int3
              num_adapters, PK_ADAPTER_MAX);
     PK_CHECK(rank > 0 && rank % 8 == 0 && rank <= PK_ADAPTER_MAX_RANK,
              "rank %d: a multiple of 8 up to %d", rank, PK_ADAPTER_MAX_RANK);
-    PK_CHECK((int64_t)num_adapters * N <= 0x7fffffff, "%d adapters of %d rows: more than 32 bits count",
-             num_adapters, N);
     if (M == 0) return PK_OK;
     PK_CHECK(K % 64 == 0 && N % 64 == 0, "K (%d) and N (%d) must be multiples of 64", K, N);
     PK_CHECK(epilogue >= PK_GEMM_STORE && epilogue <= PK_GEMM_BIAS, "bad epilogue %d", epilogue);

@@ -24,20 +24,21 @@ __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
-// Bounded wait that gives up at once when another wait of the CTA already has.
-__device__ __forceinline__ void ring_wait(uint64_t *bar, uint32_t parity, volatile int *failed,
+// Bounded wait that gives up (false) at once when another wait of the CTA already has.
+__device__ __forceinline__ bool ring_wait(uint64_t *bar, uint32_t parity, volatile int *failed,
                                           int32_t *error) {
-    if (mbar_try_wait(bar, parity)) return;
-    if (*failed) return;
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*failed) return false;
     const uint64_t t0 = globaltimer_ns();
     while (!mbar_try_wait(bar, parity)) {
-        if (*failed) return;
+        if (*failed) return false;
         if (globaltimer_ns() - t0 > kWaitLimitNs) {
             *failed = 1;
             raise(error, PK_DEV_TIMEOUT);
-            return;
+            return false;
         }
     }
+    return true;
 }
 
 // kv_map's copy of a page's rows from `row` on (a multiple of 8): groups of 8 rows, in

@@ -20,9 +20,8 @@
 // each other's latencies.  Warps that shared
 // a row tile met in a barrier at its end and cost 5000 cycles a row tile, however short
 // (160 requests of up to 500 tokens, 8 heads: 41 us).
-// P is rounded to bf16 for the product, relative 2^-9 of each weight, below the
-// rounding of the bf16 V that it multiplies; the sum that normalises keeps fp32
-// weights.  Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
+// P is rounded to bf16 for the product, by 2^-8 of each weight at most, as the bf16 V
+// that it multiplies has been; the sum that normalises keeps fp32 weights.  Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
 // other waits return at once.
 #include <math.h>
 
@@ -220,8 +219,8 @@ __device__ __forceinline__ void attend(const CUtensorMap &kv_map, const TreePara
         for (int t = w.t0; t < w.t1; t += kStride, phase ^= 1) {
             const int k0 = t * kTile;
             const bool own = k0 + kTile > w.ctx;   // some of the step's own tokens, or the end
-            ring_wait(&full[0], phase, failed, p.error);
-            __syncwarp();
+            // (a wait that gave up: nothing more is requested)
+            if (!__all_sync(0xffffffffu, ring_wait(&full[0], phase, failed, p.error))) break;
             float s[kN][4];
 #pragma unroll
             for (int n = 0; n < kN; ++n)
@@ -289,8 +288,7 @@ __device__ __forceinline__ void attend(const CUtensorMap &kv_map, const TreePara
                 o[n][2] *= keep[1];
                 o[n][3] *= keep[1];
             }
-            ring_wait(&full[1], phase, failed, p.error);
-            __syncwarp();
+            if (!__all_sync(0xffffffffu, ring_wait(&full[1], phase, failed, p.error))) break;
             // values that are not finite among the step's own rows
             const bool odd = own && clean_values<DH>(vs, k0, w.ctx, len);
 #pragma unroll
@@ -401,9 +399,10 @@ __device__ __forceinline__ void attend(const CUtensorMap &kv_map, const TreePara
         w = work.u;
         pages = then;
     }
-    if (*failed) {   // leave no copy in flight
+    if (*failed) {   // leave no copy in flight: this tile's, or the next one's K
+        mbar_wait_bounded(&full[0], phase, kWaitLimitNs);
+        mbar_wait_bounded(&full[1], phase, kWaitLimitNs);
         mbar_wait_bounded(&full[0], phase ^ 1, kWaitLimitNs);
-        mbar_wait_bounded(&full[1], phase ^ 1, kWaitLimitNs);
     }
 }
 
@@ -563,8 +562,10 @@ __global__ void __launch_bounds__(128, 3) tree_attn_f32_kernel(const TreeParams 
                 l[i] = l[i] * keep + a + b;
 #pragma unroll
                 for (int n = 0; n < NV; ++n) o[i][n] *= keep;
-                sp[(i * 4 + warp) * kTile + lane] = a;
-                sp[(i * 4 + warp) * kTile + lane + 32] = b;
+                // a key that the row does not see: -0, so that a weight too small for
+                // fp32 keeps its value's inf or NaN
+                sp[(i * 4 + warp) * kTile + lane] = s[i][0] == -INFINITY ? -0.f : a;
+                sp[(i * 4 + warp) * kTile + lane + 32] = s[i][1] == -INFINITY ? -0.f : b;
             }
             __syncwarp();
             // (rows past the end were staged as zeros, their weights are zero)
@@ -584,8 +585,8 @@ __global__ void __launch_bounds__(128, 3) tree_attn_f32_kernel(const TreeParams 
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
 #pragma unroll
-                        for (int n = 0; n < NV; ++n)   // a key that the row does not see has no
-                            o[i][n] += y[k] != 0.f ? y[k] * v[k][n] : 0.f;   // part, even inf
+                        for (int n = 0; n < NV; ++n)   // an unseen key has no part, even inf
+                            o[i][n] += __float_as_int(y[k]) >= 0 ? y[k] * v[k][n] : 0.f;
                 }
             }
             __syncwarp();
@@ -659,13 +660,14 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
         for (int c = c0 + w0; c <= c1; c += step) {
             const int64_t k = at(c, c0, in_tile);
             const float2 ml = *reinterpret_cast<const float2 *>(p.ws_ml + k * 2);
-            const float f = exp2f(ml.x - top);
+            const bool saw = ml.x != -INFINITY;   // (a part that saw nothing wrote no outputs)
+            const float f = saw ? exp2f(ml.x - top) : 0.f;
             sum += f * ml.y;
             const float *src = p.ws_o + k * DH + lane * NV;
 #pragma unroll
             for (int e = 0; e < NV; ++e) {
                 const float x = src[e];
-                acc[e] += f == 0.f ? 0.f : f * x;   // a part that saw nothing wrote no outputs
+                acc[e] += saw ? f * x : 0.f;
             }
         }
         return sum;

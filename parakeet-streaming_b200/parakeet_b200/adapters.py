@@ -81,7 +81,8 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
                  scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """epilogue(acc) with acc[m] = a[m] weight^T + scale[i] (a[m] down[i]^T) up[i]^T
     for row m's adapter i, a[m] weight^T for rows without one; epilogues,
-    ``residual``, ``alpha``, ``bias`` and ``out`` as in ``ops.gemm``.
+    ``residual``, ``alpha``, ``bias`` and ``out`` as in ``ops.gemm`` (``out`` may be the
+    residual, and shares nothing with ``a``).
 
     a [..., K], weight [N, K], down [num_adapters, rank, K], up [num_adapters, N,
     rank], bf16; K and N multiples of 64, rank a multiple of 8 up to 128; scale

@@ -175,6 +175,9 @@ CASES = [
     (16, 4, 2, 64, [0, 40], [200, 77], False),              # chains: a prompt
     (16, 2, 2, 128, [600], [130], False),                   # a chain whose first rows see no last range
     (8, 2, 1, 64, [3, 0, 9], [1, 1, 1], False),
+    (16, 40, 1, 64, [50, 0, 333], [1, 2, 1], True),         # a token's heads over several row tiles
+    (16, 160, 1, 128, [130, 700], [1, 3], True),            # of 128 rows too
+    (32, 48, 2, 64, [70], [9], False),
 ]
 
 
@@ -284,6 +287,27 @@ def test_a_tokens_bad_values_stay_with_the_rows_that_see_it(kernel, what):
     elif bad != bad:
         assert not bool(out[~keep].isfinite().any())
     assert pool.read_error() == 0
+
+
+@pytest.mark.parametrize("kernel", range(len(KERNELS)))
+def test_an_infinite_value_of_the_context_reaches_its_rows_whatever_its_weight(kernel):
+    """A context token whose weight is below fp32's range, with an infinite value."""
+    dtype, H, Hkv, dh, ctx, new = KERNELS[kernel]
+    rng = np.random.default_rng(70 + kernel)
+    pool, model, step, ref, parents, q = filled(rng, 16, H, Hkv, dh, ctx, new, dtype)
+    q = q.abs() + 1
+    pool.kv[:, :, 0].abs_()
+    clean = pool.attention(0, q, step).clone()
+    page = int(model.table[0, 0])
+    pool.kv[page, 0, 0, :, 5] = -200.0     # a score at least 400 below the others
+    low = pool.attention(0, q, step).clone()
+    pool.kv[page, 0, 1, :, 5, ::3] = float("inf")
+    out = pool.attention(0, q, step)
+    n = new[0]
+    assert not bool(out[:n, :, ::3].isfinite().any())
+    assert torch.equal(out[n:], clean[n:])
+    rest = [c for c in range(dh) if c % 3]
+    assert torch.equal(out[:n][..., rest], low[:n][..., rest])
 
 
 @pytest.mark.parametrize("kernel", range(len(KERNELS)))
