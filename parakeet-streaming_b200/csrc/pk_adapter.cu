@@ -6,13 +6,14 @@
 // Three launches:
 //  1. the plan (once per step: every projection of a model uses the same ids)
 //     sorts the rows by adapter, so that a 128-row tile meets few adapters, and
-//     lists each tile's (adapter, rows) pairs;
+//     lists each tile's (adapter, rows) pairs; rows of one tile stay in their order;
 //  2. S in bf16 and the rows' sorted copy, bound by reading and writing them;
 //  3. the product on the tcgen05 tensor cores, over the sorted rows; after the K
 //     blocks of x W^T each pair of the tile adds one K block S up[a]^T into the same
 //     accumulator, with the lanes of other rows disabled in the MMA: they get no zero
 //     products, so one adapter's weights, whatever they hold, do not reach another's
-//     rows.  The epilogue writes the rows back to their own places.
+//     rows.  The epilogue writes the rows back to their own places.  Rows that need no
+//     sorted copy are read before launch 2 is done.
 //
 // S is rounded to bf16 because the tensor cores take it so: off by 2^-8 of each of
 // its terms at most, as the bf16 result is of their sum.  Sums are
@@ -26,7 +27,70 @@ namespace {
 
 constexpr int kTileRows = 128;
 
+// An adapter and its rows of a tile.
+struct TilePair {
+    int adapter;
+    uint32_t rows[4];
+};
+__device__ __forceinline__ void store_pair(int32_t *at, int adapter, const uint32_t (&rows)[4]) {
+    reinterpret_cast<int4 *>(at)[0] = make_int4((int)rows[0], (int)rows[1], (int)rows[2], (int)rows[3]);
+    at[4] = adapter;
+}
+__device__ __forceinline__ void load_pair(const int32_t *at, TilePair &pr) {
+    const int4 m = *reinterpret_cast<const int4 *>(at);
+    pr.rows[0] = m.x;
+    pr.rows[1] = m.y;
+    pr.rows[2] = m.z;
+    pr.rows[3] = m.w;
+    pr.adapter = at[4];
+}
+__device__ __forceinline__ void load_pair(const int32_t *at, int &adapter) { adapter = at[4]; }
+
 // ------------------------------------------------------------------ the plan
+__device__ __forceinline__ uint32_t bits_below(int n) {
+    return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+}
+
+// Rows of one tile: they stay in their order, a thread a row.  The first row of each
+// adapter has its pair (1.8 us; 3.9 sorted as below).
+__global__ void __launch_bounds__(kTileRows)
+    adapter_plan_tile_kernel(const int32_t *ids, int rows, int adapters, AdapterLayout l,
+                             int32_t *plan, int32_t *error) {
+    __shared__ __align__(16) int s_id[kTileRows];
+    __shared__ int s_leads[4];
+    grid_dep_wait();
+    grid_dep_launch();
+    const int r = threadIdx.x, warp = r >> 5, lane = r & 31;
+    int a = r < rows ? ids[r] : -1;
+    if (a < -1 || a >= adapters) {
+        raise(error, PK_DEV_BAD_SLOT);
+        a = -1;
+    }
+    s_id[r] = a;
+    __syncthreads();
+    uint32_t in[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < kTileRows; j += 4) {
+        const int4 o = *reinterpret_cast<const int4 *>(s_id + j);
+        in[j / 32] |= (uint32_t)(o.x == a) << (j & 31) | (uint32_t)(o.y == a) << ((j + 1) & 31) |
+                      (uint32_t)(o.z == a) << ((j + 2) & 31) | (uint32_t)(o.w == a) << ((j + 3) & 31);
+    }
+    bool lead = a >= 0 && !(in[warp] & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) lead = lead && !in[w];
+    const unsigned leads = __ballot_sync(0xffffffffu, lead);
+    if (lane == 0) s_leads[warp] = __popc(leads);
+    __syncthreads();
+    int at = __popc(leads & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) at += s_leads[w];
+    if (lead) store_pair(plan + l.pairs + kPairWords * at, a, in);
+    plan[l.order + r] = min(r, rows);
+    if (r == 0) {
+        plan[l.tile_pair] = 0;
+        plan[l.tile_pair + 1] = s_leads[0] + s_leads[1] + s_leads[2] + s_leads[3];
+        plan[l.sorted] = 1;
+    }
+}
+
 __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, int rows,
                                                             int adapters, AdapterLayout l,
                                                             int32_t *plan, int32_t *error) {
@@ -124,8 +188,10 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
         for (int i = 0; i < mine; ++i) {
             const int t = t0 + i, lo = max(first - t * kTileRows, 0);
             const int hi = min(first + n - t * kTileRows, kTileRows);
-            pair[2 * (p0 + i)] = a;
-            pair[2 * (p0 + i) + 1] = lo | hi << 16;
+            uint32_t in[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) in[w] = bits_below(hi - w * 32) & ~bits_below(lo - w * 32);
+            store_pair(pair + (int64_t)kPairWords * (p0 + i), a, in);
             if (lo == 0) plan[l.tile_pair + t] = p0 + i;
         }
         __syncthreads();
@@ -183,7 +249,7 @@ template <int NT>   // 8-column tiles of S: rank <= 8 NT
 __global__ void __launch_bounds__(kShWarps * 32, NT <= 4 ? 3 : 2)
     adapter_shrink_kernel(const AdapterArgs p) {
     extern __shared__ float sh_part[];   // [warp][row][rank]
-    __shared__ int2 s_pair[kShRows];     // the group's pairs: adapter, first | end << 16
+    __shared__ int2 s_pair[kShRows];     // the group's pairs: adapter, bits of its rows
     __shared__ int s_n;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
     grid_dep_wait();
@@ -198,10 +264,12 @@ __global__ void __launch_bounds__(kShWarps * 32, NT <= 4 ? 3 : 2)
         int n = 0;
         for (int q = pair0; q < pair1; q += 32) {
             int2 pr = make_int2(0, 0);
-            if (q + lane < pair1) pr = reinterpret_cast<const int2 *>(plan + p.l.pairs)[q + lane];
-            const int lo = max((pr.y & 0xffff) - g0, 0), hi = min((pr.y >> 16) - g0, kShRows);
-            const unsigned has = __ballot_sync(0xffffffffu, lo < hi);
-            if (lo < hi) s_pair[n + __popc(has & ((1u << lane) - 1u))] = make_int2(pr.x, lo | hi << 16);
+            if (q + lane < pair1) {
+                const int32_t *at = plan + p.l.pairs + (int64_t)kPairWords * (q + lane);
+                pr = make_int2(at[4], (uint32_t)at[g0 >> 5] >> (g0 & 31) & 0xffffu);
+            }
+            const unsigned has = __ballot_sync(0xffffffffu, pr.y != 0);
+            if (pr.y) s_pair[n + __popc(has & ((1u << lane) - 1u))] = pr;
             n += __popc(has);
         }
         if (lane == 0) s_n = n;
@@ -224,7 +292,6 @@ __global__ void __launch_bounds__(kShWarps * 32, NT <= 4 ? 3 : 2)
     for (int j = first; j < max(n_pairs, 1); j += step) {
         const bool any = j < n_pairs;
         const int2 pr = any ? s_pair[j] : make_int2(0, 0);
-        const int lo = pr.y & 0xffff, hi = pr.y >> 16;
         const __nv_bfloat16 *down =
             static_cast<const __nv_bfloat16 *>(p.down) + ((int64_t)pr.x * r + fr) * p.K + fc;
         float acc[NT][4];
@@ -289,7 +356,7 @@ __global__ void __launch_bounds__(kShWarps * 32, NT <= 4 ? 3 : 2)
         __nv_bfloat16 *s = static_cast<__nv_bfloat16 *>(p.s) + m0 * r;
         for (int c = tid; c < kShRows * r; c += kShWarps * 32) {
             const int row = c / r;
-            if (row < lo || row >= hi) continue;
+            if (!(pr.y >> row & 1)) continue;
             float v = 0.f;
             for (int w = 0; w < warps; ++w) v += sh_part[w * kShRows * r + c];
             s[c] = __float2bfloat16_rn(v * scale);
@@ -323,33 +390,23 @@ __device__ __forceinline__ void umma_bf16_pair_lanes(uint32_t tmem_d, uint64_t a
         "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
         : "memory");
 }
-// Lanes outside a pair's rows, 32 a word.
-__device__ __forceinline__ void lanes_off(int range, uint32_t *off) {
-    const int lo = range & 0xffff, hi = range >> 16;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const int a = max(lo - w * 32, 0), b = min(hi - w * 32, 32);
-        const uint32_t below = b >= 32 ? 0xffffffffu : (b > 0 ? (1u << b) - 1u : 0u);
-        const uint32_t skip = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
-        off[w] = ~(below & ~skip);
-    }
-}
-
-// The pairs p0 .. p1 of a tile, read eight at a time: the first eight when the tile
-// begins, so that the reads' latency (one a pair took 0.4 us of a pair's turn) is
-// under the K blocks before them.
-struct TilePairs {
-    const int2 *pairs;
+// The pairs p0 .. p1 of a tile (T: int, the adapters alone, or TilePair), read eight
+// at a time: the first eight when the tile begins, so that the
+// reads' latency (one a pair took 0.4 us of a pair's turn) is under the K blocks before
+// them.
+template <typename T> struct TilePairs {
+    const int32_t *pairs;
     int p0, p1;
-    int2 ahead[8];
-    __device__ __forceinline__ TilePairs(const int2 *all, int from, int to)
+    T ahead[8];
+    __device__ __forceinline__ TilePairs(const int32_t *all, int from, int to)
         : pairs(all), p0(from), p1(to) {
         fetch();
     }
+    __device__ __forceinline__ bool any() const { return p0 < p1; }
     __device__ __forceinline__ void fetch() {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            ahead[i] = p0 + i < p1 ? pairs[p0 + i] : make_int2(0, 0);
+            if (p0 + i < p1) load_pair(pairs + (int64_t)kPairWords * (p0 + i), ahead[i]);
     }
     // fn(pair) for each, while it returns true
     template <typename F> __device__ __forceinline__ void each(F fn) {
@@ -400,7 +457,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     uint8_t *stage = sS + rblocks * kABytes + (warp & 3) * kStageBytes;
     const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order,
                   *sorted = p.plan + p.l.sorted;
-    const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
+    const int32_t *pairs = p.plan + p.l.pairs;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
@@ -446,13 +503,15 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 tma_load_2d(sB + kb * kBBytes, &tm.w, &full[kb], kb * kBK,
                             ((int)blockIdx.x / mtiles) * BN);
             }
-            grid_dep_wait();
+            // (the plan, and rows in their own order, are older than the kernel before, which
+            // has waited for them)
             const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
+            if (rows == &tm.xs) grid_dep_wait();
             int g = 0, with_s = 0;   // ring uses; tiles that had an S
             bool ok = true;
             for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
                 const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
-                TilePairs of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
+                TilePairs<int> of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     const int s = g % NS;
                     if (g >= pre) {
@@ -462,7 +521,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     }
                     tma_load_2d(sA + s * kABytes, rows, &full[s], kb * kBK, m0);
                 }
-                if (!ok || of_tile.p0 == of_tile.p1) continue;
+                if (!ok || !of_tile.any()) continue;
+                grid_dep_wait();   // S
                 // S once a tile (a copy for each pair made every CTA of a row tile ask for
                 // the same few lines again and again: 0.65 us a pair)
                 if (with_s >= 1 && !mbar_wait_bounded(&s_empty, (with_s - 1) & 1, kWaitLimitNs)) {
@@ -475,12 +535,12 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 mbar_arrive_expect_tx(&s_full, rblocks * kABytes);
                 for (int rb = 0; rb < rblocks; ++rb)
                     tma_load_2d(sS + rb * kABytes, &tm.s, &s_full, rb * kBK, m0);
-                of_tile.each([&](int2 pr) {
+                of_tile.each([&](int adapter) {
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         const int s = g % NS;
                         if (!(ok = free_stage(g))) return false;
                         mbar_arrive_expect_tx(&full[s], kBBytes);
-                        tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, pr.x);
+                        tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, adapter);
                     }
                     return true;
                 });
@@ -494,7 +554,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = idesc_bf16(kBM, BN);
-            grid_dep_wait();   // the plan
             int g = 0, t = 0, with_s = 0;
             auto done = [&](uint64_t *bar, uint32_t parity) {
                 if (mbar_wait_bounded(bar, parity, kWaitLimitNs)) return true;
@@ -512,7 +571,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
-                TilePairs of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
+                TilePairs<TilePair> of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     const int s = g % NS;
                     if (!ready(s)) break;
@@ -524,11 +583,10 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                                   (kb | kk) != 0);
                     umma_commit(&empty[s]);
                 }
-                const bool any = of_tile.p0 < of_tile.p1;
+                const bool any = of_tile.any();
                 if (any && !failed) done(&s_full, with_s++ & 1);
-                of_tile.each([&](int2 pr) {
-                    uint32_t off[4];
-                    lanes_off(pr.y, off);
+                of_tile.each([&](const TilePair &pr) {
+                    const uint32_t off[4] = {~pr.rows[0], ~pr.rows[1], ~pr.rows[2], ~pr.rows[3]};
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         const int s = g % NS;
                         if (failed || !ready(s)) return false;
@@ -597,6 +655,255 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     }
 }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
+// Few tiles: a cluster for each, its CTAs with a part of K each and every c-th pair of the
+// tile.  A tile is a chain of K blocks, some 0.2 us each whatever the depth of the ring,
+// and most SMs have no tile: 4 rows, K 4096, N 512, rank 8 took 23 us on a CTA a tile and
+// take 8.3 on eight; 16 rows, K and N 4096, 16 adapters: 29 and 21 on two.  The parts meet
+// in shared memory: each CTA leaves its sums there, and all of them add up and write a
+// share of the tile, in the order of the CTAs.
+constexpr int kSplitBN = 64, kSplitStages = 6, kSplitRow = kSplitBN + 4;   // floats
+template <int EPI>
+__global__ void __launch_bounds__(kAdThreads, 1)
+    adapter_gemm_split_kernel(const __grid_constant__ AdapterMaps tm, const AdapterArgs p) {
+    constexpr int BN = kSplitBN, NS = kSplitStages, kBBytes = BN * kBK * 2;
+    static_assert(kTileRows * kSplitRow * 4 <= NS * kABytes, "the sums take the ring's place");
+    extern __shared__ uint8_t gemm_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sA = smem, *sB = smem + NS * kABytes, *sS = sB + NS * kBBytes;
+    float *sums = reinterpret_cast<float *>(sA);   // [row][kSplitRow]
+    __shared__ __align__(8) uint64_t full[NS], empty[NS], tmem_full, s_full;
+    __shared__ uint32_t tmem_base;
+    __shared__ __align__(16) int32_t s_pairs[kTileRows * kPairWords];   // this CTA's
+    __shared__ volatile int failed;
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int c = gridDim.x, part = (int)cluster_ctarank(), tile = blockIdx.y;
+    const int mtiles = (p.M + kBM - 1) / kBM, mt = tile % mtiles;
+    const int m0 = mt * kBM, n0 = tile / mtiles * BN, live = min(p.M - m0, kBM);
+    const int nk = p.K / kBK, kb0 = (int)((int64_t)nk * part / c);
+    const int n_kb = (int)((int64_t)nk * (part + 1) / c) - kb0;
+    const int rblocks = (p.rank + kBK - 1) / kBK;
+    const uint32_t a_bytes = p.box_rows * kBK * 2;
+    const int pre = min(n_kb, NS);
+    const int32_t *tile_pair = p.plan + p.l.tile_pair, *pairs = p.plan + p.l.pairs,
+                  *order = p.plan + p.l.order, *sorted = p.plan + p.l.sorted;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&tmem_full, 1);
+        mbar_init(&s_full, 1);
+        failed = 0;
+        fence_mbar_init();
+        // W first: it does not depend on the kernel before
+        for (int g = 0; g < pre; ++g) {
+            mbar_arrive_expect_tx(&full[g], a_bytes + kBBytes);
+            tma_load_2d(sB + g * kBBytes, &tm.w, &full[g], (kb0 + g) * kBK, n0);
+        }
+        prefetch_tmap(&tm.up);
+        prefetch_tmap(&tm.s);
+    }
+    __syncwarp();
+    if (warp == 0) {
+        tmem_alloc(&tmem_base, BN);
+        tmem_relinquish();
+    }
+    const int pair0 = tile_pair[mt], n_pairs = (tile_pair[mt + 1] - pair0 - part + c - 1) / c;
+    const bool in_order = *sorted;
+    for (int i = threadIdx.x; i < n_pairs * 2; i += kAdThreads)
+        reinterpret_cast<int4 *>(s_pairs)[i] = reinterpret_cast<const int4 *>(
+            pairs + (int64_t)kPairWords * (pair0 + part + (i >> 1) * c))[i & 1];
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    // one lane's answer is the warp's: a lane that waits finds what another has found
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (!failed && !mbar_wait_bounded(bar, parity, kWaitLimitNs)) {
+            raise(p.error, PK_DEV_TIMEOUT);
+            failed = 1;
+        }
+        return !failed;
+    };
+    // ring stage and its phase, a step a use
+    int s = 0;
+    uint32_t phase = 0;
+    auto next = [&]() {
+        if (++s == NS) {
+            s = 0;
+            phase ^= 1;
+        }
+    };
+    // Producer and MMA warp: the whole warp walks along, so that indexes and descriptors
+    // are uniform (one lane's walk took 270 cycles a stage beside its MMAs).
+    if (warp == 0) {
+        const bool one = elect_one();
+        // rows in their own order are older than the kernel before, which has waited for
+        // them; their sorted copy is its work
+        const CUtensorMap *rows = in_order ? &tm.x : &tm.xs;
+        if (!in_order) grid_dep_wait();
+        int used = 0;   // stages requested
+        bool ok = true;
+        for (int g = 0; g < n_kb; ++g, ++used) {
+            if (g >= pre && !(ok = __all_sync(0xffffffffu, wait(&empty[s], phase ^ 1)))) break;
+            if (one) {
+                if (g >= pre) {
+                    mbar_arrive_expect_tx(&full[s], a_bytes + kBBytes);
+                    tma_load_2d(sB + s * kBBytes, &tm.w, &full[s], (kb0 + g) * kBK, n0);
+                }
+                tma_load_2d(sA + s * kABytes, rows, &full[s], (kb0 + g) * kBK, m0);
+            }
+            __syncwarp();
+            next();
+        }
+        if (ok && n_pairs > 0) {
+            grid_dep_wait();   // S
+            if (one) {
+                mbar_arrive_expect_tx(&s_full, rblocks * a_bytes);
+                for (int rb = 0; rb < rblocks; ++rb)
+                    tma_load_2d(sS + rb * kABytes, &tm.s, &s_full, rb * kBK, m0);
+            }
+            for (int i = 0; i < n_pairs && ok; ++i) {
+                const int adapter = s_pairs[i * kPairWords + 4];
+                for (int rb = 0; rb < rblocks; ++rb, ++used) {
+                    if (used >= NS && !(ok = __all_sync(0xffffffffu, wait(&empty[s], phase ^ 1)))) break;
+                    if (one) {
+                        mbar_arrive_expect_tx(&full[s], kBBytes);
+                        tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, adapter);
+                    }
+                    __syncwarp();
+                    next();
+                }
+            }
+            if (!ok) mbar_wait_bounded(&s_full, 0, kWaitLimitNs);
+        }
+        if (!ok)   // leave no copy in flight: the last NS requests
+            for (int i = 0; i < min(used, NS); ++i) {
+                s = s == 0 ? NS - 1 : s - 1;
+                if (s == NS - 1) phase ^= 1;
+                mbar_wait_bounded(&full[s], phase, kWaitLimitNs);
+            }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = idesc_bf16(kBM, BN);
+        const uint64_t a_desc = sw128_desc(smem_u32(sA)), b_desc = sw128_desc(smem_u32(sB)),
+                       s_desc = sw128_desc(smem_u32(sS));
+        const bool one = elect_one();
+        bool ok = true;
+        for (int g = 0; g < n_kb; ++g) {
+            if (!(ok = __all_sync(0xffffffffu, wait(&full[s], phase)))) break;
+            tc_fence_after();
+            if (one) {
+                const uint64_t a0 = a_desc + s * (kABytes >> 4), b0 = b_desc + s * (kBBytes >> 4);
+#pragma unroll
+                for (int kk = 0; kk < kBK / 16; ++kk)
+                    umma_bf16(tmem, a0 + kk * 2, b0 + kk * 2, idesc, (g | kk) != 0);
+                umma_commit(&empty[s]);
+            }
+            __syncwarp();
+            next();
+        }
+        if (ok && n_pairs > 0) {
+            ok = __all_sync(0xffffffffu, wait(&s_full, 0));
+            for (int i = 0; i < n_pairs && ok; ++i) {
+                const int4 in = reinterpret_cast<const int4 *>(s_pairs)[2 * i];
+                const uint32_t off[4] = {~(uint32_t)in.x, ~(uint32_t)in.y, ~(uint32_t)in.z, ~(uint32_t)in.w};
+                for (int rb = 0; rb < rblocks; ++rb) {
+                    if (!(ok = __all_sync(0xffffffffu, wait(&full[s], phase)))) break;
+                    tc_fence_after();
+                    if (one) {
+                        const uint64_t a0 = s_desc + rb * (kABytes >> 4), b0 = b_desc + s * (kBBytes >> 4);
+                        const int steps = min(kBK, p.rank - rb * kBK);
+                        for (int kk = 0; kk * 16 < steps; ++kk)
+                            umma_bf16_lanes(tmem, a0 + kk * 2, b0 + kk * 2, idesc, off);
+                        umma_commit(&empty[s]);
+                    }
+                    __syncwarp();
+                    next();
+                }
+            }
+        }
+        if (one) umma_commit(&tmem_full);
+    } else {
+        // warps 2..5: this CTA's sums, a row a lane
+        grid_dep_wait();
+        const int row = (warp & 3) * 32 + lane;
+        __all_sync(0xffffffffu, wait(&tmem_full, 0));
+        tc_fence_after();
+        if (row - lane < live) {
+            float v[64];
+            const uint32_t at = tmem + ((uint32_t)(row - lane) << 16);
+            tmem_ld32(at, *reinterpret_cast<float(*)[32]>(v));
+            tmem_ld32(at + 32, *reinterpret_cast<float(*)[32]>(v + 32));
+            if (!failed && row < live)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    *reinterpret_cast<float4 *>(sums + row * kSplitRow + 4 * i) =
+                        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+        tc_fence_before();
+    }
+    grid_dep_launch();
+    cluster_sync_all();   // every part's sums are there
+    for (int i = part * kAdThreads + (int)threadIdx.x; i < live * (BN / 8); i += c * kAdThreads) {
+        const int row = i / (BN / 8), col = i % (BN / 8) * 8, m = order[m0 + row];
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const uint32_t mine = smem_u32(sums + row * kSplitRow + col);
+        for (int r = 0; r < c; ++r) {
+            const uint32_t at = mapa_rank(mine, r);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4 x;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                             : "r"(at + h * 16)
+                             : "memory");
+                v[4 * h] += x.x;
+                v[4 * h + 1] += x.y;
+                v[4 * h + 2] += x.z;
+                v[4 * h + 3] += x.w;
+            }
+        }
+        float f[8];
+        if (is_residual(EPI))
+            unpack16(*reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.R) +
+                                                      (int64_t)m * p.ldr + n0 + col),
+                     f, static_cast<const __nv_bfloat16 *>(nullptr));
+        if (EPI == PK_GEMM_BIAS)
+            unpack16(*reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.bias) + n0 + col),
+                     f, static_cast<const __nv_bfloat16 *>(nullptr));
+        uint4 o;
+        __nv_bfloat162 *h = reinterpret_cast<__nv_bfloat162 *>(&o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (EPI == PK_GEMM_SILU) v[e] = __fdividef(v[e], 1.f + __expf(-v[e]));
+            if (is_residual(EPI)) v[e] = f[e] + p.alpha * v[e];
+            if (EPI == PK_GEMM_RESIDUAL_RELU) v[e] = fmaxf(v[e], 0.f);
+            if (EPI == PK_GEMM_BIAS) v[e] += f[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+        *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.C) + (int64_t)m * p.ldc + n0 + col) = o;
+    }
+    cluster_sync_all();   // and no part is read any more
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, BN);
+    }
+}
+
 // 3-D tile load into this CTA's shared memory, completion on an mbarrier of either
 // CTA of the pair
 __device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *map, uint32_t bar,
@@ -635,7 +942,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     uint8_t *stage = sS + rblocks * kABytes + (warp & 3) * kStageBytes;
     const int32_t *tile_pair = p.plan + p.l.tile_pair, *order = p.plan + p.l.order,
                   *sorted = p.plan + p.l.sorted;
-    const int2 *pairs = reinterpret_cast<const int2 *>(p.plan + p.l.pairs);
+    const int32_t *pairs = p.plan + p.l.pairs;
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             mbar_init(&full[s], 1);
@@ -672,15 +979,17 @@ __global__ void __launch_bounds__(kAdThreads, 1)
 
     if (warp == 0) {
         if (lane == 0) {
-            grid_dep_wait();
+            // (the plan, and rows in their own order, are older than the kernel before, which
+            // has waited for them)
             const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
+            if (rows == &tm.xs) grid_dep_wait();
             int g = 0, with_s = 0;   // ring uses; tiles that had an S
             bool ok = true;
             const uint32_t sb = mapa_rank(smem_u32(&s_full), 0);
             for (int tile = pair; tile < tiles && ok; tile += npairs) {
                 const int mt = tile % mtiles, m0 = mt * 2 * kBM + (int)rank * kBM;
                 const int n0 = (tile / mtiles) * BN + (int)rank * kHalfB;
-                TilePairs of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
+                TilePairs<int> of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     if (!(ok = free_stage(g))) break;
                     const int s = g % NS;
@@ -689,7 +998,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     tma_load_2d_pair(sB + s * kBBytes, &tm.w, fb, kb * kBK, n0);
                     tma_load_2d_pair(sA + s * kABytes, rows, fb, kb * kBK, m0);
                 }
-                if (!ok || of_tile.p0 == of_tile.p1) continue;
+                if (!ok || !of_tile.any()) continue;
+                grid_dep_wait();   // S
                 if (with_s >= 1 && !mbar_wait_bounded(&s_empty, (with_s - 1) & 1, kWaitLimitNs)) {
                     raise(p.error, PK_DEV_TIMEOUT);
                     failed = 1;
@@ -700,13 +1010,13 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 if (leader) mbar_arrive_expect_tx(&s_full, 2 * rblocks * kABytes);
                 for (int rb = 0; rb < rblocks; ++rb)
                     tma_load_2d_pair(sS + rb * kABytes, &tm.s, sb, rb * kBK, m0);
-                of_tile.each([&](int2 pr) {
+                of_tile.each([&](int adapter) {
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         if (!(ok = free_stage(g))) return false;
                         const int s = g % NS;
                         const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
                         if (leader) mbar_arrive_expect_tx(&full[s], 2 * kBBytes);
-                        tma_load_3d_pair(sB + s * kBBytes, &tm.up, fb, rb * kBK, n0, pr.x);
+                        tma_load_3d_pair(sB + s * kBBytes, &tm.up, fb, rb * kBK, n0, adapter);
                     }
                     return true;
                 });
@@ -720,7 +1030,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     } else if (warp == 1) {
         if (lane == 0 && leader) {
             constexpr uint32_t idesc = idesc_bf16(2 * kBM, BN);
-            grid_dep_wait();
             int g = 0, t = 0, with_s = 0;
             auto done = [&](uint64_t *bar, uint32_t parity) {
                 if (mbar_wait_cluster_bounded(bar, parity, kWaitLimitNs)) return true;
@@ -740,7 +1049,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
                 const int border = tile_pair[min(2 * mt + 1, halves)];   // of the two halves
-                TilePairs of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
+                TilePairs<TilePair> of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
                 for (int kb = 0; kb < nk; ++kb, ++g) {
                     const int s = g % NS;
                     if (!ready(s)) break;
@@ -753,13 +1062,16 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                     umma_commit_pair(&empty[s]);
                 }
                 int pr_at = of_tile.p0;
-                const bool any = of_tile.p0 < of_tile.p1;
+                const bool any = of_tile.any();
                 if (any && !failed) done(&s_full, with_s++ & 1);
-                of_tile.each([&](int2 pr) {
+                of_tile.each([&](const TilePair &pr) {
                     const bool odd = pr_at++ >= border;   // the second half's
                     uint32_t off[8];
-                    lanes_off(odd ? 0 : pr.y, off);
-                    lanes_off(odd ? pr.y : 0, off + 4);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        off[w] = odd ? ~0u : ~pr.rows[w];
+                        off[w + 4] = odd ? ~pr.rows[w] : ~0u;
+                    }
                     for (int rb = 0; rb < rblocks; ++rb, ++g) {
                         const int s = g % NS;
                         if (failed || !ready(s)) return false;
@@ -876,8 +1188,33 @@ int launch_product_t(const AdapterArgs &p, const AdapterMaps &tm, cudaStream_t s
     return cuda_status(cudaLaunchKernelEx(&cfg, k, tm, p), "adapter_gemm_kernel");
 }
 
+template <int EPI>
+int launch_split_t(const AdapterArgs &p, const AdapterMaps &tm, int c, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    auto k = adapter_gemm_split_kernel<EPI>;
+    constexpr size_t ring = (size_t)kSplitStages * (kABytes + kSplitBN * kBK * 2) + 1024;
+    cudaError_t e = allow_smem(k, ring + 2 * kABytes, done);
+    if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(adapter gemm)");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c, (p.M + kBM - 1) / kBM * (p.N / kSplitBN));
+    cfg.blockDim = dim3(kAdThreads);
+    cfg.dynamicSmemBytes = ring + (p.rank + kBK - 1) / kBK * kABytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = c;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
+    return cuda_status(cudaLaunchKernelEx(&cfg, k, tm, p), "adapter_gemm_split_kernel");
+}
+
+// split: CTAs a tile (of 64 columns), 0: the other kernels
 template <int BN, int NS, bool kPair = false>
-int launch_product(const AdapterArgs &p, cudaStream_t s) {
+int launch_product(const AdapterArgs &p, cudaStream_t s, int split = 0) {
     AdapterMaps tm;
     constexpr uint32_t box_n = kPair ? BN / 2 : BN;
     const uint64_t padded = (uint64_t)((p.M + kBM - 1) / kBM * kBM), rb = (uint64_t)p.rank * 2;
@@ -887,13 +1224,20 @@ int launch_product(const AdapterArgs &p, cudaStream_t s) {
     const uint64_t sd[2] = {(uint64_t)p.rank, padded}, ss[1] = {rb};
     const uint64_t ud[3] = {(uint64_t)p.rank, (uint64_t)p.N, (uint64_t)p.adapters};
     const uint64_t us[2] = {rb, rb * p.N};
-    const uint32_t abox[2] = {kBK, kBM}, wbox[2] = {kBK, box_n}, ubox[3] = {kBK, box_n, 1};
+    const uint32_t abox[2] = {kBK, (uint32_t)p.box_rows}, wbox[2] = {kBK, box_n}, ubox[3] = {kBK, box_n, 1};
     int st = encode_tmap(&tm.x, PK_DTYPE_BF16, p.x, 2, xd, xs, abox);
     if (st == PK_OK) st = encode_tmap(&tm.xs, PK_DTYPE_BF16, p.xs, 2, pd, ps, abox);
     if (st == PK_OK) st = encode_tmap(&tm.w, PK_DTYPE_BF16, p.W, 2, wd, ws, wbox);
     if (st == PK_OK) st = encode_tmap(&tm.s, PK_DTYPE_BF16, p.s, 2, sd, ss, abox);
     if (st == PK_OK) st = encode_tmap(&tm.up, PK_DTYPE_BF16, p.up, 3, ud, us, ubox);
     if (st != PK_OK) return st;
+    if (split) switch (p.epilogue) {
+            case PK_GEMM_SILU: return launch_split_t<PK_GEMM_SILU>(p, tm, split, s);
+            case PK_GEMM_RESIDUAL: return launch_split_t<PK_GEMM_RESIDUAL>(p, tm, split, s);
+            case PK_GEMM_RESIDUAL_RELU: return launch_split_t<PK_GEMM_RESIDUAL_RELU>(p, tm, split, s);
+            case PK_GEMM_BIAS: return launch_split_t<PK_GEMM_BIAS>(p, tm, split, s);
+            default: return launch_split_t<PK_GEMM_STORE>(p, tm, split, s);
+        }
     switch (p.epilogue) {
         case PK_GEMM_SILU: return launch_product_t<BN, NS, kPair, PK_GEMM_SILU>(p, tm, s);
         case PK_GEMM_RESIDUAL: return launch_product_t<BN, NS, kPair, PK_GEMM_RESIDUAL>(p, tm, s);
@@ -908,6 +1252,10 @@ int launch_product(const AdapterArgs &p, cudaStream_t s) {
 
 int launch_adapter_plan(const int32_t *ids, int rows, int adapters, int32_t *plan, int32_t *error,
                         cudaStream_t s) {
+    if (rows <= kTileRows)
+        return cuda_status(launch_pdl(adapter_plan_tile_kernel, dim3(1), dim3(kTileRows), 0, s, ids, rows,
+                                      adapters, adapter_layout(rows, adapters), plan, error),
+                           "adapter_plan_kernel");
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(adapter_plan_kernel, (PK_ADAPTER_MAX + 1) * 4, done);
     if (e == cudaSuccess)
@@ -919,6 +1267,7 @@ int launch_adapter_plan(const int32_t *ids, int rows, int adapters, int32_t *pla
 int launch_adapter_gemm(const AdapterArgs &a, cudaStream_t s) {
     AdapterArgs p = a;
     p.l = adapter_layout(p.M, p.adapters);
+    p.box_rows = kBM;
     cudaError_t e = p.rank <= 8    ? launch_shrink<1>(p, s)
                     : p.rank <= 16 ? launch_shrink<2>(p, s)
                     : p.rank <= 32 ? launch_shrink<4>(p, s)
@@ -937,6 +1286,21 @@ int launch_adapter_gemm(const AdapterArgs &a, cudaStream_t s) {
         return launch_product<256, 5, true>(p, s);
     if (p.N % 256 == 0 && mtiles * (p.N / 256) >= 2 * sms) return launch_product<256, 3>(p, s);
     if (p.N % 128 == 0 && mtiles * (p.N / 128) >= sms) return launch_product<128, 5>(p, s);
+    // two CTAs a tile while there are SMs for them, up to eight on half of the SMs: more
+    // clusters of four or eight do not all find room in the GPCs at once (16 tiles of
+    // K = 2048 on 1, 2, 4, 8 CTAs: 13.0, 9.2, 7.5, 13.0 us; 32: 13.9, 10.8, 10.4 us, with
+    // an adapter 12.8 on two and 16.3 on four)
+    const int tiles = mtiles * (p.N / kSplitBN), nk = p.K / kBK;
+    const int split = 8 * tiles <= sms / 2 && nk >= 8   ? 8
+                      : 4 * tiles <= sms / 2 && nk >= 4 ? 4
+                      : 2 * tiles <= sms && nk >= 2     ? 2
+                                                        : 1;
+    if (split > 1) {
+        // one row tile: no more of its rows than there are (8 a swizzle atom); the
+        // others' sums are never read
+        p.box_rows = mtiles > 1 ? kBM : (p.M + 7) / 8 * 8;
+        return launch_product<64, 6>(p, s, split);
+    }
     return launch_product<64, 6>(p, s);
 }
 

@@ -321,6 +321,7 @@ int64_t tree_attn_workspace(const pk_token_kv *kv, int batch, int rows);
 int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStream_t s);
 
 // pk_adapter.cu: plan block, int32 words
+constexpr int kPairWords = 8;
 struct AdapterLayout {
     int64_t tile_pair, order, sorted, pairs, words;
 };
@@ -330,8 +331,8 @@ inline AdapterLayout adapter_layout(int rows, int adapters) {
     l.order = 0;                         // sorted row -> row; `rows` past the last
     l.tile_pair = l.order + tiles * 128; // first pair of each tile
     l.sorted = l.tile_pair + tiles + 1;  // 1: the rows' own order is sorted
-    l.pairs = (l.sorted + 1 + 1) / 2 * 2;   // adapter, first | end << 16 row in the tile
-    l.words = l.pairs + 2 * (tiles + (adapters < rows ? adapters : rows));
+    l.pairs = (l.sorted + 1 + 3) / 4 * 4;   // adapter, 128 bits: its rows of the tile
+    l.words = l.pairs + kPairWords * (tiles + (adapters < rows ? adapters : rows));
     return l;
 }
 struct AdapterArgs {
@@ -339,6 +340,7 @@ struct AdapterArgs {
     int64_t ldx, ldw, ldc, ldr;
     void *C, *s, *xs;   // output; S and the rows' copy, sorted and padded to 128
     int M, N, K, epilogue, rank, adapters;
+    int box_rows;       // rows of a TMA copy of x, its sorted copy and S
     float alpha;
     const float *scale;
     const int32_t *plan;

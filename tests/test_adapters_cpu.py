@@ -41,13 +41,13 @@ def test_plan_refuses():
 
 def test_sizes():
     """The plan holds the sorted rows padded to 128-row tiles, a flag and, at most, a pair
-    for each adapter in use and one more for each tile."""
+    (of 8 words) for each adapter in use and one more for each tile."""
     lib = _lib.lib()
     for rows, n in [(1, 1), (128, 5), (129, 8192), (6720, 64)]:
         tiles = -(-rows // 128)
         words = lib.pk_adapter_plan_words(rows, n)
-        need = tiles * 128 + tiles + 2 + 2 * (tiles + min(rows, n))
-        assert need <= words <= need + 1
+        need = tiles * 128 + tiles + 2 + 8 * (tiles + min(rows, n))
+        assert need <= words <= need + 3
         assert lib.pk_adapter_workspace(rows, 64, 16) == tiles * 128 * (64 + 16) * 2
     assert lib.pk_adapter_plan_words(-1, 1) == -1 and lib.pk_adapter_plan_words(1, 0) == -1
     assert lib.pk_adapter_workspace(1, 64, 0) == -1
