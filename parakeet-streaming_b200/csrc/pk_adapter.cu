@@ -420,6 +420,16 @@ template <typename T> struct TilePairs {
     }
 };
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
 // A warp's rows of C and R in sorted order: the eight that this lane's pieces touch.
 struct SortedRows {
     int row[8];
@@ -483,127 +493,142 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base;
-    // wait until stage g of the ring is free; false when a wait of the CTA gave up
-    auto free_stage = [&](int g) {
-        const int u = g / NS;
-        if (u >= 1 && !failed && !mbar_wait_bounded(&empty[g % NS], (u - 1) & 1, kWaitLimitNs)) {
+    // (a lane that waits finds what another has found: the warp's answer is one)
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (!failed && !mbar_wait_bounded(bar, parity, kWaitLimitNs)) {
             raise(p.error, PK_DEV_TIMEOUT);
             failed = 1;
         }
         return !failed;
     };
-
+    // ring stage and its phase, a step a use
+    int s = 0;
+    uint32_t phase = 0;
+    auto next = [&]() {
+        if (++s == NS) {
+            s = 0;
+            phase ^= 1;
+        }
+    };
+    // Producer and MMA warp: the whole warp walks along, so that indexes and descriptors
+    // are uniform (one lane's walk took 270 cycles a stage beside its MMAs).
     if (warp == 0) {
-        if (lane == 0) {
-            // producer.  The weights of the first stages do not depend on the kernel
-            // before: they are requested ahead of the wait for it.
-            const int pre = (int)blockIdx.x < tiles ? (nk < NS ? nk : NS) : 0;
+        const bool one = elect_one();
+        // The weights of the first stages do not depend on the kernel before: they are
+        // requested ahead of the wait for it.
+        const int pre = (int)blockIdx.x < tiles ? (nk < NS ? nk : NS) : 0;
+        if (one)
             for (int kb = 0; kb < pre; ++kb) {
                 mbar_arrive_expect_tx(&full[kb], kABytes + kBBytes);
                 tma_load_2d(sB + kb * kBBytes, &tm.w, &full[kb], kb * kBK,
                             ((int)blockIdx.x / mtiles) * BN);
             }
-            // (the plan, and rows in their own order, are older than the kernel before, which
-            // has waited for them)
-            const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
-            if (rows == &tm.xs) grid_dep_wait();
-            int g = 0, with_s = 0;   // ring uses; tiles that had an S
-            bool ok = true;
-            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-                const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
-                TilePairs<int> of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
-                for (int kb = 0; kb < nk; ++kb, ++g) {
-                    const int s = g % NS;
-                    if (g >= pre) {
-                        if (!(ok = free_stage(g))) break;
+        // (the plan, and rows in their own order, are older than the kernel before, which
+        // has waited for them)
+        const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
+        if (rows == &tm.xs) grid_dep_wait();
+        int used = 0, with_s = 0;   // stages requested; tiles that had an S
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            const int mt = tile % mtiles, m0 = mt * kBM, n0 = (tile / mtiles) * BN;
+            TilePairs<int> of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
+            for (int kb = 0; kb < nk; ++kb, ++used) {
+                if (used >= NS && !(ok = __all_sync(0xffffffffu, wait(&empty[s], phase ^ 1)))) break;
+                if (one) {
+                    if (used >= pre) {
                         mbar_arrive_expect_tx(&full[s], kABytes + kBBytes);
                         tma_load_2d(sB + s * kBBytes, &tm.w, &full[s], kb * kBK, n0);
                     }
                     tma_load_2d(sA + s * kABytes, rows, &full[s], kb * kBK, m0);
                 }
-                if (!ok || !of_tile.any()) continue;
-                grid_dep_wait();   // S
-                // S once a tile (a copy for each pair made every CTA of a row tile ask for
-                // the same few lines again and again: 0.65 us a pair)
-                if (with_s >= 1 && !mbar_wait_bounded(&s_empty, (with_s - 1) & 1, kWaitLimitNs)) {
-                    raise(p.error, PK_DEV_TIMEOUT);
-                    failed = 1;
-                    ok = false;
-                    break;
-                }
-                ++with_s;
+                __syncwarp();
+                next();
+            }
+            if (!ok || !of_tile.any()) continue;
+            grid_dep_wait();   // S
+            // S once a tile (a copy for each pair made every CTA of a row tile ask for
+            // the same few lines again and again: 0.65 us a pair)
+            if (with_s >= 1 && !(ok = __all_sync(0xffffffffu, wait(&s_empty, (with_s - 1) & 1)))) break;
+            ++with_s;
+            if (one) {
                 mbar_arrive_expect_tx(&s_full, rblocks * kABytes);
                 for (int rb = 0; rb < rblocks; ++rb)
                     tma_load_2d(sS + rb * kABytes, &tm.s, &s_full, rb * kBK, m0);
-                of_tile.each([&](int adapter) {
-                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
-                        const int s = g % NS;
-                        if (!(ok = free_stage(g))) return false;
+            }
+            of_tile.each([&](int adapter) {
+                for (int rb = 0; rb < rblocks; ++rb, ++used) {
+                    if (used >= NS && !(ok = __all_sync(0xffffffffu, wait(&empty[s], phase ^ 1))))
+                        return false;
+                    if (one) {
                         mbar_arrive_expect_tx(&full[s], kBBytes);
                         tma_load_3d(sB + s * kBBytes, &tm.up, &full[s], rb * kBK, n0, adapter);
                     }
-                    return true;
-                });
+                    __syncwarp();
+                    next();
+                }
+                return true;
+            });
+        }
+        if (!ok) {   // leave no copy in flight: the last NS stages' and the last S
+            for (int i = 0; i < min(used, NS); ++i) {
+                s = s == 0 ? NS - 1 : s - 1;
+                if (s == NS - 1) phase ^= 1;
+                mbar_wait_bounded(&full[s], phase, kWaitLimitNs);
             }
-            if (!ok) {   // leave no copy in flight
-                for (int s = 0; s < NS; ++s)
-                    if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
-                if (with_s) mbar_wait_bounded(&s_full, (with_s - 1) & 1, kWaitLimitNs);
-            }
+            if (with_s) mbar_wait_bounded(&s_full, (with_s - 1) & 1, kWaitLimitNs);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_bf16(kBM, BN);
-            int g = 0, t = 0, with_s = 0;
-            auto done = [&](uint64_t *bar, uint32_t parity) {
-                if (mbar_wait_bounded(bar, parity, kWaitLimitNs)) return true;
-                raise(p.error, PK_DEV_TIMEOUT);
-                failed = 1;
-                return false;
-            };
-            auto ready = [&](int s) { return done(&full[s], (g / NS) & 1); };
-            for (int tile = blockIdx.x; tile < tiles && !failed; tile += gridDim.x, ++t) {
-                const int acc = t & 1, use = t >> 1, mt = tile % mtiles;
-                if (use >= 1 && !mbar_wait_bounded(&tmem_empty[acc], (use - 1) & 1, kWaitLimitNs)) {
-                    raise(p.error, PK_DEV_TIMEOUT);
-                    failed = 1;
-                    break;
-                }
+        constexpr uint32_t idesc = idesc_bf16(kBM, BN);
+        const bool one = elect_one();
+        const uint64_t a_desc = sw128_desc(smem_u32(sA)), b_desc = sw128_desc(smem_u32(sB)),
+                       s_desc = sw128_desc(smem_u32(sS));
+        int t = 0, with_s = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++t) {
+            const int acc = t & 1, use = t >> 1, mt = tile % mtiles;
+            if (use >= 1 && !(ok = __all_sync(0xffffffffu, wait(&tmem_empty[acc], (use - 1) & 1)))) break;
+            tc_fence_after();
+            const uint32_t d = tmem + acc * BN;
+            TilePairs<TilePair> of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
+            for (int kb = 0; kb < nk; ++kb) {
+                if (!(ok = __all_sync(0xffffffffu, wait(&full[s], phase)))) break;
                 tc_fence_after();
-                const uint32_t d = tmem + acc * BN;
-                TilePairs<TilePair> of_tile(pairs, tile_pair[mt], tile_pair[mt + 1]);
-                for (int kb = 0; kb < nk; ++kb, ++g) {
-                    const int s = g % NS;
-                    if (!ready(s)) break;
-                    tc_fence_after();
-                    const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
+                if (one) {
+                    const uint64_t a0 = a_desc + s * (kABytes >> 4), b0 = b_desc + s * (kBBytes >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kBK / 16; ++kk)
-                        umma_bf16(d, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32), idesc,
-                                  (kb | kk) != 0);
+                        umma_bf16(d, a0 + kk * 2, b0 + kk * 2, idesc, (kb | kk) != 0);
                     umma_commit(&empty[s]);
                 }
-                const bool any = of_tile.any();
-                if (any && !failed) done(&s_full, with_s++ & 1);
-                of_tile.each([&](const TilePair &pr) {
-                    const uint32_t off[4] = {~pr.rows[0], ~pr.rows[1], ~pr.rows[2], ~pr.rows[3]};
-                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
-                        const int s = g % NS;
-                        if (failed || !ready(s)) return false;
-                        tc_fence_after();
-                        const uint32_t a0 = smem_u32(sS + rb * kABytes),
-                                       b0 = smem_u32(sB + s * kBBytes);
-                        const int steps = min(kBK, p.rank - rb * kBK);
-                        for (int kk = 0; kk * 16 < steps; ++kk)
-                            umma_bf16_lanes(d, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32),
-                                            idesc, off);
-                        umma_commit(&empty[s]);
-                    }
-                    return true;
-                });
-                if (any) umma_commit(&s_empty);
-                umma_commit(&tmem_full[acc]);
+                __syncwarp();
+                next();
             }
+            if (ok && of_tile.any()) {
+                ok = __all_sync(0xffffffffu, wait(&s_full, with_s++ & 1));
+                if (ok)
+                    of_tile.each([&](const TilePair &pr) {
+                        const uint32_t off[4] = {~pr.rows[0], ~pr.rows[1], ~pr.rows[2], ~pr.rows[3]};
+                        for (int rb = 0; rb < rblocks; ++rb) {
+                            if (!(ok = __all_sync(0xffffffffu, wait(&full[s], phase)))) return false;
+                            tc_fence_after();
+                            if (one) {
+                                const uint64_t a0 = s_desc + rb * (kABytes >> 4),
+                                               b0 = b_desc + s * (kBBytes >> 4);
+                                const int steps = min(kBK, p.rank - rb * kBK);
+                                for (int kk = 0; kk * 16 < steps; ++kk)
+                                    umma_bf16_lanes(d, a0 + kk * 2, b0 + kk * 2, idesc, off);
+                                umma_commit(&empty[s]);
+                            }
+                            __syncwarp();
+                            next();
+                        }
+                        return true;
+                    });
+                if (one) umma_commit(&s_empty);
+            }
+            if (one) umma_commit(&tmem_full[acc]);
+            __syncwarp();
         }
     } else {
         // epilogue warps 2..5
@@ -653,16 +678,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 2 * BN);
     }
-}
-
-__device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "elect.sync _|p, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(r));
-    return r != 0;
 }
 
 // Few tiles: a cluster for each, its CTAs with a part of K each and every c-th pair of the
@@ -729,7 +744,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base;
-    // one lane's answer is the warp's: a lane that waits finds what another has found
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return true;
         if (!failed && !mbar_wait_bounded(bar, parity, kWaitLimitNs)) {
@@ -747,8 +761,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             phase ^= 1;
         }
     };
-    // Producer and MMA warp: the whole warp walks along, so that indexes and descriptors
-    // are uniform (one lane's walk took 270 cycles a stage beside its MMAs).
     if (warp == 0) {
         const bool one = elect_one();
         // rows in their own order are older than the kernel before, which has waited for
@@ -968,126 +980,136 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_base;
-    auto free_stage = [&](int g) {
-        const int u = g / NS;
-        if (u >= 1 && !failed && !mbar_wait_bounded(&empty[g % NS], (u - 1) & 1, kWaitLimitNs)) {
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait_cluster(bar, parity)) return true;
+        if (!failed && !mbar_wait_cluster_bounded(bar, parity, kWaitLimitNs)) {
             raise(p.error, PK_DEV_TIMEOUT);
             failed = 1;
         }
         return !failed;
     };
-
+    int s = 0;
+    uint32_t phase = 0;
+    auto next = [&]() {
+        if (++s == NS) {
+            s = 0;
+            phase ^= 1;
+        }
+    };
     if (warp == 0) {
-        if (lane == 0) {
-            // (the plan, and rows in their own order, are older than the kernel before, which
-            // has waited for them)
-            const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
-            if (rows == &tm.xs) grid_dep_wait();
-            int g = 0, with_s = 0;   // ring uses; tiles that had an S
-            bool ok = true;
-            const uint32_t sb = mapa_rank(smem_u32(&s_full), 0);
-            for (int tile = pair; tile < tiles && ok; tile += npairs) {
-                const int mt = tile % mtiles, m0 = mt * 2 * kBM + (int)rank * kBM;
-                const int n0 = (tile / mtiles) * BN + (int)rank * kHalfB;
-                TilePairs<int> of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
-                for (int kb = 0; kb < nk; ++kb, ++g) {
-                    if (!(ok = free_stage(g))) break;
-                    const int s = g % NS;
-                    const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
+        const bool one = elect_one();
+        const CUtensorMap *rows = *sorted ? &tm.x : &tm.xs;
+        if (rows == &tm.xs) grid_dep_wait();
+        int used = 0, with_s = 0;   // stages requested; tiles that had an S
+        bool ok = true;
+        const uint32_t f0 = mapa_rank(smem_u32(&full[0]), 0), sb = mapa_rank(smem_u32(&s_full), 0);
+        for (int tile = pair; tile < tiles && ok; tile += npairs) {
+            const int mt = tile % mtiles, m0 = mt * 2 * kBM + (int)rank * kBM;
+            const int n0 = (tile / mtiles) * BN + (int)rank * kHalfB;
+            TilePairs<int> of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
+            for (int kb = 0; kb < nk; ++kb, ++used) {
+                if (used >= NS && !(ok = __all_sync(0xffffffffu, wait(&empty[s], phase ^ 1)))) break;
+                if (one) {
                     if (leader) mbar_arrive_expect_tx(&full[s], kStageTx);
-                    tma_load_2d_pair(sB + s * kBBytes, &tm.w, fb, kb * kBK, n0);
-                    tma_load_2d_pair(sA + s * kABytes, rows, fb, kb * kBK, m0);
+                    tma_load_2d_pair(sB + s * kBBytes, &tm.w, f0 + s * 8, kb * kBK, n0);
+                    tma_load_2d_pair(sA + s * kABytes, rows, f0 + s * 8, kb * kBK, m0);
                 }
-                if (!ok || !of_tile.any()) continue;
-                grid_dep_wait();   // S
-                if (with_s >= 1 && !mbar_wait_bounded(&s_empty, (with_s - 1) & 1, kWaitLimitNs)) {
-                    raise(p.error, PK_DEV_TIMEOUT);
-                    failed = 1;
-                    ok = false;
-                    break;
-                }
-                ++with_s;
+                __syncwarp();
+                next();
+            }
+            if (!ok || !of_tile.any()) continue;
+            grid_dep_wait();   // S
+            if (with_s >= 1 && !(ok = __all_sync(0xffffffffu, wait(&s_empty, (with_s - 1) & 1)))) break;
+            ++with_s;
+            if (one) {
                 if (leader) mbar_arrive_expect_tx(&s_full, 2 * rblocks * kABytes);
                 for (int rb = 0; rb < rblocks; ++rb)
                     tma_load_2d_pair(sS + rb * kABytes, &tm.s, sb, rb * kBK, m0);
-                of_tile.each([&](int adapter) {
-                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
-                        if (!(ok = free_stage(g))) return false;
-                        const int s = g % NS;
-                        const uint32_t fb = mapa_rank(smem_u32(&full[s]), 0);
+            }
+            of_tile.each([&](int adapter) {
+                for (int rb = 0; rb < rblocks; ++rb, ++used) {
+                    if (used >= NS && !(ok = __all_sync(0xffffffffu, wait(&empty[s], phase ^ 1))))
+                        return false;
+                    if (one) {
                         if (leader) mbar_arrive_expect_tx(&full[s], 2 * kBBytes);
-                        tma_load_3d_pair(sB + s * kBBytes, &tm.up, fb, rb * kBK, n0, adapter);
+                        tma_load_3d_pair(sB + s * kBBytes, &tm.up, f0 + s * 8, rb * kBK, n0, adapter);
                     }
-                    return true;
-                });
+                    __syncwarp();
+                    next();
+                }
+                return true;
+            });
+        }
+        if (leader) {   // leave none of the pair's loads in flight
+            for (int i = 0; i < min(used, NS); ++i) {
+                s = s == 0 ? NS - 1 : s - 1;
+                if (s == NS - 1) phase ^= 1;
+                mbar_wait_bounded(&full[s], phase, kWaitLimitNs);
             }
-            if (leader) {   // leave none of the pair's loads in flight
-                for (int s = 0; s < NS; ++s)
-                    if (g > s) mbar_wait_bounded(&full[s], ((g - 1 - s) / NS) & 1, kWaitLimitNs);
-                if (with_s) mbar_wait_bounded(&s_full, (with_s - 1) & 1, kWaitLimitNs);
-            }
+            if (with_s) mbar_wait_bounded(&s_full, (with_s - 1) & 1, kWaitLimitNs);
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        if (leader) {
             constexpr uint32_t idesc = idesc_bf16(2 * kBM, BN);
-            int g = 0, t = 0, with_s = 0;
-            auto done = [&](uint64_t *bar, uint32_t parity) {
-                if (mbar_wait_cluster_bounded(bar, parity, kWaitLimitNs)) return true;
-                raise(p.error, PK_DEV_TIMEOUT);
-                failed = 1;
-                return false;
-            };
-            auto ready = [&](int s) { return done(&full[s], (g / NS) & 1); };
-            for (int tile = pair; tile < tiles && !failed; tile += npairs, ++t) {
+            const bool one = elect_one();
+            const uint64_t a_desc = sw128_desc(smem_u32(sA)), b_desc = sw128_desc(smem_u32(sB)),
+                           s_desc = sw128_desc(smem_u32(sS));
+            int t = 0, with_s = 0;
+            bool ok = true;
+            for (int tile = pair; tile < tiles && ok; tile += npairs, ++t) {
                 const int acc = t & 1, use = t >> 1, mt = tile % mtiles;
-                if (use >= 1 &&
-                    !mbar_wait_cluster_bounded(&tmem_empty[acc], (use - 1) & 1, kWaitLimitNs)) {
-                    raise(p.error, PK_DEV_TIMEOUT);
-                    failed = 1;
-                    break;
-                }
+                if (use >= 1 && !(ok = __all_sync(0xffffffffu, wait(&tmem_empty[acc], (use - 1) & 1)))) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
                 const int border = tile_pair[min(2 * mt + 1, halves)];   // of the two halves
                 TilePairs<TilePair> of_tile(pairs, tile_pair[2 * mt], tile_pair[min(2 * mt + 2, halves)]);
-                for (int kb = 0; kb < nk; ++kb, ++g) {
-                    const int s = g % NS;
-                    if (!ready(s)) break;
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!(ok = __all_sync(0xffffffffu, wait(&full[s], phase)))) break;
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(sA + s * kABytes), b0 = smem_u32(sB + s * kBBytes);
+                    if (one) {
+                        const uint64_t a0 = a_desc + s * (kABytes >> 4), b0 = b_desc + s * (kBBytes >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 16; ++kk)
-                        umma_bf16_pair(d, sw128_desc(a0 + kk * 32), sw128_desc(b0 + kk * 32), idesc,
-                                       (kb | kk) != 0);
-                    umma_commit_pair(&empty[s]);
+                        for (int kk = 0; kk < kBK / 16; ++kk)
+                            umma_bf16_pair(d, a0 + kk * 2, b0 + kk * 2, idesc, (kb | kk) != 0);
+                        umma_commit_pair(&empty[s]);
+                    }
+                    __syncwarp();
+                    next();
                 }
                 int pr_at = of_tile.p0;
                 const bool any = of_tile.any();
-                if (any && !failed) done(&s_full, with_s++ & 1);
-                of_tile.each([&](const TilePair &pr) {
-                    const bool odd = pr_at++ >= border;   // the second half's
-                    uint32_t off[8];
+                if (any && ok) ok = __all_sync(0xffffffffu, wait(&s_full, with_s++ & 1));
+                if (ok)
+                    of_tile.each([&](const TilePair &pr) {
+                        const bool odd = pr_at++ >= border;   // the second half's
+                        uint32_t off[8];
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        off[w] = odd ? ~0u : ~pr.rows[w];
-                        off[w + 4] = odd ? ~pr.rows[w] : ~0u;
-                    }
-                    for (int rb = 0; rb < rblocks; ++rb, ++g) {
-                        const int s = g % NS;
-                        if (failed || !ready(s)) return false;
-                        tc_fence_after();
-                        const uint32_t a0 = smem_u32(sS + rb * kABytes), b0 = smem_u32(sB + s * kBBytes);
-                        const int steps = min(kBK, p.rank - rb * kBK);
-                        for (int kk = 0; kk * 16 < steps; ++kk)
-                            umma_bf16_pair_lanes(d, sw128_desc(a0 + kk * 32),
-                                                 sw128_desc(b0 + kk * 32), idesc, off);
-                        umma_commit_pair(&empty[s]);
-                    }
-                    return true;
-                });
-                if (failed) break;
-                if (any) umma_commit_pair(&s_empty);
-                umma_commit_pair(&tmem_full[acc]);
+                        for (int w = 0; w < 4; ++w) {
+                            off[w] = odd ? ~0u : ~pr.rows[w];
+                            off[w + 4] = odd ? ~pr.rows[w] : ~0u;
+                        }
+                        for (int rb = 0; rb < rblocks; ++rb) {
+                            if (!(ok = __all_sync(0xffffffffu, wait(&full[s], phase)))) return false;
+                            tc_fence_after();
+                            if (one) {
+                                const uint64_t a0 = s_desc + rb * (kABytes >> 4),
+                                               b0 = b_desc + s * (kBBytes >> 4);
+                                const int steps = min(kBK, p.rank - rb * kBK);
+                                for (int kk = 0; kk * 16 < steps; ++kk)
+                                    umma_bf16_pair_lanes(d, a0 + kk * 2, b0 + kk * 2, idesc, off);
+                                umma_commit_pair(&empty[s]);
+                            }
+                            __syncwarp();
+                            next();
+                        }
+                        return true;
+                    });
+                if (!ok) break;
+                if (one) {
+                    if (any) umma_commit_pair(&s_empty);
+                    umma_commit_pair(&tmem_full[acc]);
+                }
+                __syncwarp();
             }
         }
     } else {
