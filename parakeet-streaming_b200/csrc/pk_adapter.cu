@@ -420,16 +420,6 @@ template <typename T> struct TilePairs {
     }
 };
 
-__device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "elect.sync _|p, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(r));
-    return r != 0;
-}
-
 // A warp's rows of C and R in sorted order: the eight that this lane's pieces touch.
 struct SortedRows {
     int row[8];

@@ -190,50 +190,62 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         Work work(p, blockIdx.x);
         constexpr uint32_t id_s = idesc_bf16(kRows, kKeys);
         constexpr uint32_t id_o = idesc_bf16(kRows, DH) | (1u << 16);   // B MN-major
-        const uint32_t q0 = smem_u32(sq);
+        const uint64_t q0 = tile_desc(smem_u32(sq), S::kGroup), ring0 = tile_desc(smem_u32(ring), S::kGroup);
+        // the whole warp walks along, so that indexes and descriptors are uniform
+        const bool one = elect_one();
         int it = 0, j = 0, unit = 0;   // ring use, tile and unit of this CTA
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            return __all_sync(0xffffffffu, ring_wait(bar, parity, &failed, p.error));
+        };
+        bool ok = true;
         // S of a tile whose K is ring use `use`, over the P of the tile two before, whose
         // product has to be done with it
         auto scores = [&](int use, int tile) {
             const int s = use % NS;
-            if (tile >= 2) ring_wait(&o_done[tile & 1], ((tile >> 1) - 1) & 1, &failed, p.error);
-            ring_wait(&full[s], (use / NS) & 1, &failed, p.error);
+            if (tile >= 2) ok = ok && wait(&o_done[tile & 1], ((tile >> 1) - 1) & 1);
+            ok = ok && wait(&full[s], (use / NS) & 1);
+            if (!ok) return;
             tc_fence_after();
-            const uint32_t k0 = smem_u32(ring + s * S::kSlot);
+            if (one) {
+                const uint64_t k0 = ring0 + s * (S::kSlot >> 4);
 #pragma unroll
-            for (int kk = 0; kk < DH / 16; ++kk) {
-                const uint32_t off = (kk / 4) * 1024 + (kk % 4) * 32;
-                umma_bf16(tmem + S::kS + (tile & 1) * kKeys, tile_desc(q0 + off, S::kGroup),
-                          tile_desc(k0 + off, S::kGroup), id_s, kk != 0);
+                for (int kk = 0; kk < DH / 16; ++kk) {
+                    const uint32_t off = ((kk / 4) * 1024 + (kk % 4) * 32) >> 4;
+                    umma_bf16(tmem + S::kS + (tile & 1) * kKeys, q0 + off, k0 + off, id_s, kk != 0);
+                }
+                umma_commit(&empty[s]);
+                umma_commit(&s_full[tile & 1]);
             }
-            umma_commit(&empty[s]);
-            umma_commit(&s_full[tile & 1]);
+            __syncwarp();
         };
-        while (!failed && work.next()) {
+        while (ok && work.next()) {
             const int n = work.u.t1 - work.u.t0;
             if (n <= 0) continue;
-            ring_wait(&q_full, unit & 1, &failed, p.error);
+            ok = wait(&q_full, unit & 1);
             ++unit;
             tc_fence_after();
             scores(it, j);
-            for (int i = 0; i < n && !failed; ++i, ++j, it += 2) {
+            for (int i = 0; i < n && ok; ++i, ++j, it += 2) {
                 if (i + 1 < n) scores(it + 2, j + 1);
                 const int s = (it + 1) % NS;
-                ring_wait(&full[s], ((it + 1) / NS) & 1, &failed, p.error);
-                ring_wait(&p_full[j & 1], (j >> 1) & 1, &failed, p.error);
-                if (failed) break;
+                ok = ok && wait(&full[s], ((it + 1) / NS) & 1) && wait(&p_full[j & 1], (j >> 1) & 1);
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t v0 = smem_u32(ring + s * S::kSlot);
+                if (one) {
+                    const uint64_t v0 = ring0 + s * (S::kSlot >> 4);
 #pragma unroll
-                for (int kk = 0; kk < kKeys / 16; ++kk)
-                    umma_bf16_ts(tmem + S::kO + (j & 1) * DH,
-                                 tmem + S::kS + (j & 1) * kKeys + kk * 8,
-                                 tile_desc(v0 + kk * 2 * S::kGroup, S::kGroup), id_o, (i > 1) | (kk != 0));
-                umma_commit(&empty[s]);
-                umma_commit(&o_done[j & 1]);
+                    for (int kk = 0; kk < kKeys / 16; ++kk)
+                        umma_bf16_ts(tmem + S::kO + (j & 1) * DH,
+                                     tmem + S::kS + (j & 1) * kKeys + kk * 8,
+                                     v0 + kk * (2 * S::kGroup >> 4), id_o, (i > 1) | (kk != 0));
+                    umma_commit(&empty[s]);
+                    umma_commit(&o_done[j & 1]);
+                }
+                __syncwarp();
             }
         }
-        umma_commit(&idle);   // no MMA is left when the CTA frees its TMEM
+        if (one) umma_commit(&idle);   // no MMA is left when the CTA frees its TMEM
+        __syncwarp();
         mbar_wait_bounded(&idle, 0, kWaitLimitNs);
     };
 
@@ -242,7 +254,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 0) produce();
-        else if (warp == 1 && lane == 0) multiply();
+        else if (warp == 1) multiply();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         Work work(p, blockIdx.x);
