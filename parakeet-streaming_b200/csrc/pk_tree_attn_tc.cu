@@ -3,18 +3,22 @@
 //
 // Bound by reading K and V as long as a request's rows fit one tile: 128 keys of a
 // 128-wide head are 64 KB, 2800 cycles of an SM's share of the memory rate, for
-// 1024 cycles of MMAs and 1024 of exponentials, but some 2400 of a warpgroup's whole
-// softmax (loads from TMEM, maximum, sum, conversions).  So one CTA an SM, and two
-// softmax warpgroups that take every other tile:
-//   warp 0      pages of K and V by TMA into a ring of slots (a slot: one tile of
-//               K or of V), running ahead over the CTA's units
-//   warp 1      one thread issues S_j = Q K_j^T (both from shared memory, fp32 in
-//               TMEM, two buffers) and O += P_j V_j (P from TMEM, V from shared
-//               memory as it lies: a row-major [keys][dim] tile is the MN-major
-//               operand), O in TMEM, one for the even tiles and one for the odd
-//   warps 4..11 a thread per row (TMEM lane), warps 4..7 for the even tiles: the row's
-//               scores without a shuffle, maximum, exp2, P as bf16 over the scores,
-//               fp32 sum; maxima, sums and O of the two meet at the end of a unit
+// 1024 cycles of MMAs and 1024 of exponentials.  But a tile is a chain - S, the softmax
+// of 128 scores a thread (loads from TMEM, maximum, exp2, sum, conversions), O - of some
+// 5000 cycles, and beginning and ending a row tile another.  So one CTA an SM with two
+// workers, each with a share of the step's line, a ring of its own and its own warps:
+//   warps 0, 2   pages of K and V by TMA into a ring of slots (a slot: one tile of K or
+//                of V), running ahead over the worker's units
+//   warps 1, 3   S = Q K^T (both from shared memory, fp32 in TMEM) and O += P V (P
+//                from TMEM, V from shared memory as it lies: a row-major [keys][dim]
+//                tile is the MN-major operand), O in TMEM
+//   warps 4..11  four a worker, a thread per row (TMEM lane): the row's scores without a
+//                shuffle, maximum, exp2, P as bf16 over the scores, fp32 sum; the next
+//                unit's queries ahead of the epilogue
+// Two groups that took every other tile of one worker's units and met at their ends took
+// 140 us for 32 requests x 8 heads of 128 with up to 128 rows and 8000 tokens, this takes
+// 124; 160 x 8 heads of 64 with 21 rows and 2000 tokens: 171 and 135; a single request of
+// 131,000 tokens, whose shares are cut twice as often: 98 and 101.
 // The running maximum is raised, and O scaled for it, only when a row's scores pass
 // the one in use by more than 2^8: weights stay below 256, which the fp32 sums and
 // bf16's exponent hold, and most tiles touch O in the MMA alone.
@@ -33,9 +37,10 @@ template <int DH>
 struct TcShape {
     static constexpr int kSlot = kKeys * DH * 2;       // one tile of K, V or Q
     static constexpr int kGroup = DH / 64 * 1024;      // 8 rows of one
-    static constexpr int kSlots = 5 * (128 / DH);      // 160 KB
-    static constexpr int kSmem = (kSlots + 1) * kSlot + 1024;
-    // TMEM columns: S twice (P over it), O twice
+    static constexpr int kSlots = DH == 64 ? 5 : 2;    // a worker's, beside its Q
+    static constexpr int kWorker = (kSlots + 1) * kSlot;
+    static constexpr int kSmem = 2 * kWorker + 1024;
+    // TMEM columns: each worker's S (P over it), each worker's O
     static constexpr int kS = 0, kO = 2 * kKeys, kTmem = 512;
 };
 
@@ -71,7 +76,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-// barrier of one softmax group (four warps) that also ORs a flag over them
+// barrier of one worker's softmax warps (four) that also ORs a flag over them
 __device__ __forceinline__ bool group_any(int group, bool v) {
     uint32_t r;
     asm volatile(
@@ -84,9 +89,6 @@ __device__ __forceinline__ bool group_any(int group, bool v) {
         : "memory");
     return r != 0;
 }
-// barrier of both groups
-__device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
 // Bits of keys rel0 .. rel0 + 31 of the step's own tokens that a row sees.
 __device__ __forceinline__ uint32_t seen_bits(int trees, uint64_t mask, int node, int rel0) {
     if (rel0 <= -32) return 0xffffffffu;
@@ -105,32 +107,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     using S = TcShape<DH>;
     constexpr int NS = S::kSlots;
     extern __shared__ uint8_t tree_smem[];
-    uint8_t *sq = reinterpret_cast<uint8_t *>(
-        (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023));
-    uint8_t *ring = sq + S::kSlot;
-    __shared__ __align__(8) uint64_t full[NS], empty[NS], q_full, s_full[2], p_full[2], o_done[2],
-        idle;
-    __shared__ float s_max[2][kRows], s_sum[2][kRows];
-    __shared__ int s_odd[2];
+    __shared__ __align__(8) uint64_t bars[2][2 * NS + 5];   // of each worker
     __shared__ uint32_t tmem_base;
     __shared__ volatile int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // worker 0: warps 0 and 1 (copies, MMAs) and 4 .. 7 (softmax); worker 1: 2, 3, 8 .. 11
+    const int w = warp < 4 ? warp >> 1 : (warp >> 2) - 1;
+    uint8_t *sq = reinterpret_cast<uint8_t *>(
+                      (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023)) +
+                  w * S::kWorker;
+    uint8_t *ring = sq + S::kSlot;
+    uint64_t *full = bars[w], *empty = full + NS, *q_full = empty + NS, *s_full = q_full + 1,
+             *p_full = s_full + 1, *o_done = p_full + 1, *idle = o_done + 1;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < NS; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+        for (int v = 0; v < 2; ++v) {
+            for (int s = 0; s < 2 * NS + 5; ++s) mbar_init(&bars[v][s], s == 2 * NS || s == 2 * NS + 2 ? 4 : 1);
         }
-        mbar_init(&q_full, 8);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&o_done[i], 1);
-        }
-        mbar_init(&idle, 1);
         failed = 0;
         fence_mbar_init();
         prefetch_tmap(&kv_map);
     }
+    __syncwarp();
     if (warp == 0) {
         tmem_alloc(&tmem_base, S::kTmem);
         tmem_relinquish();
@@ -141,23 +138,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = tmem_base;
     grid_dep_wait();
     grid_dep_launch();
+    const int worker = w * gridDim.x + blockIdx.x;   // neighbouring shares on different SMs
+
     auto produce = [&]() {
-        // producer: lanes issue a tile's boxes, K then V
+        // lanes issue a tile's boxes, K then V
         const int ps = 1 << p.ps_shift, rows_box = min(ps, kTokRowsBox);
         const int box_of = lane;
         const uint32_t bytes = rows_box * DH * 2;
         int it = 0;
         bool stop = false;   // the warp's, so that its lanes stay together
-        Work work(p, blockIdx.x);
+        Work work(p, worker);
         Pages pages, then;
         bool more = work.next();
-        Unit w = work.u;
-        if (more) pages.open(p, w);
+        Unit u = work.u;
+        if (more) pages.open(p, u);
         while (more && !stop) {
             more = work.next();
             if (more) then.open(p, work.u);
-            const int len = w.ctx + w.count;
-            for (int t = w.t0; t < w.t1 && !stop; ++t) {
+            const int len = u.ctx + u.count;
+            for (int t = u.t0; t < u.t1 && !stop; ++t) {
                 const int k0 = t * kKeys, n = (min(kKeys, len - k0) + rows_box - 1) / rows_box;
                 // lanes without a box ask for the last one's page
                 int page = pages.get((k0 + min(box_of, n - 1) * rows_box) >> p.ps_shift);
@@ -176,10 +175,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     __syncwarp();
                     if (box_of < n)
                         tma_load_rows(ring + s * S::kSlot + box_of * bytes, &kv_map, &full[s], in_page,
-                                      ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + w.head);
+                                      ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + u.head);
                 }
             }
-            w = work.u;
+            u = work.u;
             pages = then;
         }
         if (stop)   // leave no copy in flight
@@ -187,141 +186,157 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (it > s) mbar_wait_bounded(&full[s], ((it - 1 - s) / NS) & 1, kWaitLimitNs);
     };
     auto multiply = [&]() {
-        Work work(p, blockIdx.x);
+        Work work(p, worker);
         constexpr uint32_t id_s = idesc_bf16(kRows, kKeys);
         constexpr uint32_t id_o = idesc_bf16(kRows, DH) | (1u << 16);   // B MN-major
         const uint64_t q0 = tile_desc(smem_u32(sq), S::kGroup), ring0 = tile_desc(smem_u32(ring), S::kGroup);
+        const uint32_t st = tmem + S::kS + w * kKeys, ot = tmem + S::kO + w * DH;
         // the whole warp walks along, so that indexes and descriptors are uniform
         const bool one = elect_one();
-        int it = 0, j = 0, unit = 0;   // ring use, tile and unit of this CTA
         auto wait = [&](uint64_t *bar, uint32_t parity) {
             return __all_sync(0xffffffffu, ring_wait(bar, parity, &failed, p.error));
         };
+        int s = 0, unit = 0;   // ring slot, unit of this worker
+        uint32_t phase = 0, j = 0;   // of the ring, tile of this worker
         bool ok = true;
-        // S of a tile whose K is ring use `use`, over the P of the tile two before, whose
-        // product has to be done with it
-        auto scores = [&](int use, int tile) {
-            const int s = use % NS;
-            if (tile >= 2) ok = ok && wait(&o_done[tile & 1], ((tile >> 1) - 1) & 1);
-            ok = ok && wait(&full[s], (use / NS) & 1);
-            if (!ok) return;
-            tc_fence_after();
-            if (one) {
-                const uint64_t k0 = ring0 + s * (S::kSlot >> 4);
-#pragma unroll
-                for (int kk = 0; kk < DH / 16; ++kk) {
-                    const uint32_t off = ((kk / 4) * 1024 + (kk % 4) * 32) >> 4;
-                    umma_bf16(tmem + S::kS + (tile & 1) * kKeys, q0 + off, k0 + off, id_s, kk != 0);
-                }
-                umma_commit(&empty[s]);
-                umma_commit(&s_full[tile & 1]);
+        auto next = [&]() {
+            if (++s == NS) {
+                s = 0;
+                phase ^= 1;
             }
-            __syncwarp();
         };
         while (ok && work.next()) {
             const int n = work.u.t1 - work.u.t0;
             if (n <= 0) continue;
-            ok = wait(&q_full, unit & 1);
+            ok = wait(q_full, unit & 1);
             ++unit;
-            tc_fence_after();
-            scores(it, j);
-            for (int i = 0; i < n && ok; ++i, ++j, it += 2) {
-                if (i + 1 < n) scores(it + 2, j + 1);
-                const int s = (it + 1) % NS;
-                ok = ok && wait(&full[s], ((it + 1) / NS) & 1) && wait(&p_full[j & 1], (j >> 1) & 1);
+            for (int i = 0; i < n && ok; ++i, ++j) {
+                // S over the P of the tile before, whose product has to be done with it
+                ok = (j == 0 || wait(o_done, (j - 1) & 1)) && wait(&full[s], phase);
+                if (!ok) break;
+                tc_fence_after();
+                if (one) {
+                    const uint64_t k0 = ring0 + s * (S::kSlot >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < DH / 16; ++kk) {
+                        const uint32_t off = ((kk / 4) * 1024 + (kk % 4) * 32) >> 4;
+                        umma_bf16(st, q0 + off, k0 + off, id_s, kk != 0);
+                    }
+                    umma_commit(&empty[s]);
+                    umma_commit(s_full);
+                }
+                __syncwarp();
+                next();
+                ok = wait(&full[s], phase) && wait(p_full, j & 1);
                 if (!ok) break;
                 tc_fence_after();
                 if (one) {
                     const uint64_t v0 = ring0 + s * (S::kSlot >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        umma_bf16_ts(tmem + S::kO + (j & 1) * DH,
-                                     tmem + S::kS + (j & 1) * kKeys + kk * 8,
-                                     v0 + kk * (2 * S::kGroup >> 4), id_o, (i > 1) | (kk != 0));
+                        umma_bf16_ts(ot, st + kk * 8, v0 + kk * (2 * S::kGroup >> 4), id_o,
+                                     (i > 0) | (kk != 0));
                     umma_commit(&empty[s]);
-                    umma_commit(&o_done[j & 1]);
+                    umma_commit(o_done);
                 }
                 __syncwarp();
+                next();
             }
         }
-        if (one) umma_commit(&idle);   // no MMA is left when the CTA frees its TMEM
+        if (one) umma_commit(idle);   // no MMA is left when the CTA frees its TMEM
         __syncwarp();
-        mbar_wait_bounded(&idle, 0, kWaitLimitNs);
+        mbar_wait_bounded(idle, 0, kWaitLimitNs);
     };
 
     // a row's scores take 128 registers: 208 for the softmax warps out of the launch's
     // 168 x 384, 88 for the other warpgroup (128 x 88 + 256 x 208 = 64512)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 0) produce();
-        else if (warp == 1) multiply();
+        if (warp & 1) multiply();
+        else produce();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        Work work(p, blockIdx.x);
-        // softmax group g takes the CTA's tiles j with j % 2 == g; thread = row (TMEM
-        // lane) 32 (warp % 4) + lane of the tile
-        const int g = (warp >> 2) - 1, quad = warp & 3, rt = quad * 32 + lane;
+        Work work(p, worker);
+        // thread = row (TMEM lane) 32 (warp % 4) + lane of the tile
+        const int quad = warp & 3, rt = quad * 32 + lane;
         const int gt = threadIdx.x & 127;   // thread in the group
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const uint32_t st = tmem + lanes + S::kS + g * kKeys, ot = tmem + lanes + S::kO + g * DH;
+        const uint32_t st = tmem + lanes + S::kS + w * kKeys, ot = tmem + lanes + S::kO + w * DH;
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
         __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
-        int it = 0, j = 0;   // ring use and tile of the unit's first tile
-        while (work.next()) {
-            const Unit &w = work.u;
-            const int r = w.rt * kRows + rt, n = w.t1 - w.t0, len = w.ctx + w.count;
-            const bool live = r < w.count * p.group;
-            const int node = live ? r / p.group : -1;
-            const int64_t row = w.row0 + (live ? node : 0);
-            const int64_t qh = (int64_t)w.head * p.group + (live ? r - node * p.group : 0);
-            uint64_t mask = 0;
-            if (live && p.trees) mask = reinterpret_cast<const uint64_t *>(p.step + p.l.mask)[row];
+        // this thread's row of a unit
+        struct Row {
+            Unit u;
+            int node;   // -1: none
+            int64_t row, qh;
+            uint64_t mask;
+        } now, then;
+        bool more;
+        // the next unit's row, its query to shared memory: ahead of the epilogue of the unit
+        // before, whose scores have all been read
+        auto advance = [&](Row &x) {
+            more = work.next();
+            if (!more) return;
+            x.u = work.u;
+            const int r = x.u.rt * kRows + rt;
+            const bool live = r < x.u.count * p.group;
+            x.node = live ? r / p.group : -1;
+            x.row = x.u.row0 + (live ? x.node : 0);
+            x.qh = (int64_t)x.u.head * p.group + (live ? r - x.node * p.group : 0);
+            x.mask = 0;
+            if (live && p.trees) x.mask = reinterpret_cast<const uint64_t *>(p.step + p.l.mask)[x.row];
+            if (x.u.t1 <= x.u.t0) return;
+            const uint4 *src = reinterpret_cast<const uint4 *>(q + x.row * p.q_rs + x.qh * p.q_hs);
+#pragma unroll
+            for (int c = 0; c < DH / 8; ++c)
+                *reinterpret_cast<uint4 *>(sq + tile_at<DH>(rt, c)) =
+                    live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) arrive(q_full);
+        };
+        advance(now);
+        int s = 0;                   // ring slot
+        uint32_t phase = 0, j = 0;   // of the ring, tile of this worker
+        auto next = [&]() {
+            if (++s == NS) {
+                s = 0;
+                phase ^= 1;
+            }
+        };
+        while (more) {
+            const Unit &u = now.u;
+            const int len = u.ctx + u.count;
             float m = -INFINITY, l = 0.f;   // the maximum in use (scaled), the sum
             bool odd = false;               // a value that is not finite among the own rows
-            if (n > 0) {
-                // the tile's queries, half a group; the MMAs that read the last ones are
-                // done, since both groups have read their scores
-                const uint4 *src = reinterpret_cast<const uint4 *>(q + row * p.q_rs + qh * p.q_hs);
-#pragma unroll
-                for (int i = 0; i < DH / 16; ++i) {
-                    const int c = g * (DH / 16) + i;
-                    *reinterpret_cast<uint4 *>(sq + tile_at<DH>(rt, c)) =
-                        live ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_async_proxy();
-                __syncwarp();
-                if (lane == 0) arrive(&q_full);
-            }
-            int mine = 0;   // tiles of this group in the unit
-            for (int i = (g ^ j) & 1; i < n; i += 2, ++mine) {
-                const int tile = j + i, use = it + 2 * i;
-                const int k0 = (w.t0 + i) * kKeys;
-                ring_wait(&s_full[g], (tile >> 1) & 1, &failed, p.error);
+            for (int t = u.t0; t < u.t1; ++t, ++j) {
+                const int k0 = t * kKeys;
+                next();   // V's slot
+                ring_wait(s_full, j & 1, &failed, p.error);
                 __syncwarp();
                 tc_fence_after();
-                float s[kKeys];
+                float sc[kKeys];
 #pragma unroll
                 for (int c = 0; c < kKeys / 32; ++c)
-                    tmem_ld32(st + c * 32, *reinterpret_cast<float(*)[32]>(s + c * 32));
-                if (k0 + kKeys > w.ctx) {   // some of the step's own tokens, or the end
-                    const int sv = (use + 1) % NS;
+                    tmem_ld32(st + c * 32, *reinterpret_cast<float(*)[32]>(sc + c * 32));
+                if (k0 + kKeys > u.ctx) {   // some of the step's own tokens, or the end
 #pragma unroll
                     for (int c = 0; c < kKeys / 32; ++c) {
-                        const uint32_t bits = seen_bits(p.trees, mask, node, k0 + c * 32 - w.ctx);
+                        const uint32_t bits =
+                            seen_bits(p.trees, now.mask, now.node, k0 + c * 32 - u.ctx);
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (!(bits >> e & 1)) s[c * 32 + e] = -INFINITY;
+                            if (!(bits >> e & 1)) sc[c * 32 + e] = -INFINITY;
                     }
                     // V rows past the end hold what the page held before, and a token's
                     // values may be inf or NaN: zero in the product, where a weight of
                     // zero would not keep them out; the epilogue adds the latter to the
                     // rows that see them
-                    ring_wait(&full[sv], ((use + 1) / NS) & 1, &failed, p.error);
-                    uint8_t *vs = ring + sv * S::kSlot;
+                    ring_wait(&full[s], phase, &failed, p.error);
+                    uint8_t *vs = ring + s * S::kSlot;
                     bool bad = false;
-                    for (int c = gt; c < kKeys * DH / 8; c += 128) {
+                    for (int c = max(u.ctx - k0, 0) * (DH / 8) + gt; c < kKeys * DH / 8; c += 128) {
                         const int vr = c / (DH / 8), ch = c % (DH / 8), key = k0 + vr;
-                        if (key < w.ctx) continue;
                         uint4 *at = reinterpret_cast<uint4 *>(vs + tile_at<DH>(vr, ch));
                         uint4 x = make_uint4(0u, 0u, 0u, 0u);
                         if (key < len) {
@@ -345,11 +360,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         *at = x;
                     }
                     fence_async_proxy();
-                    odd |= group_any(g, bad);
+                    odd |= group_any(w, bad);
                 }
-                float tops[4] = {s[0], s[1], s[2], s[3]};
+                float tops[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
-                for (int e = 4; e < kKeys; ++e) tops[e & 3] = fmaxf(tops[e & 3], s[e]);
+                for (int e = 4; e < kKeys; ++e) tops[e & 3] = fmaxf(tops[e & 3], sc[e]);
                 float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 top = top == -INFINITY ? top : __fmul_rn(top, p.scale_log2);
                 const bool raise_it = top > m + kRaise || (m == -INFINITY && top > m);
@@ -357,10 +372,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const float keep = raise_it ? ex2(m - top) : 1.f;
                     if (raise_it) m = top;
                     l *= keep;
-                    if (mine > 0) {   // O has the group's tiles before
-                        ring_wait(&o_done[g], ((tile >> 1) - 1) & 1, &failed, p.error);
-                        __syncwarp();
-                        tc_fence_after();
+                    if (t > u.t0) {   // (S came after the product of the tile before)
 #pragma unroll 1
                         for (int c = 0; c < DH / 32; ++c) {
                             float o[32];
@@ -379,8 +391,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     uint32_t x[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float a = ex2(s[c * 64 + 2 * e] * p.scale_log2 - base);
-                        const float b = ex2(s[c * 64 + 2 * e + 1] * p.scale_log2 - base);
+                        const float a = ex2(sc[c * 64 + 2 * e] * p.scale_log2 - base);
+                        const float b = ex2(sc[c * 64 + 2 * e + 1] * p.scale_log2 - base);
                         sum[(2 * e) & 3] += a;
                         sum[(2 * e + 1) & 3] += b;
                         x[e] = pack2(a, b);
@@ -391,60 +403,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(&p_full[g]);
+                if (lane == 0) arrive(p_full);
+                next();   // the next K's
             }
-            // the last tile of each group in O, and the groups' maxima and sums
-            const int last = j + n - 1;   // the CTA's last tile; the other group's is the one before
+            advance(then);
+            // O after the unit's last tile
+            const int n = u.t1 - u.t0;
             if (n > 0) {
-                if (n > 1 || (last & 1) == 0)
-                    ring_wait(&o_done[0], ((last & 1 ? last - 1 : last) >> 1) & 1, &failed, p.error);
-                if (n > 1 || (last & 1) == 1)
-                    ring_wait(&o_done[1], ((last & 1 ? last : last - 1) >> 1) & 1, &failed, p.error);
+                ring_wait(o_done, (j - 1) & 1, &failed, p.error);
                 __syncwarp();
                 tc_fence_after();
             }
-            j += n > 0 ? n : 0;
-            it += n > 0 ? 2 * n : 0;
-            s_max[g][rt] = m;
-            s_sum[g][rt] = l;
-            if (gt == 0) s_odd[g] = odd;
-            groups_sync();
-            odd = s_odd[0] | s_odd[1];
-            // a group without a tile has O that was never written: a factor of 0 and no
-            // product with it
-            const float ma = s_max[0][rt], mb = s_max[1][rt], mm = fmaxf(ma, mb);
-            const float ref = mm == -INFINITY ? 0.f : mm;
-            const float fa = ex2(ma - ref), fb = ex2(mb - ref);
-            const float ls = fa * s_sum[0][rt] + fb * s_sum[1][rt];
-            const bool has_a = n > 1 || (n == 1 && (last & 1) == 0),
-                       has_b = n > 1 || (n == 1 && (last & 1) == 1);
-            const float inv = 1.f / ls;
-            float *dst = p.ws_o + ((int64_t)w.part * kRows + rt) * DH;
-            __nv_bfloat16 *o_row = out + row * p.o_rs + qh * p.o_hs;
+            const float inv = 1.f / l;
+            float *dst = p.ws_o + ((int64_t)u.part * kRows + rt) * DH;
+            __nv_bfloat16 *o_row = out + now.row * p.o_rs + now.qh * p.o_hs;
 #pragma unroll 1
-            for (int c = g * (DH / 64); c < (g + 1) * (DH / 64); ++c) {   // half the columns each
-                float o[32], x[32];
+            for (int c = 0; c < DH / 32; ++c) {
+                float o[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = 0.f;
-                if (has_a) {
-                    tmem_ld32(tmem + lanes + S::kO + c * 32, x);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = fa * x[e];
-                }
-                if (has_b) {
-                    tmem_ld32(tmem + lanes + S::kO + DH + c * 32, x);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] += fb * x[e];
-                }
-                if (!live) continue;
+                __syncwarp();
+                if (n > 0) tmem_ld32(ot + c * 32, o);
+                if (now.node < 0) continue;
                 if (odd) {
                     // the values that were kept out of the product, for the keys that
                     // the row sees: they make the sum inf or NaN, whatever their weight
 #pragma unroll 1
-                    for (int key = max(w.ctx, w.t0 * kKeys); key < min(len, w.t1 * kKeys); ++key) {
-                        const int rel = key - w.ctx;
-                        if (!(seen_bits(p.trees, mask, node, rel) & 1)) continue;
-                        const __nv_bfloat16 *v = value_row<DH>(p, w, key) + c * 32;
+                    for (int key = max(u.ctx, u.t0 * kKeys); key < min(len, u.t1 * kKeys); ++key) {
+                        if (!(seen_bits(p.trees, now.mask, now.node, key - u.ctx) & 1)) continue;
+                        const __nv_bfloat16 *v = value_row<DH>(p, u, key) + c * 32;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
                             const float y = __bfloat162float(v[e]);
@@ -452,7 +439,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                     }
                 }
-                if (w.part >= 0) {
+                if (u.part >= 0) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         reinterpret_cast<float4 *>(dst + c * 32)[e] =
@@ -467,11 +454,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             pack2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
                 }
             }
-            if (g == 0 && w.part >= 0 && live)
-                *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)w.part * kRows + rt) * 2) =
-                    make_float2(mm, ls);
-            tc_fence_before();
-            groups_sync();   // O and the exchange are free again
+            if (u.part >= 0 && now.node >= 0)
+                *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)u.part * kRows + rt) * 2) =
+                    make_float2(m, l);
+            tc_fence_before();   // O is free again when this group's next P is there
+            __syncwarp();
+            now = then;
         }
     }
     tc_fence_before();
@@ -483,18 +471,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 }
 
 template <int DH>
-cudaError_t launch(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
+cudaError_t launch(const pk_token_kv *kv, const TreeParams &p, int workers, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_smem(tree_tc_kernel<DH>, TcShape<DH>::kSmem, done);
     if (e != cudaSuccess) return e;
+    const int ctas = workers < kv->sms ? workers : kv->sms;   // few workers: an SM each
     return launch_pdl(tree_tc_kernel<DH>, dim3(ctas), dim3(kTcThreads), TcShape<DH>::kSmem, s,
                       kv->kv_map, p);
 }
 
 }  // namespace
 
-cudaError_t launch_tree_tc(const pk_token_kv *kv, const TreeParams &p, int ctas, cudaStream_t s) {
-    return kv->d.head_dim == 64 ? launch<64>(kv, p, ctas, s) : launch<128>(kv, p, ctas, s);
+cudaError_t launch_tree_tc(const pk_token_kv *kv, const TreeParams &p, int workers, cudaStream_t s) {
+    return kv->d.head_dim == 64 ? launch<64>(kv, p, workers, s) : launch<128>(kv, p, workers, s);
 }
 
 }  // namespace pk
