@@ -242,7 +242,7 @@ inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
     if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, (kv->d.head_dim == 64 ? 3 : 2) * kv->sms, 1, 1};
     if (mean <= 16) return {16, kTokRowsBox, tok_workers(kv->d.head_dim) * kv->sms, 8, 1};
-    return {128, 128, 2 * kv->sms, 3, kv->d.head_dim == 64 ? 2 : 3};
+    return {128, 64, 2 * kv->sms, 6, 4};
 }
 
 // Step block, int32 words: header, then arrays at these offsets.  The step's work

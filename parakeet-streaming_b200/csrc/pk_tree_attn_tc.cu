@@ -30,18 +30,29 @@
 namespace pk {
 namespace {
 
-constexpr int kRows = 128, kKeys = 128, kTcThreads = 128 + 256;
+constexpr int kRows = 128, kKeys = 64, kTcThreads = 128 + 256;
 constexpr float kRaise = 8.f;   // log2 of how far scores may pass the maximum in use
 
 template <int DH>
 struct TcShape {
-    static constexpr int kSlot = kKeys * DH * 2;       // one tile of K, V or Q
+    static constexpr int kSlot = kKeys * DH * 2;       // one tile of K or V
+    static constexpr int kQ = kRows * DH * 2;
     static constexpr int kGroup = DH / 64 * 1024;      // 8 rows of one
-    static constexpr int kSlots = DH == 64 ? 5 : 2;    // a worker's, beside its Q
-    static constexpr int kWorker = (kSlots + 1) * kSlot;
+    static constexpr int kSlots = DH == 64 ? 10 : 5;   // a worker's, beside its Q
+    static constexpr int kWorker = kQ + kSlots * kSlot;
     static constexpr int kSmem = 2 * kWorker + 1024;
-    // TMEM columns: each worker's S (P over it), each worker's O
-    static constexpr int kS = 0, kO = 2 * kKeys, kTmem = 512;
+    // TMEM columns: each worker's S, twice (P over it), each worker's O
+    static constexpr int kS = 0, kO = 4 * kKeys, kTmem = 512;
+    // barriers of a worker: slots full and empty, then
+    // (S, P and O of even and odd tiles have barriers of their own: two tiles are under way)
+    enum {
+        kQFull = 2 * kSlots,
+        kIdle,
+        kODone,
+        kSFull = kODone + 2,
+        kPFull = kSFull + 2,
+        kBars = kPFull + 2
+    };
 };
 
 // O += P V: A from TMEM (bf16 pairs), B MN-major
@@ -73,6 +84,43 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+// a row's scores: one wait for their loads
+__device__ __forceinline__ void tmem_ld_scores(uint32_t taddr, float (&v)[kKeys]) {
+    uint32_t r[kKeys];
+#pragma unroll
+    for (int c = 0; c < kKeys; c += 32)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+            "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+            "%28, %29, %30, %31}, [%32];"
+            : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]),
+              "=r"(r[c + 5]), "=r"(r[c + 6]), "=r"(r[c + 7]), "=r"(r[c + 8]), "=r"(r[c + 9]),
+              "=r"(r[c + 10]), "=r"(r[c + 11]), "=r"(r[c + 12]), "=r"(r[c + 13]), "=r"(r[c + 14]),
+              "=r"(r[c + 15]), "=r"(r[c + 16]), "=r"(r[c + 17]), "=r"(r[c + 18]), "=r"(r[c + 19]),
+              "=r"(r[c + 20]), "=r"(r[c + 21]), "=r"(r[c + 22]), "=r"(r[c + 23]), "=r"(r[c + 24]),
+              "=r"(r[c + 25]), "=r"(r[c + 26]), "=r"(r[c + 27]), "=r"(r[c + 28]), "=r"(r[c + 29]),
+              "=r"(r[c + 30]), "=r"(r[c + 31])
+            : "r"(taddr + c));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) v[i] = __uint_as_float(r[i]);
+}
+// two fp32 operations an instruction
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    return (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float low2(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float high2(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
 __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -107,7 +155,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     using S = TcShape<DH>;
     constexpr int NS = S::kSlots;
     extern __shared__ uint8_t tree_smem[];
-    __shared__ __align__(8) uint64_t bars[2][2 * NS + 5];   // of each worker
+    __shared__ __align__(8) uint64_t bars[2][S::kBars];   // of each worker
     __shared__ uint32_t tmem_base;
     __shared__ volatile int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -116,13 +164,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint8_t *sq = reinterpret_cast<uint8_t *>(
                       (reinterpret_cast<uintptr_t>(tree_smem) + 1023) & ~uintptr_t(1023)) +
                   w * S::kWorker;
-    uint8_t *ring = sq + S::kSlot;
-    uint64_t *full = bars[w], *empty = full + NS, *q_full = empty + NS, *s_full = q_full + 1,
-             *p_full = s_full + 1, *o_done = p_full + 1, *idle = o_done + 1;
+    uint8_t *ring = sq + S::kQ;
+    uint64_t *full = bars[w], *empty = full + NS, *q_full = full + S::kQFull,
+             *s_full = full + S::kSFull, *p_full = full + S::kPFull, *o_done = full + S::kODone,
+             *idle = full + S::kIdle;
     if (threadIdx.x == 0) {
-        for (int v = 0; v < 2; ++v) {
-            for (int s = 0; s < 2 * NS + 5; ++s) mbar_init(&bars[v][s], s == 2 * NS || s == 2 * NS + 2 ? 4 : 1);
-        }
+        for (int v = 0; v < 2; ++v)
+            for (int s = 0; s < S::kBars; ++s)
+                mbar_init(&bars[v][s], s == S::kQFull || s >= S::kPFull ? 4 : 1);
         failed = 0;
         fence_mbar_init();
         prefetch_tmap(&kv_map);
@@ -155,28 +204,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         while (more && !stop) {
             more = work.next();
             if (more) then.open(p, work.u);
+            // K of a tile ahead of V of the one before: the order of their products
             const int len = u.ctx + u.count;
-            for (int t = u.t0; t < u.t1 && !stop; ++t) {
-                const int k0 = t * kKeys, n = (min(kKeys, len - k0) + rows_box - 1) / rows_box;
-                // lanes without a box ask for the last one's page
-                int page = pages.get((k0 + min(box_of, n - 1) * rows_box) >> p.ps_shift);
-                if (page < 0 || page >= p.num_pages) {
-                    raise(p.error, PK_DEV_BAD_PAGE);
-                    page = 0;
+            int last = 0;   // the page of this lane's box of the tile before
+            for (int t = u.t0; t <= u.t1 && u.t0 < u.t1 && !stop; ++t) {
+                int page = last;
+                if (t < u.t1) {
+                    const int k0 = t * kKeys, n = (min(kKeys, len - k0) + rows_box - 1) / rows_box;
+                    // lanes without a box ask for the last one's page
+                    page = pages.get((k0 + min(box_of, n - 1) * rows_box) >> p.ps_shift);
+                    if (page < 0 || page >= p.num_pages) {
+                        raise(p.error, PK_DEV_BAD_PAGE);
+                        page = 0;
+                    }
                 }
-                const int in_page = (k0 + box_of * rows_box) & (ps - 1);
 #pragma unroll
-                for (int v = 0; v < 2; ++v, ++it) {
+                for (int v = 0; v < 2; ++v) {
+                    const int tile = t - v;   // V of the tile before
+                    if (tile < u.t0 || tile >= u.t1) continue;
+                    const int k0 = tile * kKeys, n = (min(kKeys, len - k0) + rows_box - 1) / rows_box;
                     const int s = it % NS, use = it / NS;
+                    ++it;
                     if (use) ring_wait(&empty[s], (use - 1) & 1, &failed, p.error);
                     stop = __any_sync(0xffffffffu, failed != 0);
-                    if (stop) break;
+                    if (stop) {
+                        --it;
+                        break;
+                    }
                     if (lane == 0) mbar_arrive_expect_tx(&full[s], n * bytes);
                     __syncwarp();
                     if (box_of < n)
-                        tma_load_rows(ring + s * S::kSlot + box_of * bytes, &kv_map, &full[s], in_page,
-                                      ((page * p.num_layers + p.layer) * 2 + v) * p.kv_heads + u.head);
+                        tma_load_rows(ring + s * S::kSlot + box_of * bytes, &kv_map, &full[s],
+                                      (k0 + box_of * rows_box) & (ps - 1),
+                                      (((v ? last : page) * p.num_layers + p.layer) * 2 + v) * p.kv_heads +
+                                          u.head);
                 }
+                last = page;
             }
             u = work.u;
             pages = then;
@@ -190,7 +253,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         constexpr uint32_t id_s = idesc_bf16(kRows, kKeys);
         constexpr uint32_t id_o = idesc_bf16(kRows, DH) | (1u << 16);   // B MN-major
         const uint64_t q0 = tile_desc(smem_u32(sq), S::kGroup), ring0 = tile_desc(smem_u32(ring), S::kGroup);
-        const uint32_t st = tmem + S::kS + w * kKeys, ot = tmem + S::kO + w * DH;
+        const uint32_t st = tmem + S::kS + w * 2 * kKeys, ot = tmem + S::kO + w * DH;
         // the whole warp walks along, so that indexes and descriptors are uniform
         const bool one = elect_one();
         auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -205,39 +268,44 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 phase ^= 1;
             }
         };
+        // S of a tile, over the P of the tile two before: the products issued so far, of
+        // tiles below j, have to be done with it
+        auto scores = [&](uint32_t tile) {
+            ok = ok && (j == 0 || wait(&o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)) && wait(&full[s], phase);
+            if (!ok) return;
+            tc_fence_after();
+            if (one) {
+                const uint64_t k0 = ring0 + s * (S::kSlot >> 4);
+#pragma unroll
+                for (int kk = 0; kk < DH / 16; ++kk) {
+                    const uint32_t off = ((kk / 4) * 1024 + (kk % 4) * 32) >> 4;
+                    umma_bf16(st + (tile & 1) * kKeys, q0 + off, k0 + off, id_s, kk != 0);
+                }
+                umma_commit(&empty[s]);
+                umma_commit(&s_full[tile & 1]);
+            }
+            __syncwarp();
+            next();
+        };
         while (ok && work.next()) {
             const int n = work.u.t1 - work.u.t0;
             if (n <= 0) continue;
             ok = wait(q_full, unit & 1);
             ++unit;
+            scores(j);
             for (int i = 0; i < n && ok; ++i, ++j) {
-                // S over the P of the tile before, whose product has to be done with it
-                ok = (j == 0 || wait(o_done, (j - 1) & 1)) && wait(&full[s], phase);
-                if (!ok) break;
-                tc_fence_after();
-                if (one) {
-                    const uint64_t k0 = ring0 + s * (S::kSlot >> 4);
-#pragma unroll
-                    for (int kk = 0; kk < DH / 16; ++kk) {
-                        const uint32_t off = ((kk / 4) * 1024 + (kk % 4) * 32) >> 4;
-                        umma_bf16(st, q0 + off, k0 + off, id_s, kk != 0);
-                    }
-                    umma_commit(&empty[s]);
-                    umma_commit(s_full);
-                }
-                __syncwarp();
-                next();
-                ok = wait(&full[s], phase) && wait(p_full, j & 1);
+                if (i + 1 < n) scores(j + 1);
+                ok = ok && wait(&full[s], phase) && wait(&p_full[j & 1], (j >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 if (one) {
                     const uint64_t v0 = ring0 + s * (S::kSlot >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        umma_bf16_ts(ot, st + kk * 8, v0 + kk * (2 * S::kGroup >> 4), id_o,
-                                     (i > 0) | (kk != 0));
+                        umma_bf16_ts(ot, st + (j & 1) * kKeys + kk * 8, v0 + kk * (2 * S::kGroup >> 4),
+                                     id_o, (i > 0) | (kk != 0));
                     umma_commit(&empty[s]);
-                    umma_commit(o_done);
+                    umma_commit(&o_done[j & 1]);
                 }
                 __syncwarp();
                 next();
@@ -248,20 +316,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_wait_bounded(idle, 0, kWaitLimitNs);
     };
 
-    // a row's scores take 128 registers: 208 for the softmax warps out of the launch's
-    // 168 x 384, 88 for the other warpgroup (128 x 88 + 256 x 208 = 64512)
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp & 1) multiply();
         else produce();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         Work work(p, worker);
         // thread = row (TMEM lane) 32 (warp % 4) + lane of the tile
         const int quad = warp & 3, rt = quad * 32 + lane;
         const int gt = threadIdx.x & 127;   // thread in the group
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const uint32_t st = tmem + lanes + S::kS + w * kKeys, ot = tmem + lanes + S::kO + w * DH;
+        const uint32_t st0 = tmem + lanes + S::kS + w * 2 * kKeys, ot = tmem + lanes + S::kO + w * DH;
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q);
         __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
         // this thread's row of a unit
@@ -296,29 +360,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 0) arrive(q_full);
         };
         advance(now);
-        int s = 0;                   // ring slot
-        uint32_t phase = 0, j = 0;   // of the ring, tile of this worker
-        auto next = [&]() {
-            if (++s == NS) {
-                s = 0;
-                phase ^= 1;
-            }
-        };
+        uint32_t it = 0, j = 0;   // ring use and tile of this worker where the unit begins
         while (more) {
             const Unit &u = now.u;
             const int len = u.ctx + u.count;
             float m = -INFINITY, l = 0.f;   // the maximum in use (scaled), the sum
             bool odd = false;               // a value that is not finite among the own rows
-            for (int t = u.t0; t < u.t1; ++t, ++j) {
-                const int k0 = t * kKeys;
-                next();   // V's slot
-                ring_wait(s_full, j & 1, &failed, p.error);
+            const int n = u.t1 - u.t0;
+            for (int i = 0; i < n; ++i, ++j) {
+                const int k0 = (u.t0 + i) * kKeys;
+                const uint32_t st = st0 + (j & 1) * kKeys;
+                ring_wait(&s_full[j & 1], (j >> 1) & 1, &failed, p.error);
                 __syncwarp();
                 tc_fence_after();
                 float sc[kKeys];
-#pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c)
-                    tmem_ld32(st + c * 32, *reinterpret_cast<float(*)[32]>(sc + c * 32));
+                tmem_ld_scores(st, sc);
                 if (k0 + kKeys > u.ctx) {   // some of the step's own tokens, or the end
 #pragma unroll
                     for (int c = 0; c < kKeys / 32; ++c) {
@@ -332,8 +388,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     // values may be inf or NaN: zero in the product, where a weight of
                     // zero would not keep them out; the epilogue adds the latter to the
                     // rows that see them
-                    ring_wait(&full[s], phase, &failed, p.error);
-                    uint8_t *vs = ring + s * S::kSlot;
+                    const uint32_t use = it + (i + 1 < n ? 2 * i + 2 : 2 * i + 1);
+                    ring_wait(&full[use % NS], (use / NS) & 1, &failed, p.error);
+                    uint8_t *vs = ring + use % NS * S::kSlot;
                     bool bad = false;
                     for (int c = max(u.ctx - k0, 0) * (DH / 8) + gt; c < kKeys * DH / 8; c += 128) {
                         const int vr = c / (DH / 8), ch = c % (DH / 8), key = k0 + vr;
@@ -372,7 +429,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const float keep = raise_it ? ex2(m - top) : 1.f;
                     if (raise_it) m = top;
                     l *= keep;
-                    if (t > u.t0) {   // (S came after the product of the tile before)
+                    if (i > 0) {   // O has the unit's tiles before
+                        ring_wait(&o_done[(j - 1) & 1], ((j - 1) >> 1) & 1, &failed, p.error);
+                        __syncwarp();
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DH / 32; ++c) {
                             float o[32];
@@ -385,32 +445,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t scale2 = pair2(p.scale_log2, p.scale_log2), base2 = pair2(-base, -base);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int c = 0; c < kKeys / 64; ++c) {
                     uint32_t x[32];
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float a = ex2(sc[c * 64 + 2 * e] * p.scale_log2 - base);
-                        const float b = ex2(sc[c * 64 + 2 * e + 1] * p.scale_log2 - base);
-                        sum[(2 * e) & 3] += a;
-                        sum[(2 * e + 1) & 3] += b;
+                        const uint64_t y =
+                            fma2(pair2(sc[c * 64 + 2 * e], sc[c * 64 + 2 * e + 1]), scale2, base2);
+                        const float a = ex2(low2(y)), b = ex2(high2(y));
+                        sum[e & 1] = add2(sum[e & 1], pair2(a, b));
                         x[e] = pack2(a, b);
                     }
                     tmem_st32(st + c * 32, x);   // P over the scores, all of them read
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l += (low2(sum[0]) + high2(sum[0])) + (low2(sum[1]) + high2(sum[1]));
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(p_full);
-                next();   // the next K's
+                if (lane == 0) arrive(&p_full[j & 1]);
             }
+            it += 2 * max(n, 0);
             advance(then);
             // O after the unit's last tile
-            const int n = u.t1 - u.t0;
             if (n > 0) {
-                ring_wait(o_done, (j - 1) & 1, &failed, p.error);
+                ring_wait(&o_done[(j - 1) & 1], ((j - 1) >> 1) & 1, &failed, p.error);
                 __syncwarp();
                 tc_fence_after();
             }
