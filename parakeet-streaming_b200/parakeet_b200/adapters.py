@@ -89,8 +89,9 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
     float32 [num_adapters] or None.  The plan's rows are those of ``a`` flattened."""
     dev, shape = a.device, a.shape
     N, K = weight.shape if weight.dim() == 2 else (0, 0)
+    ldw, wcol = weight.stride() if K else (0, 0)
     if a.dtype is not _BF16 or weight.dtype is not _BF16 or not a.is_cuda or weight.device != dev \
-            or shape[-1] != K or weight.stride(1) != 1:
+            or shape[-1] != K or wcol != 1:
         raise ValueError("adapter_gemm needs bf16 operands a [..., K] and weight [N, K], rows "
                          "contiguous, on one CUDA device")
     n = plan.num_adapters
@@ -135,7 +136,7 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
         raise ValueError(f"rank {rank}: a multiple of 8 up to {PK_ADAPTER_MAX_RANK}")
     # (rows padded to 128 of K and of rank; a buffer of this call's own)
     ws = a.new_empty((M + 127) // 128 * 128 * (K + rank))
-    _launch(dev, lib().pk_adapter_gemm, ap, lda, weight.data_ptr(), weight.stride(0), M, N, K,
+    _launch(dev, lib().pk_adapter_gemm, ap, lda, weight.data_ptr(), ldw, M, N, K,
             out.data_ptr(), N, epi, r, ldr, b, alpha, down.data_ptr(), up.data_ptr(), rank, n, sc,
             plan.block.data_ptr(), ws.data_ptr(), _error_word(dev), _stream(dev))
     return out if flat and out.dim() == 2 else out.reshape(*a.shape[:-1], N)
