@@ -235,14 +235,15 @@ constexpr int kTokRowsBox = 64;
 constexpr int tok_workers(int head_dim) { return head_dim == 64 ? 12 : 6; }
 // bf16: row tiles of 16 by mma.sync, a warp a worker, where they hold an average
 // request (its K/V is read once per row tile); of 128 by tcgen05, two workers a CTA,
-// otherwise (160 requests of 21 rows, 8 heads of 64: 500 tokens 54 us by the former, 73
-// by the latter, 2000 tokens 138 and 135; one request of 24 rows and 20,000 tokens 30
-// and 23; 32 x 8 heads of 128 with 28 rows, 8000 tokens 203 and 114).  float32: 16.
+// otherwise (160 requests of 21 rows, 8 heads of 64: 500 tokens 54 us by the former, 64
+// by the latter, 2000 tokens 138 and 128; one request of 24 rows and 20,000 tokens 30
+// and 23; 32 x 8 heads of 128 with 28 rows, 8000 tokens 203 and 113; the lengths, which
+// also tell them apart, are known on the device only).  float32: 16.
 inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
     if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, (kv->d.head_dim == 64 ? 3 : 2) * kv->sms, 1, 1};
     if (mean <= 16) return {16, kTokRowsBox, tok_workers(kv->d.head_dim) * kv->sms, 8, 1};
-    return {128, 64, 2 * kv->sms, 6, 4};
+    return {128, 64, 2 * kv->sms, 6, 4};   // a row tile's ends: 5 to 7 us, four tiles
 }
 
 // Step block, int32 words: header, then arrays at these offsets.  The step's work

@@ -2,11 +2,12 @@
 // on the 5th-generation tensor cores.
 //
 // Bound by reading K and V as long as a request's rows fit one tile: 128 keys of a
-// 128-wide head are 64 KB, 2800 cycles of an SM's share of the memory rate, for
-// 1024 cycles of MMAs and 1024 of exponentials.  But a tile is a chain - S, the softmax
-// of 128 scores a thread (loads from TMEM, maximum, exp2, sum, conversions), O - of some
-// 5000 cycles, and beginning and ending a row tile another.  So one CTA an SM with two
-// workers, each with a share of the step's line, a ring of its own and its own warps:
+// 128-wide head are 64 KB, 2800 cycles of an SM's share of the memory rate, for some
+// 1400 cycles of MMAs and 1024 of exponentials (without either the kernel takes as long).
+// But a tile is a chain - S, the softmax (loads from TMEM, maximum, exp2, sum,
+// conversions), O - and beginning and ending a row tile another.  So one CTA an SM with
+// two workers, each with a share of the step's line, a ring of its own and its own warps,
+// and S of the next tile (of 64 keys) under the softmax of this one:
 //   warps 0, 2   pages of K and V by TMA into a ring of slots (a slot: one tile of K or
 //                of V), running ahead over the worker's units
 //   warps 1, 3   S = Q K^T (both from shared memory, fp32 in TMEM) and O += P V (P
@@ -15,10 +16,11 @@
 //   warps 4..11  four a worker, a thread per row (TMEM lane): the row's scores without a
 //                shuffle, maximum, exp2, P as bf16 over the scores, fp32 sum; the next
 //                unit's queries ahead of the epilogue
-// Two groups that took every other tile of one worker's units and met at their ends took
-// 140 us for 32 requests x 8 heads of 128 with up to 128 rows and 8000 tokens, this takes
-// 124; 160 x 8 heads of 64 with 21 rows and 2000 tokens: 171 and 135; a single request of
-// 131,000 tokens, whose shares are cut twice as often: 98 and 101.
+// Two groups that took every other tile (of 128 keys) of one worker's units and met at
+// their ends took 140 us for 32 requests x 8 heads of 128 with up to 128 rows and 8000
+// tokens, this takes 125 (4.8 TB/s); 160 x 8 heads of 64 with 21 rows and 2000 tokens: 171
+// and 128; 160 x 8 heads of 128 with 33 rows and 500 tokens: 135 and 93; a single request
+// of 131,000 tokens, whose shares are cut twice as often: 98 and 102 (5.3 TB/s).
 // The running maximum is raised, and O scaled for it, only when a row's scores pass
 // the one in use by more than 2^8: weights stay below 256, which the fp32 sums and
 // bf16's exponent hold, and most tiles touch O in the MMA alone.
