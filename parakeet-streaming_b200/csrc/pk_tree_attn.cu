@@ -626,10 +626,8 @@ template <int DH, typename T, bool kTeam>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     constexpr int NV = DH / 32;
     __shared__ float s_acc[8][DH], s_sum[8];
-    grid_dep_wait();
     grid_dep_launch();
     const int64_t share = p.step[kTokShare];
-    if (share == 0) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t n = (int64_t)p.rows * p.heads;
     const int bm = p.shape.rows;
@@ -687,10 +685,16 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
         for (int e = 0; e < NV; ++e) dst[e] = Elem<T>::from_f(acc[e] * inv);
     };
     const int step = kTeam ? 8 : 1, first = kTeam ? warp : 0;
-    for (int64_t i = kTeam ? blockIdx.x : (int64_t)blockIdx.x * 8 + warp; i < n;
-         i += (int64_t)gridDim.x * (kTeam ? 1 : 8)) {
-        int c0, c1, in_tile;
-        if (!find(i, c0, c1, in_tile)) continue;
+    const int64_t i0 = kTeam ? blockIdx.x : (int64_t)blockIdx.x * 8 + warp;
+    int c0, c1, in_tile;
+    // the step's tables are older than the kernel before, which has waited for them: the
+    // first entry is found while that one ends
+    bool cut = share > 0 && find(i0, c0, c1, in_tile);
+    grid_dep_wait();
+    if (share == 0) return;
+    for (int64_t i = i0; i < n; i += (int64_t)gridDim.x * (kTeam ? 1 : 8)) {
+        if (i != i0) cut = find(i, c0, c1, in_tile);
+        if (!cut) continue;
         float acc[NV] = {};
         const float top = highest(c0, c1, in_tile);
         const float sum = add(c0, c1, in_tile, top, first, step, acc);
