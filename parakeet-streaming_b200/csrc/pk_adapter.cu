@@ -232,9 +232,12 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
 // sums of its own rows only, so no product of another adapter's weights reaches a row;
 // with few groups the passes are CTAs of their own (blockIdx.y).
 //
-// Reading x and writing its copy bound it: 6720 x 4096, rank 32, 64 adapters, 110 MB.
-// Tiles staged in shared memory with a barrier a stage took 46 us.
+// Reading x and writing its copy bound it: 6720 x 4096, rank 32, 64 adapters, 126 MB,
+// 34 us.  Tiles staged in shared memory with a barrier a stage took 46.
 constexpr int kShWarps = 8, kShRows = 16;
+// x a block ahead where the registers of two CTAs an SM hold it (rank 32: 34 us for 38 at
+// three CTAs without; rank 16: level; rank 64, where it spills: 16 us slower)
+constexpr bool shrink_ahead(int nt) { return nt == 4; }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -246,7 +249,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
 }
 
 template <int NT>   // 8-column tiles of S: rank <= 8 NT
-__global__ void __launch_bounds__(kShWarps * 32, NT <= 4 ? 3 : 2)
+__global__ void __launch_bounds__(kShWarps * 32, NT < 4 ? 3 : 2)
     adapter_shrink_kernel(const AdapterArgs p) {
     extern __shared__ float sh_part[];   // [warp][row][rank]
     __shared__ int2 s_pair[kShRows];     // the group's pairs: adapter, bits of its rows
@@ -299,12 +302,24 @@ __global__ void __launch_bounds__(kShWarps * 32, NT <= 4 ? 3 : 2)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-        for (int kb = warp; kb < nk; kb += kShWarps) {
-            uint4 a[2][2];   // columns fc .. + 7 of both halves of the block
+        uint4 a[2][2], next[2][2];   // columns fc .. + 7 of both halves of the block
+        auto fetch = [&](int kb, uint4 (&to)[2][2]) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                a[h][0] = in0 ? *reinterpret_cast<const uint4 *>(x0 + kb * 64 + h * 32) : zero;
-                a[h][1] = in1 ? *reinterpret_cast<const uint4 *>(x1 + kb * 64 + h * 32) : zero;
+                to[h][0] = in0 ? *reinterpret_cast<const uint4 *>(x0 + kb * 64 + h * 32) : zero;
+                to[h][1] = in1 ? *reinterpret_cast<const uint4 *>(x1 + kb * 64 + h * 32) : zero;
+            }
+        };
+        if (shrink_ahead(NT) && warp < nk) fetch(warp, next);
+        for (int kb = warp; kb < nk; kb += kShWarps) {
+            if (shrink_ahead(NT)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) a[h][i] = next[h][i];
+                if (kb + kShWarps < nk) fetch(kb + kShWarps, next);
+            } else {
+                fetch(kb, a);
             }
             constexpr int kAtOnce = NT < 8 ? NT : 8;   // tiles of S whose rows are in registers
 #pragma unroll
