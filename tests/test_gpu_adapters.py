@@ -118,11 +118,21 @@ def test_id_patterns(kind):
     check(run(d, scaled=False), reference(d, "store", scaled=False))
 
 
-def test_adapters_do_not_reach_other_rows():
+@pytest.mark.parametrize("K,N,rank", [(1024, 64, 16), (64, 128, 8), (512, 128, 72), (2048, 320, 128)])
+@pytest.mark.parametrize("M", [128, 100, 256])
+def test_an_adapter_a_row(M, K, N, rank):
+    """As many pairs in a tile as it has rows; K split over 8, 1, 8 and 4 CTAs a tile."""
+    d = make(M, N, K, rank, 260, M + rank)
+    d["ids"] = torch.randperm(260)[:M].int().cuda()
+    check(run(d, "silu"), reference(d, "silu"))
+
+
+@pytest.mark.parametrize("M,N,K", [(200, 128, 128), (100, 128, 512), (2400, 2048, 2048), (2500, 256, 64)])
+def test_adapters_do_not_reach_other_rows(M, N, K):
     """Inf and NaN in an adapter's weights, or in a row, stay with that adapter's
     rows and that row."""
-    d = make(200, 128, 128, 16, 6, 3)
-    d["ids"] = (torch.arange(200) % 7 - 1).int().cuda()
+    d = make(M, N, K, 16, 6, 3)
+    d["ids"] = (torch.arange(M) % 7 - 1).int().cuda()
     clean = run(d)
     d["down"][2, 3, 5] = float("nan")
     d["up"][4] = float("inf")
