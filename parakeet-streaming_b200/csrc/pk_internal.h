@@ -227,12 +227,20 @@ struct TokShape {
     int ctas;    // workers: CTAs, or warps of the 16-row bf16 kernel
     int least;   // key tiles that a worker takes before a request's are split over several
     int lead;    // what beginning a row tile costs, in key tiles
+    // so many row tiles of so many key tiles at most: a CTA each, its warps sharing it (24
+    // requests of up to 553 tokens, 4 heads of 128: 27 us in shares, 11 so)
+    int team, team_keys;
+    // workers that get a share of their own before shares grow from two key tiles to
+    // `least` (two requests of up to 5908 tokens, one head of 128: 24 us at 8 tiles, 14 at
+    // two; 160 of up to 500, 8 heads of 64: 27 at 8, 34 at 4)
+    int busy;
 };
 // Most rows of a page that one TMA copy brings, and keys of a tile of the 16-row
 // kernel; its workers an SM, with two tiles of shared memory each (8 KB, or 16 for
 // 128-wide heads).
 constexpr int kTokRowsBox = 64;
 constexpr int tok_workers(int head_dim) { return head_dim == 64 ? 12 : 6; }
+constexpr int tok_warps(int head_dim) { return head_dim == 64 ? 4 : 6; }   // of a CTA
 // bf16: row tiles of 16 by mma.sync, a warp a worker, where they hold an average
 // request (its K/V is read once per row tile); of 128 by tcgen05, two workers a CTA,
 // otherwise (160 requests of 21 rows, 8 heads of 64: 500 tokens 54 us by the former, 64
@@ -241,17 +249,20 @@ constexpr int tok_workers(int head_dim) { return head_dim == 64 ? 12 : 6; }
 // also tell them apart, are known on the device only).  float32: 16.
 inline TokShape tok_shape(const pk_token_kv *kv, int batch, int rows) {
     const int64_t mean = ((int64_t)rows + batch - 1) / (batch > 0 ? batch : 1) * kv->group;
-    if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, (kv->d.head_dim == 64 ? 3 : 2) * kv->sms, 1, 1};
-    if (mean <= 16) return {16, kTokRowsBox, tok_workers(kv->d.head_dim) * kv->sms, 8, 1};
-    return {128, 64, 2 * kv->sms, 6, 4};   // a row tile's ends: 5 to 7 us, four tiles
+    if (kv->d.dtype == PK_DTYPE_F32) return {16, 64, (kv->d.head_dim == 64 ? 3 : 2) * kv->sms, 1, 1, 0, 0, 1};
+    if (mean <= 16) {
+        const int workers = tok_workers(kv->d.head_dim), warps = tok_warps(kv->d.head_dim);
+        return {16, kTokRowsBox, workers * kv->sms, 8, 1, workers / warps * kv->sms, 4 * warps, 4 * kv->sms};
+    }
+    return {128, 64, 2 * kv->sms, 6, 4, 0, 0, 2 * kv->sms};   // a row tile's ends: 5 to 7 us, four tiles
 }
 
 // Step block, int32 words: header, then arrays at these offsets.  The step's work
 // is a line of key tiles, request by request, K/V head by head, row tile by row
 // tile; worker c takes tiles [c * share, (c + 1) * share), whatever they belong to, so
-// that every worker has the same number however the lengths are spread (share 0: a
-// row tile each).
-enum TokHeader { kTokShare = 0, kTokRows, kTokFree, kTokHeaderWords = 16 };
+// that every worker has the same number however the lengths are spread (share 0: kTokPer
+// whole row tiles each).
+enum TokHeader { kTokShare = 0, kTokRows, kTokFree, kTokPer, kTokHeaderWords = 16 };
 struct TokLayout {
     // work: int64 first place (share 0: row tile) of each request; first: the request
     // that each worker begins in (-1: no work); take: first new page; held: pages before

@@ -203,15 +203,20 @@ __device__ void begin_plan(const TokParams &p) {
     longest = __reduce_max_sync(0xffffffffu, longest);
     if ((threadIdx.x & 31) == 0 && longest) atomicMax(&s_longest, longest);
 
-    // the attention's line of tiles: an equal share of it a CTA, but the shape's least
-    // at least; a row tile each where there are no more of them than CTAs and none is
-    // longer than that
+    // the attention's line of tiles: an equal share of it a worker, but the shape's least
+    // at least (and two, while few workers have any); whole row tiles where the most of
+    // them that a worker gets are no longer than that, or where a CTA takes one (167
+    // requests of 14 rows and a few tokens, 8 heads: 33 us in shares, 15 whole)
     const int64_t items_before = block_exclusive_sum64(items, total, s_scan);
     const int64_t all_items = total * p.kv_heads;
     int64_t before = block_exclusive_sum64(tiles, total, s_scan);
     int64_t all = total * p.kv_heads;
-    int64_t share = max((all + p.shape.ctas - 1) / p.shape.ctas, (int64_t)(p.shape.least + p.shape.lead));
-    const bool whole = all_items <= p.shape.ctas && s_longest <= p.shape.least;
+    const int least = min((int64_t)p.shape.least, max(all / p.shape.busy, (int64_t)2));
+    int64_t share = max((all + p.shape.ctas - 1) / p.shape.ctas, (int64_t)(least + p.shape.lead));
+    const int64_t per = max((all_items + p.shape.ctas - 1) / p.shape.ctas, (int64_t)1);
+    const bool whole = per * (s_longest + p.shape.lead) <=
+                           max(share, (int64_t)(p.shape.least + p.shape.lead)) ||
+                       (all_items <= p.shape.team && s_longest <= p.shape.team_keys);
     if (whole) {
         share = 0;
         before = items_before;
@@ -226,10 +231,11 @@ __device__ void begin_plan(const TokParams &p) {
     if (threadIdx.x == 0) {
         work[p.batch] = all;
         st[kTokShare] = (int)min(share, (int64_t)0x7fffffff);
+        st[kTokPer] = (int)per;
         *d.free_count = free_n - (int)min(all_takes, (int64_t)s_taken);
     }
     // CTAs behind the last tile
-    const int64_t used = whole ? all : (all + share - 1) / share;
+    const int64_t each = whole ? per : share, used = (all + each - 1) / each;
     for (int64_t c = used + threadIdx.x; c < p.shape.ctas; c += blockDim.x) st[p.l.first + c] = -1;
 }
 
@@ -317,7 +323,7 @@ __device__ void begin_fill(const TokParams &p, int w, int nw) {
     int32_t *st = p.step;
     const int lane = threadIdx.x & 31;
     const int free_n = st[kTokFree];
-    const int64_t share = max(st[kTokShare], 1);
+    const int64_t share = st[kTokShare] > 0 ? st[kTokShare] : st[kTokPer];
     const int64_t *work = reinterpret_cast<const int64_t *>(st + p.l.work);
     for (int b = w; b < p.batch; b += nw) {
         const int ctx = st[p.l.context + b];

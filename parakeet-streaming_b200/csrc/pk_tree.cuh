@@ -83,8 +83,8 @@ struct Work {
         if (b < 0) return;
         load();
         const int64_t *work = reinterpret_cast<const int64_t *>(p.step + p.l.work);
-        const int64_t from = whole ? (int64_t)c : (int64_t)c * share, local = from - work[b];
-        left = (int)min(whole ? (int64_t)1 : (int64_t)share, work[p.batch] - from);
+        const int64_t each = whole ? p.step[kTokPer] : share, from = c * each, local = from - work[b];
+        left = (int)min(each, work[p.batch] - from);
         int64_t item = local;
         at = 0;
         if (!whole) {

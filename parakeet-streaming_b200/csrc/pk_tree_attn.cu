@@ -33,8 +33,7 @@ namespace {
 constexpr int kTile = kTokRowsBox;   // keys
 // Workers (warps) of a CTA and CTAs an SM: what registers and shared memory hold.
 template <int DH> struct TreeShape {
-    static constexpr int kWarps = DH == 64 ? 4 : 6, kCtas = DH == 64 ? 3 : 1;
-    static_assert(kWarps * kCtas == tok_workers(DH), "workers");
+    static constexpr int kWarps = tok_warps(DH), kCtas = tok_workers(DH) / kWarps;
     static constexpr int kSlot = kTile * DH * 2;   // a tile of K or of V
     static constexpr int kSmem = kWarps * 2 * kSlot + 1024;
 };
@@ -755,11 +754,13 @@ cudaError_t launch_join(const TreeParams &p, int sms, cudaStream_t s) {
 int64_t max_items(const pk_token_kv *kv, int batch, int rows, const TokShape &sh) {
     return ((int64_t)rows * kv->group / sh.rows + batch) * kv->d.num_kv_heads;
 }
-// No row tile of such a step is shared by CTAs: as begin_plan decides, for the
-// longest request that the pool holds.
+// No row tile of such a step is shared by workers: as begin_plan decides, for the
+// longest requests that the pool holds.
 bool never_shared(const pk_token_kv *kv, int batch, int rows, const TokShape &sh) {
-    return (int64_t)kv->d.table_width << kv->ps_shift <= (int64_t)sh.least * sh.keys &&
-           max_items(kv, batch, rows, sh) <= sh.ctas;
+    const int64_t items = max_items(kv, batch, rows, sh), per = (items + sh.ctas - 1) / sh.ctas;
+    const int64_t longest = (((int64_t)kv->d.table_width << kv->ps_shift) + sh.keys - 1) / sh.keys;
+    return per * (longest + sh.lead) <= sh.least + sh.lead ||
+           (items <= sh.team && longest <= sh.team_keys);
 }
 
 }  // namespace
@@ -800,7 +801,7 @@ int launch_tree_attention(const pk_token_kv *kv, const TreeAttnArgs &a, cudaStre
     p.ws_ml = a.ws ? a.ws + (int64_t)2 * p.shape.ctas * p.shape.rows * d.head_dim : nullptr;
     p.error = d.error;
     const bool shared = !never_shared(kv, a.batch, a.rows, p.shape);
-    // without sharing a CTA has one row tile, so those behind the last have none
+    // workers without a row tile are not started
     const int64_t items = max_items(kv, a.batch, a.rows, p.shape);
     const int ctas = shared || items > p.shape.ctas ? p.shape.ctas : (int)items;
     cudaError_t e = p.shape.rows == 128 ? launch_tree_tc(kv, p, ctas, s)

@@ -96,10 +96,10 @@ def test_calls_refuse(pool):
 
 
 def test_workspace_needed_when_requests_can_be_split():
-    """A pool whose requests may pass 512 tokens splits their keys; without a
-    workspace the call is refused."""
+    """A pool whose requests may be long splits their keys; without a workspace the
+    call is refused."""
     lib, h = _lib.lib(), ctypes.c_void_p()
-    assert lib.pk_token_kv_create(ctypes.byref(make_desc(table_width=64)), ctypes.byref(h)) == 0
+    assert lib.pk_token_kv_create(ctypes.byref(make_desc(table_width=256)), ctypes.byref(h)) == 0
     assert lib.pk_token_attention_workspace(h, 1, 1) > 0
     assert lib.pk_token_attention(h, 0, FAKE, 512, 64, 0.1, 1, 1, 0, FAKE, FAKE, 512, 64, None,
                                   None) == _lib.PK_EINVAL
