@@ -575,6 +575,26 @@ def test_one_token_of_one_kv_head(dh, nl):
     assert pool.read_error() == 0
 
 
+@pytest.mark.parametrize("dtype,H,Hkv,dh,batch,most_ctx,most_new", [
+    (torch.bfloat16, 8, 8, 64, 260, 5, 3), (torch.bfloat16, 16, 8, 128, 150, 20, 7),
+    (torch.bfloat16, 32, 8, 64, 90, 40, 12), (torch.bfloat16, 8, 8, 128, 80, 9, 60),
+    (torch.float32, 8, 8, 64, 120, 30, 4), (torch.bfloat16, 8, 8, 64, 30, 900, 4),
+    (torch.bfloat16, 4, 4, 128, 20, 1400, 2), (torch.bfloat16, 2, 1, 128, 3, 2500, 8)])
+def test_many_short_requests_and_few_long_ones(dtype, H, Hkv, dh, batch, most_ctx, most_new):
+    """More row tiles than workers, a few whole ones each; a CTA's warps on one longer
+    row tile; small shares of few row tiles."""
+    rng = np.random.default_rng(batch)
+    ctx = rng.integers(0, most_ctx + 1, batch).tolist()
+    new = rng.integers(0, most_new + 1, batch).tolist()
+    ctx[0], new[0] = most_ctx, most_new
+    pool, model, step, ref, parents, q = filled(rng, 16, H, Hkv, dh, ctx, new, dtype)
+    want, mean_abs, reach = reference(pool, model, ref, parents, q)
+    out = torch.full_like(q, 7.0)
+    pool.attention(0, q, step, out=out)
+    bound(out.double().cpu().numpy(), want, mean_abs, reach, dtype, most_ctx + most_new, dh)
+    assert pool.read_error() == 0
+
+
 @pytest.mark.parametrize("kernel", range(len(KERNELS)))
 def test_out_may_be_the_query(kernel):
     dtype, H, Hkv, dh, ctx, new = KERNELS[kernel]
