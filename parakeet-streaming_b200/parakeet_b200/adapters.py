@@ -64,7 +64,8 @@ def adapter_plan(ids: torch.Tensor, num_adapters: int) -> AdapterPlan:
 
 
 def _operand(t, shape, dtype, dev, name):
-    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or t.device != dev:
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or \
+            t.get_device() != dev.index:
         raise ValueError(f"{name} must be a contiguous {dtype} {shape} tensor on {dev}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
 

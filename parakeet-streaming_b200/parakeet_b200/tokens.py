@@ -103,6 +103,7 @@ class TokenKVPool:
             raise RuntimeError("TokenKVPool needs a CUDA device")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
         if max_tokens <= 0 or page_size <= 0 or num_slots <= 0:
             raise ValueError("max_tokens, page_size and num_slots must be positive")
         self.num_layers, self.num_heads, self.num_kv_heads = num_layers, num_heads, num_kv_heads
@@ -148,7 +149,7 @@ class TokenKVPool:
     # ------------------------------------------------------------ checks
     def _i32(self, t, n, name):
         """The length of an int32 vector, which has to be ``n`` where given."""
-        if t.dtype is not torch.int32 or t.device != self.device:
+        if t.dtype is not torch.int32 or t.get_device() != self._index:
             raise TypeError(f"{name}: expected int32 on {self.device}, got {t.dtype} on {t.device}")
         if t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
             raise ValueError(f"{name}: expected a contiguous [{'n' if n is None else n}] tensor, "
@@ -164,23 +165,25 @@ class TokenKVPool:
             step.open = False
 
     def _rows(self, t, heads, rows, name):
-        """t [..., rows, heads * head_dim] or [..., rows, heads, head_dim] as the latter."""
-        if t.dtype is not self.dtype or t.device != self.device:
+        """Leading dimensions and strides of t, [..., rows, heads, head_dim] or
+        [..., rows, heads * head_dim]: (leading, all strides, row stride, head stride)."""
+        if t.dtype is not self.dtype or t.get_device() != self._index:
             raise TypeError(f"{name}: expected {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
-        shape = t.shape
-        # (one row of one 64-wide head in several layers fits the former but for its rows)
-        if len(shape) < 3 or shape[-3:] != (rows, heads, self.head_dim):
-            if len(shape) < 2 or shape[-1] != heads * self.head_dim:
-                raise ValueError(f"{name}: expected [..., {rows}, {heads}, {self.head_dim}], got "
-                                 f"{tuple(shape)}")
-            t = t.unflatten(-1, (heads, self.head_dim))
-            shape = t.shape
-        if len(shape) < 3 or shape[-3] != rows:
-            raise ValueError(f"{name}: expected [..., {rows}, {heads}, {self.head_dim}], got "
-                             f"{tuple(shape)}")
-        if t.stride(-1) != 1:
+        shape, strides, dh = t.shape, t.stride(), self.head_dim
+        n = len(shape)
+        if n >= 3 and shape[-1] == dh and shape[-2] == heads and shape[-3] == rows:
+            rs, hs, column = strides[-3:]
+            n -= 3
+        elif n >= 2 and shape[-1] == heads * dh and shape[-2] == rows:
+            rs, column = strides[-2:]
+            hs = dh
+            n -= 2
+        else:
+            raise ValueError(f"{name}: expected [..., {rows}, {heads}, {dh}] or [..., {rows}, "
+                             f"{heads * dh}], got {tuple(shape)}")
+        if column != 1:
             raise ValueError(f"{name}: last dimension must be contiguous")
-        return t
+        return n, strides, rs, hs
 
     # ------------------------------------------------------------ allocator
     def reset(self, page_order=None):
@@ -260,14 +263,13 @@ class TokenKVPool:
         [nl, rows, ...] of layers layer .. layer + nl - 1, with any row and head
         strides (slices of a fused projection)."""
         self._step(step)
-        H = self.num_kv_heads
-        key, value = self._rows(key, H, step.rows, "key"), self._rows(value, H, step.rows, "value")
-        strides = key.stride()
-        if len(strides) > 4 or value.shape != key.shape or value.stride() != strides:
+        leading, strides, rs, hs = self._rows(key, self.num_kv_heads, step.rows, "key")
+        if leading > 1 or self._rows(value, self.num_kv_heads, step.rows, "value")[1] != strides or \
+                value.shape != key.shape:
             raise ValueError("key and value must have the same shape and strides")
-        nl, ls = (key.shape[0], strides[0]) if len(strides) == 4 else (1, 0)
+        nl, ls = (key.shape[0], strides[0]) if leading else (1, 0)
         _launch(self.device, self._lib.pk_token_append, self._h, layer, nl, key.data_ptr(),
-                value.data_ptr(), ls, strides[-3], strides[-2], step.batch, step.rows, step.trees,
+                value.data_ptr(), ls, rs, hs, step.batch, step.rows, step.trees,
                 step.block.data_ptr(), _stream(self.device))
 
     def attention(self, layer: int, query: torch.Tensor, step: TokenStep,
@@ -279,8 +281,8 @@ class TokenKVPool:
         be the query itself).
         Rows of no request, and of refused ones, are left as they were."""
         self._step(step)
-        q = self._rows(query, self.num_heads, step.rows, "query")
-        if q.dim() != 3:
+        leading, _, qrs, qhs = self._rows(query, self.num_heads, step.rows, "query")
+        if leading:
             raise ValueError(f"query: one layer's rows, got {tuple(query.shape)}")
         if out is None:
             out = query.new_empty(query.shape)
@@ -288,12 +290,11 @@ class TokenKVPool:
         elif out.shape != query.shape:
             raise ValueError(f"out: expected {tuple(query.shape)}, got {tuple(out.shape)}")
         else:
-            ors, ohs, _ = self._rows(out, self.num_heads, step.rows, "out").stride()
-        qrs, qhs, _ = q.stride()
+            _, _, ors, ohs = self._rows(out, self.num_heads, step.rows, "out")
         dev, need, ws = self.device, step._workspace, None
         if need:   # a buffer of this call's own: the steps' layers may run side by side
             ws = step.block.new_empty(need // 4).data_ptr()
-        _launch(dev, self._lib.pk_token_attention, self._h, layer, q.data_ptr(), qrs, qhs,
+        _launch(dev, self._lib.pk_token_attention, self._h, layer, query.data_ptr(), qrs, qhs,
                 self.head_dim ** -0.5 if scale is None else scale, step.batch, step.rows, step.trees,
                 step.block.data_ptr(), out.data_ptr(), ors, ohs, ws, _stream(dev))
         return out
