@@ -211,9 +211,13 @@ __device__ void begin_plan(const TokParams &p) {
     const int64_t all_items = total * p.kv_heads;
     int64_t before = block_exclusive_sum64(tiles, total, s_scan);
     int64_t all = total * p.kv_heads;
-    const int least = min((int64_t)p.shape.least, max(all / p.shape.busy, (int64_t)2));
-    int64_t share = max((all + p.shape.ctas - 1) / p.shape.ctas, (int64_t)(least + p.shape.lead));
-    const int64_t per = max((all_items + p.shape.ctas - 1) / p.shape.ctas, (int64_t)1);
+    // (divisions, 0.3 us each, only where their results are not the bounds)
+    const int least = all >= (int64_t)p.shape.least * p.shape.busy ? p.shape.least
+                      : all < 3 * (int64_t)p.shape.busy            ? min(p.shape.least, 2)
+                                                                   : (int)(all / p.shape.busy);
+    int64_t share = least + p.shape.lead;
+    if (all > share * p.shape.ctas) share = (all + p.shape.ctas - 1) / p.shape.ctas;
+    const int64_t per = all_items <= p.shape.ctas ? 1 : (all_items + p.shape.ctas - 1) / p.shape.ctas;
     const bool whole = per * (s_longest + p.shape.lead) <=
                            max(share, (int64_t)(p.shape.least + p.shape.lead)) ||
                        (all_items <= p.shape.team && s_longest <= p.shape.team_keys);
@@ -235,7 +239,7 @@ __device__ void begin_plan(const TokParams &p) {
         *d.free_count = free_n - (int)min(all_takes, (int64_t)s_taken);
     }
     // CTAs behind the last tile
-    const int64_t each = whole ? per : share, used = (all + each - 1) / each;
+    const int64_t each = whole ? per : share, used = each == 1 ? all : (all + each - 1) / each;
     for (int64_t c = used + threadIdx.x; c < p.shape.ctas; c += blockDim.x) st[p.l.first + c] = -1;
 }
 
