@@ -6,7 +6,8 @@
 // Three launches:
 //  1. the plan (once per step: every projection of a model uses the same ids)
 //     sorts the rows by adapter, so that a 128-row tile meets few adapters, and
-//     lists each tile's (adapter, rows) pairs; rows of one tile stay in their order;
+//     lists each tile's (adapter, rows) pairs; an adapter's rows stay in their order, and
+//     the rows of a single tile in theirs;
 //  2. S in bf16 and the rows' sorted copy, bound by reading and writing them;
 //  3. the product on the tcgen05 tensor cores, over the sorted rows; after the K
 //     blocks of x W^T each pair of the tile adds one K block S up[a]^T into the same
@@ -17,7 +18,7 @@
 //
 // S is rounded to bf16 because the tensor cores take it so: off by 2^-8 of each of
 // its terms at most, as the bf16 result is of their sum.  Sums are
-// fp32 throughout and in a fixed order.
+// fp32 throughout and in an order that the ids alone give.
 #include "pk_common.cuh"
 #include "pk_internal.h"
 #include "pk_umma.cuh"
@@ -91,101 +92,142 @@ __global__ void __launch_bounds__(kTileRows)
     }
 }
 
+// More rows than a tile's: a counting sort.  The rows are cut into chunks of neighbouring
+// ones, with counts of their own, and a row's place is its adapter's first one, the
+// adapter's rows in the chunks before and its rank among those of the chunk, which one warp
+// walks: rows of an adapter stay in their order.  (Places handed out by atomics go by which
+// warp comes first, and a row near a tile's border with them from one tile to the other,
+// where a split product adds its terms in another order.  They took 3.9 us for 320 rows of
+// 32 adapters and 9.1 for 6720 of 64, this takes 5.0 and 10.9; 6720 of 8192 adapters, whose
+// counts leave room for five chunks, 24 and 44.)
+constexpr int kPlanCounts = 50 * 1024;   // words of shared memory
+struct PlanCut {
+    int chunks;   // as many as the counts leave room for, 32 at most
+    int warps;    // that count the rows of each
+    int steps;    // groups of 32 rows of each
+};
+PlanCut plan_cut(int rows, int adapters) {
+    const int groups = (rows + 31) / 32, room = kPlanCounts / (adapters + 1) - 1;
+    PlanCut c;
+    c.chunks = room < 32 ? room : 32;
+    c.warps = 32 / c.chunks;
+    c.steps = (groups + c.chunks - 1) / c.chunks;
+    return c;
+}
 __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, int rows,
                                                             int adapters, AdapterLayout l,
-                                                            int32_t *plan, int32_t *error) {
-    extern __shared__ int s_bin[];   // [adapters + 1] (the last: rows without one)
-    __shared__ int s_warp[33], s_base, s_pairs, s_moved;
+                                                            PlanCut cut, int32_t *plan,
+                                                            int32_t *error) {
+    // counts, then places [chunk][adapters + 1] (the last: rows without one); each
+    // adapter's first place
+    extern __shared__ int s_bins[];
+    __shared__ int s_warp[2][33], s_moved;
     grid_dep_wait();
     grid_dep_launch();
-    const int tid = threadIdx.x, lane = tid & 31, bins = adapters + 1;
-    const int tiles = (rows + kTileRows - 1) / kTileRows;
-    for (int i = tid; i < bins; i += blockDim.x) s_bin[i] = 0;
-    if (tid == 0) s_base = s_pairs = s_moved = 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = adapters + 1;
+    const int tiles = (rows + kTileRows - 1) / kTileRows, steps = cut.steps;
+    const int chunk = warp / cut.warps, sub = warp - chunk * cut.warps;
+    const bool mine = chunk < cut.chunks;
+    const int row0 = chunk * steps * 32 + lane;   // of the chunk
+    const int of = chunk * bins, firsts = cut.chunks * bins;
+    for (int i = tid; i < firsts; i += blockDim.x) s_bins[i] = 0;
+    if (tid == 0) s_moved = 0;
     __syncthreads();
-    // a thread's rows tid, tid + 1024, ...: the first kHeld of them are read once, all
-    // at a time
+    // kHeld of the warp's steps of its chunk at a time, their ids requested together
     constexpr int kHeld = 8;
-    const int padded = (rows + 31) / 32 * 32;
-    auto bin_of = [&](int r) {   // -1 behind the last row
-        if (r >= rows) return -1;
-        const int a = ids[r];
-        return a >= 0 && a < adapters ? a : adapters;
+    bool bad = false;
+    auto read = [&](int r) { return ids[min(r, rows - 1)]; };
+    auto bin_of = [&](int r, int id) {   // -1 behind the last row
+        const int a = id >= 0 && id < adapters ? id : adapters;
+        bad |= id < -1 || id >= adapters;
+        return r < rows ? a : -1;
     };
     int held[kHeld];
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = bin_of(tid + i * 1024);
-    // one atomic for a warp whose rows agree, one a row otherwise (a match over the
-    // warp's ids costs more than the conflicts that it saves)
-    auto count = [&](int a) {
-        if (__all_sync(0xffffffffu, a == __shfl_sync(0xffffffffu, a, 0))) {
-            if (lane == 0 && a >= 0) atomicAdd(&s_bin[a], 32);
-        } else if (a >= 0) {
-            atomicAdd(&s_bin[a], 1);
-        }
-    };
     bool moved = false;   // a row whose adapter is above the next one's
-    auto look = [&](int r, int a) {
-        int next = __shfl_down_sync(0xffffffffu, a, 1);
-        if (lane == 31) next = bin_of(r + 1);
-        moved |= r + 1 < rows && a > next;
-        if (r < rows && (ids[r] < -1 || ids[r] >= adapters)) raise(error, PK_DEV_BAD_SLOT);
-    };
+    if (mine)
+        for (int s0 = sub; s0 < steps; s0 += kHeld * cut.warps) {
+            int next[kHeld];   // the row behind each step
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-        if (i * 1024 < rows) {
-            count(held[i]);
-            look(tid + i * 1024, held[i]);
+            for (int i = 0; i < kHeld; ++i) {
+                const int step = s0 + i * cut.warps;
+                held[i] = next[i] = 0;
+                if (step < steps) {
+                    held[i] = read(row0 + step * 32);
+                    next[i] = read(row0 - lane + step * 32 + 32);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                const int step = s0 + i * cut.warps;
+                if (step >= steps) break;
+                const int a = held[i] = bin_of(row0 + step * 32, held[i]);
+                // one atomic for a warp whose rows agree, one a row otherwise
+                if (__all_sync(0xffffffffu, a == __shfl_sync(0xffffffffu, a, 0))) {
+                    if (lane == 0 && a >= 0) atomicAdd(&s_bins[of + a], 32);
+                } else if (a >= 0) {
+                    atomicAdd(&s_bins[of + a], 1);
+                }
+                const int b = __shfl_down_sync(0xffffffffu, a, 1);
+                const int after = lane == 31 ? bin_of(row0 + step * 32 + 1, next[i]) : b;
+                moved |= after >= 0 && a > after;
+            }
         }
-    for (int r = tid + kHeld * 1024; r < padded; r += 1024) {
-        const int a = bin_of(r);
-        count(a);
-        look(r, a);
-    }
+    if (bad) raise(error, PK_DEV_BAD_SLOT);
     if (moved) s_moved = 1;
-    __syncthreads();
     // each adapter's first sorted row and first pair (it has one for each tile that
     // its rows touch), 1024 adapters at a time
     int32_t *pair = plan + l.pairs;
     for (int i = tid; i < tiles + 1; i += blockDim.x) plan[l.tile_pair + i] = 0x7fffffff;
+    __syncthreads();
+    int base = 0, pairs = 0;   // rows and pairs of the adapters before
     for (int a0 = 0; a0 < bins; a0 += blockDim.x) {
-        const int a = a0 + tid, n = a < bins ? s_bin[a] : 0;
-        auto scan = [&](int v, int &total) {
+        const int a = a0 + tid;
+        int n = 0;
+        if (a < bins)
+            for (int c0 = 0; c0 < cut.chunks; c0 += 8) {   // the chunks' places from first on
+                int here[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    here[c] = c0 + c < cut.chunks ? s_bins[(c0 + c) * bins + a] : 0;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    if (c0 + c < cut.chunks) s_bins[(c0 + c) * bins + a] = n;
+                    n += here[c];
+                }
+            }
+        auto scan = [&](int v, int &total, int (&sums)[33]) {
             int x = v;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int y = __shfl_up_sync(0xffffffffu, x, o);
                 if (lane >= o) x += y;
             }
-            if (lane == 31) s_warp[tid >> 5] = x;
+            if (lane == 31) sums[warp] = x;
             __syncthreads();
-            if (tid < 32) {
-                int t = s_warp[tid];
+            if (warp == 0) {
+                int t = sums[lane];
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int y = __shfl_up_sync(0xffffffffu, t, o);
                     if (lane >= o) t += y;
                 }
-                s_warp[tid] = t;
-                if (tid == 31) s_warp[32] = t;
+                sums[lane] = t;
+                if (lane == 31) sums[32] = t;
             }
             __syncthreads();
-            total = s_warp[32];
-            const int res = (tid >= 32 ? s_warp[(tid >> 5) - 1] : 0) + x - v;
-            __syncthreads();
-            return res;
+            total = sums[32];
+            return (warp > 0 ? sums[warp - 1] : 0) + x - v;
         };
         int total;
-        const int first = s_base + scan(n, total);
-        __syncthreads();
-        if (tid == 0) s_base += total;
+        const int first = base + scan(n, total, s_warp[0]);
+        base += total;
         const int t0 = first / kTileRows, t1 = n ? (first + n - 1) / kTileRows : t0 - 1;
-        const int mine = a < adapters && n ? t1 - t0 + 1 : 0;
-        const int p0 = s_pairs + scan(mine, total);
-        __syncthreads();
-        if (tid == 0) s_pairs += total;
-        if (a < bins) s_bin[a] = first;   // the sort's running position
-        for (int i = 0; i < mine; ++i) {
+        const int parts = a < adapters && n ? t1 - t0 + 1 : 0;
+        // (the barriers of this scan part the other's uses of its sums, and the other way)
+        const int p0 = pairs + scan(parts, total, s_warp[1]);
+        pairs += total;
+        if (a < bins) s_bins[firsts + a] = first;
+        for (int i = 0; i < parts; ++i) {
             const int t = t0 + i, lo = max(first - t * kTileRows, 0);
             const int hi = min(first + n - t * kTileRows, kTileRows);
             uint32_t in[4];
@@ -194,28 +236,48 @@ __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t *ids, 
             store_pair(pair + (int64_t)kPairWords * (p0 + i), a, in);
             if (lo == 0) plan[l.tile_pair + t] = p0 + i;
         }
-        __syncthreads();
     }
+    __syncthreads();
     // tiles that no adapter's rows begin: past all of them
     for (int i = tid; i < tiles + 1; i += blockDim.x)
-        if (plan[l.tile_pair + i] == 0x7fffffff) plan[l.tile_pair + i] = s_pairs;
+        if (plan[l.tile_pair + i] == 0x7fffffff) plan[l.tile_pair + i] = pairs;
     const bool resort = s_moved != 0;
-    auto place = [&](int r, int a) {
-        int at = r;
-        if (resort) {
-            if (__all_sync(0xffffffffu, a == __shfl_sync(0xffffffffu, a, 0))) {
-                if (lane == 0 && a >= 0) at = atomicAdd(&s_bin[a], 32);
-                at = __shfl_sync(0xffffffffu, at, 0) + lane;
-            } else if (a >= 0) {
-                at = atomicAdd(&s_bin[a], 1);
+    const int bits = 32 - __clz(adapters);
+    const unsigned below = (1u << lane) - 1u;
+    if (mine && sub == 0)
+        for (int s0 = 0; s0 < steps; s0 += kHeld) {
+            const bool others = steps > kHeld || cut.warps > 1;   // than were counted last
+            if (others) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i)
+                    if (s0 + i < steps) held[i] = read(row0 + (s0 + i) * 32);
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (s0 + i >= steps) break;
+                const int r = row0 + (s0 + i) * 32, a = others ? bin_of(r, held[i]) : held[i];
+                int at = r;
+                if (resort) {
+                    // the lanes of the same adapter, by a ballot for each of its bits
+                    unsigned same = __ballot_sync(0xffffffffu, a >= 0);
+                    if (!__all_sync(0xffffffffu, a == __shfl_sync(0xffffffffu, a, 0)))
+#pragma unroll 4
+                        for (int b = 0; b < bits; ++b) {
+                            const unsigned has = __ballot_sync(0xffffffffu, a >> b & 1);
+                            same &= a >> b & 1 ? has : ~has;
+                        }
+                    int before = 0;
+                    if (a >= 0) before = s_bins[of + a] + __popc(same & below);
+                    __syncwarp();   // read by all
+                    if (a >= 0) {
+                        if (same >> lane == 1) s_bins[of + a] = before + 1;   // the last
+                        at = s_bins[firsts + a] + before;
+                    }
+                    __syncwarp();
+                }
+                if (a >= 0) plan[l.order + at] = r;
             }
         }
-        if (a >= 0) plan[l.order + at] = r;
-    };
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-        if (i * 1024 < rows) place(tid + i * 1024, held[i]);
-    for (int r = tid + kHeld * 1024; r < padded; r += 1024) place(r, bin_of(r));
     if (tid == 0) plan[l.sorted] = !resort;
     for (int r = rows + tid; r < tiles * kTileRows; r += blockDim.x) plan[l.order + r] = rows;
 }
@@ -1284,10 +1346,12 @@ int launch_adapter_plan(const int32_t *ids, int rows, int adapters, int32_t *pla
                                       adapters, adapter_layout(rows, adapters), plan, error),
                            "adapter_plan_kernel");
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = allow_smem(adapter_plan_kernel, (PK_ADAPTER_MAX + 1) * 4, done);
+    cudaError_t e = allow_smem(adapter_plan_kernel, kPlanCounts * 4, done);
+    const PlanCut cut = plan_cut(rows, adapters);
     if (e == cudaSuccess)
-        e = launch_pdl(adapter_plan_kernel, dim3(1), dim3(1024), (size_t)(adapters + 1) * 4, s, ids,
-                       rows, adapters, adapter_layout(rows, adapters), plan, error);
+        e = launch_pdl(adapter_plan_kernel, dim3(1), dim3(1024),
+                       (size_t)(cut.chunks + 1) * (adapters + 1) * 4, s, ids, rows, adapters,
+                       adapter_layout(rows, adapters), cut, plan, error);
     return cuda_status(e, "adapter_plan_kernel");
 }
 
