@@ -540,6 +540,8 @@ int64_t pk_token_step_words(const pk_token_kv *kv, int32_t batch, int32_t rows, 
  * range, no room in its table row, rows past `rows`, no pages left) sets its
  * error bit and is left out: CONTEXT -1, its rows' SLOT_MAP -1, no state
  * changed; the others are served.  A bad parent counts as -1 (PK_DEV_BAD_COUNT).
+ * A token whose table entry names no page of the pool has SLOT_MAP -1
+ * (PK_DEV_BAD_PAGE): it is neither appended nor moved.
  * Needs no host read: lengths stay on the device, so a step can be captured. */
 int pk_token_begin_step(pk_token_kv *kv, const int32_t *slots, const int32_t *counts,
                         int32_t batch, const int32_t *parents, int32_t rows, int32_t *step,

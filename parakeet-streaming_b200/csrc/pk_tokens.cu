@@ -105,11 +105,18 @@ __device__ __forceinline__ int ceil_shift(int64_t n, int shift) {
     return (int)((n + (1 << shift) - 1) >> shift);
 }
 
-// Page i of a request: a held one, or the step's (free stack, top first).
-__device__ __forceinline__ int page_of(const TokParams &p, int slot, int held, int first,
-                                       int free_n, int i) {
-    return i < held ? p.d.page_table[(int64_t)slot * p.d.table_width + i]
-                    : p.d.free_pages[free_n - 1 - (first + i - held)];
+// The cache row of a request's token: in a held page, or one of the step's (free stack, top
+// first).  -1, and an error bit, where the table or the stack names no page of the pool.
+__device__ __forceinline__ int row_of(const TokParams &p, int slot, int held, int first, int free_n,
+                                      int tok) {
+    const int i = tok >> p.ps_shift;
+    const int page = i < held ? p.d.page_table[(int64_t)slot * p.d.table_width + i]
+                              : p.d.free_pages[free_n - 1 - (first + i - held)];
+    if ((unsigned)page >= (unsigned)p.d.num_pages) {
+        raise(p.d.error, PK_DEV_BAD_PAGE);
+        return -1;
+    }
+    return (page << p.ps_shift) | (tok & ((1 << p.ps_shift) - 1));
 }
 
 template <int NK>
@@ -309,12 +316,9 @@ __device__ void tree_rows(const TokParams &p, int b, int lane) {
     for (int h = 0; h < 2; ++h) {
         const int j = lane + 32 * h;
         if (j < n) {
-            const int tok = ctx + j;
-            const int page = page_of(p, slot, held, first, free_n, tok >> p.ps_shift);
             st[p.l.request + r0 + j] = b;
             st[p.l.position + r0 + j] = ctx + depth[h];
-            st[p.l.slot_map + r0 + j] =
-                (page << p.ps_shift) | (tok & ((1 << p.ps_shift) - 1));
+            st[p.l.slot_map + r0 + j] = row_of(p, slot, held, first, free_n, ctx + j);
             mask[r0 + j] = (int64_t)m[h];
         }
     }
@@ -359,9 +363,7 @@ __device__ void begin_fill(const TokParams &p, int w, int nw) {
             const int ctx = st[p.l.context + lo];
             if (ctx >= 0) {
                 pos = ctx + r - st[p.l.row_start + lo];
-                const int page = page_of(p, st[p.l.slot + lo], st[p.l.held + lo],
-                                         st[p.l.take + lo], free_n, pos >> p.ps_shift);
-                map = (page << p.ps_shift) | (pos & ((1 << p.ps_shift) - 1));
+                map = row_of(p, st[p.l.slot + lo], st[p.l.held + lo], st[p.l.take + lo], free_n, pos);
             }
         }
         st[p.l.request + r] = req;
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(256)
         const int c = (int)(i - r * per_row), h = c / per_head, e = c - h * per_head;
         const int map = a.step[slot_map + r];
         if (map < 0) continue;
-        if (map >> ps_shift >= d.num_pages) {   // a table that names no page of the pool
+        if (map >> ps_shift >= d.num_pages) {   // a step block that was written to
             raise(d.error, PK_DEV_BAD_PAGE);
             continue;
         }
@@ -469,11 +471,12 @@ __global__ void __launch_bounds__(256)
     if (threadIdx.x < PK_TOK_MAX_TREE && (path >> threadIdx.x & 1) &&
         (int)threadIdx.x >= in_place) {
         const int rank = __popcll(path & ((1ull << threadIdx.x) - 1ull));
-        int src = step[l.slot_map + r0 + threadIdx.x], dst = step[l.slot_map + r0 + rank];
+        int src = step[l.slot_map + r0 + threadIdx.x];
+        const int dst = step[l.slot_map + r0 + rank];
         if ((unsigned)src >> ps_shift >= (unsigned)d.num_pages ||
             (unsigned)dst >> ps_shift >= (unsigned)d.num_pages) {
             raise(d.error, PK_DEV_BAD_PAGE);
-            src = dst = 0;
+            src = -1;   // not moved
         }
         s_src[rank - in_place] = src;
         s_dst[rank - in_place] = dst;
@@ -495,10 +498,12 @@ __global__ void __launch_bounds__(256)
             uint4 v[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
-                if (i + k < moves) v[k] = *reinterpret_cast<const uint4 *>(at(s_src[i + k]));
+                if (i + k < moves && s_src[i + k] >= 0)
+                    v[k] = *reinterpret_cast<const uint4 *>(at(s_src[i + k]));
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
-                if (i + k < moves) *reinterpret_cast<uint4 *>(at(s_dst[i + k])) = v[k];
+                if (i + k < moves && s_src[i + k] >= 0)
+                    *reinterpret_cast<uint4 *>(at(s_dst[i + k])) = v[k];
         }
     }
 }
