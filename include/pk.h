@@ -539,7 +539,11 @@ int64_t pk_token_step_words(const pk_token_kv *kv, int32_t batch, int32_t rows, 
  * A request that cannot be served (slot out of range or twice, count out of
  * range, no room in its table row, rows past `rows`, no pages left) sets its
  * error bit and is left out: CONTEXT -1, its rows' SLOT_MAP -1, no state
- * changed; the others are served.  A bad parent counts as -1 (PK_DEV_BAD_COUNT).
+ * changed; the others are served.  Pages go out in batch order and nobody
+ * overtakes: from the first request on that needs more pages than are left,
+ * every later one that needs any is left out too (PK_DEV_POOL_EXHAUSTED), even
+ * where there would be enough for it; those that need none are served.  Name a
+ * request that may be refused last.  A bad parent counts as -1 (PK_DEV_BAD_COUNT).
  * A token whose table entry names no page of the pool has SLOT_MAP -1
  * (PK_DEV_BAD_PAGE): it is neither appended nor moved.
  * Needs no host read: lengths stay on the device, so a step can be captured. */

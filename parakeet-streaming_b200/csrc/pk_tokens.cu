@@ -179,7 +179,8 @@ __device__ void begin_plan(const TokParams &p) {
         st[kTokFree] = free_n;
     }
 
-    // pages, in batch order: requests past the end of the stack are left out
+    // pages, in batch order: from the first request that finds too few on, those that need
+    // any are left out (nobody overtakes, and one prefix sum decides)
     int64_t first = block_exclusive_sum64(takes, total, s_scan);
     const int64_t all_takes = total;
     int64_t tiles = 0;

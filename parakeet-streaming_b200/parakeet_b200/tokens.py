@@ -208,7 +208,10 @@ class TokenKVPool:
 
         A request that cannot be served (a slot out of range or named twice, a
         count out of range, no room or no pages left) sets its bit of ``error``
-        and is left out: context -1, its rows not appended nor attended."""
+        and is left out: context -1, its rows not appended nor attended.  Pages go out
+        in batch order and nobody overtakes: behind a request that finds too few, the
+        later ones that need any are left out too, even where enough for them are left
+        (those that need none are served)."""
         B = self._i32(slots, None, "slots")
         self._i32(counts, B, "counts")
         trees = parents is not None
