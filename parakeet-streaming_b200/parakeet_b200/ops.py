@@ -25,6 +25,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 def _stream(device) -> int:
     """The device's current stream as a raw handle (torch.cuda.current_stream
     builds an object for it, 2 us of a call)."""
+    if device.type != "cuda":   # as torch does: no kernel is given host pointers
+        raise ValueError(f"expected a cuda device, but got: {device}")
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
