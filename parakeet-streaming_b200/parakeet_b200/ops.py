@@ -31,7 +31,9 @@ def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-_current_device = torch._C._cuda_getDevice
+# (torch.cuda.current_device without its check of the state; a torch without CUDA has
+# neither, and may still import this)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _launch(device, fn, *args) -> None:

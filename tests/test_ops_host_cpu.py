@@ -1,8 +1,12 @@
 """Host side of the calls, on a machine without a GPU: what they refuse before any
 launch, what they keep alive until one is made, and what importing needs."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
+from conftest import REPO
 from parakeet_b200 import ops
 from parakeet_b200.modules.subsample import ConvSubsampling
 
@@ -36,3 +40,17 @@ def test_host_tensors_are_refused_before_a_launch(no_launch):
     with pytest.raises(ValueError, match="cuda device"):
         sub.forward_stream(torch.zeros(1, 80, 16))
     ops._gemm_error.pop(a.device, None)
+
+
+def test_imports_where_torch_has_no_cuda_bindings():
+    code = ("import sys, torch\n"
+            "for name in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, name)\n"
+            f"sys.path[:0] = [{REPO!r}, {REPO + '/parakeet-streaming_b200'!r}]\n"
+            "import parakeet_b200\n"
+            "from parakeet_b200.ops import gemm_supported, layer_norm\n"
+            "a = torch.zeros(4, 64)\n"
+            "assert not gemm_supported(a, a)\n"
+            "layer_norm(a, torch.nn.LayerNorm(64))\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
