@@ -294,12 +294,13 @@ class TokenKVPool:
             raise ValueError(f"out: expected {tuple(query.shape)}, got {tuple(out.shape)}")
         else:
             _, _, ors, ohs = self._rows(out, self.num_heads, step.rows, "out")
-        dev, need, ws = self.device, step._workspace, None
-        if need:   # a buffer of this call's own: the steps' layers may run side by side
-            ws = step.block.new_empty(need // 4).data_ptr()
+        # a buffer of this call's own (the step's layers may run side by side), held until
+        # both of its launches are made: another thread's call may be between them
+        dev, need = self.device, step._workspace
+        ws = step.block.new_empty(need // 4) if need else None
         _launch(dev, self._lib.pk_token_attention, self._h, layer, query.data_ptr(), qrs, qhs,
                 self.head_dim ** -0.5 if scale is None else scale, step.batch, step.rows, step.trees,
-                step.block.data_ptr(), out.data_ptr(), ors, ohs, ws, _stream(dev))
+                step.block.data_ptr(), out.data_ptr(), ors, ohs, _ptr(ws), _stream(dev))
         return out
 
 

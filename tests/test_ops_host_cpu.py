@@ -2,12 +2,13 @@
 launch, what they keep alive until one is made, and what importing needs."""
 import subprocess
 import sys
+import weakref
 
 import pytest
 import torch
 
 from conftest import REPO
-from parakeet_b200 import ops
+from parakeet_b200 import ops, tokens
 from parakeet_b200.modules.subsample import ConvSubsampling
 
 
@@ -54,3 +55,37 @@ def test_imports_where_torch_has_no_cuda_bindings():
             "layer_norm(a, torch.nn.LayerNorm(64))\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_attention_keeps_its_workspace_until_it_has_launched(monkeypatch):
+    """The call's two launches share it.  Given back before them, it could go to a call
+    that another thread makes on the same stream, between the two."""
+    made = []
+
+    class Block:
+        """A step's block that remembers what was allocated beside it."""
+
+        def new_empty(self, n):
+            t = torch.empty(n)
+            made.append((weakref.ref(t), t.data_ptr()))
+            return t
+
+        def data_ptr(self):
+            return 64
+
+    launches = []
+
+    def launch(device, fn, *args):
+        ref, ptr = made[-1]
+        assert ref() is not None and ptr in args
+        launches.append(fn)
+
+    monkeypatch.setattr(tokens, "_launch", launch)
+    monkeypatch.setattr(tokens, "_stream", lambda device: 0)
+    pool = object.__new__(tokens.TokenKVPool)
+    pool.dtype, pool.device, pool._index = torch.float32, torch.device("cpu"), -1
+    pool.num_heads, pool.num_kv_heads, pool.head_dim, pool._h = 2, 1, 64, None
+    pool._lib = NoLaunch()
+    step = tokens.TokenStep(pool, Block(), 1, 3, False, (0,) * 6, 4096)
+    pool.attention(0, torch.zeros(3, 2, 64), step)
+    assert len(launches) == 1 and len(made) == 1
