@@ -797,7 +797,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         prefetch_tmap(&tm.up);
         prefetch_tmap(&tm.s);
     }
-    __syncwarp();
     if (warp == 0) {
         tmem_alloc(&tmem_base, BN);
         tmem_relinquish();

@@ -75,6 +75,7 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, uint32_t group) {
            ((uint64_t)(group >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    __syncwarp();
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
         "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
@@ -88,6 +89,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 }
 // a row's scores: one wait for their loads
 __device__ __forceinline__ void tmem_ld_scores(uint32_t taddr, float (&v)[kKeys]) {
+    __syncwarp();
     uint32_t r[kKeys];
 #pragma unroll
     for (int c = 0; c < kKeys; c += 32)
@@ -129,6 +131,7 @@ __device__ __forceinline__ void tmem_wait_st() {
 // barrier of one worker's softmax warps (four) that also ORs a flag over them
 __device__ __forceinline__ bool group_any(int group, bool v) {
     uint32_t r;
+    __syncwarp();
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
@@ -178,7 +181,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         fence_mbar_init();
         prefetch_tmap(&kv_map);
     }
-    __syncwarp();
     if (warp == 0) {
         tmem_alloc(&tmem_base, S::kTmem);
         tmem_relinquish();
