@@ -188,12 +188,15 @@ class TokenKVPool:
     # ------------------------------------------------------------ allocator
     def reset(self, page_order=None):
         """Every request empty, every page free; pages are taken from the end of
-        ``page_order`` (default 0 .. num_pages - 1)."""
+        ``page_order`` (default 0 .. num_pages - 1), which lists every page once (looked
+        at where it is on the host; a device tensor's values are taken as they are)."""
         order = None
         if page_order is not None:
-            order = torch.as_tensor(page_order, dtype=torch.int32).to(self.device).contiguous()
-            if order.numel() != self.num_pages:
+            order = torch.as_tensor(page_order, dtype=torch.int32)
+            if order.numel() != self.num_pages or not order.is_cuda and not torch.equal(
+                    order.flatten().sort().values, torch.arange(self.num_pages, dtype=torch.int32)):
                 raise ValueError("page_order must list every page once")
+            order = order.to(self.device).contiguous()
         self._order = order
         _launch(self.device, self._lib.pk_token_reset, self._h, _ptr(order), _stream(self.device))
 

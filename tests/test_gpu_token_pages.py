@@ -87,3 +87,21 @@ def test_requests_behind_one_that_found_too_few_pages_get_none(batch):
     pool.end_step(step, i32(np.full(batch, -1)))
     step = pool.begin_step(i32(np.arange(1, batch)), i32(n[1:]), int(n[1:].sum()))
     assert all(c == 10 for c in step.context.tolist()) and int(pool.free_count) == 1
+
+
+@pytest.mark.parametrize("kind", [list, np.array, lambda o: torch.tensor(o)])
+@pytest.mark.parametrize("order", [[0, 1, 2, 2], [0, 1, 2, 4], [-1, 0, 1, 2], [0, 1, 2], [0, 1, 2, 3, 3]])
+def test_an_order_that_does_not_list_every_page_once_is_refused(order, kind):
+    """Two requests would share a page."""
+    args = dict(num_layers=1, num_heads=1, num_kv_heads=1, head_dim=64, num_slots=2, max_tokens=32,
+                num_pages=4, page_size=16, device=DEV)
+    with pytest.raises(ValueError, match="every page once"):
+        TokenKVPool(**args, page_order=kind(order))
+    pool = TokenKVPool(**args, page_order=kind([2, 0, 3, 1]))
+    step = pool.begin_step(i32([0]), i32([20]), 20)
+    pool.end_step(step, i32([19]))
+    with pytest.raises(ValueError, match="every page once"):
+        pool.reset(kind(order))
+    assert pool.lengths.tolist() == [20, 0] and pool.page_table.tolist()[0] == [1, 3]
+    pool.reset(kind([0, 1, 2, 3]))
+    assert pool.free_pages.tolist() == [0, 1, 2, 3] and pool.lengths.tolist() == [0, 0]
