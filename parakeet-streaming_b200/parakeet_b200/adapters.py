@@ -29,7 +29,8 @@ def _error_word(device) -> int:
     if err is None:
         if torch.cuda.is_current_stream_capturing():   # a replay would clear it again
             raise RuntimeError("a device's first adapter call cannot be captured: make one before")
-        err = _gemm_error[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        # (another thread may have made it meanwhile: one word a device)
+        err = _gemm_error.setdefault(device, torch.zeros(1, dtype=torch.int32, device=device))
     return err.data_ptr()
 
 

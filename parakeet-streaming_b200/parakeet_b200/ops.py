@@ -124,8 +124,8 @@ def gemm(a: torch.Tensor, weight: torch.Tensor, epilogue: str = "store",
     if epilogue == "bias" and (bias is None or not bias.is_contiguous()):
         raise ValueError("the bias epilogue needs a contiguous bias")
     err = _gemm_error.get(a.device)
-    if err is None:
-        err = _gemm_error[a.device] = torch.zeros(1, dtype=torch.int32, device=a.device)
+    if err is None:   # (another thread may have made it meanwhile: one word a device)
+        err = _gemm_error.setdefault(a.device, torch.zeros(1, dtype=torch.int32, device=a.device))
     check(lib().pk_gemm_bf16(a2.data_ptr(), a2.stride(0), weight.data_ptr(), weight.stride(0), M,
                              N, K, out.data_ptr(), N, GEMM_EPILOGUES[epilogue], _ptr(r2),
                              r2.stride(0) if r2 is not None else 0, _ptr(bias), float(alpha),

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from conftest import REPO
-from parakeet_b200 import ops, tokens
+from parakeet_b200 import adapters, ops, tokens
 from parakeet_b200.modules.subsample import ConvSubsampling
 
 
@@ -89,3 +89,33 @@ def test_attention_keeps_its_workspace_until_it_has_launched(monkeypatch):
     step = tokens.TokenStep(pool, Block(), 1, 3, False, (0,) * 6, 4096)
     pool.attention(0, torch.zeros(3, 2, 64), step)
     assert len(launches) == 1 and len(made) == 1
+
+
+@pytest.mark.parametrize("who", ["gemm", "adapters"])
+def test_a_devices_error_word_is_one_whoever_makes_it_first(monkeypatch, who):
+    """Two threads' first calls: the word that one of them gives to its kernel is the one
+    that stays, not a tensor that is freed under the kernel."""
+    device = torch.device("cpu")
+    monkeypatch.setattr(ops, "_gemm_error", {})
+    monkeypatch.setattr(adapters, "_gemm_error", ops._gemm_error)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    zeros, others = torch.zeros, []
+
+    def zeros_while_another_thread_is_faster(*shape, **kw):
+        if not others:
+            others.append(zeros(1, dtype=torch.int32))
+            ops._gemm_error[device] = others[0]
+        return zeros(*shape, **kw)
+
+    monkeypatch.setattr(torch, "zeros", zeros_while_another_thread_is_faster)
+    if who == "adapters":
+        given = adapters._error_word(device)
+    else:
+        calls = []
+        monkeypatch.setattr(ops, "_stream", lambda device: 0)
+        monkeypatch.setattr(ops, "lib", lambda: type("L", (), {
+            "pk_gemm_bf16": staticmethod(lambda *args: calls.append(args) or 0)}))
+        a = torch.ones(4, 64, dtype=torch.bfloat16)
+        ops.gemm(a, torch.ones(64, 64, dtype=torch.bfloat16))
+        given = calls[0][-2]
+    assert ops._gemm_error[device] is others[0] and given == others[0].data_ptr()
