@@ -15,14 +15,15 @@
 // two slots of shared memory, one for a tile of 64 keys and one for its V (TMA, a page a
 // copy, 128B swizzle).  It requests the next K as soon as it has read one and the next
 // V likewise, across its units, computes S = Q K^T and O += P V with mma.sync m16n8k16
-// and waits for nobody: 12 such chains an SM for 64-wide heads, 6 for 128 (a tile takes
-// a warp some 2600 cycles; its 16 KB are 700 of an SM's share of the memory rate) hide
-// each other's latencies.  Warps that shared
-// a row tile met in a barrier at its end and cost 5000 cycles a row tile, however short
-// (160 requests of up to 500 tokens, 8 heads: 41 us).
+// and waits for nobody: 12 such chains an SM for 64-wide heads, 6 for 128, hide each
+// other's latencies.  Where every worker has the same, memory bounds it (160 requests of
+// 505 tokens, 8 heads of 64, eight key tiles a warp: 36 us, 4.6 TB/s); where lengths differ
+// and a worker has one row tile, the longest one's chain does (62 to 500 tokens: 27 us for
+// 97 MB).  Warps that shared a row tile met in a barrier at its end and cost 5000 cycles a
+// row tile, however short (the same: 41 us).
 // P is rounded to bf16 for the product, by 2^-8 of each weight at most, as the bf16 V
-// that it multiplies has been; the sum that normalises keeps fp32 weights.  Every wait is bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's
-// other waits return at once.
+// that it multiplies has been; the sum that normalises keeps fp32 weights.  Every wait is
+// bounded: one that runs out sets PK_DEV_TIMEOUT, and the CTA's other waits return at once.
 #include <math.h>
 
 #include "pk_tree.cuh"

@@ -20,7 +20,7 @@
 // their ends took 140 us for 32 requests x 8 heads of 128 with up to 128 rows and 8000
 // tokens, this takes 125 (4.8 TB/s); 160 x 8 heads of 64 with 21 rows and 2000 tokens: 171
 // and 128; 160 x 8 heads of 128 with 33 rows and 500 tokens: 135 and 93; a single request
-// of 131,000 tokens, whose shares are cut twice as often: 98 and 102 (5.3 TB/s).
+// of 131,000 tokens, whose shares are cut twice as often: 98 and 103 (5.2 TB/s).
 // The running maximum is raised, and O scaled for it, only when a row's scores pass
 // the one in use by more than 2^8: weights stay below 256, which the fp32 sums and
 // bf16's exponent hold, and most tiles touch O in the MMA alone.

@@ -88,7 +88,12 @@ def adapter_gemm(a: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: 
 
     a [..., K], weight [N, K], down [num_adapters, rank, K], up [num_adapters, N,
     rank], bf16; K and N multiples of 64, rank a multiple of 8 up to 128; scale
-    float32 [num_adapters] or None.  The plan's rows are those of ``a`` flattened."""
+    float32 [num_adapters] or None.  The plan's rows are those of ``a`` flattened.
+
+    Sums are float32, added in an order that the plan's ids alone give.  The low-rank
+    scale[i] (a[m] down[i]^T) is rounded to bf16 before its product with ``up``, as the
+    tensor cores take it: off by 2^-8 of each term at most, beside the result's own
+    rounding."""
     dev, shape = a.device, a.shape
     N, K = weight.shape if weight.dim() == 2 else (0, 0)
     ldw, wcol = weight.stride() if K else (0, 0)

@@ -285,7 +285,11 @@ class TokenKVPool:
         the rows before and themselves).  query [rows, H, dh] (or [rows, H * dh]);
         ``scale`` defaults to dh ** -0.5; returns ``out`` in the query's shape (it may
         be the query itself).
-        Rows of no request, and of refused ones, are left as they were."""
+        Rows of no request, and of refused ones, are left as they were.
+
+        Sums are float32.  A bfloat16 pool's weights are rounded to bfloat16 for the
+        product with the values, as the tensor cores take them: off by 2^-8 of each term
+        at most, beside the result's own rounding.  A float32 pool rounds neither."""
         self._step(step)
         leading, _, qrs, qhs = self._rows(query, self.num_heads, step.rows, "query")
         if leading:
