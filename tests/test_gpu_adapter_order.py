@@ -52,3 +52,22 @@ def test_split_products_of_several_row_tiles_give_the_same_bits(M, N, K, n):
                 busy = busy @ busy * 1e-2
         assert torch.equal(run(d), first)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,adapters", [(700, 5), (9500, 2000), (9500, 8192)])
+def test_bad_ids_among_many_rows(rows, adapters):
+    """They count as none, and are reported wherever they are."""
+    from parakeet_b200 import _lib, ops
+    device = torch.device("cuda", torch.cuda.current_device())
+    for at in (0, 31, 32, rows // 2, rows - 1):
+        for bad in (-2, adapters, 2 ** 31 - 1, -2 ** 31):
+            ids = ids_of("random", rows, adapters, at)
+            ids[at] = bad
+            plan = adapter_plan(torch.from_numpy(ids).cuda(), adapters)
+            want = np.argsort(np.where((ids < 0) | (ids >= adapters), adapters, ids), kind="stable")
+            assert np.array_equal(plan.block[:rows].cpu().numpy(), want)
+            err = ops._gemm_error[device]
+            assert int(err.item()) == _lib.PK_DEV_BAD_SLOT
+            err.zero_()
+    adapter_plan(torch.from_numpy(ids_of("random", rows, adapters, 1)).cuda(), adapters)
+    assert int(ops._gemm_error[device].item()) == 0
