@@ -576,7 +576,8 @@ int pk_token_attention(pk_token_kv *kv, int32_t layer, const void *query, int64_
  * The rows on its path are moved behind the context in order of depth, in
  * every layer, and lengths grow by the path's tokens.  Pages stay with the
  * request (the next step's tokens need them).  A bad last[b] sets
- * PK_DEV_BAD_COUNT and keeps nothing. */
+ * PK_DEV_BAD_COUNT and keeps nothing, and so does a request whose pages of the
+ * step have been given back (truncated, or the pool reset) since it began. */
 int pk_token_end_step(pk_token_kv *kv, const int32_t *last, int32_t batch, int32_t rows,
                       int32_t trees, const int32_t *step, void *stream);
 

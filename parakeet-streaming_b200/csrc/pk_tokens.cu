@@ -456,7 +456,14 @@ __global__ void __launch_bounds__(256)
     const int ctx = step[l.context + b];
     if (ctx < 0) return;
     const int r0 = step[l.row_start + b], n = step[l.row_start + b + 1] - r0;
+    const int slot = step[l.slot + b];
     int keep = last[b];
+    // pages given back since the step began: the request has been cut (or the pool
+    // reset), and a length past its pages would read what others write there
+    if (((int64_t)d.held[slot] << ps_shift) < (int64_t)ctx + n) {
+        if (layer == 0 && threadIdx.x == 0) raise(d.error, PK_DEV_BAD_COUNT);
+        return;
+    }
     if (keep < -1 || keep >= n) {
         if (layer == 0 && threadIdx.x == 0) raise(d.error, PK_DEV_BAD_COUNT);
         keep = -1;
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(256)
     if (trees && keep >= 0)
         path = (unsigned long long)reinterpret_cast<const int64_t *>(step + l.mask)[r0 + keep];
     const int kept = trees ? __popcll(path) : keep + 1;
-    if (layer == 0 && threadIdx.x == 0) d.lengths[step[l.slot + b]] = ctx + kept;
+    if (layer == 0 && threadIdx.x == 0) d.lengths[slot] = ctx + kept;
     // a path of nodes 0, 1, ... is in place already (every chain)
     if (!trees || path == (kept >= 64 ? ~0ull : (1ull << kept) - 1ull)) return;
     const int in_place = __ffsll(~path) - 1;   // nodes 0 .. in_place - 1 stay

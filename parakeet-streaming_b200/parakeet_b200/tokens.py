@@ -246,7 +246,8 @@ class TokenKVPool:
         """Keep of each request the path to its node ``last[b]`` (int32 [B]; -1:
         nothing; a chain's ``n - 1``: all): its K/V rows are moved behind the
         context in every layer and ``lengths`` grows by them.  Pages stay with
-        the request."""
+        the request.  A request that gave pages of the step back since it began
+        (``truncate``, ``reset``) keeps nothing of it and sets PK_DEV_BAD_COUNT."""
         self._i32(last, step.batch, "last")
         self._step(step, ending=True)
         _launch(self.device, self._lib.pk_token_end_step, self._h, last.data_ptr(), step.batch,

@@ -105,3 +105,41 @@ def test_an_order_that_does_not_list_every_page_once_is_refused(order, kind):
     assert pool.lengths.tolist() == [20, 0] and pool.page_table.tolist()[0] == [1, 3]
     pool.reset(kind([0, 1, 2, 3]))
     assert pool.free_pages.tolist() == [0, 1, 2, 3] and pool.lengths.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("trees", [True, False])
+@pytest.mark.parametrize("cut", ["release", "shorter", "reset"])
+def test_a_step_is_not_ended_over_pages_given_back(cut, trees):
+    """A request cut while its step is open (a client that left) keeps nothing of the
+    step: its length never passes the pages it holds.  The others are ended."""
+    pool = TokenKVPool(2, 2, 2, 64, 3, 200, page_size=16, device=DEV)
+    slots, model = np.arange(3), TokenPoolModel(3, 200, pool.num_pages, 16)
+    grow(pool, model, slots, np.array([30, 40, 50]))
+    n = i32([20, 20, 20])
+    # the path 1, 2, .. 19: rows are moved
+    parents = i32(np.tile(np.concatenate([[-1, -1], np.arange(1, 19)]), 3)) if trees else None
+    step = pool.begin_step(i32(slots), n, 60, parents)
+    k = torch.randn(2, 60, 2, 64, device=DEV).to(torch.bfloat16)
+    pool.append(0, k, k, step)
+    if cut == "reset":
+        pool.reset()
+    else:
+        pool.truncate(i32([1]), i32([0 if cut == "release" else 10]))
+    before, held = pool.kv.clone(), pool.held.tolist()
+    pool.end_step(step, i32([19, 19, 19]))
+    kept = 19 if trees else 20
+    assert pool.read_error() == _lib.PK_DEV_BAD_COUNT
+    assert pool.lengths.tolist() == {"release": [30 + kept, 0, 50 + kept],
+                                     "shorter": [30 + kept, 10, 50 + kept], "reset": [0, 0, 0]}[cut]
+    assert pool.held.tolist() == held
+    left = step.slot_map[20:40].long()
+    for plane in (0, 1):
+        assert torch.equal(pool.kv[left // 16, :, plane, :, left % 16],
+                           before[left // 16, :, plane, :, left % 16])
+    # the request goes on
+    pool.error.zero_()
+    start = pool.lengths[1].item()
+    step = pool.begin_step(i32([1]), i32([3]), 3)
+    assert step.context.tolist() == [start]
+    pool.end_step(step, i32([2]))
+    assert pool.lengths[1].item() == start + 3 and pool.read_error() == 0
